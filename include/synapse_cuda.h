@@ -302,6 +302,76 @@ syn_status_t syn_cuda_kvcache_truncate(syn_cuda_kvcache_t *cache, size_t seq,
 syn_status_t syn_cuda_kvcache_reset(syn_cuda_kvcache_t *cache, size_t seq,
                                     void *stream);
 
+/* ------------------------------------------------------------------ */
+/* Beam search on the paged cache (no counterpart in the reference,    */
+/* which decodes one greedy sequence, generation/pipeline.rs:197-280). */
+/* ------------------------------------------------------------------ */
+
+/* Device pointers of one layer's K and V pools of a paged cache, [n_pages]
+ * [page][n_kv_heads*head_dim] f32 (layers follow one another), and of the
+ * page table, int32 [batch][pages_per_seq], -1 = none. For reading; the
+ * table belongs to the library. SYN_ERR_UNSUPPORTED on a contiguous cache. */
+syn_status_t syn_cuda_kvcache_pool(const syn_cuda_kvcache_t *cache, size_t layer,
+                                   float **k, float **v);
+syn_status_t syn_cuda_kvcache_page_table(const syn_cuda_kvcache_t *cache,
+                                         const int32_t **table,
+                                         size_t *pages_per_seq);
+/* The empty sequence dst gets the first len positions of src: the full pages
+ * are shared (and freed when their last holder lets go), the rows of a partly
+ * filled last page are copied into a page of its own. A sequence that is
+ * truncated into a shared page and grows again gets its own copy first. Paged
+ * caches only; not while the stream is captured; SYN_ERR_OUT_OF_MEMORY
+ * without a free page, nothing changed. */
+syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t *cache, size_t src, size_t dst,
+                                   size_t len, void *stream);
+/* Beams follow their parents: of n distinct sequences (host array) in groups
+ * of `beams` (2..256; 1 changes nothing) of equal committed length, member i
+ * of a group takes the context of member parents[i] (device int32 [n],
+ * indices within the group, as syn_cuda_beam_select writes them; an index out
+ * of range keeps the member's own). All layers; positions beyond the
+ * committed length are not carried over. Full pages move by their table
+ * entries; the partly filled last page stays private: one child of each parent
+ * (the parent itself, else its lowest child) takes it over, the others copy
+ * its rows into the pages of the members without children, in ascending order.
+ * Nothing synchronises. Pages that no member holds any more are counted free
+ * at the next truncate, reset or fork of any sequence, which read the tables
+ * back. May be captured; a sequence reordered by a graph has its table read
+ * back at every such call. Paged caches only. */
+syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t *cache, size_t n,
+                                      const int32_t *seqs, const int32_t *parents,
+                                      size_t beams, void *stream);
+/* Batched append: n_tokens[i] new rows of sequence seqs[i] (host arrays, seqs
+ * distinct), the rows of all sequences one after another in q / k / v (row
+ * stride ld). Headwise RMSNorm of q and k (weights may be NULL = identity) and
+ * RoPE at the cache positions len .. len+n_tokens-1; q goes to q_out (row
+ * stride ldq; q_out may be q), k and the raw v to the cache. The lengths are
+ * not advanced. Rows of a replayed graph beyond max_seq or the pages that
+ * were reserved write nothing. Reductions in parallel order. */
+syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
+    syn_cuda_kvcache_t *cache, size_t layer, size_t n_seqs, const int32_t *seqs,
+    const size_t *n_tokens, const float *q, const float *k, const float *v, size_t ld,
+    size_t n_heads, const float *q_norm, const float *k_norm, float eps,
+    const float *rope_cos, const float *rope_sin, float *q_out, size_t ldq,
+    void *stream);
+/* The k best continuations of each group of beams. Row g*beams + b of logits
+ * (stride ld) is beam b of group g; a candidate (b, t) has the value
+ * scores[g*beams+b] + logits[t] - logsumexp(logits), compared in 64 bits; equal
+ * values go to the lower beam, then to the larger logit, then to the lower
+ * token. NaN counts as -inf, +inf as the largest float. A beam with finished[row] != 0 (may be NULL) has the one candidate
+ * (eos, its score); its others are -inf. Outputs [groups][k], best first:
+ * value, beam within the group, token, and (optional) whether the
+ * continuation is finished (its beam was, or the token is eos; eos < 0: no
+ * such token, finished must be NULL). The outputs may be the inputs where
+ * k == beams. beams, k <= 64, k <= beams*vocab, vocab <= 2^25, at most 65535
+ * rows. Scratch belongs to the
+ * context, as for syn_cuda_qmatmul. */
+syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t *ctx, const float *logits, size_t ld,
+                                  size_t groups, size_t beams, size_t vocab,
+                                  const float *scores, const uint8_t *finished,
+                                  int32_t eos, size_t k, float *out_scores,
+                                  int32_t *out_parents, int32_t *out_tokens,
+                                  uint8_t *out_finished, void *stream);
+
 /* cached_attention_decode (ops/attention.rs:24-147) for sequences
  * [0, batch), one new token each: headwise RMSNorm of q and k (q_norm /
  * k_norm may be NULL = identity), RoPE at position len, K and raw V

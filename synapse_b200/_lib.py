@@ -83,6 +83,16 @@ SIGNATURES = {
     "syn_cuda_kvcache_create_paged": (c_st, [c_vp, c_size, c_size, c_size, c_size, c_size, c_size,
                                              c_size, ctypes.POINTER(c_vp)]),
     "syn_cuda_kvcache_pages_free": (c_st, [c_vp, ctypes.POINTER(c_size)]),
+    "syn_cuda_kvcache_pool": (c_st, [c_vp, c_size, ctypes.POINTER(c_vp), ctypes.POINTER(c_vp)]),
+    "syn_cuda_kvcache_page_table": (c_st, [c_vp, ctypes.POINTER(c_vp), ctypes.POINTER(c_size)]),
+    "syn_cuda_kvcache_fork": (c_st, [c_vp, c_size, c_size, c_size, c_vp]),
+    "syn_cuda_kvcache_reorder": (c_st, [c_vp, c_size, c_vp, c_vp, c_size, c_vp]),
+    "syn_cuda_qk_norm_rope_kv_append_batch": (c_st, [c_vp, c_size, c_size, c_vp, c_vp, c_vp, c_vp,
+                                                     c_vp, c_size, c_size, c_vp, c_vp,
+                                                     ctypes.c_float, c_vp, c_vp, c_vp, c_size,
+                                                     c_vp]),
+    "syn_cuda_beam_select": (c_st, [c_vp, c_vp, c_size, c_size, c_size, c_size, c_vp, c_vp,
+                                    ctypes.c_int32, c_size, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "syn_cuda_model_set_kv_paging": (c_st, [c_vp, c_size, c_size]),
     "syn_cuda_model_kv_pages_free": (c_st, [c_vp, ctypes.POINTER(c_size)]),
     "syn_cuda_decode_step_slots": (c_st, [c_vp, c_size, c_vp, c_vp, c_vp, c_vp]),

@@ -392,6 +392,8 @@ class KVCache:
                  n_pages=0):
         self.max_seq, self.n_kv, self.hd = max_seq, n_kv_heads, head_dim
         self.layers, self.batch = num_layers, batch
+        self.page, self.n_pages = page, n_pages
+        self.device = ctx.device
         h = ctypes.c_void_p()
         _check(lib().syn_cuda_kvcache_create_paged(ctx.handle, max_seq, n_kv_heads, head_dim,
                                                    num_layers, batch, page, n_pages,
@@ -417,6 +419,51 @@ class KVCache:
         n = self.max_seq * self.n_kv * self.hd
         return _wrap_device(k.value, n, (self.max_seq, self.n_kv * self.hd)), \
             _wrap_device(v.value, n, (self.max_seq, self.n_kv * self.hd))
+
+    def pages(self, layer=None):
+        """(K, V) torch views of a paged cache's pools, [n_pages, page, n_kv,
+        hd] of one layer or [layers, ...] of all (syn_cuda_kvcache_pool)."""
+        k, v = ctypes.c_void_p(), ctypes.c_void_p()
+        _check(lib().syn_cuda_kvcache_pool(self.handle, layer or 0, ctypes.byref(k),
+                                           ctypes.byref(v)), "kvcache_pool")
+        shape = (self.n_pages, self.page, self.n_kv, self.hd)
+        if layer is None:
+            shape = (self.layers,) + shape
+        return tuple(_wrap_device(p.value, _numel(shape), shape, device=self.device)
+                     for p in (k, v))
+
+    def device_table(self):
+        """The page table as a torch view, int32 [batch, pages per sequence],
+        -1 = none (syn_cuda_kvcache_page_table). For reading."""
+        p, n = ctypes.c_void_p(), ctypes.c_size_t()
+        _check(lib().syn_cuda_kvcache_page_table(self.handle, ctypes.byref(p), ctypes.byref(n)),
+               "kvcache_page_table")
+        return _wrap_device(p.value, self.batch * n.value, (self.batch, n.value), "<i4",
+                            self.device)
+
+    def fork(self, src, dst, length=None):
+        """The empty sequence dst gets the first `length` (default: all)
+        positions of src; full pages are shared (syn_cuda_kvcache_fork)."""
+        length = self.length(src) if length is None else length
+        _check(lib().syn_cuda_kvcache_fork(self.handle, _index(src), _index(dst), _index(length),
+                                           self._stream()), "kvcache_fork")
+
+    def reorder(self, seqs, parents, beams):
+        """Sequence seqs[i] takes the context of its group's member parents[i]
+        (int32 on the device, as from beam_select), in groups of `beams`
+        (syn_cuda_kvcache_reorder)."""
+        seqs = _int32_array(seqs)
+        _need_cuda(parents)
+        if parents.dtype != torch.int32 or parents.numel() != len(seqs):
+            raise SynapseError(4, "kvcache_reorder")
+        _need_device(self.device, parents)
+        if not seqs:
+            return
+        _check(lib().syn_cuda_kvcache_reorder(self.handle, len(seqs), seqs, _ptr(parents),
+                                              _index(beams), self._stream()), "kvcache_reorder")
+
+    def _stream(self):
+        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
 
     def append(self, layer, k, v, seq=0):
         _need_cuda(k, v)
@@ -451,14 +498,47 @@ class KVCache:
             pass
 
 
-def _wrap_device(addr, numel, shape):
+def _wrap_device(addr, numel, shape, typestr="<f4", device=None):
     """A torch view of library-owned device memory (no copy, no ownership)."""
     class _Iface:
         pass
     it = _Iface()
-    it.__cuda_array_interface__ = {"shape": (numel,), "typestr": "<f4", "data": (addr, False),
+    it.__cuda_array_interface__ = {"shape": (numel,), "typestr": typestr, "data": (addr, False),
                                    "version": 3, "strides": None}
-    return torch.as_tensor(it, device="cuda").view(*shape)
+    return torch.as_tensor(it, device="cuda" if device is None else f"cuda:{device}").view(*shape)
+
+
+def _numel(shape):
+    n = 1
+    for d in shape:
+        n *= d
+    return n
+
+
+def _index(v):
+    """A size or index argument of the C ABI, which has no negative ones."""
+    if v < 0:
+        raise SynapseError(2, f"negative argument {v}")
+    return int(v)
+
+
+def _int32_array(values):
+    values = [int(v) for v in values]
+    if any(not -2**31 <= v < 2**31 for v in values):
+        raise SynapseError(2, "index out of range")
+    return (ctypes.c_int32 * len(values))(*values)
+
+
+def _need_device(device, *ts):
+    for t in ts:
+        if t is not None and t.device.index != device:
+            raise SynapseError(2, f"expected tensors on cuda:{device}")
+
+
+def _need_f32(*ts):
+    for t in ts:
+        if t is not None and t.dtype != torch.float32:
+            raise SynapseError(2, "expected float32 tensors")
 
 
 def attention_decode(cache, layer, qkv, n_heads, q_norm, k_norm, eps, cos_t, sin_t, window=0,
@@ -497,6 +577,86 @@ def attention_prefill(cache, layer, qkv, n_heads, q_norm, k_norm, eps, cos_t, si
         ctypes.c_void_p(base + 4 * (qd + kvd)), ld, n_heads, _ptr(q_norm), _ptr(k_norm),
         float(eps), _ptr(cos_t), _ptr(sin_t), _ptr(out), qd, _stream(qkv)), "attention_prefill")
     return out
+
+
+def _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t):
+    """Shapes, types and device of the rows [q | k | v] and what rotates them."""
+    _need_cuda(qkv, cos_t, sin_t, *(t for t in (q_norm, k_norm) if t is not None))
+    _need_f32(qkv, cos_t, sin_t, q_norm, k_norm)
+    _need_device(cache.device, qkv, cos_t, sin_t, q_norm, k_norm)
+    _index(layer)
+    if qkv.dim() != 2 or qkv.shape[1] < (n_heads + 2 * cache.n_kv) * cache.hd or n_heads < 1:
+        raise SynapseError(4, "qkv rows")
+    half = cache.hd // 2
+    if any(t.numel() < cache.max_seq * half for t in (cos_t, sin_t)):
+        raise SynapseError(4, "rope tables")
+    if any(t is not None and t.numel() != cache.hd for t in (q_norm, k_norm)):
+        raise SynapseError(4, "head norms")
+
+
+def qk_norm_rope_kv_append_batch(cache, layer, seqs, n_tokens, qkv, n_heads, q_norm, k_norm, eps,
+                                 cos_t, sin_t, q_out=None):
+    """Appends n_tokens[i] new rows [q | k | v] of each sequence seqs[i], one
+    sequence after another in qkv: headwise norms, RoPE at the cache positions,
+    K and raw V into the cache (syn_cuda_qk_norm_rope_kv_append_batch). Returns
+    the normalised and rotated q rows [rows, n_heads*hd]; the lengths are not
+    advanced."""
+    _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t)
+    seqs, counts = _int32_array(seqs), [_index(t) for t in n_tokens]
+    qd, kvd, ld = n_heads * cache.hd, cache.n_kv * cache.hd, qkv.shape[1]
+    if len(counts) != len(seqs) or sum(counts) != qkv.shape[0]:
+        raise SynapseError(4, "qk_norm_rope_kv_append_batch")
+    if q_out is None:
+        q_out = torch.empty(qkv.shape[0], qd, dtype=torch.float32, device=qkv.device)
+    else:
+        _need_cuda(q_out)
+        _need_f32(q_out)
+        _need_device(cache.device, q_out)
+        if q_out.shape != (qkv.shape[0], qd):
+            raise SynapseError(4, "q_out")
+    if qkv.shape[0] == 0:
+        return q_out
+    base = qkv.data_ptr()
+    _check(lib().syn_cuda_qk_norm_rope_kv_append_batch(
+        cache.handle, layer, len(seqs), seqs, (ctypes.c_size_t * len(counts))(*counts),
+        ctypes.c_void_p(base), ctypes.c_void_p(base + 4 * qd),
+        ctypes.c_void_p(base + 4 * (qd + kvd)), ld, n_heads, _ptr(q_norm), _ptr(k_norm),
+        float(eps), _ptr(cos_t), _ptr(sin_t), _ptr(q_out), qd, _stream(qkv)),
+        "qk_norm_rope_kv_append_batch")
+    return q_out
+
+
+def beam_select(ctx, logits, scores, beams, k=None, finished=None, eos=-1):
+    """The k (default: beams) best continuations of each group of beams
+    (syn_cuda_beam_select): logits [groups*beams, vocab], scores
+    [groups*beams], finished uint8 [groups*beams] or None. Returns (scores f32,
+    parents int32, tokens int32, finished uint8), each [groups, k], best first."""
+    k = beams if k is None else k
+    for t in (logits, scores, finished):
+        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda):
+            raise SynapseError(2, "expected CUDA tensors")
+    _need_f32(logits, scores)
+    _need_device(ctx.device, logits, scores, finished)
+    if logits.dim() != 2 or beams < 1 or k < 1 or logits.shape[0] % beams:
+        raise SynapseError(4, "beam_select")
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+        raise SynapseError(5, "beam_select")
+    _need_cuda(scores, *([finished] if finished is not None else []))
+    if scores.numel() != rows or (finished is not None and finished.numel() != rows):
+        raise SynapseError(4, "beam_select")
+    if finished is not None and finished.dtype != torch.uint8:
+        raise SynapseError(2, "finished")
+    g, dev = rows // beams, logits.device
+    s = torch.empty(g, k, dtype=torch.float32, device=dev)
+    pt = torch.empty(2, g, k, dtype=torch.int32, device=dev)
+    f = torch.empty(g, k, dtype=torch.uint8, device=dev)
+    if rows:
+        _check(lib().syn_cuda_beam_select(
+            ctx.handle, _ptr(logits), logits.stride(0) if rows > 1 else vocab, g, beams, vocab,
+            _ptr(scores), _ptr(finished), int(eos), k, _ptr(s), _ptr(pt[0]), _ptr(pt[1]), _ptr(f),
+            _stream(logits)), "beam_select")
+    return s, pt[0], pt[1], f
 
 
 # ---------------------------------------------------------------------------

@@ -1,0 +1,929 @@
+// beam.cu -- beam search around the paged KV cache: sequences that share
+// their leading pages (fork), the batched append of new tokens, the choice of
+// the best continuations over beams x vocabulary, and the reordering of the
+// beams' caches after it. The reference decodes one greedy sequence
+// (generation/pipeline.rs:197-280) and has no counterpart.
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "internal.cuh"
+
+namespace syn {
+namespace {
+
+syn_status_t launched(cudaError_t e, const char* where) {
+  if (e == cudaSuccess) return SYN_OK;
+  set_last_cuda_error(e, where);
+  return SYN_ERR_CUDA;
+}
+
+bool capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  cudaStreamIsCapturing(st, &cs);
+  return cs != cudaStreamCaptureStatusNone;
+}
+
+// ---------------------------------------------------------------------------
+// One page's first rows to another page: grid (chunks, layers, K / V)
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) k_kv_copy_page(float4* k, float4* v, size_t layer4,
+                                                      size_t src4, size_t dst4, int n4) {
+  float4* p = (blockIdx.z ? v : k) + blockIdx.y * layer4;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n4; i += gridDim.x * 256)
+    p[dst4 + i] = p[src4 + i];
+}
+
+// ---------------------------------------------------------------------------
+// Reordering of beams. Group members are numbered 0..B-1; member i takes the
+// context of member par(i). Full pages move by their table entries alone. The
+// last, partly filled page of every member stays private, since it is written
+// next: of a parent's children one (the parent itself if it is among them,
+// else the lowest) takes the page over, and each other child copies it into
+// the page of a member that has no child, matched in ascending order. No page
+// is both read and written, so the copies need no second buffer.
+// ---------------------------------------------------------------------------
+constexpr int RO_MAX = 256;  // sequences per call (by value in the launch)
+
+struct ReorderArgs {
+  float4 *k, *v;
+  size_t layer4;   // float4s between layers
+  int* ptab;
+  int maxp, page, row4;  // row4: float4s of one position
+  const int32_t* parents;
+  int n, beams;
+  int seq[RO_MAX];
+  int len[RO_MAX / 2];  // per group (beams >= 2)
+};
+
+__device__ __forceinline__ int ro_parent(const int32_t* par, int i, int beams) {
+  const int p = par[i];
+  return p >= 0 && p < beams ? p : i;  // out of range: the member keeps its own
+}
+
+// Where member i's last page comes from: {member whose page it takes, 1 if
+// the parent's rows have to be copied into it}.
+__device__ __forceinline__ int2 ro_tail(const int* par, int i, int beams) {
+  const int p = par[i];
+  int keeper = -1;
+  if (par[p] == p) {
+    keeper = p;
+  } else {
+    for (int j = 0; j < beams && keeper < 0; j++)
+      if (par[j] == p) keeper = j;
+  }
+  if (keeper == i) return make_int2(p, 0);
+  // rank of i among the children that keep no page, then the childless member of that rank
+  int rank = 0;
+  for (int j = 0; j < i; j++) {
+    const int pj = par[j];
+    bool keeps = pj == j;
+    if (!keeps && par[pj] != pj) {
+      keeps = true;
+      for (int u = 0; u < j; u++)
+        if (par[u] == pj) keeps = false;
+    }
+    rank += !keeps;
+  }
+  for (int j = 0; j < beams; j++) {
+    bool child = false;
+    for (int u = 0; u < beams; u++) child |= par[u] == j;
+    if (!child && rank-- == 0) return make_int2(j, 1);
+  }
+  return make_int2(i, 0);  // not reached: as many childless members as copies
+}
+
+// The copies: grid (chunks, n, layers)
+__global__ void __launch_bounds__(256) k_reorder_copy(const __grid_constant__ ReorderArgs a) {
+  __shared__ int par[RO_MAX];
+  __shared__ int2 t;
+  const int i = blockIdx.y, g0 = i / a.beams * a.beams;
+  for (int j = threadIdx.x; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
+  __syncthreads();
+  if (threadIdx.x == 0) t = ro_tail(par, i - g0, a.beams);
+  __syncthreads();
+  const int len = a.len[i / a.beams], tail = len % a.page;
+  if (!t.y || !tail) return;
+  const int col = len / a.page;
+  const int src = a.ptab[(size_t)a.seq[g0 + par[i - g0]] * a.maxp + col];
+  const int dst = a.ptab[(size_t)a.seq[g0 + t.x] * a.maxp + col];
+  if (src < 0 || dst < 0) return;
+  const int n4 = tail * a.row4;
+  const size_t s4 = (size_t)src * a.page * a.row4, d4 = (size_t)dst * a.page * a.row4;
+  float4* k = a.k + blockIdx.z * a.layer4;
+  float4* v = a.v + blockIdx.z * a.layer4;
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < n4; j += gridDim.x * 256) {
+    k[d4 + j] = k[s4 + j];
+    v[d4 + j] = v[s4 + j];
+  }
+}
+
+// The tables: grid (column chunks of 32, groups), after the copies
+__global__ void __launch_bounds__(256) k_reorder_tables(const __grid_constant__ ReorderArgs a) {
+  __shared__ int par[RO_MAX], from[RO_MAX];
+  extern __shared__ int old[];  // [beams][33]
+  const int g0 = blockIdx.y * a.beams, len = a.len[blockIdx.y];
+  const int full = len / a.page, cols = (len + a.page - 1) / a.page;
+  const int c0 = blockIdx.x * 32;
+  if (c0 >= cols) return;
+  for (int j = threadIdx.x; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
+  for (int t = threadIdx.x; t < a.beams * 32; t += 256) {
+    const int b = t >> 5, c = c0 + (t & 31);
+    if (c < cols) old[b * 33 + (t & 31)] = a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c];
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < a.beams; j += 256) from[j] = ro_tail(par, j, a.beams).x;
+  __syncthreads();
+  for (int t = threadIdx.x; t < a.beams * 32; t += 256) {
+    const int b = t >> 5, c = c0 + (t & 31);
+    if (c < cols)
+      a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c] = old[(c < full ? par[b] : from[b]) * 33 + (t & 31)];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Batched append: rows of new tokens of several sequences, row t of sequence s
+// at position len[s] + t. Per head row: x' = x * w / sqrt(mean(x^2) + eps)
+// (q and k, where a norm weight is given), then the rotation of the pairs
+// (i, i + hd/2) by the position's angle; q goes to q_out, k and the raw v to
+// the position's cache row.
+// LP lanes (a power of two) take one head row, VEC pairs each; ONE: a head row
+// is one step of its lanes, kept in registers between the sum and the rotation.
+// Bound by HBM for prompts, by its launch for single tokens.
+// ---------------------------------------------------------------------------
+constexpr int AP_MAX = 256;  // sequences per launch (by value)
+constexpr int AP_THREADS = 256;
+
+struct AppendArgs {
+  const float *q, *k, *v;
+  long long ld;
+  float* q_out;
+  long long ldq;
+  int n_heads, n_kv, hd;
+  const float *qn, *kn;
+  float eps;
+  const float *cos_t, *sin_t;
+  float *kc, *vc;  // this layer
+  const int* ptab;
+  int page, maxp, max_seq;
+  const int* len;
+  int n;
+  int seq[AP_MAX];
+  int row0[AP_MAX + 1];  // first row of each sequence; [n] = rows
+};
+
+template <int VEC> struct ApVec;
+template <> struct ApVec<4> { using T = float4; };
+template <> struct ApVec<1> { using T = float; };
+
+template <int VEC, int LP, bool ONE>
+__global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_constant__ AppendArgs a) {
+  using T = typename ApVec<VEC>::T;
+  const int heads = a.n_heads + 2 * a.n_kv, half = a.hd >> 1, nv = half / VEC;
+  const long long unit = (long long)blockIdx.x * (AP_THREADS / LP) + threadIdx.x / LP;
+  const int lane = threadIdx.x % LP;
+  const int row = (int)(unit / heads), h = (int)(unit - (long long)row * heads);
+  const bool live = row < a.row0[a.n];
+  int s = 0;
+  if (live)
+    for (int step = AP_MAX / 2; step; step >>= 1)  // the last sequence that starts at or before row
+      if (s + step < a.n && a.row0[s + step] <= row) s += step;
+  const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+  const float* src = nullptr;
+  if (live)
+    src = (is_q ? a.q + (long long)h * a.hd
+                : is_v ? a.v + (long long)(h - a.n_heads - a.n_kv) * a.hd
+                       : a.k + (long long)(h - a.n_heads) * a.hd) +
+          (long long)row * a.ld;
+  const float* w = is_q ? a.qn : is_v ? nullptr : a.kn;
+  griddep_wait();
+  T x1[1], x2[1];
+  float scale = 1.0f;
+  if (ONE && live && lane < nv) {
+    x1[0] = reinterpret_cast<const T*>(src)[lane];
+    x2[0] = reinterpret_cast<const T*>(src + half)[lane];
+  }
+  if (a.qn || a.kn) {  // (uniform: the shuffles need every lane)
+    float acc = 0.0f;
+    if (live && w)
+      for (int i = lane; i < nv; i += LP) {
+        T b1, b2;
+        if (ONE) {
+          b1 = x1[0];
+          b2 = x2[0];
+        } else {
+          b1 = reinterpret_cast<const T*>(src)[i];
+          b2 = reinterpret_cast<const T*>(src + half)[i];
+        }
+        const float* f1 = reinterpret_cast<const float*>(&b1);
+        const float* f2 = reinterpret_cast<const float*>(&b2);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], acc));
+      }
+#pragma unroll
+    for (int o = LP / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    scale = 1.0f / sqrtf(acc / (float)a.hd + a.eps);
+  }
+  griddep_launch();
+  if (!live) return;
+  const int pos = a.len[a.seq[s]] + row - a.row0[s];
+  if (pos >= a.max_seq) return;  // (a replayed graph that has run past the cache)
+  float* dst;
+  if (is_q) {
+    dst = a.q_out + (long long)row * a.ldq + (long long)h * a.hd;
+  } else {
+    size_t slot = (size_t)a.seq[s] * a.max_seq + pos;
+    if (a.ptab) {
+      const int pg = a.ptab[(size_t)a.seq[s] * a.maxp + pos / a.page];
+      if (pg < 0) return;
+      slot = (size_t)pg * a.page + pos % a.page;
+    }
+    dst = (is_v ? a.vc + (size_t)(h - a.n_heads - a.n_kv) * a.hd
+                : a.kc + (size_t)(h - a.n_heads) * a.hd) +
+          slot * a.n_kv * a.hd;
+  }
+  const float* ct = a.cos_t + (size_t)pos * half;
+  const float* st = a.sin_t + (size_t)pos * half;
+  for (int i = lane; i < nv; i += LP) {
+    T b1, b2;
+    if (ONE) {
+      b1 = x1[0];
+      b2 = x2[0];
+    } else {
+      b1 = reinterpret_cast<const T*>(src)[i];
+      b2 = reinterpret_cast<const T*>(src + half)[i];
+    }
+    if (!is_v) {
+      float* f1 = reinterpret_cast<float*>(&b1);
+      float* f2 = reinterpret_cast<float*>(&b2);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const int d = i * VEC + e;
+        float y1 = f1[e], y2 = f2[e];
+        if (w) {
+          y1 *= w[d] * scale;
+          y2 *= w[half + d] * scale;
+        }
+        const float c = ct[d], sn = st[d];
+        f1[e] = y1 * c - y2 * sn;
+        f2[e] = y2 * c + y1 * sn;
+      }
+    }
+    reinterpret_cast<T*>(dst)[i] = b1;
+    reinterpret_cast<T*>(dst + half)[i] = b2;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Beam selection. Candidate (b, t) of a group has the value
+//   score_b + (x_bt - logsumexp(x_b)),
+// compared in 64 bits; equal values go to the lower beam, then to the larger
+// logit, then to the lower token. NaN logits count as -inf and +inf as the
+// largest float. A finished beam has one candidate, (eos, score_b); its others
+// are -inf.
+//
+// k_beam_scan, CTA = (segment of a row): one pass over the logits. Within a
+// row the value is monotone in x, so the segment's k best logits are all that
+// can be chosen from it: they are found exactly with 64-bit keys (ordered bits
+// of x, then the lower index). The k-th largest of the threads' own maxima
+// bounds the k-th best from below; what reaches it (at most k * EPT elements)
+// goes to shared memory and is ranked by counting.
+// k_beam_pick, CTA = group: logsumexp of each row from the segments' (max,
+// sum); the k-th best list head bounds the result from below, so at most k
+// lists and k * k elements are ranked.
+// ---------------------------------------------------------------------------
+constexpr int BS_THREADS = 256, BS_KMAX = 64, BS_BMAX = 64;
+
+__device__ __forceinline__ uint32_t ord32(float x) {  // order-preserving, > 0 for every float
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unord32(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint64_t ord64(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ double unord64(uint64_t o) {
+  return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
+__device__ __forceinline__ float tame(float x) {
+  return x != x ? -INFINITY : fminf(x, 3.402823466e+38f) + 0.0f;  // (-0 becomes 0)
+}
+
+struct BeamArgs {
+  const float* x;
+  long long ld;
+  int beams, vocab, k, nseg, vec;
+  const float* scores;
+  const uint8_t* fin;
+  int eos;
+  uint64_t* cand;  // [rows][nseg][k], best first, 0 = none
+  float2* part;    // [rows][nseg] (max, sum of exp(x - max))
+  float* out_s;
+  int32_t *out_p, *out_t;
+  uint8_t* out_f;
+};
+
+template <int EPT>
+__global__ void __launch_bounds__(BS_THREADS) k_beam_scan(const BeamArgs a) {
+  constexpr int SEG = BS_THREADS * EPT;
+  __shared__ uint64_t tmax[BS_THREADS];
+  __shared__ uint64_t list[BS_KMAX * EPT];
+  __shared__ uint64_t bound;
+  __shared__ int cnt;
+  __shared__ float red[BS_THREADS / 32];
+  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = seg * SEG;
+  griddep_wait();
+  float v[EPT];
+  const bool fin = a.fin && a.fin[row];
+  const float* xr = a.x + (long long)row * a.ld;
+#pragma unroll
+  for (int j = 0; j < EPT / 4; j++) {
+    const int i = base + (j * BS_THREADS + tid) * 4;
+    if (fin) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[j * 4 + e] = i + e == a.eos ? 0.0f : -INFINITY;
+    } else if (a.vec && i + 4 <= a.vocab) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(xr + i));
+      v[j * 4] = f.x;
+      v[j * 4 + 1] = f.y;
+      v[j * 4 + 2] = f.z;
+      v[j * 4 + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[j * 4 + e] = i + e < a.vocab ? __ldg(xr + i + e) : -INFINITY;
+    }
+  }
+  if (tid == 0) {
+    bound = 0;
+    cnt = 0;
+  }
+  float m = -INFINITY;
+  uint64_t best = 0;
+#pragma unroll
+  for (int j = 0; j < EPT; j++) {
+    v[j] = tame(v[j]);
+    m = fmaxf(m, v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < EPT; j++) {  // ascending index: the first of equals stays
+    const int i = base + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3);
+    if (v[j] == m && !best && i < a.vocab) best = (uint64_t)ord32(m) << 32 | (uint32_t)~i;
+  }
+  tmax[tid] = best;
+  const float wm = warp_max(m);
+  if (lane == 0) red[warp] = wm;
+  __syncthreads();
+  float M = red[0];
+#pragma unroll
+  for (int w = 1; w < BS_THREADS / 32; w++) M = fmaxf(M, red[w]);
+  // sum of exp over the segment, and the k-th largest of the threads' maxima
+  float s = 0.0f;
+  if (M > -INFINITY) {
+#pragma unroll
+    for (int j = 0; j < EPT; j++) s += expf(v[j] - M);
+  }
+  int above = 0;
+  for (int j = 0; j < BS_THREADS; j++) above += tmax[j] > best;
+  if (best && above == a.k - 1) bound = best;
+  s = warp_sum(s);
+  __syncthreads();
+  if (lane == 0) red[warp] = s;
+  const uint64_t T = bound ? bound : 1;
+#pragma unroll
+  for (int j = 0; j < EPT; j++) {
+    const int i = base + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3);
+    const uint64_t key = (uint64_t)ord32(v[j]) << 32 | (uint32_t)~i;
+    if (i < a.vocab && key >= T) list[atomicAdd(&cnt, 1)] = key;
+  }
+  __syncthreads();
+  griddep_launch();
+  const int n = cnt;
+  uint64_t* out = a.cand + ((size_t)row * a.nseg + seg) * a.k;
+  for (int i = tid; i < n; i += BS_THREADS) {
+    const uint64_t key = list[i];
+    int r = 0;
+    for (int j = 0; j < n; j++) r += list[j] > key;
+    if (r < a.k) out[r] = key;
+  }
+  for (int i = n + tid; i < a.k; i += BS_THREADS) out[i] = 0;
+  if (tid == 0) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < BS_THREADS / 32; w++) t += red[w];
+    a.part[(size_t)row * a.nseg + seg] = make_float2(M, t);
+  }
+}
+
+// A candidate is ord64 of its value (0 = none) and, for equal values, beam,
+// logit and token in 6, 32 and 25 bits, the larger the earlier.
+constexpr int BS_TBITS = 25;
+__device__ __forceinline__ bool over(uint64_t v, uint64_t i, uint64_t w, uint64_t j) {
+  return v > w || (v == w && i > j);
+}
+
+__global__ void __launch_bounds__(BS_THREADS) k_beam_pick(const BeamArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  // heads [nh] and then the finalists [k*k] use the same space
+  uint64_t* lv = reinterpret_cast<uint64_t*>(raw);
+  const int lists = a.beams * a.nseg, cap = max(a.k * a.k, a.k * ((lists + BS_THREADS - 1) / BS_THREADS));
+  uint64_t* li = lv + cap;
+  __shared__ uint64_t tv[BS_THREADS], ti[BS_THREADS];
+  __shared__ double lse[BS_BMAX];
+  __shared__ float sc[BS_BMAX];
+  __shared__ uint8_t fin[BS_BMAX];
+  __shared__ uint64_t bv, bi;
+  __shared__ int cnt;
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r0 = g * a.beams;
+  griddep_wait();
+  for (int b = warp; b < a.beams; b += BS_THREADS / 32) {
+    const float2* p = a.part + (size_t)(r0 + b) * a.nseg;
+    float M = -INFINITY;
+    for (int i = lane; i < a.nseg; i += 32) M = fmaxf(M, p[i].x);
+    M = warp_max(M);
+    double s = 0.0;
+    for (int i = lane; i < a.nseg; i += 32)
+      if (p[i].x > -INFINITY) s += (double)p[i].y * exp((double)p[i].x - (double)M);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) {
+      lse[b] = M > -INFINITY ? (double)M + log(s) : 0.0;
+      sc[b] = tame(a.scores[r0 + b]);
+      fin[b] = a.fin ? a.fin[r0 + b] : 0;
+    }
+  }
+  if (tid == 0) {
+    bv = 0;
+    bi = 0;
+    cnt = 0;
+  }
+  __syncthreads();
+  const uint64_t* cand = a.cand + (size_t)r0 * a.nseg * a.k;
+  auto value = [&](int b, uint64_t key, uint64_t& v, uint64_t& i) {
+    v = 0;
+    i = 0;
+    if (!key) return;
+    v = ord64((double)sc[b] + ((double)unord32((uint32_t)(key >> 32)) - lse[b]));
+    i = (uint64_t)(BS_BMAX - 1 - b) << (32 + BS_TBITS) | key >> 32 << BS_TBITS |
+        ((uint32_t)key & ((1u << BS_TBITS) - 1));
+  };
+  // the k-th best of the threads' best list heads ...
+  uint64_t mv = 0;
+  uint64_t mi = 0;
+  for (int l = tid; l < lists; l += BS_THREADS) {
+    uint64_t v, i;
+    value(l / a.nseg, cand[(size_t)l * a.k], v, i);
+    if (over(v, i, mv, mi)) {
+      mv = v;
+      mi = i;
+    }
+  }
+  tv[tid] = mv;
+  ti[tid] = mi;
+  __syncthreads();
+  int above = 0;
+  for (int j = 0; j < BS_THREADS; j++) above += over(tv[j], ti[j], mv, mi);
+  if (mv && above == a.k - 1) {
+    bv = mv;
+    bi = mi;
+  }
+  __syncthreads();
+  uint64_t Tv = bv;
+  uint64_t Ti = bi;
+  // ... and, where a thread has several lists, of the heads that reach it
+  if (lists > BS_THREADS) {
+    for (int l = tid; l < lists; l += BS_THREADS) {
+      uint64_t v, i;
+      value(l / a.nseg, cand[(size_t)l * a.k], v, i);
+      if (v && !over(Tv, Ti, v, i)) {
+        const int c = atomicAdd(&cnt, 1);
+        lv[c] = v;
+        li[c] = i;
+      }
+    }
+    __syncthreads();
+    const int n = cnt;
+    for (int c = tid; c < n; c += BS_THREADS) {
+      int r = 0;
+      for (int j = 0; j < n; j++) r += over(lv[j], li[j], lv[c], li[c]);
+      if (r == a.k - 1) {
+        bv = lv[c];
+        bi = li[c];
+      }
+    }
+    __syncthreads();
+    Tv = bv;
+    Ti = bi;
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+  }
+  // at most k lists reach it: their elements that do
+  for (int l = tid; l < lists; l += BS_THREADS) {
+    const int b = l / a.nseg;
+    for (int j = 0; j < a.k; j++) {
+      uint64_t v, i;
+      value(b, cand[(size_t)l * a.k + j], v, i);
+      if (!v || over(Tv, Ti, v, i)) break;  // best first
+      const int c = atomicAdd(&cnt, 1);
+      lv[c] = v;
+      li[c] = i;
+    }
+  }
+  __syncthreads();
+  griddep_launch();
+  const int n = cnt;
+  for (int c = tid; c < n; c += BS_THREADS) {
+    const uint64_t v = lv[c];
+    const uint64_t i = li[c];
+    int r = 0;
+    for (int j = 0; j < n; j++) r += over(lv[j], li[j], v, i);
+    if (r < a.k) {
+      const int b = BS_BMAX - 1 - (int)(i >> (32 + BS_TBITS));
+      const int t = (int)((1u << BS_TBITS) - 1 - ((uint32_t)i & ((1u << BS_TBITS) - 1)));
+      const size_t o = (size_t)g * a.k + r;
+      a.out_s[o] = (float)unord64(v);
+      a.out_p[o] = b;
+      a.out_t[o] = t;
+      if (a.out_f) a.out_f[o] = fin[b] || t == a.eos;
+    }
+  }
+}
+
+// Segments of a row: 8, 16 or 32 elements per thread, the largest with which
+// the grid still gives every SM two CTAs.
+int beam_ept(size_t rows, size_t vocab, int sms) {
+  for (int e = 32; e > 8; e >>= 1)
+    if (rows * ((vocab + BS_THREADS * e - 1) / (BS_THREADS * e)) >= 2 * (size_t)sms) return e;
+  return 8;
+}
+
+}  // namespace
+
+syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, cudaStream_t st) {
+  const size_t row4 = c->n_kv * c->hd / 4, page4 = c->page * row4;
+  const int n4 = (int)(rows * row4);
+  if (!n4) return SYN_OK;
+  for (size_t l0 = 0; l0 < c->layers; l0 += 32768) {
+    const unsigned nl = (unsigned)std::min<size_t>(c->layers - l0, 32768);
+    const size_t layer4 = c->n_pages * page4;
+    k_kv_copy_page<<<dim3((unsigned)std::min(8, (n4 + 255) / 256), nl, 2), 256, 0, st>>>(
+        reinterpret_cast<float4*>(c->k) + l0 * layer4, reinterpret_cast<float4*>(c->v) + l0 * layer4,
+        layer4, src * page4, dst * page4, n4);
+  }
+  SYN_LAUNCH_CHECK("k_kv_copy_page");
+  return SYN_OK;
+}
+
+syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
+  if (!c->page || c->stale[seq] == 1) return SYN_OK;  // (a reorder leaves private last pages)
+  if (c->stale[seq] && !capturing(st)) {
+    syn_status_t s = kv_sync(c, st);
+    if (s) return s;
+  }
+  const size_t col = c->len[seq] / c->page;
+  if (col >= c->maxp) return SYN_OK;
+  int* e = c->ptab_h + seq * c->maxp + col;
+  if (*e < 0 || c->refs[*e] <= 1) return SYN_OK;
+  if (capturing(st)) return SYN_ERR_UNSUPPORTED;  // a replay would copy again
+  if (!c->n_free) {
+    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
+  const int old = *e, own = c->free_pages[c->n_free - 1];
+  syn_status_t s = kv_copy_page(c, old, own, c->len[seq] % c->page, st);
+  if (s) return s;
+  c->n_free--;
+  c->refs[old]--;
+  c->refs[own] = 1;
+  *e = own;
+  c->shrunk[seq]++;
+  SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + seq * c->maxp + col, e, sizeof(int),
+                               cudaMemcpyHostToDevice, st));
+  return SYN_OK;
+}
+
+syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st) {
+  if (!c->page || !c->n_stale) return SYN_OK;
+  if (capturing(st)) return SYN_ERR_UNSUPPORTED;
+  SYN_CUDA_TRY(cudaDeviceSynchronize());
+  const size_t entries = c->batch * c->maxp;
+  SYN_CUDA_TRY(cudaMemcpy(c->ptab_h, c->d_ptab, entries * sizeof(int), cudaMemcpyDeviceToHost));
+  std::fill(c->refs, c->refs + c->n_pages, 0);
+  for (size_t i = 0; i < entries; i++)
+    if (c->ptab_h[i] >= 0) c->refs[c->ptab_h[i]]++;
+  c->n_free = 0;
+  for (size_t p = c->n_pages; p-- > 0;)
+    if (!c->refs[p]) c->free_pages[c->n_free++] = (int)p;
+  c->n_stale = 0;
+  for (size_t b = 0; b < c->batch; b++) {
+    if (c->stale[b] == 1) c->stale[b] = 0;
+    c->n_stale += c->stale[b] != 0;  // (2: permuted by a captured graph, at any time)
+  }
+  return SYN_OK;
+}
+
+syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
+                               const int32_t* parents, size_t beams, const size_t* lens,
+                               cudaStream_t st) {
+  ReorderArgs a;
+  a.k = reinterpret_cast<float4*>(c->k);
+  a.v = reinterpret_cast<float4*>(c->v);
+  a.row4 = (int)(c->n_kv * c->hd / 4);
+  a.layer4 = c->n_pages * c->page * a.row4;
+  a.ptab = c->d_ptab;
+  a.maxp = (int)c->maxp;
+  a.page = (int)c->page;
+  a.parents = parents;
+  a.n = (int)n;
+  a.beams = (int)beams;
+  size_t cols = 0, tail = 0;
+  for (size_t i = 0; i < n; i++) a.seq[i] = seqs[i];
+  for (size_t g = 0; g < n / beams; g++) {
+    a.len[g] = (int)lens[g];
+    cols = std::max(cols, (lens[g] + c->page - 1) / c->page);
+    tail = std::max(tail, lens[g] % c->page);
+  }
+  if (!cols) return SYN_OK;
+  if (tail) {
+    const unsigned ch = (unsigned)std::min<size_t>(16, (tail * a.row4 + 255) / 256);
+    for (size_t l0 = 0; l0 < c->layers; l0 += 32768) {
+      const unsigned nl = (unsigned)std::min<size_t>(c->layers - l0, 32768);
+      ReorderArgs b = a;
+      b.k += l0 * a.layer4;
+      b.v += l0 * a.layer4;
+      k_reorder_copy<<<dim3(ch, (unsigned)n, nl), 256, 0, st>>>(b);
+    }
+    SYN_LAUNCH_CHECK("k_reorder_copy");
+  }
+  k_reorder_tables<<<dim3((unsigned)((cols + 31) / 32), (unsigned)(n / beams)), 256,
+                     beams * 33 * sizeof(int), st>>>(a);
+  SYN_LAUNCH_CHECK("k_reorder_tables");
+  return SYN_OK;
+}
+
+syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, size_t n,
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st) {
+  const syn_cuda_kvcache_t* c = at.cache;
+  const size_t kvd = c->n_kv * c->hd;
+  const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
+  size_t done = 0;
+  for (size_t i0 = 0; i0 < n; i0 += AP_MAX) {
+    AppendArgs a;
+    a.n = (int)std::min<size_t>(AP_MAX, n - i0);
+    size_t rows = 0;
+    for (int i = 0; i < a.n; i++) {
+      a.seq[i] = seqs[i0 + i];
+      a.row0[i] = (int)rows;
+      rows += counts[i0 + i];
+    }
+    a.row0[a.n] = (int)rows;
+    if (rows) {
+      a.q = at.q + done * at.ld;
+      a.k = at.k + done * at.ld;
+      a.v = at.v + done * at.ld;
+      a.ld = (long long)at.ld;
+      a.q_out = q_out + done * ldq;
+      a.ldq = (long long)ldq;
+      a.n_heads = (int)at.n_heads;
+      a.n_kv = (int)c->n_kv;
+      a.hd = (int)c->hd;
+      a.qn = at.qn;
+      a.kn = at.kn;
+      a.eps = at.eps;
+      a.cos_t = at.cos_t;
+      a.sin_t = at.sin_t;
+      a.kc = c->k + at.layer * rows_per_layer * kvd;
+      a.vc = c->v + at.layer * rows_per_layer * kvd;
+      a.ptab = c->page ? c->d_ptab : nullptr;
+      a.page = (int)c->page;
+      a.maxp = (int)c->maxp;
+      a.max_seq = (int)c->max_seq;
+      a.len = c->d_len;
+      // 16-byte accesses where every head row's halves start on 16 bytes
+      const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+                            reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out);
+      const bool vec = c->hd % 8 == 0 && low % 16 == 0 && at.ld % 4 == 0 && ldq % 4 == 0;
+      const int lanes = (int)(c->hd / 2) / (vec ? 4 : 1);
+      void (*kern)(const AppendArgs) = nullptr;
+      int lp;
+      if (vec && lanes <= 4) kern = k_append_batch<4, 4, true>, lp = 4;
+      else if (vec && lanes <= 8) kern = k_append_batch<4, 8, true>, lp = 8;
+      else if (vec && lanes <= 16) kern = k_append_batch<4, 16, true>, lp = 16;
+      else if (vec && lanes <= 32) kern = k_append_batch<4, 32, true>, lp = 32;
+      else if (vec) kern = k_append_batch<4, 32, false>, lp = 32;
+      else kern = k_append_batch<1, 32, false>, lp = 32;
+      const size_t units = rows * (at.n_heads + 2 * c->n_kv), per = AP_THREADS / lp;
+      const size_t blocks = (units + per - 1) / per;
+      if (blocks > 0x7FFFFFFF) return SYN_ERR_UNSUPPORTED;
+      syn_status_t s = launched(launch_pdl(kern, dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a),
+                                "k_append_batch");
+      if (s) return s;
+    }
+    done += rows;
+  }
+  return SYN_OK;
+}
+
+size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms) {
+  const size_t seg = (size_t)BS_THREADS * beam_ept(rows, vocab, sms), nseg = (vocab + seg - 1) / seg;
+  return rows * nseg * (k * sizeof(uint64_t) + sizeof(float2));
+}
+
+syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
+                                size_t vocab, const float* scores, const uint8_t* fin, int eos,
+                                size_t k, float* out_s, int32_t* out_p, int32_t* out_t,
+                                uint8_t* out_f, void* scratch, int sms, cudaStream_t st) {
+  const size_t rows = groups * beams;
+  const int ept = beam_ept(rows, vocab, sms);
+  BeamArgs a;
+  a.x = x;
+  a.ld = (long long)ld;
+  a.beams = (int)beams;
+  a.vocab = (int)vocab;
+  a.k = (int)k;
+  a.nseg = (int)((vocab + (size_t)BS_THREADS * ept - 1) / ((size_t)BS_THREADS * ept));
+  a.vec = ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  a.scores = scores;
+  a.fin = fin;
+  a.eos = eos;
+  a.cand = static_cast<uint64_t*>(scratch);
+  a.part = reinterpret_cast<float2*>(a.cand + rows * a.nseg * k);
+  a.out_s = out_s;
+  a.out_p = out_p;
+  a.out_t = out_t;
+  a.out_f = out_f;
+  const size_t lists = beams * a.nseg;
+  const size_t cap = std::max(k * k, k * ((lists + BS_THREADS - 1) / BS_THREADS));
+  const size_t smem = cap * 2 * sizeof(uint64_t);
+  if (smem > 200 * 1024) return SYN_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)a.nseg, (unsigned)rows);
+  void (*scan)(const BeamArgs) = ept == 32 ? k_beam_scan<32> : ept == 16 ? k_beam_scan<16> : k_beam_scan<8>;
+  syn_status_t s = launched(launch_pdl(scan, grid, dim3(BS_THREADS), 0, st, a), "k_beam_scan");
+  if (s) return s;
+  if (smem > 40 * 1024)
+    SYN_CUDA_TRY(cudaFuncSetAttribute(k_beam_pick, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      200 * 1024));
+  return launched(launch_pdl(k_beam_pick, dim3((unsigned)groups), dim3(BS_THREADS), smem, st, a),
+                  "k_beam_pick");
+}
+
+}  // namespace syn
+
+using namespace syn;
+
+extern "C" {
+
+syn_status_t syn_cuda_kvcache_pool(const syn_cuda_kvcache_t* c, size_t layer, float** k, float** v) {
+  if (!c) return SYN_ERR_NULL_PTR;
+  if (layer >= c->layers) return SYN_ERR_INVALID_ARG;
+  if (!c->page) return SYN_ERR_UNSUPPORTED;
+  const size_t off = layer * c->n_pages * c->page * c->n_kv * c->hd;
+  if (k) *k = c->k + off;
+  if (v) *v = c->v + off;
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_kvcache_page_table(const syn_cuda_kvcache_t* c, const int32_t** table,
+                                         size_t* pages_per_seq) {
+  if (!c) return SYN_ERR_NULL_PTR;
+  if (!c->page) return SYN_ERR_UNSUPPORTED;
+  if (table) *table = c->d_ptab;
+  if (pages_per_seq) *pages_per_seq = c->maxp;
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t* c, size_t src, size_t dst, size_t len,
+                                   void* stream) {
+  if (!c) return SYN_ERR_NULL_PTR;
+  if (!c->page) return SYN_ERR_UNSUPPORTED;
+  if (src >= c->batch || dst >= c->batch || src == dst || len > c->len[src] || c->len[dst])
+    return SYN_ERR_INVALID_ARG;
+  DeviceGuard g(c->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (capturing(st)) return SYN_ERR_UNSUPPORTED;  // the tables are kept on the host
+  syn_status_t s = kv_sync(c, st);
+  if (s) return s;
+  int *from = c->ptab_h + src * c->maxp, *to = c->ptab_h + dst * c->maxp;
+  if (to[0] >= 0 && (s = kv_release(c, dst, 0, st))) return s;  // pages taken for a call, never committed
+  const size_t full = len / c->page, tail = len % c->page;
+  if (tail && !c->n_free) {
+    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
+  for (size_t i = 0; i < full; i++) {
+    to[i] = from[i];
+    c->refs[to[i]]++;
+  }
+  if (tail) {
+    to[full] = c->free_pages[--c->n_free];
+    c->refs[to[full]] = 1;
+    if ((s = kv_copy_page(c, from[full], to[full], tail, st))) return s;
+  }
+  c->shrunk[dst]++;
+  if (len)
+    SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + dst * c->maxp, to, (full + (tail != 0)) * sizeof(int),
+                                 cudaMemcpyHostToDevice, st));
+  if ((s = launch_kv_set(c, dst, (int)len, 0, st))) return s;
+  c->len[dst] = len;
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
+                                      const int32_t* parents, size_t beams, void* stream) {
+  if (!c || !seqs || !parents) return SYN_ERR_NULL_PTR;
+  if (!c->page) return SYN_ERR_UNSUPPORTED;
+  if (!n) return SYN_OK;
+  if (!beams || n % beams) return SYN_ERR_SHAPE_MISMATCH;
+  std::vector<uint8_t> seen(c->batch, 0);
+  for (size_t i = 0; i < n; i++) {
+    if (seqs[i] < 0 || (size_t)seqs[i] >= c->batch || seen[seqs[i]]) return SYN_ERR_INVALID_ARG;
+    seen[seqs[i]] = 1;
+    if (c->len[seqs[i]] != c->len[seqs[i - i % beams]]) return SYN_ERR_INVALID_ARG;
+  }
+  if (beams > RO_MAX) return SYN_ERR_UNSUPPORTED;
+  if (beams == 1) return SYN_OK;
+  DeviceGuard g(c->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  syn_status_t s;
+  for (size_t i = 0; i < n; i++)
+    if ((s = kv_own_page(c, seqs[i], st))) return s;
+  const size_t per = RO_MAX / beams * beams;
+  for (size_t i0 = 0; i0 < n; i0 += per) {
+    const size_t m = std::min(per, n - i0);
+    size_t lens[RO_MAX];
+    for (size_t i = 0; i < m; i += beams) lens[i / beams] = c->len[seqs[i0 + i]];
+    if ((s = launch_kv_reorder(c, m, seqs + i0, parents + i0, beams, lens, st))) return s;
+  }
+  const uint8_t mark = capturing(st) ? 2 : 1;
+  for (size_t i = 0; i < n; i++) {
+    c->n_stale += !c->stale[seqs[i]];
+    c->stale[seqs[i]] = std::max(c->stale[seqs[i]], mark);
+  }
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
+    syn_cuda_kvcache_t* c, size_t layer, size_t n_seqs, const int32_t* seqs, const size_t* n_tokens,
+    const float* q, const float* k, const float* v, size_t ld, size_t n_heads, const float* q_norm,
+    const float* k_norm, float eps, const float* rope_cos, const float* rope_sin, float* q_out,
+    size_t ldq, void* stream) {
+  if (!c || !seqs || !n_tokens || !q || !k || !v || !rope_cos || !rope_sin || !q_out)
+    return SYN_ERR_NULL_PTR;
+  if (layer >= c->layers) return SYN_ERR_INVALID_ARG;
+  if (!n_heads || n_heads % c->n_kv) return SYN_ERR_SHAPE_MISMATCH;
+  std::vector<uint8_t> seen(c->batch, 0);
+  size_t rows = 0;
+  for (size_t i = 0; i < n_seqs; i++) {
+    if (seqs[i] < 0 || (size_t)seqs[i] >= c->batch || seen[seqs[i]]) return SYN_ERR_INVALID_ARG;
+    seen[seqs[i]] = 1;
+    if (n_tokens[i] > c->max_seq || c->len[seqs[i]] + n_tokens[i] > c->max_seq)
+      return SYN_ERR_INVALID_ARG;  // CacheFull
+    rows += n_tokens[i];
+  }
+  if (!rows) return SYN_OK;
+  if (rows > 0x7FFFFFFF) return SYN_ERR_UNSUPPORTED;
+  if (ld < c->hd || ldq < n_heads * c->hd) return SYN_ERR_SHAPE_MISMATCH;
+  DeviceGuard g(c->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  syn_status_t s;
+  for (size_t i = 0; i < n_seqs; i++)
+    if (n_tokens[i] && (s = kv_reserve(c, seqs[i], c->len[seqs[i]] + n_tokens[i], st))) return s;
+  AttnArgs a{const_cast<float*>(q), k, v, ld, n_heads, q_norm, k_norm, eps, rope_cos, rope_sin, 0, c,
+             layer, nullptr, 0};
+  return launch_append_batch(a, q_out, ldq, n_seqs, seqs, n_tokens, st);
+}
+
+syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t* ctx, const float* logits, size_t ld,
+                                  size_t groups, size_t beams, size_t vocab, const float* scores,
+                                  const uint8_t* finished, int32_t eos, size_t k, float* out_scores,
+                                  int32_t* out_parents, int32_t* out_tokens, uint8_t* out_finished,
+                                  void* stream) {
+  if (!ctx || !logits || !scores || !out_scores || !out_parents || !out_tokens)
+    return SYN_ERR_NULL_PTR;
+  if (!groups) return SYN_OK;
+  if (!beams || !vocab || !k) return SYN_ERR_INVALID_DIMENSIONS;
+  if (ld < vocab) return SYN_ERR_SHAPE_MISMATCH;
+  if (beams > BS_BMAX || k > BS_KMAX || vocab > 1u << BS_TBITS || groups > 0x7FFFFFFF ||
+      groups * beams > 65535)
+    return SYN_ERR_UNSUPPORTED;
+  if (k > beams * vocab) return SYN_ERR_INVALID_ARG;
+  if (finished && (eos < 0 || (size_t)eos >= vocab)) return SYN_ERR_INVALID_ARG;
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  syn_status_t s = grow_scratch(&ctx->beam, &ctx->beam_bytes,
+                                beam_scratch_bytes(groups * beams, vocab, k, ctx->sms), st);
+  if (s) return s;
+  return launch_beam_select(logits, ld, groups, beams, vocab, scores, finished, eos, k, out_scores,
+                            out_parents, out_tokens, out_finished, ctx->beam, ctx->sms, st);
+}
+
+}  // extern "C"

@@ -95,10 +95,9 @@ size_t layout(syn_cuda_weight_s* w, uint8_t* base) {
   return off;
 }
 
-// Grows one of the context's scratch buffers (zero-filled). Growth frees the
-// old buffer, so it waits for the device first; it is refused while `st` is
-// being captured into a graph.
-syn_status_t grow(void** buf, size_t* cap, size_t bytes, cudaStream_t st) {
+}  // namespace
+
+syn_status_t grow_scratch(void** buf, size_t* cap, size_t bytes, cudaStream_t st) {
   if (bytes <= *cap) return SYN_OK;
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
@@ -118,14 +117,12 @@ syn_status_t grow(void** buf, size_t* cap, size_t bytes, cudaStream_t st) {
   return SYN_OK;
 }
 
-}  // namespace
-
 syn_status_t ensure_scratch(syn_cuda_ctx_s* ctx, const syn_cuda_weight_s* w, size_t m,
                             cudaStream_t st) {
-  syn_status_t s = grow(reinterpret_cast<void**>(&ctx->part), &ctx->part_bytes,
+  syn_status_t s = grow_scratch(reinterpret_cast<void**>(&ctx->part), &ctx->part_bytes,
                         gemv_partial_bytes(w->fmt, m, w->n, w->kp, w->k), st);
   if (s != SYN_OK) return s;
-  return grow(reinterpret_cast<void**>(&ctx->cnt), &ctx->cnt_bytes, gemv_counter_bytes(m, w->n),
+  return grow_scratch(reinterpret_cast<void**>(&ctx->cnt), &ctx->cnt_bytes, gemv_counter_bytes(m, w->n),
               st);
 }
 
@@ -250,6 +247,7 @@ syn_status_t syn_cuda_context_destroy(syn_cuda_ctx_t* ctx) {
     cudaFree(ctx->part);
     cudaFree(ctx->cnt);
     cudaFree(ctx->abuf);
+    cudaFree(ctx->beam);
     cudaFree(ctx->err);
     tp_release(ctx);
   }
@@ -423,7 +421,7 @@ syn_status_t syn_cuda_qmatmul(syn_cuda_ctx_t* ctx, const syn_cuda_weight_t* w, c
   cudaStream_t st = (cudaStream_t)stream;
   const int chunked = (w->fmt == SYN_QFMT_INT8_KN && m > 16) ? 1 : 0;
   if (m >= gemm_min_rows(w->fmt, w->n)) {
-    syn_status_t s = grow(reinterpret_cast<void**>(&ctx->abuf), &ctx->abuf_bytes,
+    syn_status_t s = grow_scratch(reinterpret_cast<void**>(&ctx->abuf), &ctx->abuf_bytes,
                           gemm_a_bytes(w->fmt, m, w->kp), st);
     if (s != SYN_OK) return s;
     return launch_qgemm(w, x, w->k, nullptr, nullptr, m, y, w->n, chunked, ctx->abuf, ctx->err,
@@ -445,7 +443,7 @@ syn_status_t syn_cuda_qmatmul_int8_prequant(syn_cuda_ctx_t* ctx, const syn_cuda_
   if (!g.ok) return SYN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
   if (m >= gemm_min_rows(w->fmt, w->n)) {
-    syn_status_t s = grow(reinterpret_cast<void**>(&ctx->abuf), &ctx->abuf_bytes,
+    syn_status_t s = grow_scratch(reinterpret_cast<void**>(&ctx->abuf), &ctx->abuf_bytes,
                           gemm_a_bytes(w->fmt, m, w->kp), st);
     if (s != SYN_OK) return s;
     return launch_qgemm(w, nullptr, w->k, x_i8, scales_x, m, y, w->n, m > 16 ? 1 : 0, ctx->abuf,

@@ -1,6 +1,8 @@
 // internal.cuh -- library-private types shared by the .cu files.
 #pragma once
 
+#include <utility>
+
 #include "common.cuh"
 
 // One context per device and per issuing stream: the scratch buffers are
@@ -15,6 +17,8 @@ struct syn_cuda_ctx_s {
   size_t cnt_bytes;
   uint8_t* abuf;     // activations prepared for the tensor-core GEMM
   size_t abuf_bytes;
+  void* beam;        // beam selection: the segments' candidates and sums
+  size_t beam_bytes;
   int* err;          // device-side error word (e.g. SYN_ERR_TIMEOUT)
   void* nccl;        // tensor-parallel communicator (ncclComm_t) or nullptr
   int tp_rank, tp_world;
@@ -69,6 +73,15 @@ struct syn_cuda_kvcache_s {
   int* d_ptab;       // device copy
   int* free_pages;   // stack of free page ids (host)
   size_t n_free;
+  // A page can be in several sequences' tables (syn_cuda_kvcache_fork). refs
+  // counts its table entries; it is free at zero. syn_cuda_kvcache_reorder
+  // permutes table rows on the device: until kv_sync the host rows of those
+  // sequences are stale (the same set of pages, in other rows). shrunk[s]
+  // counts the events after which pages that s shared may no longer be.
+  int* refs;         // [n_pages]
+  uint8_t* stale;    // [batch]
+  size_t n_stale;
+  size_t* shrunk;    // [batch]
 };
 
 namespace syn {
@@ -134,6 +147,10 @@ struct GemvNorm {
 syn_status_t launch_qgemv_norm(const syn_cuda_weight_s* w, const GemvNorm& nm, float* y,
                                float* part, size_t part_cap, int* cnt, int* err,
                                cudaStream_t st);
+// Grows one of the context's scratch buffers (zero-filled). Growth frees the
+// old buffer, so it waits for the device first; it is refused while `st` is
+// being captured into a graph.
+syn_status_t grow_scratch(void** buf, size_t* cap, size_t bytes, cudaStream_t st);
 // Grows the context's GEMV scratch for m rows of w (refused during capture).
 syn_status_t ensure_scratch(syn_cuda_ctx_s* ctx, const syn_cuda_weight_s* w, size_t m,
                             cudaStream_t st);
@@ -215,6 +232,14 @@ struct AttnArgs {
 // table, copied to the device on `st`); SYN_ERR_OUT_OF_MEMORY when the pool
 // is exhausted. No-op for a contiguous cache.
 syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st);
+// The page that the next position of seq goes into, if other sequences hold it
+// too, is replaced by a copy (SYN_ERR_UNSUPPORTED while `st` is captured).
+syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
+// Copies rows [0, rows) of page src to page dst, K and V of all layers.
+syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, cudaStream_t st);
+// Reads the table rows that were permuted on the device back to the host and
+// recounts the pages (synchronises the device; refused while `st` is captured).
+syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st);
 // Frees the pages of seq beyond position keep_len (drains `st` first).
 syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cudaStream_t st);
 // Decode step of sequences [0, batch): norm/RoPE/append of the new token,
@@ -263,6 +288,22 @@ syn_status_t launch_kv_advance_slots(syn_cuda_kvcache_t* c, const int* slots, si
 // Device length of sequence seq: set to value (add=0) or advanced by it.
 syn_status_t launch_kv_set(syn_cuda_kvcache_t* c, size_t seq, int value, int add, cudaStream_t st);
 
+// ---- beam search (beam.cu) ----
+// New rows of n sequences (counts[i] rows of seqs[i], host arrays, pages
+// reserved) normalised, rotated and appended; q rows to q_out.
+syn_status_t launch_append_batch(const AttnArgs& a, float* q_out, size_t ldq, size_t n,
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st);
+// Groups of `beams` sequences (seqs and lens on the host, parents on the
+// device) take over their parents' contexts; at most 256 sequences.
+syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
+                               const int32_t* parents, size_t beams, const size_t* lens,
+                               cudaStream_t st);
+size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms);
+syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
+                                size_t vocab, const float* scores, const uint8_t* fin, int eos,
+                                size_t k, float* out_s, int32_t* out_p, int32_t* out_t,
+                                uint8_t* out_f, void* scratch, int sms, cudaStream_t st);
+
 // ---- tensor parallelism (tp.cu) ----
 // Releases the context's communicator (context destroy).
 void tp_release(syn_cuda_ctx_s* ctx);
@@ -272,5 +313,23 @@ syn_status_t tp_allreduce_sum(syn_cuda_ctx_s* ctx, float* buf, size_t count, cud
 // in rank order.
 syn_status_t tp_allgather(syn_cuda_ctx_s* ctx, const float* send, float* recv, size_t count,
                           cudaStream_t st);
+
+// Launch with programmatic stream serialisation: the kernel may start before
+// its predecessor ends and waits for it in griddep_wait().
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                       cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
 
 }  // namespace syn

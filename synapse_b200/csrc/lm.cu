@@ -41,22 +41,6 @@ __device__ __forceinline__ float chain(bool fused, float a, float b, float acc) 
   return fused ? __fmaf_rn(a, b, acc) : __fadd_rn(acc, __fmul_rn(a, b));
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                       cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
 syn_status_t allow_smem(const void* fn, size_t bytes) {
   static std::mutex mu;
   static std::set<std::pair<const void*, int>> done;
@@ -2137,16 +2121,22 @@ syn_status_t launch_attn_prefill_args(const AttnArgs& a, size_t seq, size_t ntok
 syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st) {
   if (!c->page) return SYN_OK;
   if (seq >= c->batch || new_len > c->max_seq) return SYN_ERR_INVALID_ARG;
+  if (new_len > c->len[seq]) {
+    syn_status_t s = kv_own_page(c, seq, st);
+    if (s) return s;
+  }
   int* row = c->ptab_h + seq * c->maxp;
   const size_t need = (new_len + c->page - 1) / c->page;
-  size_t first = need;
+  size_t first = need, missing = 0;
+  for (size_t i = 0; i < need; i++) missing += row[i] < 0;
+  if (missing > c->n_free) {
+    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
   for (size_t i = 0; i < need; i++) {
     if (row[i] >= 0) continue;
-    if (!c->n_free) {
-      set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
-      return SYN_ERR_OUT_OF_MEMORY;
-    }
     row[i] = c->free_pages[--c->n_free];
+    c->refs[row[i]] = 1;
     first = std::min(first, i);
   }
   if (first < need)
@@ -2160,12 +2150,15 @@ syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaS
 syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cudaStream_t st) {
   if (!c->page) return SYN_OK;
   SYN_CUDA_TRY(cudaStreamSynchronize(st));
+  syn_status_t s = kv_sync(c, st);
+  if (s) return s;
+  c->shrunk[seq]++;
   int* row = c->ptab_h + seq * c->maxp;
   const size_t keep = (keep_len + c->page - 1) / c->page;
   bool changed = false;
   for (size_t i = keep; i < c->maxp; i++)
     if (row[i] >= 0) {
-      c->free_pages[c->n_free++] = row[i];
+      if (--c->refs[row[i]] == 0) c->free_pages[c->n_free++] = row[i];
       row[i] = -1;
       changed = true;
     }
@@ -2277,7 +2270,11 @@ syn_status_t syn_cuda_kvcache_create_paged(syn_cuda_ctx_t* ctx, size_t max_seq,
     e = cudaMallocHost(&c->ptab_h, batch * c->maxp * sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc(&c->d_ptab, batch * c->maxp * sizeof(int));
     c->free_pages = e == cudaSuccess ? new (std::nothrow) int[n_pages] : nullptr;
-    if (e == cudaSuccess && !c->free_pages) e = cudaErrorMemoryAllocation;
+    c->refs = e == cudaSuccess ? new (std::nothrow) int[n_pages]() : nullptr;
+    c->stale = e == cudaSuccess ? new (std::nothrow) uint8_t[batch]() : nullptr;
+    c->shrunk = e == cudaSuccess ? new (std::nothrow) size_t[batch]() : nullptr;
+    if (e == cudaSuccess && (!c->free_pages || !c->refs || !c->stale || !c->shrunk))
+      e = cudaErrorMemoryAllocation;
     if (e == cudaSuccess) {
       for (size_t i = 0; i < batch * c->maxp; i++) c->ptab_h[i] = -1;
       for (size_t i = 0; i < n_pages; i++) c->free_pages[i] = (int)(n_pages - 1 - i);
@@ -2294,6 +2291,9 @@ syn_status_t syn_cuda_kvcache_create_paged(syn_cuda_ctx_t* ctx, size_t max_seq,
     cudaFree(c->d_ptab);
     if (c->ptab_h) cudaFreeHost(c->ptab_h);
     delete[] c->free_pages;
+    delete[] c->refs;
+    delete[] c->stale;
+    delete[] c->shrunk;
     delete[] c->len;
     delete c;
     return SYN_ERR_OUT_OF_MEMORY;
@@ -2326,6 +2326,9 @@ syn_status_t syn_cuda_kvcache_destroy(syn_cuda_kvcache_t* c) {
   cudaFree(c->d_ptab);
   if (c->ptab_h) cudaFreeHost(c->ptab_h);
   delete[] c->free_pages;
+  delete[] c->refs;
+  delete[] c->stale;
+  delete[] c->shrunk;
   delete[] c->len;
   delete c;
   return SYN_OK;
@@ -2360,7 +2363,8 @@ syn_status_t syn_cuda_kvcache_append(syn_cuda_kvcache_t* c, size_t layer, size_t
   const size_t row = c->n_kv * c->hd;
   cudaStream_t st = (cudaStream_t)stream;
   if (c->page) {  // page by page
-    syn_status_t s = kv_reserve(c, seq, c->len[seq] + n_tokens, st);
+    syn_status_t s = c->stale[seq] ? kv_sync(c, st) : SYN_OK;
+    if (s == SYN_OK) s = kv_reserve(c, seq, c->len[seq] + n_tokens, st);
     if (s) return s;
     const size_t base = layer * c->n_pages * c->page;
     for (size_t t = 0; t < n_tokens;) {
