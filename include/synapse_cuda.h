@@ -353,6 +353,38 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
     size_t n_heads, const float *q_norm, const float *k_norm, float eps,
     const float *rope_cos, const float *rope_sin, float *q_out, size_t ldq,
     void *stream);
+/* Decode attention for a batch whose sequences share leading pages: beams of a
+ * prompt, samples of a document, users behind one system prompt. A plan names
+ * the batch's rows: n_groups groups of group_rows[g] sequences each (seqs, host
+ * arrays, all distinct). _set finds for each group the leading pages that all
+ * its sequences hold, and schedules their work; what a group does not share
+ * (all of it on a contiguous cache) is computed row by row. The workspaces and
+ * the schedule belong to the plan: its calls run in stream order, one at a
+ * time; two streams or graphs that overlap need a plan each. _set is not for
+ * captured streams; a captured attention call may be replayed after a later
+ * _set of the same number of rows in groups that share (or not) as before.
+ * head_dim <= 128. Destroy the plan before its cache. */
+typedef struct syn_cuda_decode_plan_s syn_cuda_decode_plan_t;
+syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t *cache, size_t n_heads,
+                                         syn_cuda_decode_plan_t **out);
+syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t *plan);
+syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t *plan, size_t n_groups,
+                                      const size_t *group_rows, const int32_t *seqs,
+                                      void *stream);
+/* Positions that row `row` shares with its group. */
+syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t *plan, size_t row,
+                                         size_t *len);
+/* syn_cuda_attention_decode_flash for the plan's rows (row r of q / k / v / out
+ * is sequence r of the plan; q is left as it is): headwise norms, RoPE, K and V
+ * appended at each sequence's length, attention over all its positions or the
+ * last `window`. Results within f32 reassociation of the reference order. The
+ * lengths are not advanced. Cache positions that no row of a group sees (behind
+ * its sequences, outside all windows) may hold anything. SYN_ERR_INVALID_ARG when a sequence was truncated,
+ * reset or forked into since _set. */
+syn_status_t syn_cuda_attention_decode_shared(
+    syn_cuda_decode_plan_t *plan, size_t layer, const float *q, const float *k, const float *v,
+    size_t ld, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+    const float *rope_sin, size_t window, float *out, size_t ldo, void *stream);
 /* The k best continuations of each group of beams. Row g*beams + b of logits
  * (stride ld) is beam b of group g; a candidate (b, t) has the value
  * scores[g*beams+b] + logits[t] - logsumexp(logits), compared in 64 bits; equal

@@ -16,7 +16,8 @@ _API = ("QFormat", "SynapseError", "Context", "QuantizedWeight", "QuantizedLinea
         "qgemm_int8", "q4_0_gemv", "row_bytes", "rope_tables", "rmsnorm", "add_rmsnorm",
         "swiglu", "argmax", "KVCache", "attention_decode", "attention_prefill", "Model",
         "tp_unique_id", "tp_shard_linear", "GGUFFile", "SafetensorsFile", "gguf_runner_name",
-        "quantize_weights_int8_half", "qk_norm_rope_kv_append_batch", "beam_select")
+        "quantize_weights_int8_half", "qk_norm_rope_kv_append_batch", "beam_select",
+        "DecodePlan", "attention_decode_shared")
 
 __all__ = ["lib"] + list(_API)
 

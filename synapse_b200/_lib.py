@@ -91,6 +91,13 @@ SIGNATURES = {
                                                      c_vp, c_size, c_size, c_vp, c_vp,
                                                      ctypes.c_float, c_vp, c_vp, c_vp, c_size,
                                                      c_vp]),
+    "syn_cuda_decode_plan_create": (c_st, [c_vp, c_size, ctypes.POINTER(c_vp)]),
+    "syn_cuda_decode_plan_destroy": (c_st, [c_vp]),
+    "syn_cuda_decode_plan_set": (c_st, [c_vp, c_size, c_vp, c_vp, c_vp]),
+    "syn_cuda_decode_plan_prefix": (c_st, [c_vp, c_size, ctypes.POINTER(c_size)]),
+    "syn_cuda_attention_decode_shared": (c_st, [c_vp, c_size, c_vp, c_vp, c_vp, c_size, c_vp, c_vp,
+                                                ctypes.c_float, c_vp, c_vp, c_size, c_vp, c_size,
+                                                c_vp]),
     "syn_cuda_beam_select": (c_st, [c_vp, c_vp, c_size, c_size, c_size, c_size, c_vp, c_vp,
                                     ctypes.c_int32, c_size, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "syn_cuda_model_set_kv_paging": (c_st, [c_vp, c_size, c_size]),

@@ -417,8 +417,9 @@ class KVCache:
         _check(lib().syn_cuda_kvcache_view(self.handle, layer, seq, ctypes.byref(k),
                                            ctypes.byref(v)), "kvcache_view")
         n = self.max_seq * self.n_kv * self.hd
-        return _wrap_device(k.value, n, (self.max_seq, self.n_kv * self.hd)), \
-            _wrap_device(v.value, n, (self.max_seq, self.n_kv * self.hd))
+        shape = (self.max_seq, self.n_kv * self.hd)
+        return tuple(_wrap_device(p.value, n, shape, device=self.device, owner=self)
+                     for p in (k, v))
 
     def pages(self, layer=None):
         """(K, V) torch views of a paged cache's pools, [n_pages, page, n_kv,
@@ -429,7 +430,7 @@ class KVCache:
         shape = (self.n_pages, self.page, self.n_kv, self.hd)
         if layer is None:
             shape = (self.layers,) + shape
-        return tuple(_wrap_device(p.value, _numel(shape), shape, device=self.device)
+        return tuple(_wrap_device(p.value, _numel(shape), shape, device=self.device, owner=self)
                      for p in (k, v))
 
     def device_table(self):
@@ -439,7 +440,7 @@ class KVCache:
         _check(lib().syn_cuda_kvcache_page_table(self.handle, ctypes.byref(p), ctypes.byref(n)),
                "kvcache_page_table")
         return _wrap_device(p.value, self.batch * n.value, (self.batch, n.value), "<i4",
-                            self.device)
+                            self.device, self)
 
     def fork(self, src, dst, length=None):
         """The empty sequence dst gets the first `length` (default: all)
@@ -498,11 +499,13 @@ class KVCache:
             pass
 
 
-def _wrap_device(addr, numel, shape, typestr="<f4", device=None):
-    """A torch view of library-owned device memory (no copy, no ownership)."""
+def _wrap_device(addr, numel, shape, typestr="<f4", device=None, owner=None):
+    """A torch view of library-owned device memory (no copy); the view keeps
+    `owner` alive."""
     class _Iface:
         pass
     it = _Iface()
+    it.owner = owner
     it.__cuda_array_interface__ = {"shape": (numel,), "typestr": typestr, "data": (addr, False),
                                    "version": 3, "strides": None}
     return torch.as_tensor(it, device="cuda" if device is None else f"cuda:{device}").view(*shape)
@@ -624,6 +627,76 @@ def qk_norm_rope_kv_append_batch(cache, layer, seqs, n_tokens, qkv, n_heads, q_n
         float(eps), _ptr(cos_t), _ptr(sin_t), _ptr(q_out), qd, _stream(qkv)),
         "qk_norm_rope_kv_append_batch")
     return q_out
+
+
+class DecodePlan:
+    """The rows of a decode batch in groups that share leading cache pages
+    (syn_cuda_decode_plan_*), with the workspaces of its attention calls."""
+
+    def __init__(self, cache, n_heads):
+        self.cache, self.n_heads, self.rows = cache, n_heads, 0
+        self.handle = None
+        h = ctypes.c_void_p()
+        _check(lib().syn_cuda_decode_plan_create(cache.handle, _index(n_heads), ctypes.byref(h)),
+               "decode_plan_create")
+        self.handle = h
+
+    def set(self, groups):
+        """groups: lists of sequences; row r of an attention call is the r-th
+        sequence of them all."""
+        groups = [list(g) for g in groups]
+        seqs = _int32_array(s for g in groups for s in g)
+        sizes = (ctypes.c_size_t * len(groups))(*(len(g) for g in groups))
+        _check(lib().syn_cuda_decode_plan_set(self.handle, len(groups), sizes, seqs,
+                                              self.cache._stream()), "decode_plan_set")
+        self.rows = len(seqs)
+
+    def prefix(self, row):
+        """Positions that the row shares with its group."""
+        v = ctypes.c_size_t()
+        _check(lib().syn_cuda_decode_plan_prefix(self.handle, _index(row), ctypes.byref(v)),
+               "decode_plan_prefix")
+        return v.value
+
+    def close(self):
+        if self.handle:
+            lib().syn_cuda_decode_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def attention_decode_shared(plan, layer, qkv, q_norm, k_norm, eps, cos_t, sin_t, window=0,
+                            out=None):
+    """attention_decode for the plan's rows, each group's shared positions read
+    once (syn_cuda_attention_decode_shared); qkv rows [q | k | v]. Returns
+    [rows, n_heads*hd]; the cache lengths are not advanced."""
+    cache, n_heads = plan.cache, plan.n_heads
+    _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t)
+    qd, kvd, ld = n_heads * cache.hd, cache.n_kv * cache.hd, qkv.shape[1]
+    if qkv.shape[0] != plan.rows:
+        raise SynapseError(4, "attention_decode_shared")
+    if out is None:
+        out = torch.empty(plan.rows, qd, dtype=torch.float32, device=qkv.device)
+    else:
+        _need_cuda(out)
+        _need_f32(out)
+        _need_device(cache.device, out)
+        if out.shape != (plan.rows, qd):
+            raise SynapseError(4, "out")
+    if plan.rows == 0:
+        return out
+    base = qkv.data_ptr()
+    _check(lib().syn_cuda_attention_decode_shared(
+        plan.handle, layer, ctypes.c_void_p(base), ctypes.c_void_p(base + 4 * qd),
+        ctypes.c_void_p(base + 4 * (qd + kvd)), ld, _ptr(q_norm), _ptr(k_norm), float(eps),
+        _ptr(cos_t), _ptr(sin_t), _index(window), _ptr(out), qd, _stream(qkv)),
+        "attention_decode_shared")
+    return out
 
 
 def beam_select(ctx, logits, scores, beams, k=None, finished=None, eos=-1):

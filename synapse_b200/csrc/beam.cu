@@ -168,6 +168,8 @@ struct AppendArgs {
   const int* ptab;
   int page, maxp, max_seq;
   const int* len;
+  const int* seq_of;  // device: one row of each sequence seq_of[row] (replaces the lists below)
+  int rows;
   int n;
   int seq[AP_MAX];
   int row0[AP_MAX + 1];  // first row of each sequence; [n] = rows
@@ -184,9 +186,9 @@ __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_consta
   const long long unit = (long long)blockIdx.x * (AP_THREADS / LP) + threadIdx.x / LP;
   const int lane = threadIdx.x % LP;
   const int row = (int)(unit / heads), h = (int)(unit - (long long)row * heads);
-  const bool live = row < a.row0[a.n];
+  const bool live = row < a.rows;
   int s = 0;
-  if (live)
+  if (live && !a.seq_of)
     for (int step = AP_MAX / 2; step; step >>= 1)  // the last sequence that starts at or before row
       if (s + step < a.n && a.row0[s + step] <= row) s += step;
   const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
@@ -227,15 +229,16 @@ __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_consta
   }
   griddep_launch();
   if (!live) return;
-  const int pos = a.len[a.seq[s]] + row - a.row0[s];
+  const int sq = a.seq_of ? a.seq_of[row] : a.seq[s];
+  const int pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);
   if (pos >= a.max_seq) return;  // (a replayed graph that has run past the cache)
   float* dst;
   if (is_q) {
     dst = a.q_out + (long long)row * a.ldq + (long long)h * a.hd;
   } else {
-    size_t slot = (size_t)a.seq[s] * a.max_seq + pos;
+    size_t slot = (size_t)sq * a.max_seq + pos;
     if (a.ptab) {
-      const int pg = a.ptab[(size_t)a.seq[s] * a.maxp + pos / a.page];
+      const int pg = a.ptab[(size_t)sq * a.maxp + pos / a.page];
       if (pg < 0) return;
       slot = (size_t)pg * a.page + pos % a.page;
     }
@@ -667,21 +670,24 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 }
 
 syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, size_t n,
-                                 const int32_t* seqs, const size_t* counts, cudaStream_t st) {
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st,
+                                 const int* seq_of) {
   const syn_cuda_kvcache_t* c = at.cache;
   const size_t kvd = c->n_kv * c->hd;
   const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
   size_t done = 0;
-  for (size_t i0 = 0; i0 < n; i0 += AP_MAX) {
+  for (size_t i0 = 0; i0 < n; i0 += seq_of ? n : AP_MAX) {
     AppendArgs a;
-    a.n = (int)std::min<size_t>(AP_MAX, n - i0);
-    size_t rows = 0;
+    a.seq_of = seq_of;
+    a.n = seq_of ? 0 : (int)std::min<size_t>(AP_MAX, n - i0);
+    size_t rows = seq_of ? n : 0;
     for (int i = 0; i < a.n; i++) {
       a.seq[i] = seqs[i0 + i];
       a.row0[i] = (int)rows;
       rows += counts[i0 + i];
     }
     a.row0[a.n] = (int)rows;
+    a.rows = (int)rows;
     if (rows) {
       a.q = at.q + done * at.ld;
       a.k = at.k + done * at.ld;

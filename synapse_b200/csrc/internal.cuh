@@ -290,14 +290,20 @@ syn_status_t launch_kv_set(syn_cuda_kvcache_t* c, size_t seq, int value, int add
 
 // ---- beam search (beam.cu) ----
 // New rows of n sequences (counts[i] rows of seqs[i], host arrays, pages
-// reserved) normalised, rotated and appended; q rows to q_out.
+// reserved) normalised, rotated and appended; q rows to q_out. With seq_of (a
+// device array, read when the kernel runs) one row of each of its n sequences.
 syn_status_t launch_append_batch(const AttnArgs& a, float* q_out, size_t ldq, size_t n,
-                                 const int32_t* seqs, const size_t* counts, cudaStream_t st);
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st,
+                                 const int* seq_of = nullptr);
 // Groups of `beams` sequences (seqs and lens on the host, parents on the
 // device) take over their parents' contexts; at most 256 sequences.
 syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
                                const int32_t* parents, size_t beams, const size_t* lens,
                                cudaStream_t st);
+// Decode attention of a plan's rows (q, k, v, the layer and the output in a;
+// pages reserved).
+syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& a, int* err,
+                                cudaStream_t st);
 size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms);
 syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
                                 size_t vocab, const float* scores, const uint8_t* fin, int eos,

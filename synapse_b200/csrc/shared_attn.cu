@@ -1,0 +1,694 @@
+// shared_attn.cu -- decode attention for a batch whose sequences share their
+// leading cache pages (syn_cuda_kvcache_fork): beams of a prompt, samples of a
+// document, users behind one system prompt. For one query row with scores
+// s_j = q.k_j / sqrt(hd) over its positions,
+//   o = sum_j e^{s_j} v_j / sum_j e^{s_j},
+// and any partition of the positions into parts with (m_i, l_i, o_i) = (max,
+// sum of e^{s-m_i}, sum of e^{s-m_i} v) joins as M = max m_i,
+//   o = sum_i e^{m_i-M} o_i / sum_i e^{m_i-M} l_i.
+// The shared prefix of a group is one part set, computed once for all its
+// rows, so its K and V cross HBM once per step instead of once per row; each
+// row's own positions are the other. Kernels of one call:
+//   k_append_batch (beam.cu)  the new rows normalised, rotated and appended
+//   k_prefix                  the shared prefixes, on a fixed schedule
+//   k_suffix                  each row's own positions; the last CTA of a (row,
+//                             KV head) joins all parts
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "internal.cuh"
+
+// A batch of decode rows in groups. Built on the host by _set: which leading
+// pages each group shares, and the schedule of its prefix work.
+struct syn_cuda_decode_plan_s {
+  syn_cuda_kvcache_t* cache;
+  int device, sms;
+  size_t n_heads;
+  size_t rows = 0, groups = 0;
+  std::vector<int32_t> seqs;
+  std::vector<size_t> prefix, shrunk;  // per row: shared positions; the sequence's state at _set
+  // device
+  float* q = nullptr;        // rotated queries [batch][n_heads * hd]
+  int* meta = nullptr;       // MetaView, copied from meta_h
+  int* meta_h = nullptr;     // pinned
+  cudaEvent_t copied = nullptr;
+  size_t meta_ints = 0;
+  float* po = nullptr;       // partial o, prefix then suffix
+  float2* pml = nullptr;     // partial (m, l)
+  size_t part_rows = 0;      // records of po / pml
+  int* cnt = nullptr;        // arrivals per (row, KV head, chunk); zero between launches
+};
+
+namespace syn {
+namespace {
+
+constexpr int PT = 64;         // keys of a prefix tile
+constexpr int PM = 128;        // query rows of a prefix job
+constexpr int SX_THREADS = 128, SX_WARPS = 4, SX_RB = 4;
+constexpr int SX_SPLITS = 64;  // most suffix splits of a (row, KV head)
+constexpr int PARTS_MAX = 256; // most parts of one query row: those and a prefix split per SM
+
+struct Job {      // prefix work of one (group, tile of query rows, KV head)
+  int row0;       // first row of the group
+  int m0, m;      // query rows m0 .. m0+m of the group: row0 + i / G, head i % G
+  int kvh;
+  int len;        // shared positions
+  int part0;      // first partial record; split i is at part0 + i * m
+  int splits;
+};
+struct Item {     // a CTA's share of a job: key tiles t0 .. t1, partial records from part
+  int job, t0, t1, part;
+};
+
+// Offsets (ints) of the arrays in the plan's metadata block.
+struct Meta {
+  int rows, max_jobs, max_items, ctas;
+  __host__ __device__ int seq() const { return 0; }
+  __host__ __device__ int pre() const { return rows; }           // shared positions of each row
+  __host__ __device__ int job_of() const { return 2 * rows; }    // first job of the row's group, -1
+  __host__ __device__ int local() const { return 3 * rows; }     // row - first row of its group
+  __host__ __device__ int start() const { return 4 * rows; }     // [ctas + 1] items of each CTA
+  __host__ __device__ int items() const { return (start() + ctas + 1 + 3) / 4 * 4; }
+  __host__ __device__ int jobs() const { return items() + 4 * max_items; }
+  __host__ __device__ int total() const { return jobs() + 7 * max_jobs; }
+};
+
+struct SharedArgs {
+  const float* q;  // rotated
+  int n_heads, n_kv, hd, G;
+  const float *kc, *vc;  // this layer
+  const int* ptab;       // nullptr: contiguous
+  int page, maxp, max_seq;
+  const int* len;
+  int window;
+  const int* meta;
+  Meta mv;
+  float* po;
+  float2* pml;
+  int sfx0;  // first suffix record
+  int nsplit;
+  int* cnt;
+  float* out;
+  long long ldo;
+  float scale;
+  int* err;
+};
+
+__device__ __forceinline__ long long row_at(const SharedArgs& a, int sq, int pos) {
+  if (!a.ptab) return (long long)sq * a.max_seq + pos;
+  const int pg = a.ptab[(long long)sq * a.maxp + pos / a.page];
+  return pg < 0 ? -1 : (long long)pg * a.page + pos % a.page;
+}
+
+// ---------------------------------------------------------------------------
+// Prefix, plain form: CTA = its items in turn; two threads per query row.
+// ---------------------------------------------------------------------------
+constexpr int PX_THREADS = 256;
+
+template <int HDP>
+__global__ void __launch_bounds__(PX_THREADS) k_prefix(const SharedArgs a) {
+  extern __shared__ float sm[];
+  constexpr int S = HDP + 4;
+  float* sq = sm;
+  float* sk = sq + PM * S;
+  float* sv = sk + PT * S;
+  float* ss = sv + PT * S;  // [PM][PT + 1]
+  const int tid = threadIdx.x, hd = a.hd;
+  const int* meta = a.meta;
+  griddep_wait();
+  const int i0 = meta[a.mv.start() + blockIdx.x], i1 = meta[a.mv.start() + blockIdx.x + 1];
+  for (int it = i0; it < i1; it++) {
+    const Item item = reinterpret_cast<const Item*>(meta + a.mv.items())[it];
+    const Job job = reinterpret_cast<const Job*>(meta + a.mv.jobs())[item.job];
+    const int seq = meta[a.mv.seq() + job.row0];
+    for (int t = tid; t < PM * HDP; t += PX_THREADS) {
+      const int r = t / HDP, d = t % HDP;
+      float x = 0.0f;
+      if (r < job.m && d < hd) {
+        const int i = job.m0 + r;
+        x = a.q[((size_t)(job.row0 + i / a.G) * a.n_heads + job.kvh * a.G + i % a.G) * hd + d];
+      }
+      sq[r * S + d] = x;
+    }
+    const int r = tid >> 1, part = tid & 1;
+    float o[HDP / 2];
+#pragma unroll
+    for (int d = 0; d < HDP / 2; d++) o[d] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    // positions below low are outside the row's window; below all rows', they are not read
+    int low = 0, lowest = 0;
+    if (a.window) {
+      lowest = job.len;
+      for (int i = 0; i < job.m; i++) {
+        const int row = job.row0 + (job.m0 + i) / a.G;
+        const int lw = max(0, a.len[meta[a.mv.seq() + row]] + 1 - a.window);
+        lowest = min(lowest, lw);
+        if (i == r) low = lw;
+      }
+    }
+    for (int t = item.t0; t < item.t1; t++) {
+      __syncthreads();
+      for (int u = tid; u < PT * HDP; u += PX_THREADS) {
+        const int j = u / HDP, d = u % HDP, pos = t * PT + j;
+        float kx = 0.0f, vx = 0.0f;
+        if (pos < job.len && pos >= lowest && d < hd) {
+          const long long row = row_at(a, seq, pos);
+          if (row >= 0) {
+            kx = a.kc[(row * a.n_kv + job.kvh) * hd + d];
+            vx = a.vc[(row * a.n_kv + job.kvh) * hd + d];
+          }
+        }
+        sk[j * S + d] = kx;
+        sv[j * S + d] = vx;
+      }
+      __syncthreads();
+      float mt = -INFINITY;
+      for (int j = part; j < PT; j += 2) {
+        float s = 0.0f;
+        for (int d = 0; d < HDP; d++) s = fmaf(sq[r * S + d], sk[j * S + d], s);
+        const int pos = t * PT + j;
+        s = pos < job.len && pos >= low ? s * a.scale : -INFINITY;
+        ss[r * (PT + 1) + j] = s;
+        mt = fmaxf(mt, s);
+      }
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+      const float mn = fmaxf(m, mt);
+      const float corr = m == -INFINITY ? 0.0f : expf(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < HDP / 2; d++) o[d] *= corr;
+      __syncwarp();
+      for (int j = 0; j < PT; j++) {
+        const float s = ss[r * (PT + 1) + j];
+        const float p = s == -INFINITY ? 0.0f : expf(s - mn);
+        l += p;
+#pragma unroll
+        for (int d = 0; d < HDP / 2; d++) o[d] = fmaf(p, sv[j * S + part * (HDP / 2) + d], o[d]);
+      }
+      m = mn;
+      __syncwarp();
+    }
+    if (r < job.m) {
+      const size_t rec = item.part + r;
+      if (part == 0) a.pml[rec] = make_float2(m, l);
+#pragma unroll
+      for (int d = 0; d < HDP / 2; d++)
+        if (part * (HDP / 2) + d < hd) a.po[rec * hd + part * (HDP / 2) + d] = o[d];
+    }
+    __syncthreads();
+  }
+  griddep_launch();
+}
+
+// ---------------------------------------------------------------------------
+// Each row's own positions: CTA = (row, KV head and chunk of GC of its query
+// heads, split). LPR lanes take one cached row (four elements each), so a
+// warp's load is 32 / LPR rows of one KV head; the q.k partials are summed by
+// butterfly shuffles, each head keeps a running (m, l, o).
+// ---------------------------------------------------------------------------
+template <int LPR, int GC>
+__global__ void __launch_bounds__(SX_THREADS) k_suffix(const SharedArgs a, int chunks) {
+  constexpr int SUBS = 32 / LPR, STEP = SX_WARPS * SX_RB * SUBS, HDP = LPR * 4;
+  constexpr int NW = SX_WARPS * SUBS;
+  __shared__ float wst[NW][GC][2];
+  __shared__ __align__(16) float wo[NW][GC][HDP];
+  __shared__ float fac[SX_WARPS][PARTS_MAX];
+  __shared__ int last;
+  const int b = blockIdx.x, kvh = blockIdx.y / chunks, ch = blockIdx.y - kvh * chunks;
+  const int sp = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int sub = lane / LPR, l4 = lane % LPR, hd = a.hd, g0 = ch * GC;
+  const int heads = min(GC, a.G - g0);
+  griddep_wait();
+  const int sq = a.meta[a.mv.seq() + b];
+  const int pre = a.meta[a.mv.pre() + b];
+  const int pos = a.len[sq], L = pos + 1;
+  const bool full = pos >= a.max_seq;  // a replayed graph that has run past the cache
+  if (full && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
+  const int off = max(pre, a.window ? L - a.window : 0);
+  const int eff = full ? 0 : L - off;
+  int sl = (eff + a.nsplit - 1) / a.nsplit;
+  sl = (sl + SX_RB * SUBS - 1) / (SX_RB * SUBS) * (SX_RB * SUBS);
+  const int r0 = off + min(eff, sp * sl), r1 = off + min(eff, (sp + 1) * sl);
+  const bool act = l4 * 4 < hd;
+  float4 q[GC];
+#pragma unroll
+  for (int g = 0; g < GC; g++) {
+    q[g] = make_float4(0, 0, 0, 0);
+    if (g < heads && act)
+      q[g] = reinterpret_cast<const float4*>(
+          a.q + ((size_t)b * a.n_heads + kvh * a.G + g0 + g) * hd)[l4];
+  }
+  float m[GC], l[GC];
+  float4 o[GC];
+#pragma unroll
+  for (int g = 0; g < GC; g++) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+    o[g] = make_float4(0, 0, 0, 0);
+  }
+  const float4 zero = make_float4(0, 0, 0, 0);
+  auto load = [&](int rb, float4(&kr)[SX_RB], float4(&vr)[SX_RB]) {
+#pragma unroll
+    for (int j = 0; j < SX_RB; j++) {
+      const int row = rb + j * SUBS + sub;
+      kr[j] = vr[j] = zero;
+      if (row < r1 && act) {
+        const long long at = row_at(a, sq, row);
+        if (at >= 0) {
+          const size_t e = ((size_t)at * a.n_kv + kvh) * hd / 4 + l4;
+          kr[j] = reinterpret_cast<const float4*>(a.kc)[e];
+          vr[j] = reinterpret_cast<const float4*>(a.vc)[e];
+        }
+      }
+    }
+  };
+  float4 kr[SX_RB], vr[SX_RB];
+  const int rb0 = r0 + warp * SX_RB * SUBS;
+  load(rb0, kr, vr);
+  for (int rb = rb0; rb < r1; rb += STEP) {
+    float4 kn[SX_RB], vn[SX_RB];
+    load(rb + STEP, kn, vn);
+    float s[GC][SX_RB];
+#pragma unroll
+    for (int g = 0; g < GC; g++)
+#pragma unroll
+      for (int j = 0; j < SX_RB; j++)
+        s[g][j] = fmaf(q[g].x, kr[j].x, fmaf(q[g].y, kr[j].y, fmaf(q[g].z, kr[j].z, q[g].w * kr[j].w)));
+#pragma unroll
+    for (int x = LPR / 2; x; x >>= 1)
+#pragma unroll
+      for (int g = 0; g < GC; g++)
+#pragma unroll
+        for (int j = 0; j < SX_RB; j++) s[g][j] += __shfl_xor_sync(0xffffffffu, s[g][j], x);
+#pragma unroll
+    for (int g = 0; g < GC; g++) {
+      float mx = m[g];
+#pragma unroll
+      for (int j = 0; j < SX_RB; j++) {
+        s[g][j] = rb + j * SUBS + sub < r1 ? s[g][j] * a.scale : -INFINITY;
+        mx = fmaxf(mx, s[g][j]);
+      }
+      if (mx == -INFINITY) continue;
+      const float corr = m[g] == -INFINITY ? 0.0f : expf(m[g] - mx);
+      l[g] *= corr;
+      o[g].x *= corr;
+      o[g].y *= corr;
+      o[g].z *= corr;
+      o[g].w *= corr;
+#pragma unroll
+      for (int j = 0; j < SX_RB; j++) {
+        const float p = s[g][j] == -INFINITY ? 0.0f : expf(s[g][j] - mx);
+        l[g] += p;
+        o[g].x = fmaf(p, vr[j].x, o[g].x);
+        o[g].y = fmaf(p, vr[j].y, o[g].y);
+        o[g].z = fmaf(p, vr[j].z, o[g].z);
+        o[g].w = fmaf(p, vr[j].w, o[g].w);
+      }
+      m[g] = mx;
+    }
+#pragma unroll
+    for (int j = 0; j < SX_RB; j++) {
+      kr[j] = kn[j];
+      vr[j] = vn[j];
+    }
+  }
+  // join the warps and their sub-rows: one record per head of this split
+#pragma unroll
+  for (int g = 0; g < GC; g++) {
+    const int w = warp * SUBS + sub;
+    if (l4 == 0) {
+      wst[w][g][0] = m[g];
+      wst[w][g][1] = l[g];
+    }
+    *reinterpret_cast<float4*>(&wo[w][g][l4 * 4]) = o[g];
+  }
+  __syncthreads();
+  const size_t rec0 = a.sfx0 + ((size_t)b * a.n_heads + kvh * a.G + g0) * a.nsplit;
+  for (int i = tid; i < heads * hd; i += SX_THREADS) {
+    const int g = i / hd, d = i - g * hd;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; w++) M = fmaxf(M, wst[w][g][0]);
+    float O = 0.0f, Ls = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float f = wst[w][g][0] == -INFINITY ? 0.0f : expf(wst[w][g][0] - M);
+      O = fmaf(f, wo[w][g][d], O);
+      Ls = fmaf(f, wst[w][g][1], Ls);
+    }
+    const size_t rec = rec0 + (size_t)g * a.nsplit + sp;
+    a.po[rec * hd + d] = O;
+    if (d == 0) a.pml[rec] = make_float2(M, Ls);
+  }
+  __threadfence();
+  __syncthreads();
+  int* cn = a.cnt + (size_t)b * gridDim.y + blockIdx.y;
+  if (tid == 0) last = atomicAdd(cn, 1) == a.nsplit - 1;
+  __syncthreads();
+  griddep_launch();
+  if (!last) return;
+  __threadfence();
+  // join all parts of this (row, chunk): a warp per head
+  const int job0 = a.meta[a.mv.job_of() + b];
+  for (int g = warp; g < heads; g += SX_WARPS) {
+    int np = 0;
+    size_t prec = 0;
+    int pstep = 0;
+    if (pre > 0 && job0 >= 0) {
+      const int i = a.meta[a.mv.local() + b] * a.G + g0 + g, mt = i / PM;
+      const Job job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[job0 + mt * a.n_kv + kvh];
+      np = job.splits;
+      prec = job.part0 + i - job.m0;
+      pstep = job.m;
+    }
+    const int n = a.nsplit + np;
+    const size_t srec = rec0 + (size_t)g * a.nsplit;
+    auto rec = [&](int c) { return c < a.nsplit ? srec + c : prec + (size_t)(c - a.nsplit) * pstep; };
+    float M = -INFINITY;
+    for (int c = lane; c < n; c += 32) M = fmaxf(M, __ldcg(&a.pml[rec(c)]).x);
+    M = warp_max(M);
+    float lsum = 0.0f;
+    for (int c = lane; c < n; c += 32) {
+      const float2 ml = __ldcg(&a.pml[rec(c)]);
+      const float f = ml.x == -INFINITY ? 0.0f : expf(ml.x - M);
+      fac[warp][c] = f;
+      lsum += f * ml.y;
+    }
+    lsum = warp_sum(lsum);
+    __syncwarp();
+    float* orow = a.out + (long long)b * a.ldo + (long long)(kvh * a.G + g0 + g) * hd;
+    for (int d4 = lane; d4 * 4 < hd; d4 += 32) {
+      float4 ov = zero;
+      for (int c = 0; c < n; c++) {
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd) + d4);
+        const float f = fac[warp][c];
+        ov.x = fmaf(t.x, f, ov.x);
+        ov.y = fmaf(t.y, f, ov.y);
+        ov.z = fmaf(t.z, f, ov.z);
+        ov.w = fmaf(t.w, f, ov.w);
+      }
+      orow[d4 * 4] = ov.x / lsum;
+      orow[d4 * 4 + 1] = ov.y / lsum;
+      orow[d4 * 4 + 2] = ov.z / lsum;
+      orow[d4 * 4 + 3] = ov.w / lsum;
+    }
+    __syncwarp();
+  }
+  if (tid == 0) *cn = 0;
+}
+
+syn_status_t launched(cudaError_t e, const char* where) {
+  if (e == cudaSuccess) return SYN_OK;
+  set_last_cuda_error(e, where);
+  return SYN_ERR_CUDA;
+}
+
+syn_status_t more_smem(const void* fn, size_t bytes) {
+  if (bytes > 48 * 1024)
+    SYN_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return SYN_OK;
+}
+
+using SuffixK = void (*)(const SharedArgs, int);
+template <int LPR>
+SuffixK suffix_kernel(int gc) {
+  return gc == 1 ? k_suffix<LPR, 1> : gc == 2 ? k_suffix<LPR, 2> : gc == 4 ? k_suffix<LPR, 4> : k_suffix<LPR, 8>;
+}
+int chunk_heads(int G) { return G == 1 ? 1 : G == 2 ? 2 : G <= 4 ? 4 : 8; }
+
+// Most jobs and items of a batch of `batch` rows (groups of two or more share).
+size_t max_jobs(size_t batch, size_t n_kv, size_t G) {
+  return n_kv * (batch * G / PM + batch / 2 + 1);
+}
+
+Meta meta_of(const syn_cuda_decode_plan_t* p) {
+  const syn_cuda_kvcache_t* c = p->cache;
+  const size_t jobs = max_jobs(c->batch, c->n_kv, p->n_heads / c->n_kv);
+  return Meta{(int)c->batch, (int)jobs, (int)(jobs + p->sms), p->sms};
+}
+
+int suffix_splits(const syn_cuda_decode_plan_t* p) {
+  // about four CTAs per SM over all (row, KV head) pairs
+  const size_t G = p->n_heads / p->cache->n_kv, gc = chunk_heads((int)G);
+  const size_t pairs = std::max<size_t>(1, p->rows) * p->cache->n_kv * ((G + gc - 1) / gc);
+  return (int)std::max<size_t>(1, std::min<size_t>(SX_SPLITS, (4 * p->sms + pairs - 1) / pairs));
+}
+
+}  // namespace
+
+syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, int* err,
+                                cudaStream_t st) {
+  syn_cuda_kvcache_t* c = p->cache;
+  const size_t kvd = c->n_kv * c->hd, qd = p->n_heads * c->hd;
+  syn_status_t s = launch_append_batch(at, p->q, qd, p->rows, nullptr, nullptr, st,
+                                       p->meta + meta_of(p).seq());
+  if (s) return s;
+  const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
+  SharedArgs a;
+  a.q = p->q;
+  a.n_heads = (int)p->n_heads;
+  a.n_kv = (int)c->n_kv;
+  a.hd = (int)c->hd;
+  a.G = (int)(p->n_heads / c->n_kv);
+  a.kc = c->k + at.layer * rows_per_layer * kvd;
+  a.vc = c->v + at.layer * rows_per_layer * kvd;
+  a.ptab = c->page ? c->d_ptab : nullptr;
+  a.page = (int)c->page;
+  a.maxp = (int)c->maxp;
+  a.max_seq = (int)c->max_seq;
+  a.len = c->d_len;
+  a.window = (int)std::min<size_t>(at.window, c->max_seq + 1);
+  a.meta = p->meta;
+  a.mv = meta_of(p);
+  a.po = p->po;
+  a.pml = p->pml;
+  a.nsplit = suffix_splits(p);
+  a.sfx0 = (int)(p->part_rows - p->n_heads * std::max<size_t>(c->batch, 4 * p->sms + c->batch));
+  a.cnt = p->cnt;
+  a.out = at.out;
+  a.ldo = (long long)at.ldo;
+  a.scale = 1.0f / sqrtf((float)c->hd);
+  a.err = err;
+  if (p->groups < p->rows) {
+    constexpr size_t s64 = (size_t)((PM + 2 * PT) * 68 + PM * (PT + 1)) * 4;
+    constexpr size_t s128 = (size_t)((PM + 2 * PT) * 132 + PM * (PT + 1)) * 4;
+    const bool w = c->hd > 64;
+    void (*kern)(const SharedArgs) = w ? k_prefix<128> : k_prefix<64>;
+    if ((s = more_smem((const void*)kern, w ? s128 : s64))) return s;
+    s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), w ? s128 : s64, st, a), "k_prefix");
+    if (s) return s;
+  }
+  const int gc = chunk_heads(a.G), chunks = (a.G + gc - 1) / gc;
+  SuffixK sk = c->hd <= 32 ? suffix_kernel<8>(gc) : c->hd <= 64 ? suffix_kernel<16>(gc) : suffix_kernel<32>(gc);
+  return launched(launch_pdl(sk, dim3((unsigned)p->rows, (unsigned)(c->n_kv * chunks), (unsigned)a.nsplit),
+                             dim3(SX_THREADS), 0, st, a, chunks),
+                  "k_suffix");
+}
+
+}  // namespace syn
+
+using namespace syn;
+
+extern "C" {
+
+syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
+                                         syn_cuda_decode_plan_t** out) {
+  if (!c || !out) return SYN_ERR_NULL_PTR;
+  *out = nullptr;
+  if (!n_heads || n_heads % c->n_kv) return SYN_ERR_SHAPE_MISMATCH;
+  if (c->hd > 128 || c->batch > 32768 || n_heads > 65535) return SYN_ERR_UNSUPPORTED;
+  DeviceGuard g(c->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  auto* p = new (std::nothrow) syn_cuda_decode_plan_s();
+  if (!p) return SYN_ERR_OUT_OF_MEMORY;
+  p->cache = c;
+  p->device = c->device;
+  p->sms = num_sms();
+  p->n_heads = n_heads;
+  if (p->sms + SX_SPLITS > PARTS_MAX) {
+    delete p;
+    return SYN_ERR_UNSUPPORTED;
+  }
+  const Meta mv = meta_of(p);
+  p->meta_ints = mv.total();
+  // prefix records: a job's rows for each CTA that shares in it, at most one job's rows more
+  // per CTA than the batch's query rows; suffix records: nsplit of each (row, head)
+  const size_t G = n_heads / c->n_kv;
+  const size_t prefix = c->batch * n_heads + (size_t)p->sms * std::min<size_t>(PM, c->batch * G);
+  const size_t suffix = n_heads * std::max<size_t>(c->batch, 4 * p->sms + c->batch);
+  p->part_rows = prefix + suffix;
+  if (p->part_rows > 0x7FFFFFFF) {
+    delete p;
+    return SYN_ERR_UNSUPPORTED;
+  }
+  const size_t ncnt = c->batch * n_heads;
+  cudaError_t e = cudaMalloc(&p->q, c->batch * n_heads * c->hd * sizeof(float));
+  if (e == cudaSuccess) e = cudaMalloc(&p->meta, p->meta_ints * sizeof(int));
+  if (e == cudaSuccess) e = cudaMallocHost(&p->meta_h, p->meta_ints * sizeof(int));
+  if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
+  if (e == cudaSuccess) e = cudaMalloc(&p->pml, p->part_rows * sizeof(float2));
+  if (e == cudaSuccess) e = cudaMalloc(&p->cnt, ncnt * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(p->cnt, 0, ncnt * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(p->meta, 0, p->meta_ints * sizeof(int));
+  if (e == cudaSuccess) e = cudaEventCreateWithFlags(&p->copied, cudaEventDisableTiming);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e, "syn_cuda_decode_plan_create");
+    syn_cuda_decode_plan_destroy(p);
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
+  *out = p;
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
+  if (!p) return SYN_ERR_NULL_PTR;
+  DeviceGuard g(p->device);
+  cudaDeviceSynchronize();
+  cudaFree(p->q);
+  cudaFree(p->meta);
+  if (p->meta_h) cudaFreeHost(p->meta_h);
+  cudaFree(p->po);
+  cudaFree(p->pml);
+  cudaFree(p->cnt);
+  if (p->copied) cudaEventDestroy(p->copied);
+  delete p;
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups,
+                                      const size_t* group_rows, const int32_t* seqs,
+                                      void* stream) {
+  if (!p || (n_groups && (!group_rows || !seqs))) return SYN_ERR_NULL_PTR;
+  syn_cuda_kvcache_t* c = p->cache;
+  DeviceGuard g(p->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+  if (cs != cudaStreamCaptureStatusNone) return SYN_ERR_UNSUPPORTED;
+  size_t rows = 0;
+  std::vector<uint8_t> seen(c->batch, 0);
+  for (size_t i = 0; i < n_groups; i++) {
+    if (!group_rows[i] || group_rows[i] > c->batch - rows) return SYN_ERR_INVALID_ARG;
+    for (size_t j = rows; j < rows + group_rows[i]; j++) {
+      if (seqs[j] < 0 || (size_t)seqs[j] >= c->batch || seen[seqs[j]]) return SYN_ERR_INVALID_ARG;
+      seen[seqs[j]] = 1;
+    }
+    rows += group_rows[i];
+  }
+  syn_status_t s = kv_sync(c, st);
+  // (a row cut back into a shared page gets its own copy now, not in a later call)
+  for (size_t i = 0; i < rows && s == SYN_OK; i++) s = kv_own_page(c, seqs[i], st);
+  if (s) return s;
+  SYN_CUDA_TRY(cudaEventSynchronize(p->copied));  // the last copy has left meta_h
+  const Meta mv = meta_of(p);
+  const int G = (int)(p->n_heads / c->n_kv);
+  int* h = p->meta_h;
+  Job* jobs = reinterpret_cast<Job*>(h + mv.jobs());
+  Item* items = reinterpret_cast<Item*>(h + mv.items());
+  p->seqs.assign(seqs, seqs + rows);
+  p->prefix.assign(rows, 0);
+  p->shrunk.assign(rows, 0);
+  int nj = 0;
+  size_t tiles = 0, r0 = 0;
+  for (size_t i = 0; i < n_groups; i++) {
+    const size_t n = group_rows[i];
+    size_t shared = 0;  // leading positions in pages that all rows hold
+    if (n > 1 && c->page) {
+      size_t most = c->len[seqs[r0]];
+      for (size_t j = r0; j < r0 + n; j++) most = std::min(most, c->len[seqs[j]]);
+      size_t col = 0;
+      for (bool same = true; (col + 1) * c->page <= most; col++) {
+        const int pg = c->ptab_h[seqs[r0] * c->maxp + col];
+        for (size_t j = r0; j < r0 + n && same; j++) same = c->ptab_h[seqs[j] * c->maxp + col] == pg;
+        if (!same) break;
+      }
+      shared = col * c->page;
+    }
+    for (size_t j = r0; j < r0 + n; j++) {
+      h[mv.seq() + j] = seqs[j];
+      h[mv.pre() + j] = (int)shared;
+      h[mv.job_of() + j] = shared ? nj : -1;
+      h[mv.local() + j] = (int)(j - r0);
+      p->prefix[j] = shared;
+      if (c->page) p->shrunk[j] = c->shrunk[seqs[j]];
+    }
+    if (shared)
+      for (int m0 = 0; m0 < (int)n * G; m0 += PM)
+        for (int kvh = 0; kvh < (int)c->n_kv; kvh++) {
+          jobs[nj++] = Job{(int)r0, m0, std::min(PM, (int)n * G - m0), kvh, (int)shared, 0, 0};
+          tiles += (shared + PT - 1) / PT;
+        }
+    r0 += n;
+  }
+  // the tiles of all jobs, one after another, in equal shares
+  size_t ni = 0, part = 0, done = 0;
+  int j = 0;
+  size_t jt = 0;  // tiles of job j given out
+  for (int cta = 0; cta < mv.ctas; cta++) {
+    h[mv.start() + cta] = (int)ni;
+    size_t share = tiles * (cta + 1) / mv.ctas - done;
+    done += share;
+    while (share) {
+      Job& job = jobs[j];
+      const size_t nt = ((size_t)job.len + PT - 1) / PT, take = std::min(share, nt - jt);
+      if (!jt) job.part0 = (int)part;
+      items[ni++] = Item{j, (int)jt, (int)(jt + take), (int)part};
+      part += job.m;
+      job.splits++;
+      share -= take;
+      if ((jt += take) == nt) {
+        j++;
+        jt = 0;
+      }
+    }
+  }
+  h[mv.start() + mv.ctas] = (int)ni;
+  p->rows = rows;
+  p->groups = n_groups;
+  SYN_CUDA_TRY(cudaMemcpyAsync(p->meta, h, p->meta_ints * sizeof(int), cudaMemcpyHostToDevice, st));
+  SYN_CUDA_TRY(cudaEventRecord(p->copied, st));
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t* p, size_t row, size_t* len) {
+  if (!p || !len) return SYN_ERR_NULL_PTR;
+  if (row >= p->rows) return SYN_ERR_INVALID_ARG;
+  *len = p->prefix[row];
+  return SYN_OK;
+}
+
+syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t layer,
+                                              const float* q, const float* k, const float* v,
+                                              size_t ld, const float* q_norm, const float* k_norm,
+                                              float eps, const float* rope_cos,
+                                              const float* rope_sin, size_t window, float* out,
+                                              size_t ldo, void* stream) {
+  if (!p || !q || !k || !v || !rope_cos || !rope_sin || !out) return SYN_ERR_NULL_PTR;
+  syn_cuda_kvcache_t* c = p->cache;
+  if (layer >= c->layers) return SYN_ERR_INVALID_ARG;
+  if (!p->rows) return SYN_OK;
+  if (ld < c->hd || ldo < p->n_heads * c->hd) return SYN_ERR_SHAPE_MISMATCH;
+  for (size_t i = 0; i < p->rows; i++) {
+    const int sq = p->seqs[i];
+    if (c->len[sq] + 1 > c->max_seq) return SYN_ERR_INVALID_ARG;  // CacheFull
+    // what the rows shared when the plan was set, they must share still
+    if (c->len[sq] < p->prefix[i] || (c->page && c->shrunk[sq] != p->shrunk[i]))
+      return SYN_ERR_INVALID_ARG;
+  }
+  DeviceGuard g(p->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  syn_status_t s;
+  for (size_t i = 0; i < p->rows; i++)
+    if ((s = kv_reserve(c, p->seqs[i], c->len[p->seqs[i]] + 1, st))) return s;
+  AttnArgs a{const_cast<float*>(q), k, v, ld, p->n_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
+             window, c, layer, out, ldo};
+  return launch_attn_shared(p, a, nullptr, st);
+}
+
+}  // extern "C"

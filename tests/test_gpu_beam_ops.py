@@ -462,3 +462,20 @@ def test_select_refusals(ctx):
         sb.beam_select(ctx, wide, _rand((65,), 2), 65)
     assert e.value.status == 12
     assert sb.beam_select(ctx, x[:0], s[:0], 2)[0].shape == (0, 2)
+
+
+def test_views_keep_the_cache(ctx):
+    """A view of the pools outlives the last name of its cache, but not its close()."""
+    import weakref
+    cache = sb.KVCache(ctx, 16, 1, 8, 2, 2, 4, 6)
+    seen = weakref.ref(cache)
+    k, table = cache.pages(1)[0], cache.device_table()
+    del cache
+    assert seen() is not None
+    k.fill_(3.0)
+    assert float(k.sum()) == 3.0 * k.numel()
+    row = k[2:3]
+    del k, table
+    assert seen() is not None and float(row.sum()) == 96.0
+    del row
+    assert seen() is None
