@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "internal.cuh"
+#include "tcgen05.cuh"
 
 // A batch of decode rows in groups. Built on the host by _set: which leading
 // pages each group shares, and the schedule of its prefix work.
@@ -104,103 +105,444 @@ __device__ __forceinline__ long long row_at(const SharedArgs& a, int sq, int pos
 }
 
 // ---------------------------------------------------------------------------
-// Prefix, plain form: CTA = its items in turn; two threads per query row.
+// Shared prefixes on the tensor cores. A job is 128 query rows (tensor-memory
+// lanes) of one group and KV head; a CTA runs through its items' tiles of 64
+// keys:
+//   16 warps load K and V rows (a half-warp per row) straight into registers,
+//     one tile ahead, and write them as fp16 hi + lo parts, x' = x 2^-e =
+//     hi + lo with lo = fp16(x' - hi) and e from the row's largest element:
+//     22 bits, whatever the rows' magnitudes;
+//   one thread issues tcgen05.mma: S = Qh Kh + Qh Kl + Ql Kh and, with the
+//     softmax's P split the same way, O += Ph Vh + Ph Vl + Pl Vh. Q and P are
+//     A operands in tensor memory. K and V lie alike, [key][hd] in swizzled
+//     128-byte rows: K-major for S, MN-major for O, so nothing is transposed;
+//   4 warps, a thread per query row, turn S into P.
+// V's row scales go into the softmax: with V_j = V'_j 2^{e_j}, the weight of V'_j
+// is 2^{x_j}, x_j = s_j log2(e) + e_j, so the running maximum is taken over x_j,
+// P_j = 2^{x_j - M} is the size of the whole contribution, and l = sum P_j 2^{-e_j}.
+// O stays in tensor memory; it is rescaled only when the maximum grows by more
+// than 2^8 (P keeps 2^7 as its nominal top, so it stays below fp16's 2^16).
+// Waits are bounded (SYN_ERR_TIMEOUT).
 // ---------------------------------------------------------------------------
-constexpr int PX_THREADS = 256;
+constexpr int PX_SOFT = 4, PX_CONV = 16;  // warps
+constexpr int PX_MMA_WARP = PX_SOFT + PX_CONV;
+constexpr int PX_THREADS = 32 * (PX_SOFT + PX_CONV + 1);
+constexpr float P_TOP = 7.0f, P_GROW = 8.0f;
 
 template <int HDP>
-__global__ void __launch_bounds__(PX_THREADS) k_prefix(const SharedArgs a) {
-  extern __shared__ float sm[];
-  constexpr int S = HDP + 4;
-  float* sq = sm;
-  float* sk = sq + PM * S;
-  float* sv = sk + PT * S;
-  float* ss = sv + PT * S;  // [PM][PT + 1]
-  const int tid = threadIdx.x, hd = a.hd;
-  const int* meta = a.meta;
-  griddep_wait();
-  const int i0 = meta[a.mv.start() + blockIdx.x], i1 = meta[a.mv.start() + blockIdx.x + 1];
-  for (int it = i0; it < i1; it++) {
-    const Item item = reinterpret_cast<const Item*>(meta + a.mv.items())[it];
-    const Job job = reinterpret_cast<const Job*>(meta + a.mv.jobs())[item.job];
-    const int seq = meta[a.mv.seq() + job.row0];
-    for (int t = tid; t < PM * HDP; t += PX_THREADS) {
-      const int r = t / HDP, d = t % HDP;
-      float x = 0.0f;
-      if (r < job.m && d < hd) {
-        const int i = job.m0 + r;
-        x = a.q[((size_t)(job.row0 + i / a.G) * a.n_heads + job.kvh * a.G + i % a.G) * hd + d];
-      }
-      sq[r * S + d] = x;
-    }
-    const int r = tid >> 1, part = tid & 1;
-    float o[HDP / 2];
-#pragma unroll
-    for (int d = 0; d < HDP / 2; d++) o[d] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    // positions below low are outside the row's window; below all rows', they are not read
-    int low = 0, lowest = 0;
-    if (a.window) {
-      lowest = job.len;
-      for (int i = 0; i < job.m; i++) {
-        const int row = job.row0 + (job.m0 + i) / a.G;
-        const int lw = max(0, a.len[meta[a.mv.seq() + row]] + 1 - a.window);
-        lowest = min(lowest, lw);
-        if (i == r) low = lw;
-      }
-    }
-    for (int t = item.t0; t < item.t1; t++) {
-      __syncthreads();
-      for (int u = tid; u < PT * HDP; u += PX_THREADS) {
-        const int j = u / HDP, d = u % HDP, pos = t * PT + j;
-        float kx = 0.0f, vx = 0.0f;
-        if (pos < job.len && pos >= lowest && d < hd) {
-          const long long row = row_at(a, seq, pos);
-          if (row >= 0) {
-            kx = a.kc[(row * a.n_kv + job.kvh) * hd + d];
-            vx = a.vc[(row * a.n_kv + job.kvh) * hd + d];
-          }
-        }
-        sk[j * S + d] = kx;
-        sv[j * S + d] = vx;
-      }
-      __syncthreads();
-      float mt = -INFINITY;
-      for (int j = part; j < PT; j += 2) {
-        float s = 0.0f;
-        for (int d = 0; d < HDP; d++) s = fmaf(sq[r * S + d], sk[j * S + d], s);
-        const int pos = t * PT + j;
-        s = pos < job.len && pos >= low ? s * a.scale : -INFINITY;
-        ss[r * (PT + 1) + j] = s;
-        mt = fmaxf(mt, s);
-      }
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-      const float mn = fmaxf(m, mt);
-      const float corr = m == -INFINITY ? 0.0f : expf(m - mn);
-      l *= corr;
-#pragma unroll
-      for (int d = 0; d < HDP / 2; d++) o[d] *= corr;
-      __syncwarp();
-      for (int j = 0; j < PT; j++) {
-        const float s = ss[r * (PT + 1) + j];
-        const float p = s == -INFINITY ? 0.0f : expf(s - mn);
-        l += p;
-#pragma unroll
-        for (int d = 0; d < HDP / 2; d++) o[d] = fmaf(p, sv[j * S + part * (HDP / 2) + d], o[d]);
-      }
-      m = mn;
-      __syncwarp();
-    }
-    if (r < job.m) {
-      const size_t rec = item.part + r;
-      if (part == 0) a.pml[rec] = make_float2(m, l);
-#pragma unroll
-      for (int d = 0; d < HDP / 2; d++)
-        if (part * (HDP / 2) + d < hd) a.po[rec * hd + part * (HDP / 2) + d] = o[d];
-    }
-    __syncthreads();
+struct PxSmem {
+  static constexpr int PART = PT * HDP * 2;  // one fp16 part of K or V
+  static constexpr int STAGE = 4 * PART;     // K hi, K lo, V hi, V lo
+  static constexpr int BYTES = 2 * STAGE + 1024;
+};
+
+// What an item covers: tiles t0 .. t1 of its job, less those that no row sees.
+struct PxItem {
+  Job job;
+  int t0, t1, part, seq;
+  int lowest;  // no row of the job sees a position below
+};
+__device__ __forceinline__ PxItem px_item(const SharedArgs& a, int it) {  // whole warps
+  PxItem r;
+  const Item i = reinterpret_cast<const Item*>(a.meta + a.mv.items())[it];
+  r.job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[i.job];
+  r.t0 = i.t0;
+  r.t1 = i.t1;
+  r.part = i.part;
+  r.seq = a.meta[a.mv.seq() + r.job.row0];
+  r.lowest = 0;
+  if (a.window) {
+    const int first = r.job.row0 + r.job.m0 / a.G, last = r.job.row0 + (r.job.m0 + r.job.m - 1) / a.G;
+    int low = r.job.len;
+    for (int row = first + (threadIdx.x & 31); row <= last; row += 32)
+      low = min(low, a.len[a.meta[a.mv.seq() + row]] + 1 - a.window);
+    r.lowest = max(0, __reduce_min_sync(0xffffffffu, low));
+    r.t0 = min(r.t1, max(r.t0, r.lowest / PT));
   }
+  return r;
+}
+
+// 2 f32 -> packed fp16 hi and lo
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Biased exponent that scales a row with largest magnitude m to [2^13, 2^14):
+// x' = x * px_down(eb), x = x' * px_up(eb). Clamped so that both are normal.
+__device__ __forceinline__ int px_exp(float m) {
+  return min(max((int)(__float_as_uint(m) >> 23), 67), 254);
+}
+__device__ __forceinline__ float px_down(int eb) { return __uint_as_float((uint32_t)(267 - eb) << 23); }
+__device__ __forceinline__ float px_up(int eb) { return __uint_as_float((uint32_t)(eb - 13) << 23); }
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
+  using L = PxSmem<HDP>;
+  constexpr int QC = HDP / 2;  // tensor-memory columns of one part of Q
+  constexpr uint32_t C_Q = 0, C_S = 2 * QC, C_P = C_S + 2 * PT, C_O = C_P + 2 * PT, COLS = 512;
+  static_assert(C_O + HDP <= COLS, "tensor memory");
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t kfull[2], vfull[2], pfull[2], qk_done[2], pv_done[2], qfull;
+  __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT];
+  __shared__ uint32_t tbase_sh;
+  __shared__ int fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&kfull[s], PX_CONV);
+      mbar_init(&vfull[s], PX_CONV);
+      mbar_init(&pfull[s], PX_SOFT);
+      mbar_init(&qk_done[s], 1);
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(&qfull, PX_SOFT);
+    fail = 0;
+    mbar_fence_init();
+  }
+  if (warp == PX_MMA_WARP) tc_alloc(&tbase_sh, COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = tbase_sh;
+  volatile int* failed = &fail;
+  auto wait = [&](uint64_t* bar, int use) {  // a whole warp, until the use-th completion
+    const bool done = !*failed && mbar_wait_bounded(bar, use & 1);
+    if (!done) *failed = 1;
+    return __all_sync(0xffffffffu, done) != 0;
+  };
+  griddep_wait();
+  const int* start = a.meta + a.mv.start() + blockIdx.x;
+  const int i0 = start[0], i1 = start[1];
+  int n = 0;  // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
+
+  if (warp < PX_SOFT) {
+    // ---- a thread per query row ----
+    const int r = tid;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    bool ok = true;
+    for (int it = i0; it < i1 && ok; it++) {
+      const PxItem item = px_item(a, it);
+      const Job& job = item.job;
+      const bool busy = warp * 32 < job.m;  // else no row of this warp is one
+      float cq = 0.0f;
+      int low = 0;
+      if (busy) {
+        const int i = job.m0 + r, row = job.row0 + i / a.G;
+        const bool live = r < job.m;
+        const float* q = a.q + ((size_t)row * a.n_heads + job.kvh * a.G + i % a.G) * a.hd;
+        float m = 0.0f;
+        if (live)
+          for (int d = 0; d < a.hd; d += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(q + d);
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+          }
+        const int eb = px_exp(m);
+        const float down = px_down(eb);
+        cq = px_up(eb) * a.scale * 1.4426950408889634f;
+        if (a.window && live) low = max(0, a.len[a.meta[a.mv.seq() + row]] + 1 - a.window);
+        // (the last item's products are done: its O was read)
+#pragma unroll
+        for (int c = 0; c < HDP; c += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int d = 0; d < 32; d += 4) {
+            float4 f = make_float4(0, 0, 0, 0);
+            if (live && c + d < a.hd) f = *reinterpret_cast<const float4*>(q + c + d);
+            split2(f.x * down, f.y * down, hi[d / 2], lo[d / 2]);
+            split2(f.z * down, f.w * down, hi[d / 2 + 1], lo[d / 2 + 1]);
+          }
+          tc_st16(tb + lanes + C_Q + c / 2, hi);
+          tc_st16(tb + lanes + C_Q + QC + c / 2, lo);
+        }
+        tc_wait_st();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qfull);
+      auto seen = [&](int p) { return p < job.len && p >= low; };
+      float M = -INFINITY, l = 0.0f;
+      for (int t = item.t0; t < item.t1; t++, n++) {
+        const int s = n & 1, use = n >> 1;
+        // (the scales of the tile's rows come with V)
+        if (!(ok = wait(&vfull[s], use)) || !(ok = wait(&qk_done[s], use))) break;
+        tc_fence_after();
+        if (busy) {
+          float mx = -INFINITY;
+          const bool whole = t * PT + PT <= job.len && t * PT >= low;
+#pragma unroll
+          for (int c = 0; c < PT; c += 32) {
+            float x[32];
+            tc_ld32(tb + lanes + C_S + s * PT + c, x);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 ku = *reinterpret_cast<const float4*>(&kup[s][c + j]);
+              const float4 ve = *reinterpret_cast<const float4*>(&vexp[s][c + j]);
+              float y[4] = {fmaf(x[j] * ku.x, cq, ve.x), fmaf(x[j + 1] * ku.y, cq, ve.y),
+                            fmaf(x[j + 2] * ku.z, cq, ve.z), fmaf(x[j + 3] * ku.w, cq, ve.w)};
+              if (!whole)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  if (!seen(t * PT + c + j + e)) y[e] = -INFINITY;
+              mx = fmaxf(mx, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+            }
+          }
+          // a new reference only when the old one is too far below
+          const bool first = t == item.t0;
+          const bool grow = mx > M + P_GROW;  // (also from -inf)
+          const float ref = grow ? mx : M;
+          if (first) {
+            M = ref;
+          } else if (__any_sync(0xffffffffu, grow)) {
+            const float f = M == -INFINITY ? 0.0f : ex2(M - ref);
+            const bool any = M != ref;
+            M = ref;
+            l *= any ? f : 1.0f;
+            if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
+            tc_fence_after();
+            for (int c = 0; c < HDP; c += 32) {
+              float o[32];
+              tc_ld32(tb + lanes + C_O + c, o);
+              tc_wait_ld();
+              uint32_t u[32];
+#pragma unroll
+              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(any ? o[j] * f : o[j]);
+              tc_st16(tb + lanes + C_O + c, u);
+              tc_st16(tb + lanes + C_O + c + 16, u + 16);
+            }
+            tc_wait_st();
+          }
+          if (use && !(ok = wait(&pv_done[s], use - 1))) break;  // P's last reader
+          tc_fence_after();
+          const float shift = M == -INFINITY ? 0.0f : P_TOP - M;
+#pragma unroll
+          for (int c = 0; c < PT; c += 32) {
+            float x[32];
+            tc_ld32(tb + lanes + C_S + s * PT + c, x);
+            tc_wait_ld();
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int j = h; j < h + 16; j += 4) {
+                const float4 ku = *reinterpret_cast<const float4*>(&kup[s][c + j]);
+                const float4 ve = *reinterpret_cast<const float4*>(&vexp[s][c + j]);
+                const float4 vd = *reinterpret_cast<const float4*>(&vdown[s][c + j]);
+                float p[4] = {ex2(fmaf(x[j] * ku.x, cq, ve.x + shift)),
+                              ex2(fmaf(x[j + 1] * ku.y, cq, ve.y + shift)),
+                              ex2(fmaf(x[j + 2] * ku.z, cq, ve.z + shift)),
+                              ex2(fmaf(x[j + 3] * ku.w, cq, ve.w + shift))};
+                if (!whole)
+#pragma unroll
+                  for (int e = 0; e < 4; e++)
+                    if (!seen(t * PT + c + j + e)) p[e] = 0.0f;
+                l = fmaf(p[0], vd.x, fmaf(p[1], vd.y, fmaf(p[2], vd.z, fmaf(p[3], vd.w, l))));
+                split2(p[0], p[1], hi[(j - h) / 2], lo[(j - h) / 2]);
+                split2(p[2], p[3], hi[(j - h) / 2 + 1], lo[(j - h) / 2 + 1]);
+              }
+              tc_st8(tb + lanes + C_P + s * PT + (c + h) / 2, hi);
+              tc_st8(tb + lanes + C_P + s * PT + 32 + (c + h) / 2, lo);
+            }
+          }
+          tc_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[s]);
+      }
+      if (!ok) break;
+      // the item's record: O and l are both relative to 2^(M - P_TOP)
+      if (item.t1 > item.t0 && !(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
+      tc_fence_after();
+      if (busy) {
+        const size_t rec = item.part + r;
+        const bool none = item.t1 == item.t0 || M == -INFINITY;
+        if (r < job.m)
+          a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
+                            : make_float2((M - P_TOP) * 0.6931471805599453f, l);
+        for (int c = 0; c < HDP; c += 32) {
+          float o[32];
+          tc_ld32(tb + lanes + C_O + c, o);
+          tc_wait_ld();
+          if (r < job.m)
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (c + j < a.hd)
+                *reinterpret_cast<float4*>(a.po + rec * a.hd + c + j) =
+                    none ? make_float4(0, 0, 0, 0) : make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+        tc_fence_before();
+      }
+    }
+  } else if (warp == PX_MMA_WARP) {
+    // ---- one thread issues the products ----
+    constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+    constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+    const uint32_t base = smem_u32(sm);
+    bool ok = true;
+    for (int it = i0; it < i1 && ok; it++) {
+      const PxItem item = px_item(a, it);
+      const int nt = item.t1 - item.t0;
+      if (!(ok = wait(&qfull, it - i0))) break;
+      auto scores = [&](int k) {  // S of the k-th tile from here
+        const int s = k & 1, use = k >> 1;
+        if (!(ok = wait(&kfull[s], use))) return;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t kb = base + s * L::STAGE;
+#pragma unroll
+          for (int ks = 0; ks < HDP / 16; ks++) {
+            const uint32_t off = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32);
+            const uint64_t dh = tc_desc_k(kb + off), dl = tc_desc_k(kb + L::PART + off);
+            const uint32_t qh = tb + C_Q + ks * 8, d = tb + C_S + s * PT;
+            tc_mma_ts(d, qh, dh, id_s, ks > 0);
+            tc_mma_ts(d, qh, dl, id_s, 1);
+            tc_mma_ts(d, qh + QC, dh, id_s, 1);
+          }
+          tc_commit(&qk_done[s]);
+        }
+        __syncwarp();
+      };
+      if (nt) scores(n);
+      for (int t = 0; t < nt && ok; t++, n++) {
+        if (t + 1 < nt) scores(n + 1);
+        const int s = n & 1, use = n >> 1;
+        if (!ok || !(ok = wait(&vfull[s], use)) || !(ok = wait(&pfull[s], use))) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t vb = base + s * L::STAGE + 2 * L::PART;
+#pragma unroll
+          for (int ks = 0; ks < PT / 16; ks++) {
+            const uint64_t dh = tc_desc_mn(vb + ks * 2048, PT * 128), dl = tc_desc_mn(vb + L::PART + ks * 2048, PT * 128);
+            const uint32_t ph = tb + C_P + s * PT + ks * 8, d = tb + C_O;
+            tc_mma_ts(d, ph, dh, id_o, t > 0 || ks > 0);
+            tc_mma_ts(d, ph, dl, id_o, 1);
+            tc_mma_ts(d, ph + 32, dh, id_o, 1);
+          }
+          tc_commit(&pv_done[s]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ---- K and V rows to fp16 parts: half-warp hw takes K rows hw, hw + 32 of a tile, then V ----
+    const int hw = (warp - PX_SOFT) * 2 + (lane >> 4), l16 = lane & 15;
+    constexpr int NV = HDP / 64;  // float4s of a row per lane
+    int it = i0, t = 0;
+    PxItem item;
+    auto settle = [&]() {  // the next tile to load, over empty items
+      while (it < i1) {
+        item = px_item(a, it);
+        t = item.t0;
+        if (t < item.t1) return;
+        it++;
+      }
+    };
+    float4 x[4][NV];
+    auto rows = [&](long long (&at)[2]) {  // cache rows of keys hw and hw + 32 of tile t, -1 = none
+      const int j = (lane & 1) * 32 + hw, pos = t * PT + j;
+      long long p = -1;
+      if (pos < item.job.len && pos >= item.lowest) p = row_at(a, item.seq, pos);
+      at[0] = __shfl_sync(0xffffffffu, p, lane & 16);
+      at[1] = __shfl_sync(0xffffffffu, p, (lane & 16) + 1);
+    };
+    auto load = [&](int i, const float* cache, long long at) {
+#pragma unroll
+      for (int u = 0; u < NV; u++) {
+        x[i][u] = make_float4(0, 0, 0, 0);
+        const int d = u * 64 + l16 * 4;
+        if (at >= 0 && d < a.hd)
+          x[i][u] = __ldg(reinterpret_cast<const float4*>(cache + ((size_t)at * a.n_kv + item.job.kvh) * a.hd + d));
+      }
+    };
+    auto store = [&](int i, uint8_t* part, int j) {  // the row's exponent
+      float m = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NV; u++)
+        m = fmaxf(fmaxf(m, fmaxf(fabsf(x[i][u].x), fabsf(x[i][u].y))), fmaxf(fabsf(x[i][u].z), fabsf(x[i][u].w)));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const int eb = px_exp(m);
+      const float down = px_down(eb);
+#pragma unroll
+      for (int u = 0; u < NV; u++) {
+        uint2 hi, lo;
+        split2(x[i][u].x * down, x[i][u].y * down, hi.x, lo.x);
+        split2(x[i][u].z * down, x[i][u].w * down, hi.y, lo.y);
+        uint8_t* p = part + u * PT * 128 + (j >> 3) * 1024 + (j & 7) * 128 + (((l16 >> 1) ^ (j & 7)) << 4) + (l16 & 1) * 8;
+        *reinterpret_cast<uint2*>(p) = hi;
+        *reinterpret_cast<uint2*>(p + L::PART) = lo;
+      }
+      return eb;
+    };
+    settle();
+    if (it < i1) {
+      long long at[2];
+      rows(at);
+#pragma unroll
+      for (int i = 0; i < 4; i++) load(i, i < 2 ? a.kc : a.vc, at[i & 1]);
+    }
+    bool ok = true;
+    for (; it < i1 && ok; n++) {
+      const int s = n & 1, use = n >> 1;
+      uint8_t* st = sm + s * L::STAGE;
+      int ek[2];
+      // the tile after this one
+      long long at[2] = {-1, -1};
+      if (++t == item.t1) {
+        it++;
+        settle();
+      }
+      if (it < i1) rows(at);
+      if (use && !(ok = wait(&qk_done[s], use - 1))) break;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        ek[i] = store(i, st, hw + 32 * i);
+        if (it < i1) load(i, a.kc, at[i]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[s]);
+      if (use && !(ok = wait(&pv_done[s], use - 1))) break;
+#pragma unroll
+      for (int i = 2; i < 4; i++) {
+        const int j = hw + 32 * (i - 2), eb = store(i, st + 2 * L::PART, j);
+        if (l16 == 0) {  // (the softmax is done with the stage's last scales: P was used)
+          kup[s][j] = px_up(ek[i - 2]);
+          vexp[s][j] = (float)(eb - 140);
+          vdown[s][j] = px_down(eb);
+        }
+        if (it < i1) load(i, a.vc, at[i - 2]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[s]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
   griddep_launch();
+  if (*failed && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
+  if (warp == PX_MMA_WARP) {
+    tc_fence_after();
+    if (*failed && lane == 0) {  // products may be in flight: let them end before the memory goes
+      tc_commit(&qfull);
+      for (int i = 0; i < 4; i++) mbar_wait_bounded(&qfull, i & 1);
+    }
+    __syncwarp();
+    tc_dealloc(tb, COLS);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -473,12 +815,11 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.scale = 1.0f / sqrtf((float)c->hd);
   a.err = err;
   if (p->groups < p->rows) {
-    constexpr size_t s64 = (size_t)((PM + 2 * PT) * 68 + PM * (PT + 1)) * 4;
-    constexpr size_t s128 = (size_t)((PM + 2 * PT) * 132 + PM * (PT + 1)) * 4;
     const bool w = c->hd > 64;
     void (*kern)(const SharedArgs) = w ? k_prefix<128> : k_prefix<64>;
-    if ((s = more_smem((const void*)kern, w ? s128 : s64))) return s;
-    s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), w ? s128 : s64, st, a), "k_prefix");
+    const size_t smem = w ? PxSmem<128>::BYTES : PxSmem<64>::BYTES;
+    if ((s = more_smem((const void*)kern, smem))) return s;
+    s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), smem, st, a), "k_prefix");
     if (s) return s;
   }
   const int gc = chunk_heads(a.G), chunks = (a.G + gc - 1) / gc;
