@@ -108,15 +108,19 @@ __device__ __forceinline__ long long row_at(const SharedArgs& a, int sq, int pos
 // Shared prefixes on the tensor cores. A job is 128 query rows (tensor-memory
 // lanes) of one group and KV head; a CTA runs through its items' tiles of 64
 // keys:
-//   16 warps load K and V rows (a half-warp per row) straight into registers,
-//     one tile ahead, and write them as fp16 hi + lo parts, x' = x 2^-e =
-//     hi + lo with lo = fp16(x' - hi) and e from the row's largest element:
-//     22 bits, whatever the rows' magnitudes;
+//   8 warps load K and V rows (8 lanes a row) straight into registers, a tile
+//     ahead, and write them as fp16 hi + lo parts, x' = x 2^-e = hi + lo with
+//     lo = fp16(x' - hi) and e from the row's largest element: 22 bits,
+//     whatever the rows' magnitudes. An item's Q goes the same way first;
 //   one thread issues tcgen05.mma: S = Qh Kh + Qh Kl + Ql Kh and, with the
 //     softmax's P split the same way, O += Ph Vh + Ph Vl + Pl Vh. Q and P are
 //     A operands in tensor memory. K and V lie alike, [key][hd] in swizzled
 //     128-byte rows: K-major for S, MN-major for O, so nothing is transposed;
-//   4 warps, a thread per query row, turn S into P.
+//   8 warps turn S into P, two threads per query row, 32 keys each.
+// Issuing blocks while the tensor pipe is busy (a product of 64 columns takes
+// 45 cycles, one of 128 takes 65), so its warp does nothing else. Registers go
+// where they are needed (setmaxnreg): what spills goes to L2, since shared
+// memory leaves next to no L1.
 // V's row scales go into the softmax: with V_j = V'_j 2^{e_j}, the weight of V'_j
 // is 2^{x_j}, x_j = s_j log2(e) + e_j, so the running maximum is taken over x_j,
 // P_j = 2^{x_j - M} is the size of the whole contribution, and l = sum P_j 2^{-e_j}.
@@ -124,36 +128,46 @@ __device__ __forceinline__ long long row_at(const SharedArgs& a, int sq, int pos
 // than 2^8 (P keeps 2^7 as its nominal top, so it stays below fp16's 2^16).
 // Waits are bounded (SYN_ERR_TIMEOUT).
 // ---------------------------------------------------------------------------
-constexpr int PX_SOFT = 4, PX_CONV = 16;  // warps
+constexpr int PX_SOFT = 8, PX_CONV = 8;  // warps; then four of which one issues the products
 constexpr int PX_MMA_WARP = PX_SOFT + PX_CONV;
-constexpr int PX_THREADS = 32 * (PX_SOFT + PX_CONV + 1);
+constexpr int PX_THREADS = 32 * (PX_SOFT + PX_CONV + 4);
+// Registers a thread: 96 at launch (20 warps), which the softmax keeps; what the last four
+// warps give up is the converters'.
+constexpr int PX_REGS = 96, PX_REGS_SOFT = 96, PX_REGS_CONV = 120, PX_REGS_MMA = 40;
+static_assert(2 * PX_REGS_SOFT + 2 * PX_REGS_CONV + PX_REGS_MMA <= 5 * PX_REGS, "register split");
 constexpr float P_TOP = 7.0f, P_GROW = 8.0f;
 
 template <int HDP>
 struct PxSmem {
-  static constexpr int PART = PT * HDP * 2;  // one fp16 part of K or V
-  static constexpr int STAGE = 4 * PART;     // K hi, K lo, V hi, V lo
-  static constexpr int BYTES = 2 * STAGE + 1024;
+  static constexpr int PART = PT * HDP * 2;   // one fp16 part of K or V
+  static constexpr int STAGE = 4 * PART;      // K hi, K lo, V hi, V lo
+  static constexpr int QPART = PM * HDP * 2;  // one part of Q
+  static constexpr int Q = 2 * STAGE;
+  static constexpr int BYTES = Q + 2 * QPART + 1024;
 };
 
 // What an item covers: tiles t0 .. t1 of its job, less those that no row sees.
 struct PxItem {
-  Job job;
-  int t0, t1, part, seq;
+  int row0, m0, m, kvh, len, t0, t1, part, seq;
   int lowest;  // no row of the job sees a position below
 };
 __device__ __forceinline__ PxItem px_item(const SharedArgs& a, int it) {  // whole warps
   PxItem r;
   const Item i = reinterpret_cast<const Item*>(a.meta + a.mv.items())[it];
-  r.job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[i.job];
+  const Job* job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs()) + i.job;
+  r.row0 = job->row0;
+  r.m0 = job->m0;
+  r.m = job->m;
+  r.kvh = job->kvh;
+  r.len = job->len;
   r.t0 = i.t0;
   r.t1 = i.t1;
   r.part = i.part;
-  r.seq = a.meta[a.mv.seq() + r.job.row0];
+  r.seq = a.meta[a.mv.seq() + r.row0];
   r.lowest = 0;
   if (a.window) {
-    const int first = r.job.row0 + r.job.m0 / a.G, last = r.job.row0 + (r.job.m0 + r.job.m - 1) / a.G;
-    int low = r.job.len;
+    const int first = r.row0 + r.m0 / a.G, last = r.row0 + (r.m0 + r.m - 1) / a.G;
+    int low = r.len;
     for (int row = first + (threadIdx.x & 31); row <= last; row += 32)
       low = min(low, a.len[a.meta[a.mv.seq() + row]] + 1 - a.window);
     r.lowest = max(0, __reduce_min_sync(0xffffffffu, low));
@@ -162,11 +176,39 @@ __device__ __forceinline__ PxItem px_item(const SharedArgs& a, int it) {  // who
   return r;
 }
 
-// 2 f32 -> packed fp16 hi and lo
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Pairs of f32 in one register pair: one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pk(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpk(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// A pair -> packed fp16 hi and lo
+__device__ __forceinline__ void split2(f32x2 v, uint32_t& hi, uint32_t& lo) {
+  float a, b;
+  unpk(v, a, b);
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
-  const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+  unpk(fma2(pk(f.x, f.y), pk(-1.0f, -1.0f), v), a, b);
+  const __half2 r = __floats2half2_rn(a, b);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -185,16 +227,67 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
   return y;
 }
 
+template <int N>
+__device__ __forceinline__ void more_regs() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void less_regs() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ void pair_sync(int id) {  // the two warps of the same query rows
+  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
+}
+
+// Two rows, j and j + 2, of an operand of `rows` rows, 8 lanes a row (lane l has the
+// float4s l, l + 8, ...): the fp16 parts into `part` and psize bytes behind it; the
+// rows' exponents.
+template <int NV>
+__device__ __forceinline__ void px_rows(const float4 (&v)[2][NV], uint8_t* part, int psize, int rows, int j,
+                                        int (&eb)[2]) {
+  const int l8 = threadIdx.x & 7;
+  float m[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    m[i] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; u++)
+      m[i] = fmaxf(fmaxf(fmaxf(m[i], fabsf(v[i][u].x)), fabsf(v[i][u].y)), fmaxf(fabsf(v[i][u].z), fabsf(v[i][u].w)));
+  }
+#pragma unroll
+  for (int o = 4; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < 2; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int k = j + 2 * i;
+    eb[i] = px_exp(m[i]);
+    const f32x2 down = pk(px_down(eb[i]), px_down(eb[i]));
+    uint8_t* row = part + (k >> 3) * 1024 + (k & 7) * 128 + (l8 & 1) * 8;
+#pragma unroll
+    for (int u = 0; u < NV; u++) {
+      uint2 hi, lo;
+      split2(mul2(pk(v[i][u].x, v[i][u].y), down), hi.x, lo.x);
+      split2(mul2(pk(v[i][u].z, v[i][u].w), down), hi.y, lo.y);
+      uint8_t* p = row + (u >> 1) * rows * 128 + ((((u & 1) * 4 + (l8 >> 1)) ^ (k & 7)) << 4);
+      *reinterpret_cast<uint2*>(p) = hi;
+      *reinterpret_cast<uint2*>(p + psize) = lo;
+    }
+  }
+}
+
 template <int HDP>
 __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   using L = PxSmem<HDP>;
-  constexpr int QC = HDP / 2;  // tensor-memory columns of one part of Q
+  constexpr int QC = HDP / 2;   // tensor-memory columns of one part of Q
+  constexpr int NV = HDP / 32;  // float4s of a row per lane
   constexpr uint32_t C_Q = 0, C_S = 2 * QC, C_P = C_S + 2 * PT, C_O = C_P + 2 * PT, COLS = 512;
   static_assert(C_O + HDP <= COLS, "tensor memory");
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t kfull[2], vfull[2], pfull[2], qk_done[2], pv_done[2], qfull;
-  __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT];
+  __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT], qup[PM];
+  __shared__ float pmax[2][2][PM];  // [tile parity][half of the keys][row]
   __shared__ uint32_t tbase_sh;
   __shared__ int fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -224,136 +317,165 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   griddep_wait();
   const int* start = a.meta + a.mv.start() + blockIdx.x;
   const int i0 = start[0], i1 = start[1];
-  int n = 0;  // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
+  int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
+  int ord = 0;  // items with tiles so far
 
   if (warp < PX_SOFT) {
-    // ---- a thread per query row ----
-    const int r = tid;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    // ---- two threads per query row: half h has keys 32h .. 32h+31 of a tile ----
+    if constexpr (PX_REGS_SOFT < PX_REGS) less_regs<PX_REGS_SOFT>();
+    const int h = warp >> 2, r = tid & 127, pair = 1 + (warp & 3);
+    const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     bool ok = true;
     for (int it = i0; it < i1 && ok; it++) {
       const PxItem item = px_item(a, it);
-      const Job& job = item.job;
-      const bool busy = warp * 32 < job.m;  // else no row of this warp is one
+      const bool busy = (warp & 3) * 32 < item.m;  // else no row of this warp is one
+      const size_t rec = item.part + r;
+      if (item.t0 == item.t1) {  // nothing of it is in any window
+        if (r < item.m && h == 0) {
+          a.pml[rec] = make_float2(-INFINITY, 0.0f);
+          for (int d = 0; d < a.hd; d += 4)
+            *reinterpret_cast<float4*>(a.po + rec * a.hd + d) = make_float4(0, 0, 0, 0);
+        }
+        continue;
+      }
       float cq = 0.0f;
       int low = 0;
+      // the item's queries, as fp16 parts
+#pragma unroll 1
+      for (int g = 0; g < PM && g + warp * 8 < item.m; g += 64) {
+        const int l8 = lane & 7, j = g + warp * 8 + (((lane >> 3) & 1) << 2 | lane >> 4);
+        float4 v[2][NV];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int m = item.m0 + j + 2 * i;
+          const float* src =
+              a.q + ((size_t)(item.row0 + m / a.G) * a.n_heads + item.kvh * a.G + m % a.G) * a.hd;
+#pragma unroll
+          for (int u = 0; u < NV; u++) {
+            v[i][u] = make_float4(0, 0, 0, 0);
+            if (j + 2 * i < item.m && u * 32 + l8 * 4 < a.hd)
+              v[i][u] = *reinterpret_cast<const float4*>(src + u * 32 + l8 * 4);
+          }
+        }
+        int eb[2];
+        px_rows<NV>(v, sm + L::Q, L::QPART, PM, j, eb);
+        if (l8 == 0) {
+          qup[j] = px_up(eb[0]);
+          qup[j + 2] = px_up(eb[1]);
+        }
+      }
+      asm volatile("bar.sync 5, %0;" ::"n"(32 * PX_SOFT) : "memory");
       if (busy) {
-        const int i = job.m0 + r, row = job.row0 + i / a.G;
-        const bool live = r < job.m;
-        const float* q = a.q + ((size_t)row * a.n_heads + job.kvh * a.G + i % a.G) * a.hd;
-        float m = 0.0f;
-        if (live)
-          for (int d = 0; d < a.hd; d += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(q + d);
-            m = fmaxf(fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-          }
-        const int eb = px_exp(m);
-        const float down = px_down(eb);
-        cq = px_up(eb) * a.scale * 1.4426950408889634f;
-        if (a.window && live) low = max(0, a.len[a.meta[a.mv.seq() + row]] + 1 - a.window);
-        // (the last item's products are done: its O was read)
+        cq = qup[r] * a.scale * 1.4426950408889634f;
+        if (a.window && r < item.m)
+          low = max(0, a.len[a.meta[a.mv.seq() + item.row0 + (item.m0 + r) / a.G]] + 1 - a.window);
+        // (the last item's products are done: its O was read) half h brings Q's part h
+        tc_fence_after();
+        const uint8_t* q = sm + L::Q + h * L::QPART + (r >> 3) * 1024 + (r & 7) * 128;
 #pragma unroll
-        for (int c = 0; c < HDP; c += 32) {
-          uint32_t hi[16], lo[16];
+        for (int c = 0; c < HDP / 8; c += 4) {  // 16-byte chunks
+          uint4 u[4];
 #pragma unroll
-          for (int d = 0; d < 32; d += 4) {
-            float4 f = make_float4(0, 0, 0, 0);
-            if (live && c + d < a.hd) f = *reinterpret_cast<const float4*>(q + c + d);
-            split2(f.x * down, f.y * down, hi[d / 2], lo[d / 2]);
-            split2(f.z * down, f.w * down, hi[d / 2 + 1], lo[d / 2 + 1]);
-          }
-          tc_st16(tb + lanes + C_Q + c / 2, hi);
-          tc_st16(tb + lanes + C_Q + QC + c / 2, lo);
+          for (int e = 0; e < 4; e++)
+            u[e] = *reinterpret_cast<const uint4*>(q + ((c + e) >> 3) * (PM * 128) + ((((c + e) & 7) ^ (r & 7)) << 4));
+          tc_st16(tl + C_Q + h * QC + c * 4, reinterpret_cast<const uint32_t*>(u));
         }
         tc_wait_st();
         tc_fence_before();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&qfull);
-      auto seen = [&](int p) { return p < job.len && p >= low; };
-      float M = -INFINITY, l = 0.0f;
+      ord++;
+      float M = -INFINITY;
+      f32x2 l = 0;
+      const f32x2 cq2 = pk(cq, cq);
       for (int t = item.t0; t < item.t1; t++, n++) {
         const int s = n & 1, use = n >> 1;
         // (the scales of the tile's rows come with V)
         if (!(ok = wait(&vfull[s], use)) || !(ok = wait(&qk_done[s], use))) break;
-        tc_fence_after();
         if (busy) {
-          float mx = -INFINITY;
-          const bool whole = t * PT + PT <= job.len && t * PT >= low;
-#pragma unroll
-          for (int c = 0; c < PT; c += 32) {
+          tc_fence_after();
+          f32x2 y[16];
+          {
             float x[32];
-            tc_ld32(tb + lanes + C_S + s * PT + c, x);
+            tc_ld32(tl + C_S + s * PT + h * 32, x);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
-              const float4 ku = *reinterpret_cast<const float4*>(&kup[s][c + j]);
-              const float4 ve = *reinterpret_cast<const float4*>(&vexp[s][c + j]);
-              float y[4] = {fmaf(x[j] * ku.x, cq, ve.x), fmaf(x[j + 1] * ku.y, cq, ve.y),
-                            fmaf(x[j + 2] * ku.z, cq, ve.z), fmaf(x[j + 3] * ku.w, cq, ve.w)};
-              if (!whole)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                  if (!seen(t * PT + c + j + e)) y[e] = -INFINITY;
-              mx = fmaxf(mx, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+              const ulonglong2 ku = *reinterpret_cast<const ulonglong2*>(&kup[s][h * 32 + j]);
+              const ulonglong2 ve = *reinterpret_cast<const ulonglong2*>(&vexp[s][h * 32 + j]);
+              y[j / 2] = fma2(mul2(pk(x[j], x[j + 1]), ku.x), cq2, ve.x);
+              y[j / 2 + 1] = fma2(mul2(pk(x[j + 2], x[j + 3]), ku.y), cq2, ve.y);
             }
           }
-          // a new reference only when the old one is too far below
-          const bool first = t == item.t0;
+          const int vlo = low - t * PT - h * 32, vhi = item.len - t * PT - h * 32;
+          if (__any_sync(0xffffffffu, vlo > 0 || vhi < 32)) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float p, q;
+              unpk(y[j / 2], p, q);
+              if (j < vlo || j >= vhi) p = -INFINITY;
+              if (j + 1 < vlo || j + 1 >= vhi) q = -INFINITY;
+              y[j / 2] = pk(p, q);
+            }
+          }
+          float mx = -INFINITY, mx2 = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            float p, q;
+            unpk(y[j], p, q);
+            mx = fmaxf(fmaxf(mx, p), q);
+            unpk(y[j + 1], p, q);
+            mx2 = fmaxf(fmaxf(mx2, p), q);
+          }
+          mx = fmaxf(mx, mx2);
+          pmax[n & 1][h][r] = mx;
+          pair_sync(pair);
+          mx = fmaxf(mx, pmax[n & 1][h ^ 1][r]);
+          // a new reference only when the old one is too far below (the same in both halves)
           const bool grow = mx > M + P_GROW;  // (also from -inf)
           const float ref = grow ? mx : M;
-          if (first) {
+          if (t == item.t0) {
             M = ref;
           } else if (__any_sync(0xffffffffu, grow)) {
-            const float f = M == -INFINITY ? 0.0f : ex2(M - ref);
-            const bool any = M != ref;
+            const float f = !grow ? 1.0f : M == -INFINITY ? 0.0f : ex2(M - ref);
             M = ref;
-            l *= any ? f : 1.0f;
+            l = mul2(l, pk(f, f));
             if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
             tc_fence_after();
-            for (int c = 0; c < HDP; c += 32) {
-              float o[32];
-              tc_ld32(tb + lanes + C_O + c, o);
+            for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 16) {
+              float o[16];
+              tc_ld16(tl + C_O + c, o);
               tc_wait_ld();
-              uint32_t u[32];
+              uint32_t u[16];
 #pragma unroll
-              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(any ? o[j] * f : o[j]);
-              tc_st16(tb + lanes + C_O + c, u);
-              tc_st16(tb + lanes + C_O + c + 16, u + 16);
+              for (int j = 0; j < 16; j++) u[j] = __float_as_uint(o[j] * f);
+              tc_st16(tl + C_O + c, u);
             }
             tc_wait_st();
           }
           if (use && !(ok = wait(&pv_done[s], use - 1))) break;  // P's last reader
           tc_fence_after();
           const float shift = M == -INFINITY ? 0.0f : P_TOP - M;
+          const f32x2 shift2 = pk(shift, shift);
 #pragma unroll
-          for (int c = 0; c < PT; c += 32) {
-            float x[32];
-            tc_ld32(tb + lanes + C_S + s * PT + c, x);
-            tc_wait_ld();
+          for (int c = 0; c < 32; c += 16) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-              uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int j = h; j < h + 16; j += 4) {
-                const float4 ku = *reinterpret_cast<const float4*>(&kup[s][c + j]);
-                const float4 ve = *reinterpret_cast<const float4*>(&vexp[s][c + j]);
-                const float4 vd = *reinterpret_cast<const float4*>(&vdown[s][c + j]);
-                float p[4] = {ex2(fmaf(x[j] * ku.x, cq, ve.x + shift)),
-                              ex2(fmaf(x[j + 1] * ku.y, cq, ve.y + shift)),
-                              ex2(fmaf(x[j + 2] * ku.z, cq, ve.z + shift)),
-                              ex2(fmaf(x[j + 3] * ku.w, cq, ve.w + shift))};
-                if (!whole)
-#pragma unroll
-                  for (int e = 0; e < 4; e++)
-                    if (!seen(t * PT + c + j + e)) p[e] = 0.0f;
-                l = fmaf(p[0], vd.x, fmaf(p[1], vd.y, fmaf(p[2], vd.z, fmaf(p[3], vd.w, l))));
-                split2(p[0], p[1], hi[(j - h) / 2], lo[(j - h) / 2]);
-                split2(p[2], p[3], hi[(j - h) / 2 + 1], lo[(j - h) / 2 + 1]);
-              }
-              tc_st8(tb + lanes + C_P + s * PT + (c + h) / 2, hi);
-              tc_st8(tb + lanes + C_P + s * PT + 32 + (c + h) / 2, lo);
+            for (int j = 0; j < 16; j += 4) {
+              const ulonglong2 vd = *reinterpret_cast<const ulonglong2*>(&vdown[s][h * 32 + c + j]);
+              float p, q;
+              unpk(add2(y[(c + j) / 2], shift2), p, q);
+              f32x2 e = pk(ex2(p), ex2(q));
+              l = fma2(e, vd.x, l);
+              split2(e, hi[j / 2], lo[j / 2]);
+              unpk(add2(y[(c + j) / 2 + 1], shift2), p, q);
+              e = pk(ex2(p), ex2(q));
+              l = fma2(e, vd.y, l);
+              split2(e, hi[j / 2 + 1], lo[j / 2 + 1]);
             }
+            tc_st8(tl + C_P + s * PT + h * 16 + c / 2, hi);
+            tc_st8(tl + C_P + s * PT + 32 + h * 16 + c / 2, lo);
           }
           tc_wait_st();
           tc_fence_before();
@@ -363,19 +485,24 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       }
       if (!ok) break;
       // the item's record: O and l are both relative to 2^(M - P_TOP)
-      if (item.t1 > item.t0 && !(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
-      tc_fence_after();
+      if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
       if (busy) {
-        const size_t rec = item.part + r;
-        const bool none = item.t1 == item.t0 || M == -INFINITY;
-        if (r < job.m)
+        tc_fence_after();
+        float la, lb;
+        unpk(l, la, lb);
+        la += lb;
+        if (h == 1) pmax[n & 1][1][r] = la;
+        pair_sync(pair);
+        const bool none = M == -INFINITY;
+        if (h == 0 && r < item.m)
           a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
-                            : make_float2((M - P_TOP) * 0.6931471805599453f, l);
-        for (int c = 0; c < HDP; c += 32) {
+                            : make_float2((M - P_TOP) * 0.6931471805599453f, la + pmax[n & 1][1][r]);
+        pair_sync(pair);  // (the slot is the next item's)
+        for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 32) {
           float o[32];
-          tc_ld32(tb + lanes + C_O + c, o);
+          tc_ld32(tl + C_O + c, o);
           tc_wait_ld();
-          if (r < job.m)
+          if (r < item.m)
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
               if (c + j < a.hd)
@@ -385,26 +512,130 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
         tc_fence_before();
       }
     }
-  } else if (warp == PX_MMA_WARP) {
-    // ---- one thread issues the products ----
-    constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
-    constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
-    const uint32_t base = smem_u32(sm);
+  } else if (warp < PX_MMA_WARP) {
+    // ---- K and V rows to fp16 parts: 8 lanes a row, 4 rows a step; warp w has keys 8w .. 8w+7 of a
+    // tile. (A step's rows are 0, 4, 1, 5 or 2, 6, 3, 7 of the 8: their stores meet all banks.)
+    more_regs<PX_REGS_CONV>();
+    const int cw = warp - PX_SOFT, l8 = lane & 7, q4 = lane >> 3;
+    const int jj = cw * 8 + (((q4 & 1) << 2) | (q4 >> 1));  // this lane's keys: jj and jj + 2
+    const int dcol = PT / a.page, doff = PT - dcol * a.page;
+    // Three tiles are under way: x holds one's rows, `at` has the next one's places, `pg` the
+    // page numbers of the one after as they come.
+    int it = i0, left = 0;  // the item of the last tile asked for, and its tiles still to ask for
+    int len = 0, lowest = 0, pos = 0, kvh = 0, col[2], off[2];
+    const int* tab = nullptr;
+    struct Pages { int kvh, pg[2], off[2]; };  // kvh < 0: no tile
+    struct Rows { bool any; long long at[2]; };  // at < 0: no row
+    auto ask = [&]() {
+      Pages r;
+      if (left == 0) {
+        it -= (tab == nullptr);
+        while (left == 0 && ++it < i1) {
+          const PxItem item = px_item(a, it);
+          left = item.t1 - item.t0;
+          len = item.len;
+          lowest = item.lowest;
+          kvh = item.kvh;
+          tab = a.ptab + (size_t)item.seq * a.maxp;
+          pos = item.t0 * PT + jj;
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            col[i] = (pos + 2 * i) / a.page;
+            off[i] = pos + 2 * i - col[i] * a.page;
+          }
+        }
+      }
+      r.kvh = left ? kvh : -1;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int p = pos + 2 * i;
+        r.pg[i] = left && p < len && p >= lowest ? __ldg(tab + col[i]) : -1;
+        r.off[i] = off[i];
+        col[i] += dcol;
+        off[i] += doff;
+        if (off[i] >= a.page) {
+          off[i] -= a.page;
+          col[i]++;
+        }
+      }
+      pos += PT;
+      if (left) left--;
+      return r;
+    };
+    auto place = [&](const Pages& p) {
+      Rows r;
+      r.any = p.kvh >= 0;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        r.at[i] = p.pg[i] < 0 ? -1 : (((long long)p.pg[i] * a.page + p.off[i]) * a.n_kv + p.kvh) * a.hd + l8 * 4;
+      return r;
+    };
+    auto load = [&](float4 (&v)[2][NV], const float* cache, const Rows& r) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+          v[i][u] = make_float4(0, 0, 0, 0);
+          if (r.at[i] >= 0 && u * 32 + l8 * 4 < a.hd)
+            v[i][u] = __ldg(reinterpret_cast<const float4*>(cache + r.at[i] + u * 32));
+        }
+    };
+    float4 xk[2][NV], xv[2][NV];
+    Pages pages = ask();
+    Rows next = place(pages);
+    pages = ask();
+    load(xk, a.kc, next);
+    load(xv, a.vc, next);
+    bool cur = next.any;
+    next = place(pages);
+    pages = ask();
     bool ok = true;
-    for (int it = i0; it < i1 && ok; it++) {
-      const PxItem item = px_item(a, it);
-      const int nt = item.t1 - item.t0;
-      if (!(ok = wait(&qfull, it - i0))) break;
-      auto scores = [&](int k) {  // S of the k-th tile from here
+    for (; cur && ok; n++) {
+      const int s = n & 1, use = n >> 1;
+      uint8_t* st = sm + s * L::STAGE;
+      if (use && !(ok = wait(&qk_done[s], use - 1))) break;
+      int ek[2], ev[2];
+      px_rows<NV>(xk, st, L::PART, PT, jj, ek);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[s]);
+      load(xk, a.kc, next);
+      if (use && !(ok = wait(&pv_done[s], use - 1))) break;
+      px_rows<NV>(xv, st + 2 * L::PART, L::PART, PT, jj, ev);
+      if (l8 == 0) {  // (the softmax is done with the stage's last scales: P was used)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          kup[s][jj + 2 * i] = px_up(ek[i]);
+          vexp[s][jj + 2 * i] = (float)(ev[i] - 140);
+          vdown[s][jj + 2 * i] = px_down(ev[i]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[s]);
+      load(xv, a.vc, next);
+      cur = next.any;
+      next = place(pages);
+      pages = ask();
+    }
+  } else {
+    less_regs<PX_REGS_MMA>();
+    if (warp == PX_MMA_WARP) {
+      // ---- one thread issues the products ----
+      constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+      constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
+      const uint32_t base = smem_u32(sm);
+      bool ok = true;
+      auto scores = [&](int k) {  // S of tile k
         const int s = k & 1, use = k >> 1;
         if (!(ok = wait(&kfull[s], use))) return;
         tc_fence_after();
         if (lane == 0) {
           const uint32_t kb = base + s * L::STAGE;
-#pragma unroll
+#pragma unroll 2
           for (int ks = 0; ks < HDP / 16; ks++) {
-            const uint32_t off = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32);
-            const uint64_t dh = tc_desc_k(kb + off), dl = tc_desc_k(kb + L::PART + off);
+            const uint32_t o = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32);
+            const uint64_t dh = tc_desc_k(kb + o), dl = tc_desc_k(kb + L::PART + o);
             const uint32_t qh = tb + C_Q + ks * 8, d = tb + C_S + s * PT;
             tc_mma_ts(d, qh, dh, id_s, ks > 0);
             tc_mma_ts(d, qh, dl, id_s, 1);
@@ -414,120 +645,33 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
         }
         __syncwarp();
       };
-      if (nt) scores(n);
-      for (int t = 0; t < nt && ok; t++, n++) {
-        if (t + 1 < nt) scores(n + 1);
-        const int s = n & 1, use = n >> 1;
-        if (!ok || !(ok = wait(&vfull[s], use)) || !(ok = wait(&pfull[s], use))) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vb = base + s * L::STAGE + 2 * L::PART;
-#pragma unroll
-          for (int ks = 0; ks < PT / 16; ks++) {
-            const uint64_t dh = tc_desc_mn(vb + ks * 2048, PT * 128), dl = tc_desc_mn(vb + L::PART + ks * 2048, PT * 128);
-            const uint32_t ph = tb + C_P + s * PT + ks * 8, d = tb + C_O;
-            tc_mma_ts(d, ph, dh, id_o, t > 0 || ks > 0);
-            tc_mma_ts(d, ph, dl, id_o, 1);
-            tc_mma_ts(d, ph + 32, dh, id_o, 1);
+      for (int it = i0; it < i1 && ok; it++) {
+        const PxItem item = px_item(a, it);
+        const int nt = item.t1 - item.t0;
+        if (!nt) continue;
+        if (!(ok = wait(&qfull, ord++))) break;
+        scores(n);
+        for (int t = 0; t < nt && ok; t++, n++) {
+          if (t + 1 < nt) scores(n + 1);
+          const int s = n & 1, use = n >> 1;
+          if (!ok || !(ok = wait(&pfull[s], use))) break;  // (after V: the softmax waits for its scales)
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t vb = base + s * L::STAGE + 2 * L::PART;
+#pragma unroll 2
+            for (int ks = 0; ks < PT / 16; ks++) {
+              const uint64_t dh = tc_desc_mn(vb + ks * 2048, PT * 128);
+              const uint64_t dl = tc_desc_mn(vb + L::PART + ks * 2048, PT * 128);
+              const uint32_t ph = tb + C_P + s * PT + ks * 8, d = tb + C_O;
+              tc_mma_ts(d, ph, dh, id_o, t > 0 || ks > 0);
+              tc_mma_ts(d, ph, dl, id_o, 1);
+              tc_mma_ts(d, ph + 32, dh, id_o, 1);
+            }
+            tc_commit(&pv_done[s]);
           }
-          tc_commit(&pv_done[s]);
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-  } else {
-    // ---- K and V rows to fp16 parts: half-warp hw takes K rows hw, hw + 32 of a tile, then V ----
-    const int hw = (warp - PX_SOFT) * 2 + (lane >> 4), l16 = lane & 15;
-    constexpr int NV = HDP / 64;  // float4s of a row per lane
-    int it = i0, t = 0;
-    PxItem item;
-    auto settle = [&]() {  // the next tile to load, over empty items
-      while (it < i1) {
-        item = px_item(a, it);
-        t = item.t0;
-        if (t < item.t1) return;
-        it++;
-      }
-    };
-    float4 x[4][NV];
-    auto rows = [&](long long (&at)[2]) {  // cache rows of keys hw and hw + 32 of tile t, -1 = none
-      const int j = (lane & 1) * 32 + hw, pos = t * PT + j;
-      long long p = -1;
-      if (pos < item.job.len && pos >= item.lowest) p = row_at(a, item.seq, pos);
-      at[0] = __shfl_sync(0xffffffffu, p, lane & 16);
-      at[1] = __shfl_sync(0xffffffffu, p, (lane & 16) + 1);
-    };
-    auto load = [&](int i, const float* cache, long long at) {
-#pragma unroll
-      for (int u = 0; u < NV; u++) {
-        x[i][u] = make_float4(0, 0, 0, 0);
-        const int d = u * 64 + l16 * 4;
-        if (at >= 0 && d < a.hd)
-          x[i][u] = __ldg(reinterpret_cast<const float4*>(cache + ((size_t)at * a.n_kv + item.job.kvh) * a.hd + d));
-      }
-    };
-    auto store = [&](int i, uint8_t* part, int j) {  // the row's exponent
-      float m = 0.0f;
-#pragma unroll
-      for (int u = 0; u < NV; u++)
-        m = fmaxf(fmaxf(m, fmaxf(fabsf(x[i][u].x), fabsf(x[i][u].y))), fmaxf(fabsf(x[i][u].z), fabsf(x[i][u].w)));
-#pragma unroll
-      for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const int eb = px_exp(m);
-      const float down = px_down(eb);
-#pragma unroll
-      for (int u = 0; u < NV; u++) {
-        uint2 hi, lo;
-        split2(x[i][u].x * down, x[i][u].y * down, hi.x, lo.x);
-        split2(x[i][u].z * down, x[i][u].w * down, hi.y, lo.y);
-        uint8_t* p = part + u * PT * 128 + (j >> 3) * 1024 + (j & 7) * 128 + (((l16 >> 1) ^ (j & 7)) << 4) + (l16 & 1) * 8;
-        *reinterpret_cast<uint2*>(p) = hi;
-        *reinterpret_cast<uint2*>(p + L::PART) = lo;
-      }
-      return eb;
-    };
-    settle();
-    if (it < i1) {
-      long long at[2];
-      rows(at);
-#pragma unroll
-      for (int i = 0; i < 4; i++) load(i, i < 2 ? a.kc : a.vc, at[i & 1]);
-    }
-    bool ok = true;
-    for (; it < i1 && ok; n++) {
-      const int s = n & 1, use = n >> 1;
-      uint8_t* st = sm + s * L::STAGE;
-      int ek[2];
-      // the tile after this one
-      long long at[2] = {-1, -1};
-      if (++t == item.t1) {
-        it++;
-        settle();
-      }
-      if (it < i1) rows(at);
-      if (use && !(ok = wait(&qk_done[s], use - 1))) break;
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        ek[i] = store(i, st, hw + 32 * i);
-        if (it < i1) load(i, a.kc, at[i]);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[s]);
-      if (use && !(ok = wait(&pv_done[s], use - 1))) break;
-#pragma unroll
-      for (int i = 2; i < 4; i++) {
-        const int j = hw + 32 * (i - 2), eb = store(i, st + 2 * L::PART, j);
-        if (l16 == 0) {  // (the softmax is done with the stage's last scales: P was used)
-          kup[s][j] = px_up(ek[i - 2]);
-          vexp[s][j] = (float)(eb - 140);
-          vdown[s][j] = px_down(eb);
-        }
-        if (it < i1) load(i, a.vc, at[i - 2]);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[s]);
     }
   }
   tc_fence_before();
@@ -536,9 +680,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   if (*failed && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
   if (warp == PX_MMA_WARP) {
     tc_fence_after();
-    if (*failed && lane == 0) {  // products may be in flight: let them end before the memory goes
+    if (*failed && lane == 0) {  // products may be in flight: they end before the memory goes
+      mbar_init(&qfull, 1);
       tc_commit(&qfull);
-      for (int i = 0; i < 4; i++) mbar_wait_bounded(&qfull, i & 1);
+      mbar_wait_bounded(&qfull, 0);
     }
     __syncwarp();
     tc_dealloc(tb, COLS);
@@ -966,17 +1111,39 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
         }
     r0 += n;
   }
-  // the tiles of all jobs, one after another, in equal shares
-  size_t ni = 0, part = 0, done = 0;
-  int j = 0;
-  size_t jt = 0;  // tiles of job j given out
-  for (int cta = 0; cta < mv.ctas; cta++) {
+  // With no more jobs than CTAs, an item per CTA: the shortest items of which there are enough
+  // CTAs for (a CTA that goes from one job to another drains its pipeline in between). Else
+  // the tiles of all jobs, one after another, in equal shares.
+  auto tiles_of = [&](int j) { return ((size_t)jobs[j].len + PT - 1) / PT; };
+  size_t ni = 0, part = 0, done = 0, jt = 0;
+  int cta = 0;
+  if (nj && nj <= mv.ctas) {
+    size_t most = (tiles + mv.ctas - 1) / mv.ctas;
+    auto items_at = [&](size_t q) {
+      size_t k = 0;
+      for (int j = 0; j < nj; j++) k += (tiles_of(j) + q - 1) / q;
+      return k;
+    };
+    while (items_at(most) > (size_t)mv.ctas) most++;
+    for (int j = 0; j < nj; j++) {
+      Job& job = jobs[j];
+      const size_t nt = tiles_of(j);
+      job.splits = (int)((nt + most - 1) / most);
+      job.part0 = (int)part;
+      for (int i = 0; i < job.splits; i++) {
+        h[mv.start() + cta++] = (int)ni;
+        items[ni++] = Item{j, (int)(nt * i / job.splits), (int)(nt * (i + 1) / job.splits), (int)part};
+        part += job.m;
+      }
+    }
+  }
+  for (int j = 0; cta < mv.ctas; cta++) {
     h[mv.start() + cta] = (int)ni;
-    size_t share = tiles * (cta + 1) / mv.ctas - done;
+    size_t share = nj > mv.ctas ? tiles * (cta + 1) / mv.ctas - done : 0;
     done += share;
     while (share) {
       Job& job = jobs[j];
-      const size_t nt = ((size_t)job.len + PT - 1) / PT, take = std::min(share, nt - jt);
+      const size_t nt = tiles_of(j), take = std::min(share, nt - jt);
       if (!jt) job.part0 = (int)part;
       items[ni++] = Item{j, (int)jt, (int)(jt + take), (int)part};
       part += job.m;
