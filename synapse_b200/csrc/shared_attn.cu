@@ -310,8 +310,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   const uint32_t tb = tbase_sh;
   volatile int* failed = &fail;
   auto wait = [&](uint64_t* bar, int use) {  // a whole warp, until the use-th completion
-    const bool done = !*failed && mbar_wait_bounded(bar, use & 1);
-    if (!done) *failed = 1;
+    bool done = mbar_try_wait(bar, use & 1);
+    if (!done && !*failed) {
+      done = mbar_wait_bounded(bar, use & 1);
+      if (!done) *failed = 1;
+    }
     return __all_sync(0xffffffffu, done) != 0;
   };
   griddep_wait();
@@ -624,22 +627,22 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       // ---- one thread issues the products ----
       constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
       constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
-      const uint32_t base = smem_u32(sm);
+      const uint64_t kd = tc_desc_k(smem_u32(sm)), vd = tc_desc_mn(smem_u32(sm) + 2 * L::PART, PT * 128);
+      const uint32_t k_lo = (uint32_t)kd, k_hi = (uint32_t)(kd >> 32), v_lo = (uint32_t)vd, v_hi = (uint32_t)(vd >> 32);
       bool ok = true;
       auto scores = [&](int k) {  // S of tile k
         const int s = k & 1, use = k >> 1;
         if (!(ok = wait(&kfull[s], use))) return;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t kb = base + s * L::STAGE;
-#pragma unroll 2
+        if (tc_elect()) {
+          const uint32_t kb = k_lo + s * (L::STAGE >> 4), d = tb + C_S + s * PT, q = tb + C_Q;
+#pragma unroll
           for (int ks = 0; ks < HDP / 16; ks++) {
-            const uint32_t o = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32);
-            const uint64_t dh = tc_desc_k(kb + o), dl = tc_desc_k(kb + L::PART + o);
-            const uint32_t qh = tb + C_Q + ks * 8, d = tb + C_S + s * PT;
-            tc_mma_ts(d, qh, dh, id_s, ks > 0);
-            tc_mma_ts(d, qh, dl, id_s, 1);
-            tc_mma_ts(d, qh + QC, dh, id_s, 1);
+            const uint32_t o = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32) >> 4;
+            if (ks == 0) tc_mma_ts<false>(d, q, kb, k_hi, id_s);
+            else tc_mma_ts<true>(d, q + ks * 8, kb + o, k_hi, id_s);
+            tc_mma_ts<true>(d, q + ks * 8, kb + (L::PART >> 4) + o, k_hi, id_s);
+            tc_mma_ts<true>(d, q + QC + ks * 8, kb + o, k_hi, id_s);
           }
           tc_commit(&qk_done[s]);
         }
@@ -656,16 +659,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           const int s = n & 1, use = n >> 1;
           if (!ok || !(ok = wait(&pfull[s], use))) break;  // (after V: the softmax waits for its scales)
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t vb = base + s * L::STAGE + 2 * L::PART;
-#pragma unroll 2
+          if (tc_elect()) {
+            const uint32_t vb = v_lo + s * (L::STAGE >> 4), p = tb + C_P + s * PT, d = tb + C_O;
+#pragma unroll
             for (int ks = 0; ks < PT / 16; ks++) {
-              const uint64_t dh = tc_desc_mn(vb + ks * 2048, PT * 128);
-              const uint64_t dl = tc_desc_mn(vb + L::PART + ks * 2048, PT * 128);
-              const uint32_t ph = tb + C_P + s * PT + ks * 8, d = tb + C_O;
-              tc_mma_ts(d, ph, dh, id_o, t > 0 || ks > 0);
-              tc_mma_ts(d, ph, dl, id_o, 1);
-              tc_mma_ts(d, ph + 32, dh, id_o, 1);
+              const uint32_t o = ks * 2048 >> 4;
+              if (ks == 0 && t == 0) tc_mma_ts<false>(d, p, vb, v_hi, id_o);
+              else tc_mma_ts<true>(d, p + ks * 8, vb + o, v_hi, id_o);
+              tc_mma_ts<true>(d, p + ks * 8, vb + (L::PART >> 4) + o, v_hi, id_o);
+              tc_mma_ts<true>(d, p + 32 + ks * 8, vb + o, v_hi, id_o);
             }
             tc_commit(&pv_done[s]);
           }

@@ -42,13 +42,21 @@ __device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr, uint32_t next) {
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// One thread of a converged warp. Products issued under this take their operands from
+// uniform registers: 32 cycles for 64 columns where a `lane == 0` branch takes 47.
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // kind::f16, A from tensor memory (lanes = rows, two halves of K per column),
-// B from shared memory, D f32 in tensor memory.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// B from shared memory (descriptor), D f32 in tensor memory; ACC: D += A B.
+template <bool ACC>
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t id) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc));
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.eq.u32 p, %5, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(id), "n"(ACC ? 1 : 0));
 }
 // Arrives on `bar` once every product issued so far by this thread is complete.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
