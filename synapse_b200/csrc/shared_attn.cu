@@ -10,9 +10,11 @@
 // rows, so its K and V cross HBM once per step instead of once per row; each
 // row's own positions are the other. Kernels of one call:
 //   k_append_batch (beam.cu)  the new rows normalised, rotated and appended
-//   k_prefix                  the shared prefixes, on a fixed schedule
-//   k_suffix                  each row's own positions; the last CTA of a (row,
-//                             KV head) joins all parts
+//   k_prefix                  the shared prefixes of many query rows, on the
+//                             tensor cores and a fixed schedule
+//   k_span                    each row's own positions, and the shared prefixes
+//                             of few query rows
+//   k_join                    the parts of each query row
 #include <math.h>
 
 #include <algorithm>
@@ -40,7 +42,8 @@ struct syn_cuda_decode_plan_s {
   float* po = nullptr;       // partial o, prefix then suffix
   float2* pml = nullptr;     // partial (m, l)
   size_t part_rows = 0;      // records of po / pml
-  int* cnt = nullptr;        // arrivals per (row, KV head, chunk); zero between launches
+  int* starts = nullptr;     // k_span's first tile of each unit, for k_join
+  int units = 0, jobs = 0;   // k_span's units; k_prefix's jobs
 };
 
 namespace syn {
@@ -48,9 +51,12 @@ namespace {
 
 constexpr int PT = 64;         // keys of a prefix tile
 constexpr int PM = 128;        // query rows of a prefix job
-constexpr int SX_THREADS = 128, SX_WARPS = 4, SX_RB = 4;
-constexpr int SX_SPLITS = 64;  // most suffix splits of a (row, KV head)
-constexpr int PARTS_MAX = 256; // most parts of one query row: those and a prefix split per SM
+constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: warps of a CTA, keys of a tile
+constexpr int SP_V = 8;        // most query vectors of a k_span job
+constexpr int SP_FEW = 16;     // a group of at most so many query rows per KV head goes to k_span
+constexpr int ROWS_MAX = 512;  // rows of a plan
+constexpr int UNITS_MAX = ROWS_MAX + ROWS_MAX / 2;
+constexpr int PARTS_MAX = 1536;  // most parts of a query row: a k_span warp's each, a k_prefix CTA's each
 
 struct Job {      // prefix work of one (group, tile of query rows, KV head)
   int row0;       // first row of the group
@@ -64,6 +70,13 @@ struct Item {     // a CTA's share of a job: key tiles t0 .. t1, partial records
   int job, t0, t1, part;
 };
 
+// k_span's work: the positions of one row behind its prefix (n = 0), or the
+// prefix of a group of n rows from row0 on. A job is one KV head's part of it for
+// up to 8 query vectors: n_kv * nch jobs, the first job0.
+struct Unit {
+  int row0, n, pre, job0, nch;
+};
+
 // Offsets (ints) of the arrays in the plan's metadata block.
 struct Meta {
   int rows, max_jobs, max_items, ctas;
@@ -74,7 +87,9 @@ struct Meta {
   __host__ __device__ int start() const { return 4 * rows; }     // [ctas + 1] items of each CTA
   __host__ __device__ int items() const { return (start() + ctas + 1 + 3) / 4 * 4; }
   __host__ __device__ int jobs() const { return items() + 4 * max_items; }
-  __host__ __device__ int total() const { return jobs() + 7 * max_jobs; }
+  __host__ __device__ int unit_of() const { return jobs() + 7 * max_jobs; }  // k_span's prefix unit of the row, -1
+  __host__ __device__ int units() const { return unit_of() + rows; }          // prefixes first, then the rows
+  __host__ __device__ int total() const { return units() + 5 * (rows + rows / 2); }
 };
 
 struct SharedArgs {
@@ -89,9 +104,9 @@ struct SharedArgs {
   Meta mv;
   float* po;
   float2* pml;
-  int sfx0;  // first suffix record
-  int nsplit;
-  int* cnt;
+  int rows, units, span0;  // rows; k_span's units (the last `rows` are theirs) and its first record
+  int warps;               // of k_span
+  int* starts;
   float* out;
   long long ldo;
   float scale;
@@ -499,7 +514,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
         const bool none = M == -INFINITY;
         if (h == 0 && r < item.m)
           a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
-                            : make_float2((M - P_TOP) * 0.6931471805599453f, la + pmax[n & 1][1][r]);
+                            : make_float2(M - P_TOP, la + pmax[n & 1][1][r]);
         pair_sync(pair);  // (the slot is the next item's)
         for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 32) {
           float o[32];
@@ -693,200 +708,358 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Each row's own positions: CTA = (row, KV head and chunk of GC of its query
-// heads, split). LPR lanes take one cached row (four elements each), so a
-// warp's load is 32 / LPR rows of one KV head; the q.k partials are summed by
-// butterfly shuffles, each head keeps a running (m, l, o).
+// Few query vectors over a range of positions: each row's own positions, and
+// prefixes of few query rows. All jobs' tiles of 32 keys, one after another, are
+// dealt to all warps in equal, contiguous shares (the lengths are read on the
+// device), so uneven rows cost nothing. A warp works alone: bulk copies bring
+// the tile's K and V rows into its ring of three half tiles (16 bytes of padding
+// a row keep a lane per row free of bank conflicts); lane = key for the scores,
+// with q broadcast from shared memory, so no sum crosses lanes; lane = four
+// columns for the weighted sum, with the weights broadcast. A key costs about
+// 6 + 5 NQ instructions for NQ query vectors, against 43 cycles of an SM's share of
+// HBM for its 1 KB (head dim 128).
 // ---------------------------------------------------------------------------
-template <int LPR, int GC>
-__global__ void __launch_bounds__(SX_THREADS) k_suffix(const SharedArgs a, int chunks) {
-  constexpr int SUBS = 32 / LPR, STEP = SX_WARPS * SX_RB * SUBS, HDP = LPR * 4;
-  constexpr int NW = SX_WARPS * SUBS;
-  __shared__ float wst[NW][GC][2];
-  __shared__ __align__(16) float wo[NW][GC][HDP];
-  __shared__ float fac[SX_WARPS][PARTS_MAX];
-  __shared__ int last;
-  const int b = blockIdx.x, kvh = blockIdx.y / chunks, ch = blockIdx.y - kvh * chunks;
-  const int sp = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int sub = lane / LPR, l4 = lane % LPR, hd = a.hd, g0 = ch * GC;
-  const int heads = min(GC, a.G - g0);
-  griddep_wait();
-  const int sq = a.meta[a.mv.seq() + b];
-  const int pre = a.meta[a.mv.pre() + b];
-  const int pos = a.len[sq], L = pos + 1;
-  const bool full = pos >= a.max_seq;  // a replayed graph that has run past the cache
-  if (full && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
-  const int off = max(pre, a.window ? L - a.window : 0);
-  const int eff = full ? 0 : L - off;
-  int sl = (eff + a.nsplit - 1) / a.nsplit;
-  sl = (sl + SX_RB * SUBS - 1) / (SX_RB * SUBS) * (SX_RB * SUBS);
-  const int r0 = off + min(eff, sp * sl), r1 = off + min(eff, (sp + 1) * sl);
-  const bool act = l4 * 4 < hd;
-  float4 q[GC];
-#pragma unroll
-  for (int g = 0; g < GC; g++) {
-    q[g] = make_float4(0, 0, 0, 0);
-    if (g < heads && act)
-      q[g] = reinterpret_cast<const float4*>(
-          a.q + ((size_t)b * a.n_heads + kvh * a.G + g0 + g) * hd)[l4];
+__device__ __forceinline__ float redux_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct SpanJob {
+  int row0, n, pre, seq, kvh, ch, r0, r1, nq;
+};
+
+// Positions of unit u: [lo, hi)
+__device__ __forceinline__ int2 unit_range(const SharedArgs& a, const Unit& u) {
+  const int* seq = a.meta + a.mv.seq();
+  if (u.n) {
+    int lo = 0;
+    if (a.window) {
+      lo = u.pre;
+      for (int r = u.row0; r < u.row0 + u.n; r++) lo = min(lo, max(0, a.len[seq[r]] + 1 - a.window));
+    }
+    return make_int2(lo, u.pre);
   }
-  float m[GC], l[GC];
-  float4 o[GC];
-#pragma unroll
-  for (int g = 0; g < GC; g++) {
-    m[g] = -INFINITY;
-    l[g] = 0.0f;
-    o[g] = make_float4(0, 0, 0, 0);
+  const int L = a.len[seq[u.row0]] + 1;
+  if (L > a.max_seq) {  // a replayed graph that has run past the cache
+    if (a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
+    return make_int2(0, 0);
   }
-  const float4 zero = make_float4(0, 0, 0, 0);
-  auto load = [&](int rb, float4(&kr)[SX_RB], float4(&vr)[SX_RB]) {
+  return make_int2(max(u.pre, a.window ? L - a.window : 0), L);
+}
+
+// Tiles [k0, k1) of a job, by one warp; the record of each query vector.
+template <int LPR, int NQ>
+__device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job, int k0, int k1, size_t rec,
+                                         uint8_t* ring, float* qs, float2* ps, uint64_t* bars, uint32_t& used) {
+  constexpr int SUBS = 32 / LPR;
+  const int lane = threadIdx.x & 31, hd = a.hd, stride = hd * 4 + 16, slot_bytes = SP_T * stride;
+  const int sub = lane / LPR, l4 = (lane % LPR) * 4;
+  // queries, times scale * log2(e)
+  const float qscale = a.scale * 1.4426950408889634f;
+  int low[NQ];
 #pragma unroll
-    for (int j = 0; j < SX_RB; j++) {
-      const int row = rb + j * SUBS + sub;
-      kr[j] = vr[j] = zero;
-      if (row < r1 && act) {
-        const long long at = row_at(a, sq, row);
-        if (at >= 0) {
-          const size_t e = ((size_t)at * a.n_kv + kvh) * hd / 4 + l4;
-          kr[j] = reinterpret_cast<const float4*>(a.kc)[e];
-          vr[j] = reinterpret_cast<const float4*>(a.vc)[e];
+  for (int v = 0; v < NQ; v++) {
+    const int i = job.ch * SP_V + v;
+    const int row = job.row0 + (job.n ? i / a.G : 0), head = job.kvh * a.G + (job.n ? i % a.G : i);
+    low[v] = 0;
+    if (v < job.nq && job.n && a.window) low[v] = a.len[a.meta[a.mv.seq() + row]] + 1 - a.window;
+    for (int d = lane * 4; d < hd; d += 128) {
+      float4 f = make_float4(0, 0, 0, 0);
+      if (v < job.nq) f = *reinterpret_cast<const float4*>(a.q + ((size_t)row * a.n_heads + head) * hd + d);
+      *reinterpret_cast<float4*>(qs + v * hd + d) =
+          make_float4(f.x * qscale, f.y * qscale, f.z * qscale, f.w * qscale);
+    }
+  }
+  // the ring: K and V of a tile in turn; `used` counts the fills of all jobs
+  const uint32_t first = used;
+  const int nt = k1 - k0;
+  long long at = -1;  // cache row of this lane's key of the tile asked for last
+  auto ask = [&](int k) {
+    const int pos = job.r0 + (k0 + k) * SP_T + lane;
+    at = pos < job.r1 ? row_at(a, job.seq, pos) : -1;
+  };
+  auto fill = [&](int h, const float* cache) {  // half tile h (its K or V) into its slot
+    const uint32_t u = first + h;
+    uint64_t* bar = bars + u % SP_SLOTS;
+    uint8_t* dst = ring + (u % SP_SLOTS) * slot_bytes + lane * stride;
+    const uint32_t rows = __popc(__ballot_sync(0xffffffffu, at >= 0));
+    fence_async_smem();  // (the slot's last readers are past; order their accesses before the copy's)
+    if (lane == 0) mbar_expect_tx(bar, rows * hd * 4);
+    __syncwarp();
+    if (at >= 0) bulk_g2s(dst, cache + ((size_t)at * a.n_kv + job.kvh) * hd, hd * 4, bar);
+    used++;
+  };
+  auto ready = [&](int h) {
+    const uint32_t u = first + h;
+    bool ok = mbar_try_wait(bars + u % SP_SLOTS, (u / SP_SLOTS) & 1);
+    if (!ok) ok = mbar_wait_bounded(bars + u % SP_SLOTS, (u / SP_SLOTS) & 1);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  float m[NQ], l[NQ];
+  f32x2 o[NQ][2];
+#pragma unroll
+  for (int v = 0; v < NQ; v++) {
+    m[v] = -INFINITY;
+    l[v] = 0.0f;
+    o[v][0] = o[v][1] = 0;
+  }
+  ask(0);
+  fill(0, a.kc);
+  fill(1, a.vc);
+  if (nt > 1) {
+    ask(1);
+    fill(2, a.kc);
+  }
+  __syncwarp();
+  for (int k = 0; k < nt; k++) {
+    const int key = job.r0 + (k0 + k) * SP_T + lane;
+    const int nk = min(SP_T, job.r1 - job.r0 - (k0 + k) * SP_T);
+    if (!ready(2 * k)) return false;
+    f32x2 acc[NQ];
+#pragma unroll
+    for (int v = 0; v < NQ; v++) acc[v] = 0;
+    const uint8_t* kr = ring + ((first + 2 * k) % SP_SLOTS) * slot_bytes + lane * stride;
+#pragma unroll 4
+    for (int d = 0; d < hd; d += 4) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kr + d * 4);
+#pragma unroll
+      for (int v = 0; v < NQ; v++) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(qs + v * hd + d);
+        acc[v] = fma2(x.x, q.x, acc[v]);
+        acc[v] = fma2(x.y, q.y, acc[v]);
+      }
+    }
+    __syncwarp();  // (all have read the slot)
+    if (k + 1 < nt) fill(2 * k + 3, a.vc);
+    // softmax weights, twice each for the packed sums
+    float corr[NQ];
+    bool grown = false;
+#pragma unroll
+    for (int v = 0; v < NQ; v++) {
+      float x, y;
+      unpk(acc[v], x, y);
+      x = lane < nk && key >= low[v] ? x + y : -INFINITY;
+      const float mx = fmaxf(m[v], redux_max(x));
+      corr[v] = m[v] == -INFINITY ? 0.0f : ex2(m[v] - mx);
+      grown |= mx != m[v];
+      const float p = mx == -INFINITY ? 0.0f : ex2(x - mx);
+      l[v] = fmaf(l[v], corr[v], p);
+      m[v] = mx;
+      ps[lane * NQ + v] = make_float2(p, p);
+    }
+    if (grown) {
+#pragma unroll
+      for (int v = 0; v < NQ; v++) {
+        o[v][0] = mul2(o[v][0], pk(corr[v], corr[v]));
+        o[v][1] = mul2(o[v][1], pk(corr[v], corr[v]));
+      }
+    }
+    __syncwarp();
+    if (!ready(2 * k + 1)) return false;
+    const uint8_t* vr = ring + ((first + 2 * k + 1) % SP_SLOTS) * slot_bytes;
+    if (l4 < hd) {
+#pragma unroll 4
+      for (int j = sub; j < nk; j += SUBS) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vr + j * stride + l4 * 4);
+        const f32x2* p = reinterpret_cast<const f32x2*>(ps + j * NQ);
+#pragma unroll
+        for (int v = 0; v < NQ; v++) {
+          o[v][0] = fma2(p[v], x.x, o[v][0]);
+          o[v][1] = fma2(p[v], x.y, o[v][1]);
         }
       }
     }
-  };
-  float4 kr[SX_RB], vr[SX_RB];
-  const int rb0 = r0 + warp * SX_RB * SUBS;
-  load(rb0, kr, vr);
-  for (int rb = rb0; rb < r1; rb += STEP) {
-    float4 kn[SX_RB], vn[SX_RB];
-    load(rb + STEP, kn, vn);
-    float s[GC][SX_RB];
-#pragma unroll
-    for (int g = 0; g < GC; g++)
-#pragma unroll
-      for (int j = 0; j < SX_RB; j++)
-        s[g][j] = fmaf(q[g].x, kr[j].x, fmaf(q[g].y, kr[j].y, fmaf(q[g].z, kr[j].z, q[g].w * kr[j].w)));
-#pragma unroll
-    for (int x = LPR / 2; x; x >>= 1)
-#pragma unroll
-      for (int g = 0; g < GC; g++)
-#pragma unroll
-        for (int j = 0; j < SX_RB; j++) s[g][j] += __shfl_xor_sync(0xffffffffu, s[g][j], x);
-#pragma unroll
-    for (int g = 0; g < GC; g++) {
-      float mx = m[g];
-#pragma unroll
-      for (int j = 0; j < SX_RB; j++) {
-        s[g][j] = rb + j * SUBS + sub < r1 ? s[g][j] * a.scale : -INFINITY;
-        mx = fmaxf(mx, s[g][j]);
-      }
-      if (mx == -INFINITY) continue;
-      const float corr = m[g] == -INFINITY ? 0.0f : expf(m[g] - mx);
-      l[g] *= corr;
-      o[g].x *= corr;
-      o[g].y *= corr;
-      o[g].z *= corr;
-      o[g].w *= corr;
-#pragma unroll
-      for (int j = 0; j < SX_RB; j++) {
-        const float p = s[g][j] == -INFINITY ? 0.0f : expf(s[g][j] - mx);
-        l[g] += p;
-        o[g].x = fmaf(p, vr[j].x, o[g].x);
-        o[g].y = fmaf(p, vr[j].y, o[g].y);
-        o[g].z = fmaf(p, vr[j].z, o[g].z);
-        o[g].w = fmaf(p, vr[j].w, o[g].w);
-      }
-      m[g] = mx;
-    }
-#pragma unroll
-    for (int j = 0; j < SX_RB; j++) {
-      kr[j] = kn[j];
-      vr[j] = vn[j];
+    __syncwarp();
+    if (k + 2 < nt) {
+      ask(k + 2);
+      fill(2 * k + 4, a.kc);
     }
   }
-  // join the warps and their sub-rows: one record per head of this split
 #pragma unroll
-  for (int g = 0; g < GC; g++) {
-    const int w = warp * SUBS + sub;
-    if (l4 == 0) {
-      wst[w][g][0] = m[g];
-      wst[w][g][1] = l[g];
+  for (int v = 0; v < NQ; v++) {
+    float x[4];
+    unpk(o[v][0], x[0], x[1]);
+    unpk(o[v][1], x[2], x[3]);
+#pragma unroll
+    for (int s = LPR; s < 32; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] += __shfl_xor_sync(0xffffffffu, x[e], s);
+    const float sum = warp_sum(l[v]);
+    if (v < job.nq) {
+      if (lane == 0) a.pml[rec + v] = make_float2(m[v], sum);
+      if (sub == 0 && l4 < hd)
+        *reinterpret_cast<float4*>(a.po + (rec + v) * hd + l4) = make_float4(x[0], x[1], x[2], x[3]);
     }
-    *reinterpret_cast<float4*>(&wo[w][g][l4 * 4]) = o[g];
   }
-  __syncthreads();
-  const size_t rec0 = a.sfx0 + ((size_t)b * a.n_heads + kvh * a.G + g0) * a.nsplit;
-  for (int i = tid; i < heads * hd; i += SX_THREADS) {
-    const int g = i / hd, d = i - g * hd;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; w++) M = fmaxf(M, wst[w][g][0]);
-    float O = 0.0f, Ls = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-      const float f = wst[w][g][0] == -INFINITY ? 0.0f : expf(wst[w][g][0] - M);
-      O = fmaf(f, wo[w][g][d], O);
-      Ls = fmaf(f, wst[w][g][1], Ls);
+  __syncwarp();
+  return true;
+}
+
+template <int LPR>
+__global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
+  extern __shared__ __align__(16) uint8_t sraw[];
+  __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_SLOTS];
+  __shared__ int sums[SP_WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slot_bytes = SP_T * (a.hd * 4 + 16), per_warp = SP_SLOTS * slot_bytes + SP_V * a.hd * 4 + SP_T * SP_V * 8;
+  uint8_t* ring = sraw + warp * per_warp;
+  float* qs = reinterpret_cast<float*>(ring + SP_SLOTS * slot_bytes);
+  float2* ps = reinterpret_cast<float2*>(qs + SP_V * a.hd);
+  int* starts = reinterpret_cast<int*>(sraw + SP_WARPS * per_warp);  // [units + 1]
+  if (lane < SP_SLOTS) mbar_init(&bars[warp][lane], 1);
+  mbar_fence_init();
+  griddep_wait();
+  const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
+  {  // first tile of each unit
+    const int per = (a.units + SP_WARPS * 32 - 1) / (SP_WARPS * 32);
+    const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
+    int sum = 0;
+    for (int u = u0; u < u1; u++) {
+      const Unit x = units[u];
+      const int2 r = unit_range(a, x);
+      const int t = (max(0, r.y - r.x) + SP_T - 1) / SP_T * a.n_kv * x.nch;
+      starts[u] = t;
+      sum += t;
     }
-    const size_t rec = rec0 + (size_t)g * a.nsplit + sp;
-    a.po[rec * hd + d] = O;
-    if (d == 0) a.pml[rec] = make_float2(M, Ls);
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    int base = inc - sum;
+    for (int w = 0; w < warp; w++) base += sums[w];
+    for (int u = u0; u < u1; u++) {
+      const int t = starts[u];
+      starts[u] = base;
+      base += t;
+    }
+    if (u1 == a.units) starts[a.units] = base;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int u = tid; u <= a.units; u += SP_WARPS * 32) a.starts[u] = starts[u];
   }
-  __threadfence();
-  __syncthreads();
-  int* cn = a.cnt + (size_t)b * gridDim.y + blockIdx.y;
-  if (tid == 0) last = atomicAdd(cn, 1) == a.nsplit - 1;
-  __syncthreads();
+  const long long total = starts[a.units];
+  const int gw = warp * gridDim.x + blockIdx.x;
+  const long long warps = min((long long)a.warps, total);  // that have a share
+  long long t = gw < warps ? gw * total / warps : 0;
+  const long long t1 = gw < warps ? (gw + 1) * total / warps : 0;
+  uint32_t used = 0;
+  bool ok = true;
+  while (t < t1 && ok) {
+    int lo = 0, hi = a.units;  // the last unit that starts at or before t and is not empty
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (starts[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    const Unit u = units[lo];
+    const int jobs = a.n_kv * u.nch, nt = (starts[lo + 1] - starts[lo]) / jobs, r = (int)(t - starts[lo]);
+    const int jl = r / nt, k0 = r - jl * nt;
+    SpanJob job;
+    job.row0 = u.row0;
+    job.n = u.n;
+    job.pre = u.pre;
+    job.seq = a.meta[a.mv.seq() + u.row0];
+    job.kvh = jl / u.nch;
+    job.ch = jl - job.kvh * u.nch;
+    job.nq = min(SP_V, (u.n ? u.n * a.G : a.G) - job.ch * SP_V);
+    const int2 range = unit_range(a, u);
+    job.r0 = range.x;
+    job.r1 = range.y;
+    const int k1 = (int)min((long long)nt, k0 + t1 - t);
+    const size_t rec = a.span0 + (size_t)(gw + u.job0 + jl) * SP_V;
+    ok = job.nq > 4   ? span_job<LPR, 8>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+         : job.nq > 2 ? span_job<LPR, 4>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+         : job.nq > 1 ? span_job<LPR, 2>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+                      : span_job<LPR, 1>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used);
+    t += k1 - k0;
+  }
+  if (!ok && lane == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
   griddep_launch();
-  if (!last) return;
-  __threadfence();
-  // join all parts of this (row, chunk): a warp per head
-  const int job0 = a.meta[a.mv.job_of() + b];
-  for (int g = warp; g < heads; g += SX_WARPS) {
-    int np = 0;
-    size_t prec = 0;
-    int pstep = 0;
-    if (pre > 0 && job0 >= 0) {
-      const int i = a.meta[a.mv.local() + b] * a.G + g0 + g, mt = i / PM;
-      const Job job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[job0 + mt * a.n_kv + kvh];
-      np = job.splits;
-      prec = job.part0 + i - job.m0;
-      pstep = job.m;
+}
+
+// ---------------------------------------------------------------------------
+// The parts of a query row: k_span's of its own positions, and of its prefix
+// k_span's or k_prefix's. A warp per (row, head). (Maxima are in units of log2.)
+// ---------------------------------------------------------------------------
+constexpr int JN_WARPS = 4;
+
+__global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
+  __shared__ float fac[JN_WARPS][PARTS_MAX];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
+  const int i = blockIdx.x * JN_WARPS + warp, b = i / a.n_heads, head = i - b * a.n_heads;
+  griddep_wait();
+  if (b >= a.rows) return;
+  const int kvh = head / a.G, g = head - kvh * a.G;
+  const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
+  const long long total = __ldcg(a.starts + a.units), warps = min((long long)a.warps, total);
+  // records first + c * step, c < n, of a k_span unit's job and vector
+  struct Parts { size_t first; int n, step; };
+  auto span_parts = [&](int u, int idx) {
+    const Unit x = units[u];
+    const int s = __ldcg(a.starts + u), e = __ldcg(a.starts + u + 1), nt = (e - s) / (a.n_kv * x.nch);
+    const int jl = kvh * x.nch + idx / SP_V;
+    Parts p{0, 0, SP_V};
+    if (nt) {  // the warps whose shares meet its tiles
+      const long long t0 = s + (long long)jl * nt, t1 = t0 + nt;
+      const int w0 = (int)(((t0 + 1) * warps - 1) / total), w1 = (int)((t1 * warps - 1) / total);
+      p.first = a.span0 + (size_t)(w0 + x.job0 + jl) * SP_V + idx % SP_V;
+      p.n = w1 - w0 + 1;
     }
-    const int n = a.nsplit + np;
-    const size_t srec = rec0 + (size_t)g * a.nsplit;
-    auto rec = [&](int c) { return c < a.nsplit ? srec + c : prec + (size_t)(c - a.nsplit) * pstep; };
-    float M = -INFINITY;
-    for (int c = lane; c < n; c += 32) M = fmaxf(M, __ldcg(&a.pml[rec(c)]).x);
-    M = warp_max(M);
-    float lsum = 0.0f;
-    for (int c = lane; c < n; c += 32) {
-      const float2 ml = __ldcg(&a.pml[rec(c)]);
-      const float f = ml.x == -INFINITY ? 0.0f : expf(ml.x - M);
-      fac[warp][c] = f;
-      lsum += f * ml.y;
-    }
-    lsum = warp_sum(lsum);
-    __syncwarp();
-    float* orow = a.out + (long long)b * a.ldo + (long long)(kvh * a.G + g0 + g) * hd;
-    for (int d4 = lane; d4 * 4 < hd; d4 += 32) {
-      float4 ov = zero;
-      for (int c = 0; c < n; c++) {
-        const float4 t = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd) + d4);
-        const float f = fac[warp][c];
-        ov.x = fmaf(t.x, f, ov.x);
-        ov.y = fmaf(t.y, f, ov.y);
-        ov.z = fmaf(t.z, f, ov.z);
-        ov.w = fmaf(t.w, f, ov.w);
-      }
-      orow[d4 * 4] = ov.x / lsum;
-      orow[d4 * 4 + 1] = ov.y / lsum;
-      orow[d4 * 4 + 2] = ov.z / lsum;
-      orow[d4 * 4 + 3] = ov.w / lsum;
-    }
-    __syncwarp();
+    return p;
+  };
+  const int local = a.meta[a.mv.local() + b] * a.G + g;
+  const Parts own = span_parts(a.units - a.rows + b, g);
+  Parts pre{0, 0, 0};
+  const int pu = a.meta[a.mv.unit_of() + b], job0 = a.meta[a.mv.job_of() + b];
+  if (pu >= 0) {
+    pre = span_parts(pu, local);
+  } else if (job0 >= 0) {
+    const Job job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[job0 + local / PM * a.n_kv + kvh];
+    pre = Parts{(size_t)(job.part0 + local - job.m0), job.splits, job.m};
   }
-  if (tid == 0) *cn = 0;
+  const int n = min(PARTS_MAX, own.n + pre.n);
+  auto rec = [&](int c) {
+    return c < own.n ? own.first + (size_t)c * own.step : pre.first + (size_t)(c - own.n) * pre.step;
+  };
+  float M = -INFINITY;
+  for (int c = lane; c < n; c += 32) {
+    const float2 ml = __ldcg(&a.pml[rec(c)]);
+    fac[warp][c] = ml.x;
+    M = fmaxf(M, ml.x);
+  }
+  M = warp_max(M);
+  float sum = 0.0f;
+  for (int c = lane; c < n; c += 32) {
+    const float f = fac[warp][c] == -INFINITY ? 0.0f : ex2(fac[warp][c] - M);
+    fac[warp][c] = f;
+    sum += f * __ldcg(&a.pml[rec(c)]).y;
+  }
+  sum = warp_sum(sum);
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f * sum;  // (NaN stays)
+  __syncwarp();
+  griddep_launch();
+  float* orow = a.out + (long long)b * a.ldo + (long long)head * hd;
+  for (int d = lane * 4; d < hd; d += 128) {
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (int c = 0; c < n; c++) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd + d));
+      const float f = fac[warp][c];
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    }
+    orow[d] = o.x * inv;
+    orow[d + 1] = o.y * inv;
+    orow[d + 2] = o.z * inv;
+    orow[d + 3] = o.w * inv;
+  }
 }
 
 syn_status_t launched(cudaError_t e, const char* where) {
@@ -901,13 +1074,6 @@ syn_status_t more_smem(const void* fn, size_t bytes) {
   return SYN_OK;
 }
 
-using SuffixK = void (*)(const SharedArgs, int);
-template <int LPR>
-SuffixK suffix_kernel(int gc) {
-  return gc == 1 ? k_suffix<LPR, 1> : gc == 2 ? k_suffix<LPR, 2> : gc == 4 ? k_suffix<LPR, 4> : k_suffix<LPR, 8>;
-}
-int chunk_heads(int G) { return G == 1 ? 1 : G == 2 ? 2 : G <= 4 ? 4 : 8; }
-
 // Most jobs and items of a batch of `batch` rows (groups of two or more share).
 size_t max_jobs(size_t batch, size_t n_kv, size_t G) {
   return n_kv * (batch * G / PM + batch / 2 + 1);
@@ -919,11 +1085,14 @@ Meta meta_of(const syn_cuda_decode_plan_t* p) {
   return Meta{(int)c->batch, (int)jobs, (int)(jobs + p->sms), p->sms};
 }
 
-int suffix_splits(const syn_cuda_decode_plan_t* p) {
-  // about four CTAs per SM over all (row, KV head) pairs
-  const size_t G = p->n_heads / p->cache->n_kv, gc = chunk_heads((int)G);
-  const size_t pairs = std::max<size_t>(1, p->rows) * p->cache->n_kv * ((G + gc - 1) / gc);
-  return (int)std::max<size_t>(1, std::min<size_t>(SX_SPLITS, (4 * p->sms + pairs - 1) / pairs));
+// k_span: shared memory, and CTAs on an SM
+size_t span_smem(size_t hd) {
+  return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 8) + (UNITS_MAX + 1) * 4;
+}
+int span_ctas(size_t hd) { return span_smem(hd) > 112 * 1024 ? 1 : 2; }
+// Most k_span jobs of a batch
+size_t span_jobs(size_t batch, size_t n_kv, size_t G) {
+  return n_kv * (batch * ((G + SP_V - 1) / SP_V) + batch / 2 * (SP_FEW / SP_V));
 }
 
 }  // namespace
@@ -954,14 +1123,16 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.mv = meta_of(p);
   a.po = p->po;
   a.pml = p->pml;
-  a.nsplit = suffix_splits(p);
-  a.sfx0 = (int)(p->part_rows - p->n_heads * std::max<size_t>(c->batch, 4 * p->sms + c->batch));
-  a.cnt = p->cnt;
+  a.rows = (int)p->rows;
+  a.units = p->units;
+  a.warps = span_ctas(c->hd) * p->sms * SP_WARPS;
+  a.span0 = (int)(p->part_rows - (a.warps + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
+  a.starts = p->starts;
   a.out = at.out;
   a.ldo = (long long)at.ldo;
   a.scale = 1.0f / sqrtf((float)c->hd);
   a.err = err;
-  if (p->groups < p->rows) {
+  if (p->jobs) {
     const bool w = c->hd > 64;
     void (*kern)(const SharedArgs) = w ? k_prefix<128> : k_prefix<64>;
     const size_t smem = w ? PxSmem<128>::BYTES : PxSmem<64>::BYTES;
@@ -969,11 +1140,15 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
     s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), smem, st, a), "k_prefix");
     if (s) return s;
   }
-  const int gc = chunk_heads(a.G), chunks = (a.G + gc - 1) / gc;
-  SuffixK sk = c->hd <= 32 ? suffix_kernel<8>(gc) : c->hd <= 64 ? suffix_kernel<16>(gc) : suffix_kernel<32>(gc);
-  return launched(launch_pdl(sk, dim3((unsigned)p->rows, (unsigned)(c->n_kv * chunks), (unsigned)a.nsplit),
-                             dim3(SX_THREADS), 0, st, a, chunks),
-                  "k_suffix");
+  void (*span)(const SharedArgs) = c->hd <= 32 ? k_span<8> : c->hd <= 64 ? k_span<16> : k_span<32>;
+  if ((s = more_smem((const void*)span, span_smem(c->hd)))) return s;
+  s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->sms), dim3(SP_WARPS * 32), span_smem(c->hd), st, a),
+               "k_span");
+  if (s) return s;
+  const size_t joins = p->rows * p->n_heads;
+  return launched(launch_pdl(k_join, dim3((unsigned)((joins + JN_WARPS - 1) / JN_WARPS)), dim3(JN_WARPS * 32), 0,
+                             st, a),
+                  "k_join");
 }
 
 }  // namespace syn
@@ -996,30 +1171,28 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   p->device = c->device;
   p->sms = num_sms();
   p->n_heads = n_heads;
-  if (p->sms + SX_SPLITS > PARTS_MAX) {
+  if (p->sms * (1 + SP_WARPS * span_ctas(c->hd)) > PARTS_MAX) {
     delete p;
     return SYN_ERR_UNSUPPORTED;
   }
   const Meta mv = meta_of(p);
   p->meta_ints = mv.total();
   // prefix records: a job's rows for each CTA that shares in it, at most one job's rows more
-  // per CTA than the batch's query rows; suffix records: nsplit of each (row, head)
   const size_t G = n_heads / c->n_kv;
+  // per CTA than the batch's query rows; k_span records: 8 of each (warp, job) that meet
   const size_t prefix = c->batch * n_heads + (size_t)p->sms * std::min<size_t>(PM, c->batch * G);
-  const size_t suffix = n_heads * std::max<size_t>(c->batch, 4 * p->sms + c->batch);
-  p->part_rows = prefix + suffix;
+  const size_t span = (p->sms * span_ctas(c->hd) * SP_WARPS + span_jobs(c->batch, c->n_kv, G)) * SP_V;
+  p->part_rows = prefix + span;
   if (p->part_rows > 0x7FFFFFFF) {
     delete p;
     return SYN_ERR_UNSUPPORTED;
   }
-  const size_t ncnt = c->batch * n_heads;
   cudaError_t e = cudaMalloc(&p->q, c->batch * n_heads * c->hd * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->meta, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMallocHost(&p->meta_h, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->pml, p->part_rows * sizeof(float2));
-  if (e == cudaSuccess) e = cudaMalloc(&p->cnt, ncnt * sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(p->cnt, 0, ncnt * sizeof(int));
+  if (e == cudaSuccess) e = cudaMalloc(&p->starts, (UNITS_MAX + 1) * sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(p->meta, 0, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&p->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -1041,7 +1214,7 @@ syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
   if (p->meta_h) cudaFreeHost(p->meta_h);
   cudaFree(p->po);
   cudaFree(p->pml);
-  cudaFree(p->cnt);
+  cudaFree(p->starts);
   if (p->copied) cudaEventDestroy(p->copied);
   delete p;
   return SYN_OK;
@@ -1068,6 +1241,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     }
     rows += group_rows[i];
   }
+  if (rows > ROWS_MAX) return SYN_ERR_UNSUPPORTED;
   syn_status_t s = kv_sync(c, st);
   // (a row cut back into a shared page gets its own copy now, not in a later call)
   for (size_t i = 0; i < rows && s == SYN_OK; i++) s = kv_own_page(c, seqs[i], st);
@@ -1081,7 +1255,8 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   p->seqs.assign(seqs, seqs + rows);
   p->prefix.assign(rows, 0);
   p->shrunk.assign(rows, 0);
-  int nj = 0;
+  Unit* units = reinterpret_cast<Unit*>(h + mv.units());
+  int nj = 0, nu = 0, uj = 0;
   size_t tiles = 0, r0 = 0;
   for (size_t i = 0; i < n_groups; i++) {
     const size_t n = group_rows[i];
@@ -1097,15 +1272,21 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       }
       shared = col * c->page;
     }
+    const bool few = shared && n * G <= SP_FEW;
     for (size_t j = r0; j < r0 + n; j++) {
       h[mv.seq() + j] = seqs[j];
       h[mv.pre() + j] = (int)shared;
-      h[mv.job_of() + j] = shared ? nj : -1;
+      h[mv.job_of() + j] = shared && !few ? nj : -1;
+      h[mv.unit_of() + j] = few ? nu : -1;
       h[mv.local() + j] = (int)(j - r0);
       p->prefix[j] = shared;
       if (c->page) p->shrunk[j] = c->shrunk[seqs[j]];
     }
-    if (shared)
+    if (few) {
+      const int nch = ((int)n * G + SP_V - 1) / SP_V;
+      units[nu++] = Unit{(int)r0, (int)n, (int)shared, uj, nch};
+      uj += (int)c->n_kv * nch;
+    } else if (shared)
       for (int m0 = 0; m0 < (int)n * G; m0 += PM)
         for (int kvh = 0; kvh < (int)c->n_kv; kvh++) {
           jobs[nj++] = Job{(int)r0, m0, std::min(PM, (int)n * G - m0), kvh, (int)shared, 0, 0};
@@ -1158,6 +1339,13 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     }
   }
   h[mv.start() + mv.ctas] = (int)ni;
+  for (size_t j = 0; j < rows; j++) {  // each row's own positions
+    const int nch = (G + SP_V - 1) / SP_V;
+    units[nu++] = Unit{(int)j, 0, h[mv.pre() + j], uj, nch};
+    uj += (int)c->n_kv * nch;
+  }
+  p->units = nu;
+  p->jobs = nj;
   p->rows = rows;
   p->groups = n_groups;
   SYN_CUDA_TRY(cudaMemcpyAsync(p->meta, h, p->meta_ints * sizeof(int), cudaMemcpyHostToDevice, st));

@@ -122,6 +122,11 @@ CASES = [
     (3, 3, 64, 1, [9], [[1, 2, 3]]),
     (2, 4, 128, 0, [70, 3], [[4, 5], [0]]),                    # contiguous: nothing shared
     (1, 2, 64, 16, [0, 0], [[0, 5], [0]]),                     # empty sequences
+    (1, 8, 128, 64, [5000], [[40, 0, 3]]),
+    (2, 16, 64, 16, [200, 90, 333], [[3, 9, 0], [1, 1], [5] * 9]),  # few and many query rows
+    (1, 16, 96, 32, [100], [[0] * 40]),                        # five tiles of query rows
+    (1, 24, 32, 4, [37, 4], [[1, 2], [3, 4]]),                 # 24 heads a KV head
+    (4, 4, 128, 16, [], [[]]) if False else (4, 4, 128, 16, [3000], [[1]]),  # one long row
 ]
 
 
