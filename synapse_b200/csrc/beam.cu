@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <vector>
 
+#include "append.cuh"
 #include "internal.cuh"
 
 namespace syn {
@@ -142,140 +143,9 @@ __global__ void __launch_bounds__(256) k_reorder_tables(const __grid_constant__ 
   }
 }
 
-// ---------------------------------------------------------------------------
-// Batched append: rows of new tokens of several sequences, row t of sequence s
-// at position len[s] + t. Per head row: x' = x * w / sqrt(mean(x^2) + eps)
-// (q and k, where a norm weight is given), then the rotation of the pairs
-// (i, i + hd/2) by the position's angle; q goes to q_out, k and the raw v to
-// the position's cache row.
-// LP lanes (a power of two) take one head row, VEC pairs each; ONE: a head row
-// is one step of its lanes, kept in registers between the sum and the rotation.
-// Bound by HBM for prompts, by its launch for single tokens.
-// ---------------------------------------------------------------------------
-constexpr int AP_MAX = 256;  // sequences per launch (by value)
-constexpr int AP_THREADS = 256;
-
-struct AppendArgs {
-  const float *q, *k, *v;
-  long long ld;
-  float* q_out;
-  long long ldq;
-  int n_heads, n_kv, hd;
-  const float *qn, *kn;
-  float eps;
-  const float *cos_t, *sin_t;
-  float *kc, *vc;  // this layer
-  const int* ptab;
-  int page, maxp, max_seq;
-  const int* len;
-  const int* seq_of;  // device: one row of each sequence seq_of[row] (replaces the lists below)
-  int rows;
-  int n;
-  int seq[AP_MAX];
-  int row0[AP_MAX + 1];  // first row of each sequence; [n] = rows
-};
-
-template <int VEC> struct ApVec;
-template <> struct ApVec<4> { using T = float4; };
-template <> struct ApVec<1> { using T = float; };
-
 template <int VEC, int LP, bool ONE>
 __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_constant__ AppendArgs a) {
-  using T = typename ApVec<VEC>::T;
-  const int heads = a.n_heads + 2 * a.n_kv, half = a.hd >> 1, nv = half / VEC;
-  const long long unit = (long long)blockIdx.x * (AP_THREADS / LP) + threadIdx.x / LP;
-  const int lane = threadIdx.x % LP;
-  const int row = (int)(unit / heads), h = (int)(unit - (long long)row * heads);
-  const bool live = row < a.rows;
-  int s = 0;
-  if (live && !a.seq_of)
-    for (int step = AP_MAX / 2; step; step >>= 1)  // the last sequence that starts at or before row
-      if (s + step < a.n && a.row0[s + step] <= row) s += step;
-  const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
-  const float* src = nullptr;
-  if (live)
-    src = (is_q ? a.q + (long long)h * a.hd
-                : is_v ? a.v + (long long)(h - a.n_heads - a.n_kv) * a.hd
-                       : a.k + (long long)(h - a.n_heads) * a.hd) +
-          (long long)row * a.ld;
-  const float* w = is_q ? a.qn : is_v ? nullptr : a.kn;
-  griddep_wait();
-  T x1[1], x2[1];
-  float scale = 1.0f;
-  if (ONE && live && lane < nv) {
-    x1[0] = reinterpret_cast<const T*>(src)[lane];
-    x2[0] = reinterpret_cast<const T*>(src + half)[lane];
-  }
-  if (a.qn || a.kn) {  // (uniform: the shuffles need every lane)
-    float acc = 0.0f;
-    if (live && w)
-      for (int i = lane; i < nv; i += LP) {
-        T b1, b2;
-        if (ONE) {
-          b1 = x1[0];
-          b2 = x2[0];
-        } else {
-          b1 = reinterpret_cast<const T*>(src)[i];
-          b2 = reinterpret_cast<const T*>(src + half)[i];
-        }
-        const float* f1 = reinterpret_cast<const float*>(&b1);
-        const float* f2 = reinterpret_cast<const float*>(&b2);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) acc = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], acc));
-      }
-#pragma unroll
-    for (int o = LP / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    scale = 1.0f / sqrtf(acc / (float)a.hd + a.eps);
-  }
-  griddep_launch();
-  if (!live) return;
-  const int sq = a.seq_of ? a.seq_of[row] : a.seq[s];
-  const int pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);
-  if (pos >= a.max_seq) return;  // (a replayed graph that has run past the cache)
-  float* dst;
-  if (is_q) {
-    dst = a.q_out + (long long)row * a.ldq + (long long)h * a.hd;
-  } else {
-    size_t slot = (size_t)sq * a.max_seq + pos;
-    if (a.ptab) {
-      const int pg = a.ptab[(size_t)sq * a.maxp + pos / a.page];
-      if (pg < 0) return;
-      slot = (size_t)pg * a.page + pos % a.page;
-    }
-    dst = (is_v ? a.vc + (size_t)(h - a.n_heads - a.n_kv) * a.hd
-                : a.kc + (size_t)(h - a.n_heads) * a.hd) +
-          slot * a.n_kv * a.hd;
-  }
-  const float* ct = a.cos_t + (size_t)pos * half;
-  const float* st = a.sin_t + (size_t)pos * half;
-  for (int i = lane; i < nv; i += LP) {
-    T b1, b2;
-    if (ONE) {
-      b1 = x1[0];
-      b2 = x2[0];
-    } else {
-      b1 = reinterpret_cast<const T*>(src)[i];
-      b2 = reinterpret_cast<const T*>(src + half)[i];
-    }
-    if (!is_v) {
-      float* f1 = reinterpret_cast<float*>(&b1);
-      float* f2 = reinterpret_cast<float*>(&b2);
-#pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const int d = i * VEC + e;
-        float y1 = f1[e], y2 = f2[e];
-        if (w) {
-          y1 *= w[d] * scale;
-          y2 *= w[half + d] * scale;
-        }
-        const float c = ct[d], sn = st[d];
-        f1[e] = y1 * c - y2 * sn;
-        f2[e] = y2 * c + y1 * sn;
-      }
-    }
-    reinterpret_cast<T*>(dst)[i] = b1;
-    reinterpret_cast<T*>(dst + half)[i] = b2;
-  }
+  append_rows<VEC, LP, ONE>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -670,17 +540,12 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 }
 
 syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, size_t n,
-                                 const int32_t* seqs, const size_t* counts, cudaStream_t st,
-                                 const int* seq_of) {
-  const syn_cuda_kvcache_t* c = at.cache;
-  const size_t kvd = c->n_kv * c->hd;
-  const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st) {
   size_t done = 0;
-  for (size_t i0 = 0; i0 < n; i0 += seq_of ? n : AP_MAX) {
-    AppendArgs a;
-    a.seq_of = seq_of;
-    a.n = seq_of ? 0 : (int)std::min<size_t>(AP_MAX, n - i0);
-    size_t rows = seq_of ? n : 0;
+  for (size_t i0 = 0; i0 < n; i0 += AP_MAX) {
+    AppendArgs a = append_args(at, q_out, ldq, done);
+    a.n = (int)std::min<size_t>(AP_MAX, n - i0);
+    size_t rows = 0;
     for (int i = 0; i < a.n; i++) {
       a.seq[i] = seqs[i0 + i];
       a.row0[i] = (int)rows;
@@ -689,41 +554,14 @@ syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, s
     a.row0[a.n] = (int)rows;
     a.rows = (int)rows;
     if (rows) {
-      a.q = at.q + done * at.ld;
-      a.k = at.k + done * at.ld;
-      a.v = at.v + done * at.ld;
-      a.ld = (long long)at.ld;
-      a.q_out = q_out + done * ldq;
-      a.ldq = (long long)ldq;
-      a.n_heads = (int)at.n_heads;
-      a.n_kv = (int)c->n_kv;
-      a.hd = (int)c->hd;
-      a.qn = at.qn;
-      a.kn = at.kn;
-      a.eps = at.eps;
-      a.cos_t = at.cos_t;
-      a.sin_t = at.sin_t;
-      a.kc = c->k + at.layer * rows_per_layer * kvd;
-      a.vc = c->v + at.layer * rows_per_layer * kvd;
-      a.ptab = c->page ? c->d_ptab : nullptr;
-      a.page = (int)c->page;
-      a.maxp = (int)c->maxp;
-      a.max_seq = (int)c->max_seq;
-      a.len = c->d_len;
-      // 16-byte accesses where every head row's halves start on 16 bytes
-      const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
-                            reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out);
-      const bool vec = c->hd % 8 == 0 && low % 16 == 0 && at.ld % 4 == 0 && ldq % 4 == 0;
-      const int lanes = (int)(c->hd / 2) / (vec ? 4 : 1);
-      void (*kern)(const AppendArgs) = nullptr;
-      int lp;
-      if (vec && lanes <= 4) kern = k_append_batch<4, 4, true>, lp = 4;
-      else if (vec && lanes <= 8) kern = k_append_batch<4, 8, true>, lp = 8;
-      else if (vec && lanes <= 16) kern = k_append_batch<4, 16, true>, lp = 16;
-      else if (vec && lanes <= 32) kern = k_append_batch<4, 32, true>, lp = 32;
-      else if (vec) kern = k_append_batch<4, 32, false>, lp = 32;
-      else kern = k_append_batch<1, 32, false>, lp = 32;
-      const size_t units = rows * (at.n_heads + 2 * c->n_kv), per = AP_THREADS / lp;
+      const AppendShape sh = append_shape(a);
+      void (*kern)(const AppendArgs) = !sh.vec      ? k_append_batch<1, 32, false>
+                                       : !sh.one    ? k_append_batch<4, 32, false>
+                                       : sh.lp == 4 ? k_append_batch<4, 4, true>
+                                       : sh.lp == 8 ? k_append_batch<4, 8, true>
+                                       : sh.lp == 16 ? k_append_batch<4, 16, true>
+                                                     : k_append_batch<4, 32, true>;
+      const size_t units = rows * (a.n_heads + 2 * a.n_kv), per = AP_THREADS / sh.lp;
       const size_t blocks = (units + per - 1) / per;
       if (blocks > 0x7FFFFFFF) return SYN_ERR_UNSUPPORTED;
       syn_status_t s = launched(launch_pdl(kern, dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a),

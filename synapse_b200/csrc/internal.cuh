@@ -290,11 +290,9 @@ syn_status_t launch_kv_set(syn_cuda_kvcache_t* c, size_t seq, int value, int add
 
 // ---- beam search (beam.cu) ----
 // New rows of n sequences (counts[i] rows of seqs[i], host arrays, pages
-// reserved) normalised, rotated and appended; q rows to q_out. With seq_of (a
-// device array, read when the kernel runs) one row of each of its n sequences.
+// reserved) normalised, rotated and appended; q rows to q_out.
 syn_status_t launch_append_batch(const AttnArgs& a, float* q_out, size_t ldq, size_t n,
-                                 const int32_t* seqs, const size_t* counts, cudaStream_t st,
-                                 const int* seq_of = nullptr);
+                                 const int32_t* seqs, const size_t* counts, cudaStream_t st);
 // Groups of `beams` sequences (seqs and lens on the host, parents on the
 // device) take over their parents' contexts; at most 256 sequences.
 syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,

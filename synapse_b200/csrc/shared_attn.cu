@@ -9,18 +9,19 @@
 // The shared prefix of a group is one part set, computed once for all its
 // rows, so its K and V cross HBM once per step instead of once per row; each
 // row's own positions are the other. Kernels of one call:
-//   k_append_batch (beam.cu)  the new rows normalised, rotated and appended
-//   k_prefix                  the shared prefixes of many query rows, on the
-//                             tensor cores and a fixed schedule
-//   k_span                    each row's own positions, and the shared prefixes
-//                             of few query rows
-//   k_join                    the parts of each query row
+//   k_begin   the new rows normalised, rotated and appended; k_span's shares
+//   k_prefix  the shared prefixes of many query rows, on the tensor cores and a
+//             schedule made on the host
+//   k_span    each row's own positions, and the shared prefixes of few query
+//             rows
+//   k_join    the parts of each query row
 #include <math.h>
 
 #include <algorithm>
 #include <new>
 #include <vector>
 
+#include "append.cuh"
 #include "internal.cuh"
 #include "tcgen05.cuh"
 
@@ -42,8 +43,8 @@ struct syn_cuda_decode_plan_s {
   float* po = nullptr;       // partial o, prefix then suffix
   float2* pml = nullptr;     // partial (m, l)
   size_t part_rows = 0;      // records of po / pml
-  int* starts = nullptr;     // k_span's first tile of each unit, for k_join
-  int units = 0, jobs = 0;   // k_span's units; k_prefix's jobs
+  void* shares = nullptr;    // k_span's shares and jobs (Share, SpanJob), written by k_begin
+  int units = 0, span_jobs = 0, jobs = 0;  // k_span's units and jobs; k_prefix's jobs
 };
 
 namespace syn {
@@ -56,7 +57,6 @@ constexpr int SP_V = 8;        // most query vectors of a k_span job
 constexpr int SP_FEW = 16;     // a group of at most so many query rows per KV head goes to k_span
 constexpr int ROWS_MAX = 512;  // rows of a plan
 constexpr int UNITS_MAX = ROWS_MAX + ROWS_MAX / 2;
-constexpr int PARTS_MAX = 1536;  // most parts of a query row: a k_span warp's each, a k_prefix CTA's each
 
 struct Job {      // prefix work of one (group, tile of query rows, KV head)
   int row0;       // first row of the group
@@ -75,6 +75,19 @@ struct Item {     // a CTA's share of a job: key tiles t0 .. t1, partial records
 // up to 8 query vectors: n_kv * nch jobs, the first job0.
 struct Unit {
   int row0, n, pre, job0, nch;
+};
+
+// A k_span warp's share: n tiles from tile k0 of a job on.
+struct Share {
+  int job, k0, n, pad;
+};
+// A k_span job: query vectors (row, g), (row, g + 1), ..., where g counts the heads of
+// KV head kvh, over the positions r0 .. r1 of a sequence; its tiles; the warps that
+// take part.
+struct SpanJob {
+  int seq, kvh, nq, row;
+  int g, r0, r1, nt;
+  int prefix, w0, nw, pad;
 };
 
 // Offsets (ints) of the arrays in the plan's metadata block.
@@ -105,19 +118,15 @@ struct SharedArgs {
   float* po;
   float2* pml;
   int rows, units, span0;  // rows; k_span's units (the last `rows` are theirs) and its first record
-  int warps;               // of k_span
-  int* starts;
+  int warps, span_jobs;    // of k_span
+  int after_prefix;        // k_prefix runs before it
+  struct Share* shares;
+  struct SpanJob* sjobs;
   float* out;
   long long ldo;
   float scale;
   int* err;
 };
-
-__device__ __forceinline__ long long row_at(const SharedArgs& a, int sq, int pos) {
-  if (!a.ptab) return (long long)sq * a.max_seq + pos;
-  const int pg = a.ptab[(long long)sq * a.maxp + pos / a.page];
-  return pg < 0 ? -1 : (long long)pg * a.page + pos % a.page;
-}
 
 // ---------------------------------------------------------------------------
 // Shared prefixes on the tensor cores. A job is 128 query rows (tensor-memory
@@ -215,6 +224,9 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   f32x2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
+}
+__device__ __forceinline__ void acc2(f32x2& acc, f32x2 a, f32x2 b) {  // acc += a b
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 // A pair -> packed fp16 hi and lo
 __device__ __forceinline__ void split2(f32x2 v, uint32_t& hi, uint32_t& lo) {
@@ -333,6 +345,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     return __all_sync(0xffffffffu, done) != 0;
   };
   griddep_wait();
+  griddep_launch();
   const int* start = a.meta + a.mv.start() + blockIdx.x;
   const int i0 = start[0], i1 = start[1];
   int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
@@ -693,7 +706,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   }
   tc_fence_before();
   __syncthreads();
-  griddep_launch();
   if (*failed && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
   if (warp == PX_MMA_WARP) {
     tc_fence_after();
@@ -725,10 +737,6 @@ __device__ __forceinline__ float redux_max(float x) {
   return y;
 }
 
-struct SpanJob {
-  int row0, n, pre, seq, kvh, ch, r0, r1, nq;
-};
-
 // Positions of unit u: [lo, hi)
 __device__ __forceinline__ int2 unit_range(const SharedArgs& a, const Unit& u) {
   const int* seq = a.meta + a.mv.seq();
@@ -748,52 +756,153 @@ __device__ __forceinline__ int2 unit_range(const SharedArgs& a, const Unit& u) {
   return make_int2(max(u.pre, a.window ? L - a.window : 0), L);
 }
 
-// Tiles [k0, k1) of a job, by one warp; the record of each query vector.
-template <int LPR, int NQ>
+// Deals the tiles of all units to k_span's warps: tile t of T is warp w's where
+// floor(w T / W) <= t < floor((w + 1) T / W), so of tile t the warp is
+// ceil((t + 1) W / T) - 1. Every block finds the units' first tiles; the shares and
+// jobs are divided among the blocks' threads.
+__device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int blocks) {
+  __shared__ int starts[UNITS_MAX + 1], lows[UNITS_MAX], highs[UNITS_MAX], sums[AP_THREADS / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
+  const int per = (a.units + AP_THREADS - 1) / AP_THREADS;
+  const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
+  int sum = 0;
+  for (int u = u0; u < u1; u++) {
+    const Unit x = units[u];
+    const int2 r = unit_range(a, x);
+    const int t = (max(0, r.y - r.x) + SP_T - 1) / SP_T * a.n_kv * x.nch;
+    starts[u] = t;
+    lows[u] = r.x;
+    highs[u] = r.y;
+    sum += t;
+  }
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  int base = inc - sum;
+  for (int w = 0; w < warp; w++) base += sums[w];
+  for (int u = u0; u < u1; u++) {
+    const int t = starts[u];
+    starts[u] = base;
+    base += t;
+  }
+  if (u1 == a.units) starts[a.units] = base;
+  __syncthreads();
+  const int total = starts[a.units], warps = min(a.warps, total);
+  // the last unit whose first tile (or job) is at or before x; an empty one starts where the next does
+  auto find = [&](int x, auto&& at) {
+    int lo = 0, hi = a.units;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (at(mid) <= x) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  for (int w = block * AP_THREADS + tid; w < a.warps; w += blocks * AP_THREADS) {
+    Share s{0, 0, 0, 0};
+    if (w < warps) {
+      const int t0 = (int)((long long)w * total / warps), t1 = (int)((long long)(w + 1) * total / warps);
+      const int u = find(t0, [&](int i) { return starts[i]; });
+      const Unit x = units[u];
+      const int nt = (starts[u + 1] - starts[u]) / (a.n_kv * x.nch), r = t0 - starts[u];
+      s = Share{x.job0 + r / nt, r % nt, t1 - t0, 0};
+    }
+    a.shares[w] = s;
+  }
+  for (int j = block * AP_THREADS + tid; j < a.span_jobs; j += blocks * AP_THREADS) {
+    const int u = find(j, [&](int i) { return units[i].job0; });
+    const Unit x = units[u];
+    const int jl = j - x.job0, kvh = jl / x.nch, v0 = (jl - kvh * x.nch) * SP_V;
+    SpanJob s;
+    s.seq = a.meta[a.mv.seq() + x.row0];
+    s.kvh = kvh;
+    s.nq = min(SP_V, (x.n ? x.n * a.G : a.G) - v0);
+    s.row = x.row0 + (x.n ? v0 / a.G : 0);
+    s.g = x.n ? v0 % a.G : v0;
+    s.r0 = lows[u];
+    s.r1 = highs[u];
+    s.nt = (starts[u + 1] - starts[u]) / (a.n_kv * x.nch);
+    s.prefix = x.n > 0;
+    s.w0 = s.nw = s.pad = 0;
+    if (s.nt) {
+      const long long t0 = starts[u] + (long long)jl * s.nt, t1 = t0 + s.nt;
+      s.w0 = (int)(((t0 + 1) * warps - 1) / total);
+      s.nw = (int)((t1 * warps - 1) / total) - s.w0 + 1;
+    }
+    a.sjobs[j] = s;
+  }
+}
+
+// The append, and in the last `deal` blocks the shares.
+template <int VEC, int LP, bool ONE>
+__global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ AppendArgs p,
+                                                      const __grid_constant__ SharedArgs a, int deal) {
+  const int block = (int)blockIdx.x - ((int)gridDim.x - deal);
+  if (block < 0) {
+    append_rows<VEC, LP, ONE>(p);
+  } else {
+    griddep_wait();
+    griddep_launch();
+    deal_shares(a, block, deal);
+  }
+}
+
+// Tiles [k0, k1) of a job, by one warp; the record of each query vector. HD: the
+// head dim where it is 64 or 128, else 0.
+template <int LPR, int HD, int NQ>
 __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job, int k0, int k1, size_t rec,
                                          uint8_t* ring, float* qs, float2* ps, uint64_t* bars, uint32_t& used) {
   constexpr int SUBS = 32 / LPR;
-  const int lane = threadIdx.x & 31, hd = a.hd, stride = hd * 4 + 16, slot_bytes = SP_T * stride;
+  const int lane = threadIdx.x & 31, hd = HD ? HD : a.hd, stride = hd * 4 + 16, slot_bytes = SP_T * stride;
   const int sub = lane / LPR, l4 = (lane % LPR) * 4;
-  // queries, times scale * log2(e)
-  const float qscale = a.scale * 1.4426950408889634f;
-  int low[NQ];
-#pragma unroll
-  for (int v = 0; v < NQ; v++) {
-    const int i = job.ch * SP_V + v;
-    const int row = job.row0 + (job.n ? i / a.G : 0), head = job.kvh * a.G + (job.n ? i % a.G : i);
-    low[v] = 0;
-    if (v < job.nq && job.n && a.window) low[v] = a.len[a.meta[a.mv.seq() + row]] + 1 - a.window;
-    for (int d = lane * 4; d < hd; d += 128) {
-      float4 f = make_float4(0, 0, 0, 0);
-      if (v < job.nq) f = *reinterpret_cast<const float4*>(a.q + ((size_t)row * a.n_heads + head) * hd + d);
-      *reinterpret_cast<float4*>(qs + v * hd + d) =
-          make_float4(f.x * qscale, f.y * qscale, f.z * qscale, f.w * qscale);
-    }
-  }
   // the ring: K and V of a tile in turn; `used` counts the fills of all jobs
-  const uint32_t first = used;
   const int nt = k1 - k0;
-  long long at = -1;  // cache row of this lane's key of the tile asked for last
-  auto ask = [&](int k) {
-    const int pos = job.r0 + (k0 + k) * SP_T + lane;
-    at = pos < job.r1 ? row_at(a, job.seq, pos) : -1;
+  // the place of this lane's key in the tile that is asked for next
+  int pos = job.r0 + k0 * SP_T + lane, col = a.ptab ? pos / a.page : 0, off = pos - col * a.page;
+  const int dcol = a.ptab ? SP_T / a.page : 0, doff = SP_T - dcol * a.page;
+  long long at = -1;  // offset of its row in the cache, -1 = none
+  auto ask = [&]() {
+    long long row = -1;
+    if (pos < job.r1) {
+      if (a.ptab) {
+        const int pg = __ldg(a.ptab + (size_t)job.seq * a.maxp + col);
+        if (pg >= 0) row = (long long)pg * a.page + off;
+      } else {
+        row = (long long)job.seq * a.max_seq + pos;
+      }
+    }
+    at = row < 0 ? -1 : (row * a.n_kv + job.kvh) * hd;
+    pos += SP_T;
+    col += dcol;
+    off += doff;
+    if (a.ptab && off >= a.page) {
+      off -= a.page;
+      col++;
+    }
   };
-  auto fill = [&](int h, const float* cache) {  // half tile h (its K or V) into its slot
-    const uint32_t u = first + h;
-    uint64_t* bar = bars + u % SP_SLOTS;
-    uint8_t* dst = ring + (u % SP_SLOTS) * slot_bytes + lane * stride;
+  uint32_t fslot = used % SP_SLOTS, rslot = fslot, rpar = (used / SP_SLOTS) & 1;
+  auto fill = [&](const float* cache) {  // the next half tile (K or V) into the next slot
+    uint64_t* bar = bars + fslot;
     const uint32_t rows = __popc(__ballot_sync(0xffffffffu, at >= 0));
     fence_async_smem();  // (the slot's last readers are past; order their accesses before the copy's)
     if (lane == 0) mbar_expect_tx(bar, rows * hd * 4);
     __syncwarp();
-    if (at >= 0) bulk_g2s(dst, cache + ((size_t)at * a.n_kv + job.kvh) * hd, hd * 4, bar);
-    used++;
+    if (at >= 0) bulk_g2s(ring + fslot * slot_bytes + lane * stride, cache + at, hd * 4, bar);
+    fslot = fslot == SP_SLOTS - 1 ? 0 : fslot + 1;
   };
-  auto ready = [&](int h) {
-    const uint32_t u = first + h;
-    bool ok = mbar_try_wait(bars + u % SP_SLOTS, (u / SP_SLOTS) & 1);
-    if (!ok) ok = mbar_wait_bounded(bars + u % SP_SLOTS, (u / SP_SLOTS) & 1);
+  const uint8_t* tile = nullptr;
+  auto ready = [&]() {  // the next half tile is in `tile`
+    bool ok = mbar_try_wait(bars + rslot, rpar);
+    if (!ok) ok = mbar_wait_bounded(bars + rslot, rpar);
+    tile = ring + rslot * slot_bytes;
+    rpar ^= rslot == SP_SLOTS - 1;
+    rslot = rslot == SP_SLOTS - 1 ? 0 : rslot + 1;
     return __all_sync(0xffffffffu, ok) != 0;
   };
   float m[NQ], l[NQ];
@@ -804,41 +913,65 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
     l[v] = 0.0f;
     o[v][0] = o[v][1] = 0;
   }
-  ask(0);
-  fill(0, a.kc);
-  fill(1, a.vc);
+  ask();
+  fill(a.kc);
+  fill(a.vc);
   if (nt > 1) {
-    ask(1);
-    fill(2, a.kc);
+    ask();
+    fill(a.kc);
+  }
+  used += 2 * nt;
+  // queries, times scale * log2(e)
+  const float qscale = a.scale * 1.4426950408889634f;
+  int low[NQ];
+  {
+    int row = job.row, g = job.g;
+#pragma unroll
+    for (int v = 0; v < NQ; v++) {
+      low[v] = 0;
+      const bool live = v < job.nq;
+      if (live && job.prefix && a.window) low[v] = a.len[a.meta[a.mv.seq() + row]] + 1 - a.window;
+      const float* q = a.q + ((size_t)row * a.n_heads + job.kvh * a.G + g) * hd;
+      for (int d = lane * 4; d < hd; d += 128) {
+        float4 f = make_float4(0, 0, 0, 0);
+        if (live) f = *reinterpret_cast<const float4*>(q + d);
+        *reinterpret_cast<float4*>(qs + v * hd + d) =
+            make_float4(f.x * qscale, f.y * qscale, f.z * qscale, f.w * qscale);
+      }
+      if (++g == a.G) {
+        g = 0;
+        row++;
+      }
+    }
   }
   __syncwarp();
   for (int k = 0; k < nt; k++) {
     const int key = job.r0 + (k0 + k) * SP_T + lane;
     const int nk = min(SP_T, job.r1 - job.r0 - (k0 + k) * SP_T);
-    if (!ready(2 * k)) return false;
-    f32x2 acc[NQ];
+    if (!ready()) return false;
+    f32x2 acc[NQ][2];
 #pragma unroll
-    for (int v = 0; v < NQ; v++) acc[v] = 0;
-    const uint8_t* kr = ring + ((first + 2 * k) % SP_SLOTS) * slot_bytes + lane * stride;
+    for (int v = 0; v < NQ; v++) acc[v][0] = acc[v][1] = 0;
+    const uint8_t* kr = tile + lane * stride;
 #pragma unroll 4
     for (int d = 0; d < hd; d += 4) {
       const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kr + d * 4);
 #pragma unroll
       for (int v = 0; v < NQ; v++) {
         const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(qs + v * hd + d);
-        acc[v] = fma2(x.x, q.x, acc[v]);
-        acc[v] = fma2(x.y, q.y, acc[v]);
+        acc2(acc[v][0], x.x, q.x);
+        acc2(acc[v][1], x.y, q.y);
       }
     }
     __syncwarp();  // (all have read the slot)
-    if (k + 1 < nt) fill(2 * k + 3, a.vc);
+    if (k + 1 < nt) fill(a.vc);
     // softmax weights, twice each for the packed sums
     float corr[NQ];
     bool grown = false;
 #pragma unroll
     for (int v = 0; v < NQ; v++) {
       float x, y;
-      unpk(acc[v], x, y);
+      unpk(add2(acc[v][0], acc[v][1]), x, y);
       x = lane < nk && key >= low[v] ? x + y : -INFINITY;
       const float mx = fmaxf(m[v], redux_max(x));
       corr[v] = m[v] == -INFINITY ? 0.0f : ex2(m[v] - mx);
@@ -856,24 +989,23 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
       }
     }
     __syncwarp();
-    if (!ready(2 * k + 1)) return false;
-    const uint8_t* vr = ring + ((first + 2 * k + 1) % SP_SLOTS) * slot_bytes;
+    if (!ready()) return false;
     if (l4 < hd) {
 #pragma unroll 4
       for (int j = sub; j < nk; j += SUBS) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vr + j * stride + l4 * 4);
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(tile + j * stride + l4 * 4);
         const f32x2* p = reinterpret_cast<const f32x2*>(ps + j * NQ);
 #pragma unroll
         for (int v = 0; v < NQ; v++) {
-          o[v][0] = fma2(p[v], x.x, o[v][0]);
-          o[v][1] = fma2(p[v], x.y, o[v][1]);
+          acc2(o[v][0], p[v], x.x);
+          acc2(o[v][1], p[v], x.y);
         }
       }
     }
     __syncwarp();
     if (k + 2 < nt) {
-      ask(k + 2);
-      fill(2 * k + 4, a.kc);
+      ask();
+      fill(a.kc);
     }
   }
 #pragma unroll
@@ -896,90 +1028,47 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
   return true;
 }
 
-template <int LPR>
+template <int LPR, int HD>
 __global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
   extern __shared__ __align__(16) uint8_t sraw[];
   __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_SLOTS];
-  __shared__ int sums[SP_WARPS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot_bytes = SP_T * (a.hd * 4 + 16), per_warp = SP_SLOTS * slot_bytes + SP_V * a.hd * 4 + SP_T * SP_V * 8;
   uint8_t* ring = sraw + warp * per_warp;
   float* qs = reinterpret_cast<float*>(ring + SP_SLOTS * slot_bytes);
   float2* ps = reinterpret_cast<float2*>(qs + SP_V * a.hd);
-  int* starts = reinterpret_cast<int*>(sraw + SP_WARPS * per_warp);  // [units + 1]
   if (lane < SP_SLOTS) mbar_init(&bars[warp][lane], 1);
   mbar_fence_init();
-  griddep_wait();
-  const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
-  {  // first tile of each unit
-    const int per = (a.units + SP_WARPS * 32 - 1) / (SP_WARPS * 32);
-    const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
-    int sum = 0;
-    for (int u = u0; u < u1; u++) {
-      const Unit x = units[u];
-      const int2 r = unit_range(a, x);
-      const int t = (max(0, r.y - r.x) + SP_T - 1) / SP_T * a.n_kv * x.nch;
-      starts[u] = t;
-      sum += t;
-    }
-    int inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
-    }
-    if (lane == 31) sums[warp] = inc;
-    __syncthreads();
-    int base = inc - sum;
-    for (int w = 0; w < warp; w++) base += sums[w];
-    for (int u = u0; u < u1; u++) {
-      const int t = starts[u];
-      starts[u] = base;
-      base += t;
-    }
-    if (u1 == a.units) starts[a.units] = base;
-    __syncthreads();
-    if (blockIdx.x == 0)
-      for (int u = tid; u <= a.units; u += SP_WARPS * 32) a.starts[u] = starts[u];
-  }
-  const long long total = starts[a.units];
-  const int gw = warp * gridDim.x + blockIdx.x;
-  const long long warps = min((long long)a.warps, total);  // that have a share
-  long long t = gw < warps ? gw * total / warps : 0;
-  const long long t1 = gw < warps ? (gw + 1) * total / warps : 0;
+  __syncwarp();
+  // Behind k_prefix this kernel needs nothing of it: k_begin is complete where k_prefix has
+  // let it begin, and so it runs on every SM that k_prefix has left.
+  if (!a.after_prefix) griddep_wait();
+  griddep_launch();
+  const int gw = warp * gridDim.x + blockIdx.x;  // (neighbouring shares on different SMs)
+  const int4 sh = __ldcg(reinterpret_cast<const int4*>(a.shares) + gw);
+  int j = sh.x, k0 = sh.y, left = sh.z;
   uint32_t used = 0;
   bool ok = true;
-  while (t < t1 && ok) {
-    int lo = 0, hi = a.units;  // the last unit that starts at or before t and is not empty
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (starts[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    const Unit u = units[lo];
-    const int jobs = a.n_kv * u.nch, nt = (starts[lo + 1] - starts[lo]) / jobs, r = (int)(t - starts[lo]);
-    const int jl = r / nt, k0 = r - jl * nt;
-    SpanJob job;
-    job.row0 = u.row0;
-    job.n = u.n;
-    job.pre = u.pre;
-    job.seq = a.meta[a.mv.seq() + u.row0];
-    job.kvh = jl / u.nch;
-    job.ch = jl - job.kvh * u.nch;
-    job.nq = min(SP_V, (u.n ? u.n * a.G : a.G) - job.ch * SP_V);
-    const int2 range = unit_range(a, u);
-    job.r0 = range.x;
-    job.r1 = range.y;
-    const int k1 = (int)min((long long)nt, k0 + t1 - t);
-    const size_t rec = a.span0 + (size_t)(gw + u.job0 + jl) * SP_V;
-    ok = job.nq > 4   ? span_job<LPR, 8>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-         : job.nq > 2 ? span_job<LPR, 4>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-         : job.nq > 1 ? span_job<LPR, 2>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-                      : span_job<LPR, 1>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used);
-    t += k1 - k0;
+  while (left > 0 && ok) {
+    union {
+      int4 v[3];
+      SpanJob job;
+    };
+#pragma unroll
+    for (int i = 0; i < 3; i++) v[i] = __ldcg(reinterpret_cast<const int4*>(a.sjobs + j) + i);
+    const int k1 = min(job.nt, k0 + left);
+    const size_t rec = a.span0 + (size_t)(gw + j) * SP_V;
+    if (k1 > k0)
+      ok = job.nq > 4   ? span_job<LPR, HD, 8>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+           : job.nq > 2 ? span_job<LPR, HD, 4>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+           : job.nq > 1 ? span_job<LPR, HD, 2>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
+                        : span_job<LPR, HD, 1>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used);
+    left -= k1 - k0;
+    k0 = 0;
+    j++;
   }
   if (!ok && lane == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
-  griddep_launch();
+  if (a.after_prefix) griddep_wait();  // (k_join waits for this kernel's end, and so for k_prefix's)
 }
 
 // ---------------------------------------------------------------------------
@@ -989,76 +1078,77 @@ __global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
 constexpr int JN_WARPS = 4;
 
 __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
-  __shared__ float fac[JN_WARPS][PARTS_MAX];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
   const int i = blockIdx.x * JN_WARPS + warp, b = i / a.n_heads, head = i - b * a.n_heads;
-  griddep_wait();
-  if (b >= a.rows) return;
+  if (b >= a.rows) {
+    griddep_wait();
+    return;
+  }
   const int kvh = head / a.G, g = head - kvh * a.G;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
-  const long long total = __ldcg(a.starts + a.units), warps = min((long long)a.warps, total);
-  // records first + c * step, c < n, of a k_span unit's job and vector
+  // Records first + c * step, c < n. (The plan and k_begin's jobs may be read before the
+  // wait: k_span begins, and lets this kernel begin, after them.)
   struct Parts { size_t first; int n, step; };
   auto span_parts = [&](int u, int idx) {
     const Unit x = units[u];
-    const int s = __ldcg(a.starts + u), e = __ldcg(a.starts + u + 1), nt = (e - s) / (a.n_kv * x.nch);
-    const int jl = kvh * x.nch + idx / SP_V;
-    Parts p{0, 0, SP_V};
-    if (nt) {  // the warps whose shares meet its tiles
-      const long long t0 = s + (long long)jl * nt, t1 = t0 + nt;
-      const int w0 = (int)(((t0 + 1) * warps - 1) / total), w1 = (int)((t1 * warps - 1) / total);
-      p.first = a.span0 + (size_t)(w0 + x.job0 + jl) * SP_V + idx % SP_V;
-      p.n = w1 - w0 + 1;
-    }
-    return p;
+    const int j = x.job0 + kvh * x.nch + idx / SP_V;
+    const int4 s = __ldcg(reinterpret_cast<const int4*>(a.sjobs + j) + 2);  // prefix, w0, nw
+    return Parts{a.span0 + (size_t)(s.y + j) * SP_V + idx % SP_V, s.z, SP_V};
   };
+  const int pu = a.meta[a.mv.unit_of() + b], job0 = a.meta[a.mv.job_of() + b];
   const int local = a.meta[a.mv.local() + b] * a.G + g;
   const Parts own = span_parts(a.units - a.rows + b, g);
   Parts pre{0, 0, 0};
-  const int pu = a.meta[a.mv.unit_of() + b], job0 = a.meta[a.mv.job_of() + b];
   if (pu >= 0) {
     pre = span_parts(pu, local);
   } else if (job0 >= 0) {
     const Job job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[job0 + local / PM * a.n_kv + kvh];
     pre = Parts{(size_t)(job.part0 + local - job.m0), job.splits, job.m};
   }
-  const int n = min(PARTS_MAX, own.n + pre.n);
+  const int n = own.n + pre.n;
   auto rec = [&](int c) {
     return c < own.n ? own.first + (size_t)c * own.step : pre.first + (size_t)(c - own.n) * pre.step;
   };
-  float M = -INFINITY;
-  for (int c = lane; c < n; c += 32) {
-    const float2 ml = __ldcg(&a.pml[rec(c)]);
-    fac[warp][c] = ml.x;
-    M = fmaxf(M, ml.x);
-  }
+  griddep_wait();
+  const float2 none = make_float2(-INFINITY, 0.0f);
+  const float2 mine = lane < n ? __ldcg(&a.pml[rec(lane)]) : none;
+  float M = mine.x;
+  for (int c = 32 + lane; c < n; c += 32) M = fmaxf(M, __ldcg(&a.pml[rec(c)]).x);
   M = warp_max(M);
+  float4 o = make_float4(0, 0, 0, 0);
   float sum = 0.0f;
-  for (int c = lane; c < n; c += 32) {
-    const float f = fac[warp][c] == -INFINITY ? 0.0f : ex2(fac[warp][c] - M);
-    fac[warp][c] = f;
-    sum += f * __ldcg(&a.pml[rec(c)]).y;
+  const bool act = lane * 4 < hd;
+  for (int c0 = 0; c0 < n; c0 += 32) {
+    const float2 ml = c0 == 0 ? mine : c0 + lane < n ? __ldcg(&a.pml[rec(c0 + lane)]) : none;
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+    sum = fmaf(f, ml.y, sum);
+    const int k = min(32, n - c0);
+    for (int c = 0; c < k; c += 8) {  // eight records' loads in flight
+      float4 x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[e] = make_float4(0, 0, 0, 0);
+        if (act && c + e < k) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c0 + c + e) * hd) + lane);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float fc = __shfl_sync(0xffffffffu, f, (c + e) & 31);
+        o.x = fmaf(x[e].x, fc, o.x);
+        o.y = fmaf(x[e].y, fc, o.y);
+        o.z = fmaf(x[e].z, fc, o.z);
+        o.w = fmaf(x[e].w, fc, o.w);
+      }
+    }
   }
+  griddep_launch();
   sum = warp_sum(sum);
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f * sum;  // (NaN stays)
-  __syncwarp();
-  griddep_launch();
-  float* orow = a.out + (long long)b * a.ldo + (long long)head * hd;
-  for (int d = lane * 4; d < hd; d += 128) {
-    float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-    for (int c = 0; c < n; c++) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd + d));
-      const float f = fac[warp][c];
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
-      o.z = fmaf(x.z, f, o.z);
-      o.w = fmaf(x.w, f, o.w);
-    }
-    orow[d] = o.x * inv;
-    orow[d + 1] = o.y * inv;
-    orow[d + 2] = o.z * inv;
-    orow[d + 3] = o.w * inv;
+  if (act) {
+    float* orow = a.out + (long long)b * a.ldo + (long long)head * hd + lane * 4;
+    orow[0] = o.x * inv;
+    orow[1] = o.y * inv;
+    orow[2] = o.z * inv;
+    orow[3] = o.w * inv;
   }
 }
 
@@ -1087,7 +1177,7 @@ Meta meta_of(const syn_cuda_decode_plan_t* p) {
 
 // k_span: shared memory, and CTAs on an SM
 size_t span_smem(size_t hd) {
-  return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 8) + (UNITS_MAX + 1) * 4;
+  return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 8);
 }
 int span_ctas(size_t hd) { return span_smem(hd) > 112 * 1024 ? 1 : 2; }
 // Most k_span jobs of a batch
@@ -1101,9 +1191,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
                                 cudaStream_t st) {
   syn_cuda_kvcache_t* c = p->cache;
   const size_t kvd = c->n_kv * c->hd, qd = p->n_heads * c->hd;
-  syn_status_t s = launch_append_batch(at, p->q, qd, p->rows, nullptr, nullptr, st,
-                                       p->meta + meta_of(p).seq());
-  if (s) return s;
+  syn_status_t s;
   const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
   SharedArgs a;
   a.q = p->q;
@@ -1127,11 +1215,28 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.units = p->units;
   a.warps = span_ctas(c->hd) * p->sms * SP_WARPS;
   a.span0 = (int)(p->part_rows - (a.warps + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
-  a.starts = p->starts;
+  a.span_jobs = p->span_jobs;
+  a.after_prefix = p->jobs > 0;
+  a.shares = static_cast<Share*>(p->shares);
+  a.sjobs = reinterpret_cast<SpanJob*>(a.shares + a.warps);
   a.out = at.out;
   a.ldo = (long long)at.ldo;
   a.scale = 1.0f / sqrtf((float)c->hd);
   a.err = err;
+  {
+    AppendArgs ap = append_args(at, p->q, qd, 0);
+    ap.seq_of = p->meta + a.mv.seq();
+    ap.rows = a.rows;
+    const AppendShape sh = append_shape(ap);
+    void (*kern)(const AppendArgs, const SharedArgs, int) = !sh.vec       ? k_begin<1, 32, false>
+                                                            : sh.lp == 4  ? k_begin<4, 4, true>
+                                                            : sh.lp == 8  ? k_begin<4, 8, true>
+                                                                          : k_begin<4, 16, true>;
+    const size_t per = AP_THREADS / sh.lp, blocks = (p->rows * (p->n_heads + 2 * c->n_kv) + per - 1) / per;
+    const int deal = (std::max(a.warps, a.span_jobs) + AP_THREADS - 1) / AP_THREADS;
+    s = launched(launch_pdl(kern, dim3((unsigned)(blocks + deal)), dim3(AP_THREADS), 0, st, ap, a, deal), "k_begin");
+    if (s) return s;
+  }
   if (p->jobs) {
     const bool w = c->hd > 64;
     void (*kern)(const SharedArgs) = w ? k_prefix<128> : k_prefix<64>;
@@ -1140,7 +1245,11 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
     s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), smem, st, a), "k_prefix");
     if (s) return s;
   }
-  void (*span)(const SharedArgs) = c->hd <= 32 ? k_span<8> : c->hd <= 64 ? k_span<16> : k_span<32>;
+  void (*span)(const SharedArgs) = c->hd == 128  ? k_span<32, 128>
+                                   : c->hd == 64 ? k_span<16, 64>
+                                   : c->hd <= 32 ? k_span<8, 0>
+                                   : c->hd < 64  ? k_span<16, 0>
+                                                 : k_span<32, 0>;
   if ((s = more_smem((const void*)span, span_smem(c->hd)))) return s;
   s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->sms), dim3(SP_WARPS * 32), span_smem(c->hd), st, a),
                "k_span");
@@ -1171,10 +1280,6 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   p->device = c->device;
   p->sms = num_sms();
   p->n_heads = n_heads;
-  if (p->sms * (1 + SP_WARPS * span_ctas(c->hd)) > PARTS_MAX) {
-    delete p;
-    return SYN_ERR_UNSUPPORTED;
-  }
   const Meta mv = meta_of(p);
   p->meta_ints = mv.total();
   // prefix records: a job's rows for each CTA that shares in it, at most one job's rows more
@@ -1192,7 +1297,9 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   if (e == cudaSuccess) e = cudaMallocHost(&p->meta_h, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->pml, p->part_rows * sizeof(float2));
-  if (e == cudaSuccess) e = cudaMalloc(&p->starts, (UNITS_MAX + 1) * sizeof(int));
+  if (e == cudaSuccess)
+    e = cudaMalloc(&p->shares, p->sms * span_ctas(c->hd) * SP_WARPS * sizeof(Share) +
+                                   span_jobs(c->batch, c->n_kv, G) * sizeof(SpanJob));
   if (e == cudaSuccess) e = cudaMemset(p->meta, 0, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&p->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -1214,7 +1321,7 @@ syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
   if (p->meta_h) cudaFreeHost(p->meta_h);
   cudaFree(p->po);
   cudaFree(p->pml);
-  cudaFree(p->starts);
+  cudaFree(p->shares);
   if (p->copied) cudaEventDestroy(p->copied);
   delete p;
   return SYN_OK;
@@ -1345,6 +1452,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     uj += (int)c->n_kv * nch;
   }
   p->units = nu;
+  p->span_jobs = uj;
   p->jobs = nj;
   p->rows = rows;
   p->groups = n_groups;
