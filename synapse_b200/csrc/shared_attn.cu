@@ -54,7 +54,7 @@ constexpr int PT = 64;         // keys of a prefix tile
 constexpr int PM = 128;        // query rows of a prefix job
 constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: warps of a CTA, keys of a tile
 constexpr int SP_V = 8;        // most query vectors of a k_span job
-constexpr int SP_FEW = 16;     // a group of at most so many query rows per KV head goes to k_span
+constexpr int SP_FEW = 8;      // a group of at most so many query rows per KV head goes to k_span
 constexpr int ROWS_MAX = 512;  // rows of a plan
 constexpr int UNITS_MAX = ROWS_MAX + ROWS_MAX / 2;
 
@@ -67,7 +67,9 @@ struct Job {      // prefix work of one (group, tile of query rows, KV head)
   int splits;
 };
 struct Item {     // a CTA's share of a job: key tiles t0 .. t1, partial records from part
-  int job, t0, t1, part;
+  int row0, m0, m, kvh;
+  int len, t0, t1, part;
+  int seq, lowest, pad0, pad1;  // lowest: no row of the job sees a position below (set on the device)
 };
 
 // k_span's work: the positions of one row behind its prefix (n = 0), or the
@@ -99,7 +101,7 @@ struct Meta {
   __host__ __device__ int local() const { return 3 * rows; }     // row - first row of its group
   __host__ __device__ int start() const { return 4 * rows; }     // [ctas + 1] items of each CTA
   __host__ __device__ int items() const { return (start() + ctas + 1 + 3) / 4 * 4; }
-  __host__ __device__ int jobs() const { return items() + 4 * max_items; }
+  __host__ __device__ int jobs() const { return items() + 12 * max_items; }
   __host__ __device__ int unit_of() const { return jobs() + 7 * max_jobs; }  // k_span's prefix unit of the row, -1
   __host__ __device__ int units() const { return unit_of() + rows; }          // prefixes first, then the rows
   __host__ __device__ int total() const { return units() + 5 * (rows + rows / 2); }
@@ -157,7 +159,7 @@ constexpr int PX_MMA_WARP = PX_SOFT + PX_CONV;
 constexpr int PX_THREADS = 32 * (PX_SOFT + PX_CONV + 4);
 // Registers a thread: 96 at launch (20 warps), which the softmax keeps; what the last four
 // warps give up is the converters'.
-constexpr int PX_REGS = 96, PX_REGS_SOFT = 96, PX_REGS_CONV = 120, PX_REGS_MMA = 40;
+constexpr int PX_REGS = 96, PX_REGS_SOFT = 96, PX_REGS_CONV = 112, PX_REGS_MMA = 56;
 static_assert(2 * PX_REGS_SOFT + 2 * PX_REGS_CONV + PX_REGS_MMA <= 5 * PX_REGS, "register split");
 constexpr float P_TOP = 7.0f, P_GROW = 8.0f;
 
@@ -170,24 +172,14 @@ struct PxSmem {
   static constexpr int BYTES = Q + 2 * QPART + 1024;
 };
 
-// What an item covers: tiles t0 .. t1 of its job, less those that no row sees.
-struct PxItem {
-  int row0, m0, m, kvh, len, t0, t1, part, seq;
-  int lowest;  // no row of the job sees a position below
-};
-__device__ __forceinline__ PxItem px_item(const SharedArgs& a, int it) {  // whole warps
-  PxItem r;
-  const Item i = reinterpret_cast<const Item*>(a.meta + a.mv.items())[it];
-  const Job* job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs()) + i.job;
-  r.row0 = job->row0;
-  r.m0 = job->m0;
-  r.m = job->m;
-  r.kvh = job->kvh;
-  r.len = job->len;
-  r.t0 = i.t0;
-  r.t1 = i.t1;
-  r.part = i.part;
-  r.seq = a.meta[a.mv.seq() + r.row0];
+// Item it, less the tiles that no row sees. Whole warps.
+__device__ __forceinline__ Item px_item(const SharedArgs& a, int it) {
+  union {
+    int4 v[3];
+    Item r;
+  };
+#pragma unroll
+  for (int i = 0; i < 3; i++) v[i] = __ldg(reinterpret_cast<const int4*>(a.meta + a.mv.items()) + 3 * it + i);
   r.lowest = 0;
   if (a.window) {
     const int first = r.row0 + r.m0 / a.G, last = r.row0 + (r.m0 + r.m - 1) / a.G;
@@ -344,8 +336,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     }
     return __all_sync(0xffffffffu, done) != 0;
   };
-  griddep_wait();
   griddep_launch();
+  // The plan, the lengths, the page table and the shared pages are from before k_begin, which
+  // let this kernel begin when they were in place: only the queries have to be waited for.
   const int* start = a.meta + a.mv.start() + blockIdx.x;
   const int i0 = start[0], i1 = start[1];
   int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
@@ -357,8 +350,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     const int h = warp >> 2, r = tid & 127, pair = 1 + (warp & 3);
     const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     bool ok = true;
+    griddep_wait();
     for (int it = i0; it < i1 && ok; it++) {
-      const PxItem item = px_item(a, it);
+      const Item item = px_item(a, it);
       const bool busy = (warp & 3) * 32 < item.m;  // else no row of this warp is one
       const size_t rec = item.part + r;
       if (item.t0 == item.t1) {  // nothing of it is in any window
@@ -371,7 +365,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       }
       float cq = 0.0f;
       int low = 0;
-      // the item's queries, as fp16 parts
+      // the item's queries, as fp16 parts (their place may still hold the last item's O)
+      if (ord) asm volatile("bar.sync 5, %0;" ::"n"(32 * PX_SOFT) : "memory");
 #pragma unroll 1
       for (int g = 0; g < PM && g + warp * 8 < item.m; g += 64) {
         const int l8 = lane & 7, j = g + warp * 8 + (((lane >> 3) & 1) << 2 | lane >> 4);
@@ -474,14 +469,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             l = mul2(l, pk(f, f));
             if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
             tc_fence_after();
-            for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 16) {
-              float o[16];
-              tc_ld16(tl + C_O + c, o);
+#pragma unroll 1
+            for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 8) {
+              float o[8];
+              tc_ld8(tl + C_O + c, o);
               tc_wait_ld();
-              uint32_t u[16];
+              uint32_t u[8];
 #pragma unroll
-              for (int j = 0; j < 16; j++) u[j] = __float_as_uint(o[j] * f);
-              tc_st16(tl + C_O + c, u);
+              for (int j = 0; j < 8; j++) u[j] = __float_as_uint(o[j] * f);
+              tc_st8(tl + C_O + c, u);
             }
             tc_wait_st();
           }
@@ -529,17 +525,27 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
                             : make_float2(M - P_TOP, la + pmax[n & 1][1][r]);
         pair_sync(pair);  // (the slot is the next item's)
-        for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 32) {
+        // O: from rows to whole lines by way of the queries' place (its readers are long past)
+        constexpr int CH = HDP / 8;  // 16-byte chunks of a row's half
+        uint8_t* stage = sm + L::Q + warp * (32 * CH * 16);
+        for (int c = 0; c < HDP / 2; c += 32) {
           float o[32];
-          tc_ld32(tl + C_O + c, o);
+          tc_ld32(tl + C_O + h * (HDP / 2) + c, o);
           tc_wait_ld();
-          if (r < item.m)
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (c + j < a.hd)
-                *reinterpret_cast<float4*>(a.po + rec * a.hd + c + j) =
-                    none ? make_float4(0, 0, 0, 0) : make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(stage + (lane * CH + (((c + j) / 4) ^ (lane % CH))) * 16) =
+                make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
+        __syncwarp();
+        const int c = lane % CH, col = h * (HDP / 2) + c * 4, r0 = (warp & 3) * 32;
+#pragma unroll 4
+        for (int q = lane / CH; q < 32; q += 32 / CH) {
+          float4 o = *reinterpret_cast<const float4*>(stage + (q * CH + (c ^ (q % CH))) * 16);
+          if (r0 + q < item.m && col < a.hd)
+            *reinterpret_cast<float4*>(a.po + (size_t)(item.part + r0 + q) * a.hd + col) = o;
+        }
+        __syncwarp();
         tc_fence_before();
       }
     }
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       if (left == 0) {
         it -= (tab == nullptr);
         while (left == 0 && ++it < i1) {
-          const PxItem item = px_item(a, it);
+          const Item item = px_item(a, it);
           left = item.t1 - item.t0;
           len = item.len;
           lowest = item.lowest;
@@ -677,7 +683,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
         __syncwarp();
       };
       for (int it = i0; it < i1 && ok; it++) {
-        const PxItem item = px_item(a, it);
+        const Item item = px_item(a, it);
         const int nt = item.t1 - item.t0;
         if (!nt) continue;
         if (!(ok = wait(&qfull, ord++))) break;
@@ -1128,7 +1134,8 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         x[e] = make_float4(0, 0, 0, 0);
-        if (act && c + e < k) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c0 + c + e) * hd) + lane);
+        // (a part that saw nothing may hold anything)
+        if (__shfl_sync(0xffffffffu, f, (c + e) & 31) != 0.0f && act && c + e < k) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c0 + c + e) * hd) + lane);
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -1406,6 +1413,10 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   // the tiles of all jobs, one after another, in equal shares.
   auto tiles_of = [&](int j) { return ((size_t)jobs[j].len + PT - 1) / PT; };
   size_t ni = 0, part = 0, done = 0, jt = 0;
+  auto item_of = [&](const Job& job, size_t t0, size_t t1) {
+    return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
+                seqs[job.row0], 0, 0, 0};
+  };
   int cta = 0;
   if (nj && nj <= mv.ctas) {
     size_t most = (tiles + mv.ctas - 1) / mv.ctas;
@@ -1422,7 +1433,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       job.part0 = (int)part;
       for (int i = 0; i < job.splits; i++) {
         h[mv.start() + cta++] = (int)ni;
-        items[ni++] = Item{j, (int)(nt * i / job.splits), (int)(nt * (i + 1) / job.splits), (int)part};
+        items[ni++] = item_of(job, nt * i / job.splits, nt * (i + 1) / job.splits);
         part += job.m;
       }
     }
@@ -1435,7 +1446,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       Job& job = jobs[j];
       const size_t nt = tiles_of(j), take = std::min(share, nt - jt);
       if (!jt) job.part0 = (int)part;
-      items[ni++] = Item{j, (int)jt, (int)(jt + take), (int)part};
+      items[ni++] = item_of(job, jt, jt + take);
       part += job.m;
       job.splits++;
       share -= take;
