@@ -6,6 +6,7 @@ safe wrappers (crates/synapse-core/src/lib.rs:602-775) and the INT8 layer
 operate on CUDA tensors through the C ABI in include/synapse_cuda.h. torch
 is used only for device memory and the current stream.
 """
+import array
 import ctypes
 
 import torch
@@ -453,18 +454,18 @@ class KVCache:
         """Sequence seqs[i] takes the context of its group's member parents[i]
         (int32 on the device, as from beam_select), in groups of `beams`
         (syn_cuda_kvcache_reorder)."""
-        seqs = _int32_array(seqs)
-        _need_cuda(parents)
-        if parents.dtype != torch.int32 or parents.numel() != len(seqs):
+        seqs = _int32s(seqs)
+        _need_tensors(self.device, torch.int32, parents)
+        if parents.numel() != len(seqs):
             raise SynapseError(4, "kvcache_reorder")
-        _need_device(self.device, parents)
         if not seqs:
             return
-        _check(lib().syn_cuda_kvcache_reorder(self.handle, len(seqs), seqs, _ptr(parents),
-                                              _index(beams), self._stream()), "kvcache_reorder")
+        _check(lib().syn_cuda_kvcache_reorder(self.handle, len(seqs), seqs.buffer_info()[0],
+                                              parents.data_ptr(), _index(beams), self._stream()),
+               "kvcache_reorder")
 
     def _stream(self):
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return _raw_stream(self.device)
 
     def append(self, layer, k, v, seq=0):
         _need_cuda(k, v)
@@ -525,23 +526,42 @@ def _index(v):
     return int(v)
 
 
-def _int32_array(values):
-    values = [int(v) for v in values]
-    if any(not -2**31 <= v < 2**31 for v in values):
-        raise SynapseError(2, "index out of range")
-    return (ctypes.c_int32 * len(values))(*values)
+def _int32s(values):
+    """An int32 array of the C ABI; values that are no such numbers are refused."""
+    try:
+        return array.array("i", values)
+    except (TypeError, OverflowError):
+        raise SynapseError(2, "expected int32 indices") from None
 
 
-def _need_device(device, *ts):
+def _sizes(values):
+    """A size_t array of the C ABI."""
+    try:
+        return array.array("Q", values)
+    except (TypeError, OverflowError):
+        raise SynapseError(2, "expected sizes") from None
+
+
+def _raw_stream(device):
+    """The current stream of a device (a tenth of a microsecond, where making a
+    torch.cuda.Stream object takes three)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _need_tensors(device, dtype, *ts):
+    """Contiguous tensors of one type on one device (None: an argument left out)."""
     for t in ts:
-        if t is not None and t.device.index != device:
-            raise SynapseError(2, f"expected tensors on cuda:{device}")
+        if t is None:
+            continue
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype
+                and t.get_device() == device):
+            raise SynapseError(2, f"expected {dtype} tensors on cuda:{device}")
+        if not t.is_contiguous():
+            raise SynapseError(5, "expected contiguous tensors")
 
 
-def _need_f32(*ts):
-    for t in ts:
-        if t is not None and t.dtype != torch.float32:
-            raise SynapseError(2, "expected float32 tensors")
+def _addr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def attention_decode(cache, layer, qkv, n_heads, q_norm, k_norm, eps, cos_t, sin_t, window=0,
@@ -584,16 +604,15 @@ def attention_prefill(cache, layer, qkv, n_heads, q_norm, k_norm, eps, cos_t, si
 
 def _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t):
     """Shapes, types and device of the rows [q | k | v] and what rotates them."""
-    _need_cuda(qkv, cos_t, sin_t, *(t for t in (q_norm, k_norm) if t is not None))
-    _need_f32(qkv, cos_t, sin_t, q_norm, k_norm)
-    _need_device(cache.device, qkv, cos_t, sin_t, q_norm, k_norm)
+    _need_tensors(cache.device, torch.float32, qkv, cos_t, sin_t, q_norm, k_norm)
     _index(layer)
     if qkv.dim() != 2 or qkv.shape[1] < (n_heads + 2 * cache.n_kv) * cache.hd or n_heads < 1:
         raise SynapseError(4, "qkv rows")
-    half = cache.hd // 2
-    if any(t.numel() < cache.max_seq * half for t in (cos_t, sin_t)):
+    angles = cache.max_seq * (cache.hd // 2)
+    if cos_t.numel() < angles or sin_t.numel() < angles:
         raise SynapseError(4, "rope tables")
-    if any(t is not None and t.numel() != cache.hd for t in (q_norm, k_norm)):
+    if (q_norm is not None and q_norm.numel() != cache.hd) or \
+            (k_norm is not None and k_norm.numel() != cache.hd):
         raise SynapseError(4, "head norms")
 
 
@@ -605,26 +624,24 @@ def qk_norm_rope_kv_append_batch(cache, layer, seqs, n_tokens, qkv, n_heads, q_n
     the normalised and rotated q rows [rows, n_heads*hd]; the lengths are not
     advanced."""
     _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t)
-    seqs, counts = _int32_array(seqs), [_index(t) for t in n_tokens]
-    qd, kvd, ld = n_heads * cache.hd, cache.n_kv * cache.hd, qkv.shape[1]
-    if len(counts) != len(seqs) or sum(counts) != qkv.shape[0]:
+    seqs, counts = _int32s(seqs), _sizes(n_tokens)
+    rows, ld = qkv.shape
+    qd, kvd = n_heads * cache.hd, cache.n_kv * cache.hd
+    if len(counts) != len(seqs) or sum(counts) != rows:
         raise SynapseError(4, "qk_norm_rope_kv_append_batch")
     if q_out is None:
-        q_out = torch.empty(qkv.shape[0], qd, dtype=torch.float32, device=qkv.device)
+        q_out = qkv.new_empty(rows, qd)
     else:
-        _need_cuda(q_out)
-        _need_f32(q_out)
-        _need_device(cache.device, q_out)
-        if q_out.shape != (qkv.shape[0], qd):
+        _need_tensors(cache.device, torch.float32, q_out)
+        if q_out.shape != (rows, qd):
             raise SynapseError(4, "q_out")
-    if qkv.shape[0] == 0:
+    if rows == 0:
         return q_out
     base = qkv.data_ptr()
     _check(lib().syn_cuda_qk_norm_rope_kv_append_batch(
-        cache.handle, layer, len(seqs), seqs, (ctypes.c_size_t * len(counts))(*counts),
-        ctypes.c_void_p(base), ctypes.c_void_p(base + 4 * qd),
-        ctypes.c_void_p(base + 4 * (qd + kvd)), ld, n_heads, _ptr(q_norm), _ptr(k_norm),
-        float(eps), _ptr(cos_t), _ptr(sin_t), _ptr(q_out), qd, _stream(qkv)),
+        cache.handle, layer, len(seqs), seqs.buffer_info()[0], counts.buffer_info()[0], base,
+        base + 4 * qd, base + 4 * (qd + kvd), ld, n_heads, _addr(q_norm), _addr(k_norm), eps,
+        cos_t.data_ptr(), sin_t.data_ptr(), q_out.data_ptr(), qd, _raw_stream(cache.device)),
         "qk_norm_rope_kv_append_batch")
     return q_out
 
@@ -645,10 +662,10 @@ class DecodePlan:
         """groups: lists of sequences; row r of an attention call is the r-th
         sequence of them all."""
         groups = [list(g) for g in groups]
-        seqs = _int32_array(s for g in groups for s in g)
-        sizes = (ctypes.c_size_t * len(groups))(*(len(g) for g in groups))
-        _check(lib().syn_cuda_decode_plan_set(self.handle, len(groups), sizes, seqs,
-                                              self.cache._stream()), "decode_plan_set")
+        seqs, sizes = _int32s(s for g in groups for s in g), _sizes(len(g) for g in groups)
+        _check(lib().syn_cuda_decode_plan_set(self.handle, len(sizes), sizes.buffer_info()[0],
+                                              seqs.buffer_info()[0], self.cache._stream()),
+               "decode_plan_set")
         self.rows = len(seqs)
 
     def prefix(self, row):
@@ -681,21 +698,18 @@ def attention_decode_shared(plan, layer, qkv, q_norm, k_norm, eps, cos_t, sin_t,
     if qkv.shape[0] != plan.rows:
         raise SynapseError(4, "attention_decode_shared")
     if out is None:
-        out = torch.empty(plan.rows, qd, dtype=torch.float32, device=qkv.device)
+        out = qkv.new_empty(plan.rows, qd)
     else:
-        _need_cuda(out)
-        _need_f32(out)
-        _need_device(cache.device, out)
+        _need_tensors(cache.device, torch.float32, out)
         if out.shape != (plan.rows, qd):
             raise SynapseError(4, "out")
     if plan.rows == 0:
         return out
     base = qkv.data_ptr()
     _check(lib().syn_cuda_attention_decode_shared(
-        plan.handle, layer, ctypes.c_void_p(base), ctypes.c_void_p(base + 4 * qd),
-        ctypes.c_void_p(base + 4 * (qd + kvd)), ld, _ptr(q_norm), _ptr(k_norm), float(eps),
-        _ptr(cos_t), _ptr(sin_t), _index(window), _ptr(out), qd, _stream(qkv)),
-        "attention_decode_shared")
+        plan.handle, layer, base, base + 4 * qd, base + 4 * (qd + kvd), ld, _addr(q_norm),
+        _addr(k_norm), eps, cos_t.data_ptr(), sin_t.data_ptr(), _index(window), out.data_ptr(), qd,
+        _raw_stream(cache.device)), "attention_decode_shared")
     return out
 
 
@@ -705,31 +719,30 @@ def beam_select(ctx, logits, scores, beams, k=None, finished=None, eos=-1):
     [groups*beams], finished uint8 [groups*beams] or None. Returns (scores f32,
     parents int32, tokens int32, finished uint8), each [groups, k], best first."""
     k = beams if k is None else k
-    for t in (logits, scores, finished):
-        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda):
-            raise SynapseError(2, "expected CUDA tensors")
-    _need_f32(logits, scores)
-    _need_device(ctx.device, logits, scores, finished)
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype == torch.float32
+            and logits.get_device() == ctx.device):
+        raise SynapseError(2, f"expected float32 logits on cuda:{ctx.device}")
+    _need_tensors(ctx.device, torch.float32, scores)
+    _need_tensors(ctx.device, torch.uint8, finished)
     if logits.dim() != 2 or beams < 1 or k < 1 or logits.shape[0] % beams:
         raise SynapseError(4, "beam_select")
     rows, vocab = logits.shape
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+    ld, inner = logits.stride()
+    if inner != 1 or (rows > 1 and ld < vocab):
         raise SynapseError(5, "beam_select")
-    _need_cuda(scores, *([finished] if finished is not None else []))
     if scores.numel() != rows or (finished is not None and finished.numel() != rows):
         raise SynapseError(4, "beam_select")
-    if finished is not None and finished.dtype != torch.uint8:
-        raise SynapseError(2, "finished")
-    g, dev = rows // beams, logits.device
-    s = torch.empty(g, k, dtype=torch.float32, device=dev)
-    pt = torch.empty(2, g, k, dtype=torch.int32, device=dev)
-    f = torch.empty(g, k, dtype=torch.uint8, device=dev)
+    g = rows // beams
+    s, p, t = logits.new_empty((3, g, k)).unbind()
+    p, t = p.view(torch.int32), t.view(torch.int32)
+    f = scores.new_empty((g, k), dtype=torch.uint8)
     if rows:
+        at = s.data_ptr()
         _check(lib().syn_cuda_beam_select(
-            ctx.handle, _ptr(logits), logits.stride(0) if rows > 1 else vocab, g, beams, vocab,
-            _ptr(scores), _ptr(finished), int(eos), k, _ptr(s), _ptr(pt[0]), _ptr(pt[1]), _ptr(f),
-            _stream(logits)), "beam_select")
-    return s, pt[0], pt[1], f
+            ctx.handle, logits.data_ptr(), ld if rows > 1 else vocab, g, beams, vocab,
+            scores.data_ptr(), _addr(finished), int(eos), k, at, at + 4 * g * k, at + 8 * g * k,
+            f.data_ptr(), _raw_stream(ctx.device)), "beam_select")
+    return s, p, t, f
 
 
 # ---------------------------------------------------------------------------

@@ -63,6 +63,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a) {
           (long long)row * a.ld;
   const float* w = is_q ? a.qn : is_v ? nullptr : a.kn;
   griddep_wait();
+  griddep_launch();
   T x1[1], x2[1];
   float scale = 1.0f;
   if (ONE && live && lane < nv) {
@@ -90,7 +91,6 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a) {
     for (int o = LP / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     scale = 1.0f / sqrtf(acc / (float)a.hd + a.eps);
   }
-  griddep_launch();
   if (!live) return;
   const int sq = a.seq_of ? a.seq_of[row] : a.seq[s];
   const int pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);

@@ -276,7 +276,7 @@ def test_reorder_odd_parents_and_refusals(ctx):
     flat = sb.KVCache(ctx, 16, 1, 8, 1, 4)
     for c, args, status in ((flat, ([0, 1], ok[:2], 2), 12), (cache, ([0, 0], ok[:2], 2), 2),
                             (cache, ([0, 4], ok[:2], 2), 2), (cache, ([0, 1, 2], ok[:3], 2), 4),
-                            (cache, ([0, 1], ok, 2), 4), (cache, ([0, 1], ok[:2].long(), 2), 4),
+                            (cache, ([0, 1], ok, 2), 4), (cache, ([0, 1], ok[:2].long(), 2), 2),
                             (cache, ([0, 1], ok[:2].cpu(), 2), 2), (cache, ([0, 1], ok[:2], 0), 4)):
         with pytest.raises(sb.SynapseError) as e:
             c.reorder(*args)
