@@ -156,20 +156,25 @@ __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_consta
 // largest float. A finished beam has one candidate, (eos, score_b); its others
 // are -inf.
 //
-// k_beam_scan, CTA = (segment of a row): one pass over the logits. Within a
-// row the value is monotone in x, so the segment's k best logits are all that
-// can be chosen from it: they are found exactly with 64-bit keys (ordered bits
-// of x, then the lower index). The k-th largest of the threads' own maxima
-// bounds the k-th best from below; what reaches it (at most k * EPT elements)
-// goes to shared memory and is ranked by counting.
-// k_beam_pick, CTA = group: logsumexp of each row from the segments' (max,
-// sum); the k-th best list head bounds the result from below, so at most k
-// lists and k * k elements are ranked.
+// One kernel, CTA = (segment of a row). Within a row the value is monotone in x, so
+// a segment's k best logits are all that can be chosen from it. They are found
+// in one pass with 64-bit keys (ordered bits of x, then the lower index): of the
+// threads' maxima of the first tile, the smallest of the 8 warps' ceil(k / 8)-th
+// largest bounds the k-th best from below, and what reaches it is listed; the
+// same bound of the whole segment cuts the list before it is ranked. Data that
+// defeat the bound (equal or sorted logits) overflow the list and are taken
+// once more with an exact bound after each tile. The pass also sums exp(x - m),
+// with m the thread's first maximum unless a later one is more than 20 above.
+// The group's last CTA to finish joins the segments: logsumexp of each row from
+// their (max, sum), a bound on the lists' heads as above (exact where it lets
+// through more than k + 8 lists), and what reaches it ranked by counting. Which CTA
+// is last changes no result.
+// Bound by HBM for many rows (4 bytes a logit), by latency for few.
 // ---------------------------------------------------------------------------
 constexpr int BS_THREADS = 256, BS_KMAX = 64, BS_BMAX = 64;
 
 __device__ __forceinline__ uint32_t ord32(float x) {  // order-preserving, > 0 for every float
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);       // (-0 becomes 0)
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unord32(uint32_t o) {
@@ -182,17 +187,24 @@ __device__ __forceinline__ uint64_t ord64(double x) {
 __device__ __forceinline__ double unord64(uint64_t o) {
   return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
 }
+__device__ __forceinline__ float ex2f(float x) {  // 2^x, 2 ulp; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float tame(float x) {
-  return x != x ? -INFINITY : fminf(x, 3.402823466e+38f) + 0.0f;  // (-0 becomes 0)
+  return fminf(fmaxf(x, -INFINITY), 3.402823466e+38f);  // (the maximum drops a NaN)
 }
 
 struct BeamArgs {
   const float* x;
   long long ld;
-  int beams, vocab, k, nseg, vec;
+  int beams, vocab, k, nseg, tiles, vec;  // tiles of a segment
+  int cap;                                // elements that beam_pick has room for
   const float* scores;
   const uint8_t* fin;
   int eos;
+  int* cnt;        // [groups] finished segments; zero between launches
   uint64_t* cand;  // [rows][nseg][k], best first, 0 = none
   float2* part;    // [rows][nseg] (max, sum of exp(x - max))
   float* out_s;
@@ -200,96 +212,45 @@ struct BeamArgs {
   uint8_t* out_f;
 };
 
-template <int EPT>
-__global__ void __launch_bounds__(BS_THREADS) k_beam_scan(const BeamArgs a) {
-  constexpr int SEG = BS_THREADS * EPT;
-  __shared__ uint64_t tmax[BS_THREADS];
-  __shared__ uint64_t list[BS_KMAX * EPT];
-  __shared__ uint64_t bound;
-  __shared__ int cnt;
-  __shared__ float red[BS_THREADS / 32];
-  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = seg * SEG;
-  griddep_wait();
-  float v[EPT];
-  const bool fin = a.fin && a.fin[row];
-  const float* xr = a.x + (long long)row * a.ld;
-#pragma unroll
-  for (int j = 0; j < EPT / 4; j++) {
-    const int i = base + (j * BS_THREADS + tid) * 4;
-    if (fin) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[j * 4 + e] = i + e == a.eos ? 0.0f : -INFINITY;
-    } else if (a.vec && i + 4 <= a.vocab) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(xr + i));
-      v[j * 4] = f.x;
-      v[j * 4 + 1] = f.y;
-      v[j * 4 + 2] = f.z;
-      v[j * 4 + 3] = f.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[j * 4 + e] = i + e < a.vocab ? __ldg(xr + i + e) : -INFINITY;
-    }
-  }
-  if (tid == 0) {
-    bound = 0;
-    cnt = 0;
-  }
-  float m = -INFINITY;
-  uint64_t best = 0;
-#pragma unroll
-  for (int j = 0; j < EPT; j++) {
-    v[j] = tame(v[j]);
-    m = fmaxf(m, v[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < EPT; j++) {  // ascending index: the first of equals stays
-    const int i = base + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3);
-    if (v[j] == m && !best && i < a.vocab) best = (uint64_t)ord32(m) << 32 | (uint32_t)~i;
-  }
-  tmax[tid] = best;
-  const float wm = warp_max(m);
-  if (lane == 0) red[warp] = wm;
+constexpr int BS_TILE = BS_THREADS * 8;    // elements of a tile
+constexpr int BS_LIST = 1024;              // a longer list is cut ...
+constexpr int BS_CAP = BS_LIST + BS_TILE;  // ... before another tile can overflow it
+constexpr int BS_WARPS = BS_THREADS / 32;
+
+// The k-th largest of the threads' keys (0 where fewer are not 0). Whole block.
+__device__ __forceinline__ uint64_t kth_key(uint64_t key, int k, uint64_t* keys, uint64_t* kth) {
+  const int tid = threadIdx.x;
+  keys[tid] = key;
+  if (tid == 0) *kth = 0;
   __syncthreads();
-  float M = red[0];
-#pragma unroll
-  for (int w = 1; w < BS_THREADS / 32; w++) M = fmaxf(M, red[w]);
-  // sum of exp over the segment, and the k-th largest of the threads' maxima
-  float s = 0.0f;
-  if (M > -INFINITY) {
-#pragma unroll
-    for (int j = 0; j < EPT; j++) s += expf(v[j] - M);
-  }
   int above = 0;
-  for (int j = 0; j < BS_THREADS; j++) above += tmax[j] > best;
-  if (best && above == a.k - 1) bound = best;
-  s = warp_sum(s);
+  const ulonglong2* p = reinterpret_cast<const ulonglong2*>(keys);
+#pragma unroll 8
+  for (int j = 0; j < BS_THREADS / 2; j++) {
+    const ulonglong2 u = p[j];
+    above += (u.x > key) + (u.y > key);
+  }
+  if (key && above == k - 1) *kth = key;
   __syncthreads();
-  if (lane == 0) red[warp] = s;
-  const uint64_t T = bound ? bound : 1;
-#pragma unroll
-  for (int j = 0; j < EPT; j++) {
-    const int i = base + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3);
-    const uint64_t key = (uint64_t)ord32(v[j]) << 32 | (uint32_t)~i;
-    if (i < a.vocab && key >= T) list[atomicAdd(&cnt, 1)] = key;
+  return *kth;
+}
+
+// A value that at least k of the threads' values reach (0 where a warp has too few that
+// are not 0): the smallest of the warps' ceil(k / 8)-th largest. Whole block.
+__device__ __forceinline__ uint32_t low_bound(uint32_t x, int k, uint32_t* warps) {
+  const int lane = threadIdx.x & 31;
+  uint32_t top = 0;
+  for (int r = (k + BS_WARPS - 1) / BS_WARPS; r > 0; r--) {
+    top = __reduce_max_sync(0xffffffffu, x);
+    const uint32_t has = __ballot_sync(0xffffffffu, x == top);
+    if (lane == __ffs(has) - 1) x = 0;
   }
+  if (lane == 0) warps[threadIdx.x >> 5] = top;
   __syncthreads();
-  griddep_launch();
-  const int n = cnt;
-  uint64_t* out = a.cand + ((size_t)row * a.nseg + seg) * a.k;
-  for (int i = tid; i < n; i += BS_THREADS) {
-    const uint64_t key = list[i];
-    int r = 0;
-    for (int j = 0; j < n; j++) r += list[j] > key;
-    if (r < a.k) out[r] = key;
-  }
-  for (int i = n + tid; i < a.k; i += BS_THREADS) out[i] = 0;
-  if (tid == 0) {
-    float t = 0.0f;
+  uint32_t low = warps[0];
 #pragma unroll
-    for (int w = 0; w < BS_THREADS / 32; w++) t += red[w];
-    a.part[(size_t)row * a.nseg + seg] = make_float2(M, t);
-  }
+  for (int w = 1; w < BS_WARPS; w++) low = min(low, warps[w]);
+  return low;
 }
 
 // A candidate is ord64 of its value (0 = none) and, for equal values, beam,
@@ -299,29 +260,34 @@ __device__ __forceinline__ bool over(uint64_t v, uint64_t i, uint64_t w, uint64_
   return v > w || (v == w && i > j);
 }
 
-__global__ void __launch_bounds__(BS_THREADS) k_beam_pick(const BeamArgs a) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  // heads [nh] and then the finalists [k*k] use the same space
-  uint64_t* lv = reinterpret_cast<uint64_t*>(raw);
-  const int lists = a.beams * a.nseg, cap = max(a.k * a.k, a.k * ((lists + BS_THREADS - 1) / BS_THREADS));
+// The group's selection from its rows' segments. Whole block; raw: as k_beam_select's.
+__device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw, uint64_t* tv, uint64_t* ti) {
+  const int lists = a.beams * a.nseg, cap = a.cap;
+  uint64_t* lv = reinterpret_cast<uint64_t*>(raw);  // heads, then finalists
   uint64_t* li = lv + cap;
-  __shared__ uint64_t tv[BS_THREADS], ti[BS_THREADS];
   __shared__ double lse[BS_BMAX];
   __shared__ float sc[BS_BMAX];
   __shared__ uint8_t fin[BS_BMAX];
   __shared__ uint64_t bv, bi;
-  __shared__ int cnt;
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ uint32_t lows[BS_WARPS];
+  __shared__ int cnt, nsel, sel[BS_THREADS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = g * a.beams;
-  griddep_wait();
-  for (int b = warp; b < a.beams; b += BS_THREADS / 32) {
+  const uint64_t* cand = a.cand + (size_t)r0 * a.nseg * a.k;
+  // (a row's lists on all warps: lists w, w + 8, ... are warp w's)
+  const int l0 = lane * BS_WARPS + warp;
+  const uint64_t head = l0 < lists ? __ldcg(cand + (size_t)l0 * a.k) : 0;
+  for (int b = warp; b < a.beams; b += BS_WARPS) {
     const float2* p = a.part + (size_t)(r0 + b) * a.nseg;
-    float M = -INFINITY;
-    for (int i = lane; i < a.nseg; i += 32) M = fmaxf(M, p[i].x);
+    const float2 first = lane < a.nseg ? __ldcg(p + lane) : make_float2(-INFINITY, 0.0f);
+    float M = first.x;
+    for (int i = 32 + lane; i < a.nseg; i += 32) M = fmaxf(M, __ldcg(p + i).x);
     M = warp_max(M);
-    double s = 0.0;
-    for (int i = lane; i < a.nseg; i += 32)
-      if (p[i].x > -INFINITY) s += (double)p[i].y * exp((double)p[i].x - (double)M);
+    double s = first.x > -INFINITY ? (double)(first.y * ex2f((first.x - M) * 1.4426950408889634f)) : 0.0;
+    for (int i = 32 + lane; i < a.nseg; i += 32) {
+      const float2 x = __ldcg(p + i);
+      if (x.x > -INFINITY) s += (double)(x.y * ex2f((x.x - M) * 1.4426950408889634f));
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
@@ -334,9 +300,9 @@ __global__ void __launch_bounds__(BS_THREADS) k_beam_pick(const BeamArgs a) {
     bv = 0;
     bi = 0;
     cnt = 0;
+    nsel = 0;
   }
   __syncthreads();
-  const uint64_t* cand = a.cand + (size_t)r0 * a.nseg * a.k;
   auto value = [&](int b, uint64_t key, uint64_t& v, uint64_t& i) {
     v = 0;
     i = 0;
@@ -345,75 +311,100 @@ __global__ void __launch_bounds__(BS_THREADS) k_beam_pick(const BeamArgs a) {
     i = (uint64_t)(BS_BMAX - 1 - b) << (32 + BS_TBITS) | key >> 32 << BS_TBITS |
         ((uint32_t)key & ((1u << BS_TBITS) - 1));
   };
-  // the k-th best of the threads' best list heads ...
-  uint64_t mv = 0;
-  uint64_t mi = 0;
-  for (int l = tid; l < lists; l += BS_THREADS) {
+  // a bound on the k-th best of the threads' best list heads, and the lists that reach it
+  uint64_t mv, mi;
+  value(l0 / a.nseg, head, mv, mi);
+  for (int l = l0 + BS_THREADS; l < lists; l += BS_THREADS) {
     uint64_t v, i;
-    value(l / a.nseg, cand[(size_t)l * a.k], v, i);
+    value(l / a.nseg, __ldcg(cand + (size_t)l * a.k), v, i);
     if (over(v, i, mv, mi)) {
       mv = v;
       mi = i;
     }
   }
-  tv[tid] = mv;
-  ti[tid] = mi;
-  __syncthreads();
-  int above = 0;
-  for (int j = 0; j < BS_THREADS; j++) above += over(tv[j], ti[j], mv, mi);
-  if (mv && above == a.k - 1) {
-    bv = mv;
-    bi = mi;
+  uint64_t Tv = (uint64_t)low_bound((uint32_t)(mv >> 32), a.k, lows) << 32, Ti = 0;
+  for (int l = l0; l < lists; l += BS_THREADS) {
+    uint64_t v, i;
+    value(l / a.nseg, l == l0 ? head : __ldcg(cand + (size_t)l * a.k), v, i);
+    if (v && v >= Tv) {
+      const int c = atomicAdd(&nsel, 1);
+      if (c < BS_THREADS) sel[c] = l;
+    }
   }
   __syncthreads();
-  uint64_t Tv = bv;
-  uint64_t Ti = bi;
-  // ... and, where a thread has several lists, of the heads that reach it
-  if (lists > BS_THREADS) {
-    for (int l = tid; l < lists; l += BS_THREADS) {
+  // the elements of ns lists that reach the bound; whether there was room for them
+  auto gather = [&](int ns) {
+    bool fits = true;
+    for (int e = tid; e < ns * a.k; e += BS_THREADS) {
+      const int l = sel[e / a.k];
       uint64_t v, i;
-      value(l / a.nseg, cand[(size_t)l * a.k], v, i);
+      value(l / a.nseg, __ldcg(cand + (size_t)l * a.k + e % a.k), v, i);
       if (v && !over(Tv, Ti, v, i)) {
         const int c = atomicAdd(&cnt, 1);
-        lv[c] = v;
-        li[c] = i;
+        fits &= c < cap;
+        if (c < cap) {
+          lv[c] = v;
+          li[c] = i;
+        }
       }
     }
+    return !__syncthreads_or(!fits);
+  };
+  const int ns = nsel;
+  if (ns > BS_THREADS || !gather(ns)) {  // too many: the exact k-th best of the threads' best ...
+    tv[tid] = mv;
+    ti[tid] = mi;
     __syncthreads();
-    const int n = cnt;
-    for (int c = tid; c < n; c += BS_THREADS) {
-      int r = 0;
-      for (int j = 0; j < n; j++) r += over(lv[j], li[j], lv[c], li[c]);
-      if (r == a.k - 1) {
-        bv = lv[c];
-        bi = li[c];
-      }
+    if (tid == 0) nsel = cnt = 0;
+    int above = 0;
+    for (int j = 0; j < BS_THREADS; j++) above += over(tv[j], ti[j], mv, mi);
+    if (mv && above == a.k - 1) {
+      bv = mv;
+      bi = mi;
     }
     __syncthreads();
     Tv = bv;
     Ti = bi;
-    if (tid == 0) cnt = 0;
-    __syncthreads();
-  }
-  // at most k lists reach it: their elements that do
-  for (int l = tid; l < lists; l += BS_THREADS) {
-    const int b = l / a.nseg;
-    for (int j = 0; j < a.k; j++) {
-      uint64_t v, i;
-      value(b, cand[(size_t)l * a.k + j], v, i);
-      if (!v || over(Tv, Ti, v, i)) break;  // best first
-      const int c = atomicAdd(&cnt, 1);
-      lv[c] = v;
-      li[c] = i;
+    // ... and, where a thread has several lists, of the heads that reach it
+    if (lists > BS_THREADS) {
+      for (int l = tid; l < lists; l += BS_THREADS) {
+        uint64_t v, i;
+        value(l / a.nseg, __ldcg(cand + (size_t)l * a.k), v, i);
+        if (v && !over(Tv, Ti, v, i)) {
+          const int c = atomicAdd(&cnt, 1);
+          lv[c] = v;
+          li[c] = i;
+        }
+      }
+      __syncthreads();
+      const int n = cnt;
+      for (int c = tid; c < n; c += BS_THREADS) {
+        int r = 0;
+        for (int j = 0; j < n; j++) r += over(lv[j], li[j], lv[c], li[c]);
+        if (r == a.k - 1) {
+          bv = lv[c];
+          bi = li[c];
+        }
+      }
+      __syncthreads();
+      Tv = bv;
+      Ti = bi;
+      if (tid == 0) cnt = 0;
     }
+    for (int l = tid; l < lists; l += BS_THREADS) {
+      uint64_t v, i;
+      value(l / a.nseg, __ldcg(cand + (size_t)l * a.k), v, i);
+      if (v && !over(Tv, Ti, v, i)) sel[atomicAdd(&nsel, 1)] = l;
+    }
+    __syncthreads();
+    gather(nsel);  // at most k lists, k * k elements
   }
-  __syncthreads();
-  griddep_launch();
   const int n = cnt;
   for (int c = tid; c < n; c += BS_THREADS) {
     const uint64_t v = lv[c];
     const uint64_t i = li[c];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; j++) r += over(lv[j], li[j], v, i);
     if (r < a.k) {
       const int b = BS_BMAX - 1 - (int)(i >> (32 + BS_TBITS));
@@ -427,13 +418,203 @@ __global__ void __launch_bounds__(BS_THREADS) k_beam_pick(const BeamArgs a) {
   }
 }
 
-// Segments of a row: 8, 16 or 32 elements per thread, the largest with which
-// the grid still gives every SM two CTAs.
-int beam_ept(size_t rows, size_t vocab, int sms) {
-  for (int e = 32; e > 8; e >>= 1)
-    if (rows * ((vocab + BS_THREADS * e - 1) / (BS_THREADS * e)) >= 2 * (size_t)sms) return e;
-  return 8;
+// PER: elements a thread takes at a time, 8 or 16.
+template <int PER>
+__global__ void __launch_bounds__(BS_THREADS, PER == 8 ? 4 : 3) k_beam_select(const BeamArgs a) {
+  constexpr float LOG2E = 1.4426950408889634f;
+  constexpr int TILE = BS_THREADS * PER;
+  extern __shared__ __align__(16) uint8_t raw[];
+  uint64_t* list = reinterpret_cast<uint64_t*>(raw);  // [BS_CAP], then beam_pick's
+  __shared__ __align__(16) uint64_t keys[BS_THREADS], keys2[BS_THREADS];
+  __shared__ uint64_t kth;
+  __shared__ uint32_t lows[2][BS_WARPS];
+  __shared__ int cnt, kept;
+  __shared__ float2 red[BS_WARPS];
+  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = seg * a.tiles * BS_TILE, end = min(a.vocab, base + a.tiles * BS_TILE);
+  if (tid == 0) cnt = 0;
+  griddep_wait();
+  const bool fin = a.fin && a.fin[row];
+  const float* xr = a.x + (long long)row * a.ld;
+  // element e of a thread's tile is at place(t, e): float4s
+  auto place = [&](int t, int e) { return base + t * TILE + ((e >> 2) * BS_THREADS + tid) * 4 + (e & 3); };
+  auto load = [&](int t, float (&v)[PER]) {
+#pragma unroll
+    for (int h = 0; h < PER; h += 4) {
+      const int i = place(t, h);
+      if (a.vec && i + 4 <= end) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(xr + i));
+        v[h] = f.x;
+        v[h + 1] = f.y;
+        v[h + 2] = f.z;
+        v[h + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[h + e] = i + e < end ? __ldg(xr + i + e) : -INFINITY;
+      }
+    }
+  };
+  // a finished beam's logits are not read: eos first, where it is in the segment, then the
+  // lowest tokens
+  const int nt = fin ? 0 : (end - base + TILE - 1) / TILE;
+  float m = -INFINITY, s = 0.0f;
+  uint64_t T = 1;        // (no key is 0)
+  uint32_t top = 0;      // ordered bits of the thread's largest element
+  bool overflow = false;
+  float v[PER], w[PER];
+  if (nt) load(0, v);
+  for (int t = 0; t < nt; t++) {
+    if (t + 1 < nt) load(t + 1, w);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      v[e] = tame(v[e]);
+      mt = fmaxf(mt, v[e]);
+    }
+    if (mt > m + 20.0f) {  // (also from -inf)
+      s *= m > -INFINITY ? ex2f((m - mt) * LOG2E) : 0.0f;
+      m = mt;
+    }
+    if (m > -INFINITY) {
+      float p[PER];
+#pragma unroll
+      for (int e = 0; e < PER; e++) p[e] = ex2f((v[e] - m) * LOG2E);
+#pragma unroll
+      for (int o = 1; o < PER; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < PER; e += 2 * o) p[e] += p[e + o];
+      s += p[0];
+    }
+    const uint32_t here = place(t, 0) < end ? ord32(mt) : 0;
+    top = max(top, here);
+    if (t == 0) T = max(T, (uint64_t)low_bound(here, a.k, lows[0]) << 32);
+    if (here >= (uint32_t)(T >> 32)) {
+#pragma unroll
+      for (int e = 0; e < PER; e++) {
+        const int i = place(t, e);
+        const uint64_t x = (uint64_t)ord32(v[e]) << 32 | (uint32_t)~i;
+        if (i < end && x >= T) {
+          const int c = atomicAdd(&cnt, 1);
+          if (c < BS_CAP) list[c] = x;
+          else overflow = true;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < PER; e++) v[e] = w[e];
+  }
+  if (__syncthreads_or(overflow)) {  // once more, in tiles of 2048 with an exact bound after each
+    T = 1;
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+    for (int t = 0; t < a.tiles; t++) {
+      uint64_t x[12], best = 0;
+      for (int e = 0; e < 8; e++) {
+        const int i = base + t * BS_TILE + e * BS_THREADS + tid;
+        x[e] = 0;
+        if (i < end) {
+          const float f = tame(__ldg(xr + i));
+          x[e] = (uint64_t)ord32(f) << 32 | (uint32_t)~i;
+        }
+        best = max(best, x[e]);
+      }
+      if (t == 0) T = max(T, kth_key(best, a.k, keys, &kth));
+      for (int e = 0; e < 8; e++)
+        if (x[e] >= T) list[atomicAdd(&cnt, 1)] = x[e];
+      __syncthreads();
+      const int n = cnt;
+      __syncthreads();
+      if (n > BS_LIST) {  // what reaches the k-th largest of the threads' maxima: at most 12 k
+        best = 0;
+        for (int e = 0; e < 12; e++) {
+          x[e] = e * BS_THREADS + tid < n ? list[e * BS_THREADS + tid] : 0;
+          best = max(best, x[e]);
+        }
+        T = max(T, kth_key(best, a.k, keys, &kth));
+        if (tid == 0) cnt = 0;
+        __syncthreads();
+        for (int e = 0; e < 12; e++)
+          if (x[e] >= T) list[atomicAdd(&cnt, 1)] = x[e];
+        __syncthreads();
+      }
+    }
+  }
+  // (max, sum) of the segment
+  const float wm = warp_max(m);
+  const float ws = warp_sum(m > -INFINITY ? s * ex2f((m - wm) * LOG2E) : 0.0f);
+  if (lane == 0) red[warp] = make_float2(wm, ws);
+  // the list, less what the whole segment's bound excludes, ranked
+  T = max(T, (uint64_t)low_bound(top, a.k, lows[1]) << 32);
+  int n = cnt;
+  uint64_t* out = a.cand + ((size_t)row * a.nseg + seg) * a.k;
+  const uint64_t* final = list;
+  if (n > 32) {
+    if (tid == 0) kept = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += BS_THREADS) {
+      const uint64_t x = list[i];
+      if (x >= T) {
+        const int c = atomicAdd(&kept, 1);
+        if (c < BS_THREADS) keys[c] = x;
+      }
+    }
+    __syncthreads();
+    if (kept <= BS_THREADS) {
+      n = kept;
+      final = keys;
+    }
+  }
+  for (int i = tid; i < n; i += BS_THREADS) {
+    const uint64_t x = final[i];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; j++) r += final[j] > x;
+    if (r < a.k) out[r] = x;
+  }
+  // (fewer than k elements are listed only where the segment has no more)
+  for (int i = n + tid; i < a.k && !fin; i += BS_THREADS) out[i] = 0;
+  const bool has = fin && a.eos >= base && a.eos < end;
+  if (fin && tid < a.k) {
+    int i = base + tid - has;
+    i += has && i >= a.eos;
+    out[tid] = has && tid == 0 ? (uint64_t)ord32(0.0f) << 32 | (uint32_t)~a.eos
+               : i < end       ? (uint64_t)ord32(-INFINITY) << 32 | (uint32_t)~i
+                               : 0;
+  }
+  if (fin && tid == 0) {
+    a.part[(size_t)row * a.nseg + seg] = has ? make_float2(0.0f, 1.0f) : make_float2(-INFINITY, 0.0f);
+  } else if (tid == 0) {
+    float M = red[0].x, t = 0.0f;
+#pragma unroll
+    for (int i = 1; i < BS_WARPS; i++) M = fmaxf(M, red[i].x);
+#pragma unroll
+    for (int i = 0; i < BS_WARPS; i++)
+      if (red[i].x > -INFINITY) t += red[i].y * ex2f((red[i].x - M) * LOG2E);
+    a.part[(size_t)row * a.nseg + seg] = make_float2(M, t);
+  }
+  __syncthreads();
+  const int g = row / a.beams;
+  if (tid == 0) {
+    __threadfence();
+    cnt = atomicAdd(&a.cnt[g], 1);
+    __threadfence();
+  }
+  __syncthreads();
+  griddep_launch();
+  if (cnt != a.beams * a.nseg - 1) return;
+  if (tid == 0) a.cnt[g] = 0;
+  beam_pick(a, g, raw, keys, keys2);
 }
+
+// Tiles of a segment: as few as give at most four CTAs (which an SM holds) on every SM,
+// at most 16.
+int beam_tiles(size_t rows, size_t vocab, int sms) {
+  const size_t tiles = (vocab + BS_TILE - 1) / BS_TILE;
+  for (int t = 1; t < 16; t++)
+    if (rows * ((tiles + t - 1) / t) <= 4 * (size_t)sms) return t;
+  return 16;
+}
+constexpr size_t BS_GROUPS = 65536;  // arrival counters, at the front of the scratch
 
 }  // namespace
 
@@ -574,8 +755,8 @@ syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, s
 }
 
 size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms) {
-  const size_t seg = (size_t)BS_THREADS * beam_ept(rows, vocab, sms), nseg = (vocab + seg - 1) / seg;
-  return rows * nseg * (k * sizeof(uint64_t) + sizeof(float2));
+  const size_t seg = (size_t)BS_TILE * beam_tiles(rows, vocab, sms), nseg = (vocab + seg - 1) / seg;
+  return BS_GROUPS * sizeof(int) + rows * nseg * (k * sizeof(uint64_t) + sizeof(float2));
 }
 
 syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
@@ -583,37 +764,36 @@ syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t
                                 size_t k, float* out_s, int32_t* out_p, int32_t* out_t,
                                 uint8_t* out_f, void* scratch, int sms, cudaStream_t st) {
   const size_t rows = groups * beams;
-  const int ept = beam_ept(rows, vocab, sms);
   BeamArgs a;
   a.x = x;
   a.ld = (long long)ld;
   a.beams = (int)beams;
   a.vocab = (int)vocab;
   a.k = (int)k;
-  a.nseg = (int)((vocab + (size_t)BS_THREADS * ept - 1) / ((size_t)BS_THREADS * ept));
+  a.tiles = beam_tiles(rows, vocab, sms);
+  a.nseg = (int)((vocab + (size_t)BS_TILE * a.tiles - 1) / ((size_t)BS_TILE * a.tiles));
   a.vec = ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   a.scores = scores;
   a.fin = fin;
   a.eos = eos;
-  a.cand = static_cast<uint64_t*>(scratch);
+  a.cnt = static_cast<int*>(scratch);
+  a.cand = reinterpret_cast<uint64_t*>(a.cnt + BS_GROUPS);
   a.part = reinterpret_cast<float2*>(a.cand + rows * a.nseg * k);
   a.out_s = out_s;
   a.out_p = out_p;
   a.out_t = out_t;
   a.out_f = out_f;
   const size_t lists = beams * a.nseg;
-  const size_t cap = std::max(k * k, k * ((lists + BS_THREADS - 1) / BS_THREADS));
+  // k lists of k, or the heads that reach the threads' k-th best
+  const size_t cap = std::max({k * k, k * ((lists + BS_THREADS - 1) / BS_THREADS), (size_t)BS_CAP / 2});
   const size_t smem = cap * 2 * sizeof(uint64_t);
+  a.cap = (int)cap;
   if (smem > 200 * 1024) return SYN_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)a.nseg, (unsigned)rows);
-  void (*scan)(const BeamArgs) = ept == 32 ? k_beam_scan<32> : ept == 16 ? k_beam_scan<16> : k_beam_scan<8>;
-  syn_status_t s = launched(launch_pdl(scan, grid, dim3(BS_THREADS), 0, st, a), "k_beam_scan");
-  if (s) return s;
+  void (*kern)(const BeamArgs) = a.tiles > 2 ? k_beam_select<16> : k_beam_select<8>;
   if (smem > 40 * 1024)
-    SYN_CUDA_TRY(cudaFuncSetAttribute(k_beam_pick, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      200 * 1024));
-  return launched(launch_pdl(k_beam_pick, dim3((unsigned)groups), dim3(BS_THREADS), smem, st, a),
-                  "k_beam_pick");
+    SYN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+  return launched(launch_pdl(kern, dim3((unsigned)a.nseg, (unsigned)rows), dim3(BS_THREADS), smem, st, a),
+                  "k_beam_select");
 }
 
 }  // namespace syn
