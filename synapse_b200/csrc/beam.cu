@@ -166,9 +166,9 @@ __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_consta
 // once more with an exact bound after each tile. The pass also sums exp(x - m),
 // with m the thread's first maximum unless a later one is more than 20 above.
 // The group's last CTA to finish joins the segments: logsumexp of each row from
-// their (max, sum), a bound on the lists' heads as above (exact where it lets
-// through more than k + 8 lists), and what reaches it ranked by counting. Which CTA
-// is last changes no result.
+// their (max, sum), a bound on the lists' heads as above (an exact one where that
+// lets too many through), one on the elements that are left, and what reaches it
+// ranked by counting. Which CTA is last changes no result.
 // Bound by HBM for many rows (4 bytes a logit), by latency for few.
 // ---------------------------------------------------------------------------
 constexpr int BS_THREADS = 256, BS_KMAX = 64, BS_BMAX = 64;
@@ -263,13 +263,12 @@ __device__ __forceinline__ bool over(uint64_t v, uint64_t i, uint64_t w, uint64_
 // The group's selection from its rows' segments. Whole block; raw: as k_beam_select's.
 __device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw, uint64_t* tv, uint64_t* ti) {
   const int lists = a.beams * a.nseg, cap = a.cap;
-  uint64_t* lv = reinterpret_cast<uint64_t*>(raw);  // heads, then finalists
-  uint64_t* li = lv + cap;
+  ulonglong2* best = reinterpret_cast<ulonglong2*>(raw);  // (v, i) of heads, then of finalists
   __shared__ double lse[BS_BMAX];
   __shared__ float sc[BS_BMAX];
   __shared__ uint8_t fin[BS_BMAX];
   __shared__ uint64_t bv, bi;
-  __shared__ uint32_t lows[BS_WARPS];
+  __shared__ uint32_t lows[BS_WARPS], lows2[BS_WARPS];
   __shared__ int cnt, nsel, sel[BS_THREADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = g * a.beams;
@@ -342,10 +341,7 @@ __device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw
       if (v && !over(Tv, Ti, v, i)) {
         const int c = atomicAdd(&cnt, 1);
         fits &= c < cap;
-        if (c < cap) {
-          lv[c] = v;
-          li[c] = i;
-        }
+        if (c < cap) best[c] = make_ulonglong2(v, i);
       }
     }
     return !__syncthreads_or(!fits);
@@ -371,19 +367,18 @@ __device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw
         uint64_t v, i;
         value(l / a.nseg, __ldcg(cand + (size_t)l * a.k), v, i);
         if (v && !over(Tv, Ti, v, i)) {
-          const int c = atomicAdd(&cnt, 1);
-          lv[c] = v;
-          li[c] = i;
+          best[atomicAdd(&cnt, 1)] = make_ulonglong2(v, i);
         }
       }
       __syncthreads();
       const int n = cnt;
       for (int c = tid; c < n; c += BS_THREADS) {
+        const ulonglong2 x = best[c];
         int r = 0;
-        for (int j = 0; j < n; j++) r += over(lv[j], li[j], lv[c], li[c]);
+        for (int j = 0; j < n; j++) r += over(best[j].x, best[j].y, x.x, x.y);
         if (r == a.k - 1) {
-          bv = lv[c];
-          bi = li[c];
+          bv = x.x;
+          bi = x.y;
         }
       }
       __syncthreads();
@@ -399,13 +394,24 @@ __device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw
     __syncthreads();
     gather(nsel);  // at most k lists, k * k elements
   }
-  const int n = cnt;
+  int n = cnt;
+  if (n > 2 * a.k && n <= BS_THREADS) {  // a bound from all of them, and what reaches it, to the front
+    const ulonglong2 x = tid < n ? best[tid] : make_ulonglong2(0, 0);
+    const uint64_t low = (uint64_t)low_bound((uint32_t)(x.x >> 32), a.k, lows2) << 32;
+    if (tid == 0) cnt = 0;  // (the bound's barrier is past every read)
+    __syncthreads();
+    if (x.x && x.x >= low) best[atomicAdd(&cnt, 1)] = x;
+    __syncthreads();
+    n = cnt;
+  }
   for (int c = tid; c < n; c += BS_THREADS) {
-    const uint64_t v = lv[c];
-    const uint64_t i = li[c];
+    const uint64_t v = best[c].x, i = best[c].y;
     int r = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; j++) r += over(lv[j], li[j], v, i);
+    for (int j = 0; j < n; j++) {
+      const ulonglong2 x = best[j];
+      r += over(x.x, x.y, v, i);
+    }
     if (r < a.k) {
       const int b = BS_BMAX - 1 - (int)(i >> (32 + BS_TBITS));
       const int t = (int)((1u << BS_TBITS) - 1 - ((uint32_t)i & ((1u << BS_TBITS) - 1)));
@@ -459,6 +465,7 @@ __global__ void __launch_bounds__(BS_THREADS, PER == 8 ? 4 : 3) k_beam_select(co
   const int nt = fin ? 0 : (end - base + TILE - 1) / TILE;
   float m = -INFINITY, s = 0.0f;
   uint64_t T = 1;        // (no key is 0)
+  float Tf = -INFINITY;  // the least value whose keys reach T
   uint32_t top = 0;      // ordered bits of the thread's largest element
   bool overflow = false;
   float v[PER], w[PER];
@@ -488,17 +495,18 @@ __global__ void __launch_bounds__(BS_THREADS, PER == 8 ? 4 : 3) k_beam_select(co
     const uint32_t here = place(t, 0) < end ? ord32(mt) : 0;
     top = max(top, here);
     if (t == 0) T = max(T, (uint64_t)low_bound(here, a.k, lows[0]) << 32);
-    if (here >= (uint32_t)(T >> 32)) {
+    if (t == 0) Tf = T > 1 ? unord32((uint32_t)(T >> 32)) : -INFINITY;
+    if (mt >= Tf) {
 #pragma unroll
-      for (int e = 0; e < PER; e++) {
-        const int i = place(t, e);
-        const uint64_t x = (uint64_t)ord32(v[e]) << 32 | (uint32_t)~i;
-        if (i < end && x >= T) {
-          const int c = atomicAdd(&cnt, 1);
-          if (c < BS_CAP) list[c] = x;
-          else overflow = true;
+      for (int e = 0; e < PER; e++)
+        if (v[e] >= Tf) {
+          const int i = place(t, e);
+          if (i < end) {
+            const int c = atomicAdd(&cnt, 1);
+            if (c < BS_CAP) list[c] = (uint64_t)ord32(v[e]) << 32 | (uint32_t)~i;
+            else overflow = true;
+          }
         }
-      }
     }
 #pragma unroll
     for (int e = 0; e < PER; e++) v[e] = w[e];
@@ -606,13 +614,13 @@ __global__ void __launch_bounds__(BS_THREADS, PER == 8 ? 4 : 3) k_beam_select(co
   beam_pick(a, g, raw, keys, keys2);
 }
 
-// Tiles of a segment: as few as give at most four CTAs (which an SM holds) on every SM,
-// at most 16.
+// Tiles of a segment: as few as give at most two CTAs on every SM,
+// at most 8 (uneven waves then cost less than longer segments save).
 int beam_tiles(size_t rows, size_t vocab, int sms) {
   const size_t tiles = (vocab + BS_TILE - 1) / BS_TILE;
-  for (int t = 1; t < 16; t++)
-    if (rows * ((tiles + t - 1) / t) <= 4 * (size_t)sms) return t;
-  return 16;
+  for (int t = 1; t < 8; t++)
+    if (rows * ((tiles + t - 1) / t) <= 2 * (size_t)sms) return t;
+  return 8;
 }
 constexpr size_t BS_GROUPS = 65536;  // arrival counters, at the front of the scratch
 
