@@ -1,6 +1,8 @@
 // append.cuh -- the batched append of new rows to the KV cache.
 #pragma once
 
+#include <initializer_list>
+
 #include "internal.cuh"
 
 namespace syn {
@@ -12,11 +14,14 @@ namespace syn {
 // (i, i + hd/2) by the position's angle; q goes to q_out, k and the raw v to
 // the position's cache row.
 // LP lanes (a power of two) take one head row, VEC pairs each; ONE: a head row
-// is one step of its lanes, kept in registers between the sum and the rotation.
-// Bound by HBM for prompts, by its launch for single tokens.
+// is one step of its lanes, kept in registers between the sum and the rotation,
+// and HC heads of a row are under way at once, with the position found and its
+// angles read once for all of them. Bound by HBM for prompts, by its launch for
+// single tokens.
 // ---------------------------------------------------------------------------
 constexpr int AP_MAX = 256;  // sequences per launch (by value)
 constexpr int AP_THREADS = 256;
+constexpr size_t AP_FILL = 600;  // blocks from which a launch fills the device
 
 struct AppendArgs {
   const float *q, *k, *v;
@@ -42,102 +47,130 @@ template <int VEC> struct ApVec;
 template <> struct ApVec<4> { using T = float4; };
 template <> struct ApVec<1> { using T = float; };
 
-template <int VEC, int LP, bool ONE>
+template <int VEC, int LP, bool ONE, int HC>
 __device__ __forceinline__ void append_rows(const AppendArgs& a) {
+  static_assert(ONE || HC == 1, "several heads are held in registers");
   using T = typename ApVec<VEC>::T;
   const int heads = a.n_heads + 2 * a.n_kv, half = a.hd >> 1, nv = half / VEC;
+  const int groups = (heads + HC - 1) / HC;
   const long long unit = (long long)blockIdx.x * (AP_THREADS / LP) + threadIdx.x / LP;
   const int lane = threadIdx.x % LP;
-  const int row = (int)(unit / heads), h = (int)(unit - (long long)row * heads);
+  const int row = (int)(unit / groups), h0 = (int)(unit - (long long)row * groups) * HC;
   const bool live = row < a.rows;
   int s = 0;
   if (live && !a.seq_of)
     for (int step = AP_MAX / 2; step; step >>= 1)  // the last sequence that starts at or before row
       if (s + step < a.n && a.row0[s + step] <= row) s += step;
-  const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
-  const float* src = nullptr;
-  if (live)
-    src = (is_q ? a.q + (long long)h * a.hd
-                : is_v ? a.v + (long long)(h - a.n_heads - a.n_kv) * a.hd
-                       : a.k + (long long)(h - a.n_heads) * a.hd) +
-          (long long)row * a.ld;
-  const float* w = is_q ? a.qn : is_v ? nullptr : a.kn;
+  auto source = [&](int h) {
+    return (h < a.n_heads             ? a.q + (long long)h * a.hd
+            : h < a.n_heads + a.n_kv ? a.k + (long long)(h - a.n_heads) * a.hd
+                                     : a.v + (long long)(h - a.n_heads - a.n_kv) * a.hd) +
+           (long long)row * a.ld;
+  };
   griddep_wait();
   griddep_launch();
-  T x1[1], x2[1];
-  float scale = 1.0f;
-  if (ONE && live && lane < nv) {
-    x1[0] = reinterpret_cast<const T*>(src)[lane];
-    x2[0] = reinterpret_cast<const T*>(src + half)[lane];
-  }
-  if (a.qn || a.kn) {  // (uniform: the shuffles need every lane)
-    float acc = 0.0f;
-    if (live && w)
-      for (int i = lane; i < nv; i += LP) {
-        T b1, b2;
-        if (ONE) {
-          b1 = x1[0];
-          b2 = x2[0];
-        } else {
-          b1 = reinterpret_cast<const T*>(src)[i];
-          b2 = reinterpret_cast<const T*>(src + half)[i];
-        }
-        const float* f1 = reinterpret_cast<const float*>(&b1);
-        const float* f2 = reinterpret_cast<const float*>(&b2);
+  T x1[HC], x2[HC];
+  const bool mine = live && lane < nv;
+  if (ONE)
 #pragma unroll
-        for (int e = 0; e < VEC; e++) acc = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], acc));
+    for (int i = 0; i < HC; i++)
+      if (mine && h0 + i < heads) {
+        x1[i] = reinterpret_cast<const T*>(source(h0 + i))[lane];
+        x2[i] = reinterpret_cast<const T*>(source(h0 + i) + half)[lane];
       }
-#pragma unroll
-    for (int o = LP / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    scale = 1.0f / sqrtf(acc / (float)a.hd + a.eps);
+  int sq = 0, pos = 0;
+  if (live) {
+    sq = a.seq_of ? a.seq_of[row] : a.seq[s];
+    pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);
   }
-  if (!live) return;
-  const int sq = a.seq_of ? a.seq_of[row] : a.seq[s];
-  const int pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);
-  if (pos >= a.max_seq) return;  // (a replayed graph that has run past the cache)
-  float* dst;
-  if (is_q) {
-    dst = a.q_out + (long long)row * a.ldq + (long long)h * a.hd;
-  } else {
-    size_t slot = (size_t)sq * a.max_seq + pos;
-    if (a.ptab) {
-      const int pg = a.ptab[(size_t)sq * a.maxp + pos / a.page];
-      if (pg < 0) return;
-      slot = (size_t)pg * a.page + pos % a.page;
-    }
-    dst = (is_v ? a.vc + (size_t)(h - a.n_heads - a.n_kv) * a.hd
-                : a.kc + (size_t)(h - a.n_heads) * a.hd) +
-          slot * a.n_kv * a.hd;
-  }
+  const bool in = live && pos < a.max_seq;  // (a replayed graph may have run past the cache)
   const float* ct = a.cos_t + (size_t)pos * half;
   const float* st = a.sin_t + (size_t)pos * half;
-  for (int i = lane; i < nv; i += LP) {
-    T b1, b2;
-    if (ONE) {
-      b1 = x1[0];
-      b2 = x2[0];
-    } else {
-      b1 = reinterpret_cast<const T*>(src)[i];
-      b2 = reinterpret_cast<const T*>(src + half)[i];
+  T c1, s1;
+  if (ONE && mine && in) {
+    c1 = reinterpret_cast<const T*>(ct)[lane];
+    s1 = reinterpret_cast<const T*>(st)[lane];
+  }
+  long long slot = -1;  // the position's cache row
+  if (in) {
+    slot = (long long)sq * a.max_seq + pos;
+    if (a.ptab) {
+      const int pg = a.ptab[(size_t)sq * a.maxp + pos / a.page];
+      slot = pg < 0 ? -1 : (long long)pg * a.page + pos % a.page;
     }
-    if (!is_v) {
-      float* f1 = reinterpret_cast<float*>(&b1);
-      float* f2 = reinterpret_cast<float*>(&b2);
+  }
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const int d = i * VEC + e;
-        float y1 = f1[e], y2 = f2[e];
-        if (w) {
-          y1 *= w[d] * scale;
-          y2 *= w[half + d] * scale;
+  for (int i = 0; i < HC; i++) {
+    const int h = h0 + i;
+    const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+    const float* src = live && h < heads ? source(h) : nullptr;
+    const float* w = is_q ? a.qn : is_v ? nullptr : a.kn;
+    float scale = 1.0f;
+    if (a.qn || a.kn) {  // (uniform: the shuffles need every lane)
+      float acc = 0.0f;
+      if (src && w)
+        for (int j = lane; j < nv; j += LP) {
+          T b1, b2;
+          if (ONE) {
+            b1 = x1[i];
+            b2 = x2[i];
+          } else {
+            b1 = reinterpret_cast<const T*>(src)[j];
+            b2 = reinterpret_cast<const T*>(src + half)[j];
+          }
+          const float* f1 = reinterpret_cast<const float*>(&b1);
+          const float* f2 = reinterpret_cast<const float*>(&b2);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) acc = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], acc));
         }
-        const float c = ct[d], sn = st[d];
-        f1[e] = y1 * c - y2 * sn;
-        f2[e] = y2 * c + y1 * sn;
-      }
+#pragma unroll
+      for (int o = LP / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      scale = 1.0f / sqrtf(acc / (float)a.hd + a.eps);
     }
-    reinterpret_cast<T*>(dst)[i] = b1;
-    reinterpret_cast<T*>(dst + half)[i] = b2;
+    if (!src || !in || (!is_q && slot < 0)) continue;
+    float* dst = is_q ? a.q_out + (long long)row * a.ldq + (long long)h * a.hd
+                      : (is_v ? a.vc + (size_t)(h - a.n_heads - a.n_kv) * a.hd
+                              : a.kc + (size_t)(h - a.n_heads) * a.hd) +
+                            (size_t)slot * a.n_kv * a.hd;
+    for (int j = lane; j < nv; j += LP) {
+      T b1, b2, c, sn;
+      if (ONE) {
+        b1 = x1[i];
+        b2 = x2[i];
+        c = c1;
+        sn = s1;
+      } else {
+        b1 = reinterpret_cast<const T*>(src)[j];
+        b2 = reinterpret_cast<const T*>(src + half)[j];
+        c = reinterpret_cast<const T*>(ct)[j];
+        sn = reinterpret_cast<const T*>(st)[j];
+      }
+      if (!is_v) {
+        float* f1 = reinterpret_cast<float*>(&b1);
+        float* f2 = reinterpret_cast<float*>(&b2);
+        const float* fc = reinterpret_cast<const float*>(&c);
+        const float* fs = reinterpret_cast<const float*>(&sn);
+        if (w) {
+          const T w1 = reinterpret_cast<const T*>(w)[j], w2 = reinterpret_cast<const T*>(w + half)[j];
+          const float* g1 = reinterpret_cast<const float*>(&w1);
+          const float* g2 = reinterpret_cast<const float*>(&w2);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            f1[e] *= g1[e] * scale;
+            f2[e] *= g2[e] * scale;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          const float y1 = f1[e], y2 = f2[e];
+          // (written out, so that every variant rounds alike)
+          f1[e] = __fmaf_rn(y1, fc[e], -__fmul_rn(y2, fs[e]));
+          f2[e] = __fmaf_rn(y2, fc[e], __fmul_rn(y1, fs[e]));
+        }
+      }
+      reinterpret_cast<T*>(dst)[j] = b1;
+      reinterpret_cast<T*>(dst + half)[j] = b2;
+    }
   }
 }
 
@@ -148,8 +181,9 @@ struct AppendShape {
   bool vec, one;
 };
 inline AppendShape append_shape(const AppendArgs& a) {
-  const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
-                        reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out);
+  uintptr_t low = 0;
+  for (const float* p : {a.q, a.k, a.v, (const float*)a.q_out, a.cos_t, a.sin_t, a.qn, a.kn})
+    low |= reinterpret_cast<uintptr_t>(p);
   const bool vec = a.hd % 8 == 0 && low % 16 == 0 && a.ld % 4 == 0 && a.ldq % 4 == 0;
   const int lanes = a.hd / 2 / 4;
   if (!vec || lanes > 32) return {32, vec, false};

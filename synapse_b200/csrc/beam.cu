@@ -143,9 +143,14 @@ __global__ void __launch_bounds__(256) k_reorder_tables(const __grid_constant__ 
   }
 }
 
-template <int VEC, int LP, bool ONE>
+template <int VEC, int LP, bool ONE, int HC>
 __global__ void __launch_bounds__(AP_THREADS) k_append_batch(const __grid_constant__ AppendArgs a) {
-  append_rows<VEC, LP, ONE>(a);
+  append_rows<VEC, LP, ONE, HC>(a);
+}
+template <int HC>
+void (*append_kernel(int lp))(const AppendArgs) {
+  return lp == 4 ? k_append_batch<4, 4, true, HC> : lp == 8 ? k_append_batch<4, 8, true, HC>
+         : lp == 16 ? k_append_batch<4, 16, true, HC> : k_append_batch<4, 32, true, HC>;
 }
 
 // ---------------------------------------------------------------------------
@@ -426,7 +431,7 @@ __device__ __forceinline__ void beam_pick(const BeamArgs& a, int g, uint8_t* raw
 
 // PER: elements a thread takes at a time, 8 or 16.
 template <int PER>
-__global__ void __launch_bounds__(BS_THREADS, PER == 8 ? 4 : 3) k_beam_select(const BeamArgs a) {
+__global__ void __launch_bounds__(BS_THREADS, 4) k_beam_select(const BeamArgs a) {
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr int TILE = BS_THREADS * PER;
   extern __shared__ __align__(16) uint8_t raw[];
@@ -744,14 +749,14 @@ syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, s
     a.rows = (int)rows;
     if (rows) {
       const AppendShape sh = append_shape(a);
-      void (*kern)(const AppendArgs) = !sh.vec      ? k_append_batch<1, 32, false>
-                                       : !sh.one    ? k_append_batch<4, 32, false>
-                                       : sh.lp == 4 ? k_append_batch<4, 4, true>
-                                       : sh.lp == 8 ? k_append_batch<4, 8, true>
-                                       : sh.lp == 16 ? k_append_batch<4, 16, true>
-                                                     : k_append_batch<4, 32, true>;
-      const size_t units = rows * (a.n_heads + 2 * a.n_kv), per = AP_THREADS / sh.lp;
-      const size_t blocks = (units + per - 1) / per;
+      // four heads a lane group once that still fills the device
+      const size_t heads = a.n_heads + 2 * a.n_kv, per = AP_THREADS / sh.lp;
+      const bool many = sh.one && rows * heads >= 4 * per * AP_FILL;
+      void (*kern)(const AppendArgs) = !sh.vec   ? k_append_batch<1, 32, false, 1>
+                                       : !sh.one ? k_append_batch<4, 32, false, 1>
+                                       : many    ? append_kernel<4>(sh.lp)
+                                                 : append_kernel<1>(sh.lp);
+      const size_t units = rows * (many ? (heads + 3) / 4 : heads), blocks = (units + per - 1) / per;
       if (blocks > 0x7FFFFFFF) return SYN_ERR_UNSUPPORTED;
       syn_status_t s = launched(launch_pdl(kern, dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a),
                                 "k_append_batch");

@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ Ap
                                                       const __grid_constant__ SharedArgs a, int deal) {
   const int block = (int)blockIdx.x - ((int)gridDim.x - deal);
   if (block < 0) {
-    append_rows<VEC, LP, ONE>(p);
+    append_rows<VEC, LP, ONE, 1>(p);
   } else {
     griddep_wait();
     griddep_launch();
