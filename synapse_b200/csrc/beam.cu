@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <mutex>
 #include <vector>
 
 #include "append.cuh"
@@ -51,6 +52,7 @@ struct ReorderArgs {
   float4 *k, *v;
   size_t layer4;   // float4s between layers
   int* ptab;
+  int* done;  // finished blocks; zero between launches
   int maxp, page, row4;  // row4: float4s of one position
   const int32_t* parents;
   int n, beams;
@@ -95,52 +97,69 @@ __device__ __forceinline__ int2 ro_tail(const int* par, int i, int beams) {
   return make_int2(i, 0);  // not reached: as many childless members as copies
 }
 
-// The copies: grid (chunks, n, layers)
-__global__ void __launch_bounds__(256) k_reorder_copy(const __grid_constant__ ReorderArgs a) {
-  __shared__ int par[RO_MAX];
+// grid (chunks, n, layers + 1): the copies of each layer; then, column chunks by group, the
+// table entries of full pages. Those of the last pages, which the copies go by, are
+// written by the block that finishes last.
+__global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ ReorderArgs a) {
+  __shared__ int par[RO_MAX], old[RO_MAX][9];
   __shared__ int2 t;
-  const int i = blockIdx.y, g0 = i / a.beams * a.beams;
-  for (int j = threadIdx.x; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
-  __syncthreads();
-  if (threadIdx.x == 0) t = ro_tail(par, i - g0, a.beams);
-  __syncthreads();
-  const int len = a.len[i / a.beams], tail = len % a.page;
-  if (!t.y || !tail) return;
-  const int col = len / a.page;
-  const int src = a.ptab[(size_t)a.seq[g0 + par[i - g0]] * a.maxp + col];
-  const int dst = a.ptab[(size_t)a.seq[g0 + t.x] * a.maxp + col];
-  if (src < 0 || dst < 0) return;
-  const int n4 = tail * a.row4;
-  const size_t s4 = (size_t)src * a.page * a.row4, d4 = (size_t)dst * a.page * a.row4;
-  float4* k = a.k + blockIdx.z * a.layer4;
-  float4* v = a.v + blockIdx.z * a.layer4;
-  for (int j = blockIdx.x * 256 + threadIdx.x; j < n4; j += gridDim.x * 256) {
-    k[d4 + j] = k[s4 + j];
-    v[d4 + j] = v[s4 + j];
+  __shared__ int last;
+  const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch();
+  if (blockIdx.z < gridDim.z - 1) {
+    const int i = blockIdx.y, g0 = i / a.beams * a.beams;
+    for (int j = tid; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
+    __syncthreads();
+    if (tid == 0) t = ro_tail(par, i - g0, a.beams);
+    __syncthreads();
+    const int len = a.len[i / a.beams], tail = len % a.page;
+    if (t.y && tail) {
+      const int col = len / a.page;
+      const int src = a.ptab[(size_t)a.seq[g0 + par[i - g0]] * a.maxp + col];
+      const int dst = a.ptab[(size_t)a.seq[g0 + t.x] * a.maxp + col];
+      if (src >= 0 && dst >= 0) {
+        const int n4 = tail * a.row4;
+        const size_t s4 = (size_t)src * a.page * a.row4, d4 = (size_t)dst * a.page * a.row4;
+        float4* k = a.k + blockIdx.z * a.layer4;
+        float4* v = a.v + blockIdx.z * a.layer4;
+        for (int j = blockIdx.x * 256 + tid; j < n4; j += gridDim.x * 256) {
+          const float4 x = k[s4 + j], y = v[s4 + j];
+          k[d4 + j] = x;
+          v[d4 + j] = y;
+        }
+      }
+    }
+  } else if (blockIdx.y < a.n / a.beams) {
+    const int g0 = blockIdx.y * a.beams, full = a.len[blockIdx.y] / a.page;
+    for (int j = tid; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
+    for (int c0 = blockIdx.x * 8; c0 < full; c0 += gridDim.x * 8) {
+      for (int u = tid; u < a.beams * 8; u += 256) {
+        const int b = u >> 3, c = c0 + (u & 7);
+        if (c < full) old[b][u & 7] = a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c];
+      }
+      __syncthreads();
+      for (int u = tid; u < a.beams * 8; u += 256) {
+        const int b = u >> 3, c = c0 + (u & 7);
+        if (c < full) a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c] = old[par[b]][u & 7];
+      }
+      __syncthreads();
+    }
   }
-}
-
-// The tables: grid (column chunks of 32, groups), after the copies
-__global__ void __launch_bounds__(256) k_reorder_tables(const __grid_constant__ ReorderArgs a) {
-  __shared__ int par[RO_MAX], from[RO_MAX];
-  extern __shared__ int old[];  // [beams][33]
-  const int g0 = blockIdx.y * a.beams, len = a.len[blockIdx.y];
-  const int full = len / a.page, cols = (len + a.page - 1) / a.page;
-  const int c0 = blockIdx.x * 32;
-  if (c0 >= cols) return;
-  for (int j = threadIdx.x; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
-  for (int t = threadIdx.x; t < a.beams * 32; t += 256) {
-    const int b = t >> 5, c = c0 + (t & 31);
-    if (c < cols) old[b * 33 + (t & 31)] = a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c];
-  }
+  __syncthreads();  // (the block has read what it needs of the last pages' entries)
+  if (tid == 0) last = atomicAdd(a.done, 1) == (int)(gridDim.x * gridDim.y * gridDim.z) - 1;
   __syncthreads();
-  for (int j = threadIdx.x; j < a.beams; j += 256) from[j] = ro_tail(par, j, a.beams).x;
+  if (!last) return;
+  if (tid < a.n) par[tid] = ro_parent(a.parents + tid / a.beams * a.beams, tid % a.beams, a.beams);
   __syncthreads();
-  for (int t = threadIdx.x; t < a.beams * 32; t += 256) {
-    const int b = t >> 5, c = c0 + (t & 31);
-    if (c < cols)
-      a.ptab[(size_t)a.seq[g0 + b] * a.maxp + c] = old[(c < full ? par[b] : from[b]) * 33 + (t & 31)];
-  }
+  int entry = -1;
+  const int g0 = tid / a.beams * a.beams;
+  const size_t col = tid < a.n ? a.len[tid / a.beams] / a.page : 0;
+  const bool mine = tid < a.n && a.len[tid / a.beams] % a.page;
+  if (mine) entry = a.ptab[(size_t)a.seq[g0 + ro_tail(par + g0, tid - g0, a.beams).x] * a.maxp + col];
+  __syncthreads();
+  if (mine) a.ptab[(size_t)a.seq[tid] * a.maxp + col] = entry;
+  if (tid == 0) *a.done = 0;
 }
 
 template <int VEC, int LP, bool ONE, int HC>
@@ -631,6 +650,18 @@ constexpr size_t BS_GROUPS = 65536;  // arrival counters, at the front of the sc
 
 }  // namespace
 
+syn_status_t more_smem(const void* fn, size_t bytes) {
+  static std::mutex mu;
+  static std::vector<std::pair<const void*, int>> done;
+  int dev = 0;
+  SYN_CUDA_TRY(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> g(mu);
+  if (std::find(done.begin(), done.end(), std::make_pair(fn, dev)) != done.end()) return SYN_OK;
+  SYN_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.push_back({fn, dev});
+  return SYN_OK;
+}
+
 syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, cudaStream_t st) {
   const size_t row4 = c->n_kv * c->hd / 4, page4 = c->page * row4;
   const int n4 = (int)(rows * row4);
@@ -703,6 +734,7 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
   a.row4 = (int)(c->n_kv * c->hd / 4);
   a.layer4 = c->n_pages * c->page * a.row4;
   a.ptab = c->d_ptab;
+  a.done = c->d_ptab + c->batch * c->maxp;
   a.maxp = (int)c->maxp;
   a.page = (int)c->page;
   a.parents = parents;
@@ -716,21 +748,12 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
     tail = std::max(tail, lens[g] % c->page);
   }
   if (!cols) return SYN_OK;
-  if (tail) {
-    const unsigned ch = (unsigned)std::min<size_t>(16, (tail * a.row4 + 255) / 256);
-    for (size_t l0 = 0; l0 < c->layers; l0 += 32768) {
-      const unsigned nl = (unsigned)std::min<size_t>(c->layers - l0, 32768);
-      ReorderArgs b = a;
-      b.k += l0 * a.layer4;
-      b.v += l0 * a.layer4;
-      k_reorder_copy<<<dim3(ch, (unsigned)n, nl), 256, 0, st>>>(b);
-    }
-    SYN_LAUNCH_CHECK("k_reorder_copy");
-  }
-  k_reorder_tables<<<dim3((unsigned)((cols + 31) / 32), (unsigned)(n / beams)), 256,
-                     beams * 33 * sizeof(int), st>>>(a);
-  SYN_LAUNCH_CHECK("k_reorder_tables");
-  return SYN_OK;
+  if (c->layers > 65534) return SYN_ERR_UNSUPPORTED;
+  // about four 16-byte copies a thread, K and V: 28 layers x 20 beams x 28 rows of 4 KB (257 MB
+  // read and written) take 39 us; one copy a thread takes 64
+  const unsigned ch = (unsigned)std::max<size_t>(1, std::min<size_t>(16, (tail * a.row4 + 1023) / 1024));
+  return launched(launch_pdl(k_reorder, dim3(ch, (unsigned)n, (unsigned)c->layers + 1), dim3(256), 0, st, a),
+                  "k_reorder");
 }
 
 syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, size_t n,
@@ -749,14 +772,14 @@ syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, s
     a.rows = (int)rows;
     if (rows) {
       const AppendShape sh = append_shape(a);
-      // four heads a lane group once that still fills the device
+      // two heads a lane group once that still fills the device
       const size_t heads = a.n_heads + 2 * a.n_kv, per = AP_THREADS / sh.lp;
-      const bool many = sh.one && rows * heads >= 4 * per * AP_FILL;
+      const bool many = sh.one && rows * heads >= 2 * per * AP_FILL;
       void (*kern)(const AppendArgs) = !sh.vec   ? k_append_batch<1, 32, false, 1>
                                        : !sh.one ? k_append_batch<4, 32, false, 1>
-                                       : many    ? append_kernel<4>(sh.lp)
+                                       : many    ? append_kernel<2>(sh.lp)
                                                  : append_kernel<1>(sh.lp);
-      const size_t units = rows * (many ? (heads + 3) / 4 : heads), blocks = (units + per - 1) / per;
+      const size_t units = rows * (many ? (heads + 1) / 2 : heads), blocks = (units + per - 1) / per;
       if (blocks > 0x7FFFFFFF) return SYN_ERR_UNSUPPORTED;
       syn_status_t s = launched(launch_pdl(kern, dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a),
                                 "k_append_batch");
@@ -803,8 +826,10 @@ syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t
   a.cap = (int)cap;
   if (smem > 200 * 1024) return SYN_ERR_UNSUPPORTED;
   void (*kern)(const BeamArgs) = a.tiles > 2 ? k_beam_select<16> : k_beam_select<8>;
-  if (smem > 40 * 1024)
-    SYN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+  if (smem > 40 * 1024) {
+    syn_status_t s = more_smem((const void*)kern, 200 * 1024);
+    if (s) return s;
+  }
   return launched(launch_pdl(kern, dim3((unsigned)a.nseg, (unsigned)rows), dim3(BS_THREADS), smem, st, a),
                   "k_beam_select");
 }

@@ -70,7 +70,7 @@ struct syn_cuda_kvcache_s {
   // sequence grows and returned when it is truncated or reset.
   size_t page, n_pages, maxp;
   int* ptab_h;       // pinned host table [batch][maxp], -1 = none
-  int* d_ptab;       // device copy
+  int* d_ptab;       // device copy, and behind it a counter that k_reorder leaves at zero
   int* free_pages;   // stack of free page ids (host)
   size_t n_free;
   // A page can be in several sequences' tables (syn_cuda_kvcache_fork). refs
@@ -302,6 +302,9 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 // pages reserved).
 syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& a, int* err,
                                 cudaStream_t st);
+// Lets a kernel have `bytes` of dynamic shared memory on the current device (asked of the
+// runtime once per kernel and device; always with the same bytes for a kernel).
+syn_status_t more_smem(const void* fn, size_t bytes);
 size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms);
 syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
                                 size_t vocab, const float* scores, const uint8_t* fin, int eos,

@@ -2268,7 +2268,8 @@ syn_status_t syn_cuda_kvcache_create_paged(syn_cuda_ctx_t* ctx, size_t max_seq,
   if (e == cudaSuccess) e = cudaMemset(c->d_len, 0, batch * sizeof(int));
   if (e == cudaSuccess && page) {
     e = cudaMallocHost(&c->ptab_h, batch * c->maxp * sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc(&c->d_ptab, batch * c->maxp * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&c->d_ptab, (batch * c->maxp + 1) * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(c->d_ptab + batch * c->maxp, 0, sizeof(int));
     c->free_pages = e == cudaSuccess ? new (std::nothrow) int[n_pages] : nullptr;
     c->refs = e == cudaSuccess ? new (std::nothrow) int[n_pages]() : nullptr;
     c->stale = e == cudaSuccess ? new (std::nothrow) uint8_t[batch]() : nullptr;

@@ -1165,12 +1165,6 @@ syn_status_t launched(cudaError_t e, const char* where) {
   return SYN_ERR_CUDA;
 }
 
-syn_status_t more_smem(const void* fn, size_t bytes) {
-  if (bytes > 48 * 1024)
-    SYN_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return SYN_OK;
-}
-
 // Most jobs and items of a batch of `batch` rows (groups of two or more share).
 size_t max_jobs(size_t batch, size_t n_kv, size_t G) {
   return n_kv * (batch * G / PM + batch / 2 + 1);
