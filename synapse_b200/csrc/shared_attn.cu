@@ -134,7 +134,7 @@ struct SharedArgs {
 // Shared prefixes on the tensor cores. A job is 128 query rows (tensor-memory
 // lanes) of one group and KV head; a CTA runs through its items' tiles of 64
 // keys:
-//   8 warps load K and V rows (8 lanes a row) straight into registers, a tile
+//   16 warps load K and V rows (8 lanes a row) straight into registers, a tile
 //     ahead, and write them as fp16 hi + lo parts, x' = x 2^-e = hi + lo with
 //     lo = fp16(x' - hi) and e from the row's largest element: 22 bits,
 //     whatever the rows' magnitudes. An item's Q goes the same way first;
@@ -154,13 +154,13 @@ struct SharedArgs {
 // than 2^8 (P keeps 2^7 as its nominal top, so it stays below fp16's 2^16).
 // Waits are bounded (SYN_ERR_TIMEOUT).
 // ---------------------------------------------------------------------------
-constexpr int PX_SOFT = 8, PX_CONV = 8;  // warps; then four of which one issues the products
+constexpr int PX_SOFT = 8, PX_CONV = 16;  // warps; then four of which one issues the products
 constexpr int PX_MMA_WARP = PX_SOFT + PX_CONV;
 constexpr int PX_THREADS = 32 * (PX_SOFT + PX_CONV + 4);
-// Registers a thread: 96 at launch (20 warps), which the softmax keeps; what the last four
-// warps give up is the converters'.
-constexpr int PX_REGS = 96, PX_REGS_SOFT = 96, PX_REGS_CONV = 112, PX_REGS_MMA = 56;
-static_assert(2 * PX_REGS_SOFT + 2 * PX_REGS_CONV + PX_REGS_MMA <= 5 * PX_REGS, "register split");
+// Registers a thread: 72 at launch (28 warps); what the converters and the last four warps
+// give up is the softmax's.
+constexpr int PX_REGS = 72, PX_REGS_SOFT = 88, PX_REGS_CONV = 64, PX_REGS_MMA = 64;
+static_assert(2 * PX_REGS_SOFT + 4 * PX_REGS_CONV + PX_REGS_MMA <= 7 * PX_REGS, "register split");
 constexpr float P_TOP = 7.0f, P_GROW = 8.0f;
 
 template <int HDP>
@@ -258,16 +258,16 @@ __device__ __forceinline__ void pair_sync(int id) {  // the two warps of the sam
   asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
 
-// Two rows, j and j + 2, of an operand of `rows` rows, 8 lanes a row (lane l has the
+// NR rows, j, j + 2, of an operand of `rows` rows, 8 lanes a row (lane l has the
 // float4s l, l + 8, ...): the fp16 parts into `part` and psize bytes behind it; the
 // rows' exponents.
-template <int NV>
-__device__ __forceinline__ void px_rows(const float4 (&v)[2][NV], uint8_t* part, int psize, int rows, int j,
-                                        int (&eb)[2]) {
+template <int NV, int NR>
+__device__ __forceinline__ void px_rows(const float4 (&v)[NR][NV], uint8_t* part, int psize, int rows, int j,
+                                        int (&eb)[NR]) {
   const int l8 = threadIdx.x & 7;
-  float m[2];
+  float m[NR];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
+  for (int i = 0; i < NR; i++) {
     m[i] = 0.0f;
 #pragma unroll
     for (int u = 0; u < NV; u++)
@@ -276,9 +276,9 @@ __device__ __forceinline__ void px_rows(const float4 (&v)[2][NV], uint8_t* part,
 #pragma unroll
   for (int o = 4; o; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < 2; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+    for (int i = 0; i < NR; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
+  for (int i = 0; i < NR; i++) {
     const int k = j + 2 * i;
     eb[i] = px_exp(m[i]);
     const f32x2 down = pk(px_down(eb[i]), px_down(eb[i]));
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
 
   if (warp < PX_SOFT) {
     // ---- two threads per query row: half h has keys 32h .. 32h+31 of a tile ----
-    if constexpr (PX_REGS_SOFT < PX_REGS) less_regs<PX_REGS_SOFT>();
+    more_regs<PX_REGS_SOFT>();
     const int h = warp >> 2, r = tid & 127, pair = 1 + (warp & 3);
     const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     bool ok = true;
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           }
         }
         int eb[2];
-        px_rows<NV>(v, sm + L::Q, L::QPART, PM, j, eb);
+        px_rows<NV, 2>(v, sm + L::Q, L::QPART, PM, j, eb);
         if (l8 == 0) {
           qup[j] = px_up(eb[0]);
           qup[j + 2] = px_up(eb[1]);
@@ -550,19 +550,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       }
     }
   } else if (warp < PX_MMA_WARP) {
-    // ---- K and V rows to fp16 parts: 8 lanes a row, 4 rows a step; warp w has keys 8w .. 8w+7 of a
-    // tile. (A step's rows are 0, 4, 1, 5 or 2, 6, 3, 7 of the 8: their stores meet all banks.)
-    more_regs<PX_REGS_CONV>();
+    // ---- K and V rows to fp16 parts: 8 lanes a row, 4 rows of each a warp and tile. (Of 8 rows, a
+    // warp has 0, 4, 1, 5 or 2, 6, 3, 7: their stores meet all banks.)
+    less_regs<PX_REGS_CONV>();
     const int cw = warp - PX_SOFT, l8 = lane & 7, q4 = lane >> 3;
-    const int jj = cw * 8 + (((q4 & 1) << 2) | (q4 >> 1));  // this lane's keys: jj and jj + 2
+    const int jj = (cw >> 1) * 8 + (((q4 & 1) << 2) | (q4 >> 1)) + (cw & 1) * 2;  // this lane's key
     const int dcol = PT / a.page, doff = PT - dcol * a.page;
     // Three tiles are under way: x holds one's rows, `at` has the next one's places, `pg` the
     // page numbers of the one after as they come.
     int it = i0, left = 0;  // the item of the last tile asked for, and its tiles still to ask for
-    int len = 0, lowest = 0, pos = 0, kvh = 0, col[2], off[2];
+    int len = 0, lowest = 0, pos = 0, kvh = 0, col = 0, off = 0;
     const int* tab = nullptr;
-    struct Pages { int kvh, pg[2], off[2]; };  // kvh < 0: no tile
-    struct Rows { bool any; long long at[2]; };  // at < 0: no row
+    struct Pages { int kvh, pg, off; };  // kvh < 0: no tile
+    struct Rows { bool any; long long at; };  // at < 0: no row
     auto ask = [&]() {
       Pages r;
       if (left == 0) {
@@ -575,25 +575,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           kvh = item.kvh;
           tab = a.ptab + (size_t)item.seq * a.maxp;
           pos = item.t0 * PT + jj;
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            col[i] = (pos + 2 * i) / a.page;
-            off[i] = pos + 2 * i - col[i] * a.page;
-          }
+          col = pos / a.page;
+          off = pos - col * a.page;
         }
       }
       r.kvh = left ? kvh : -1;
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int p = pos + 2 * i;
-        r.pg[i] = left && p < len && p >= lowest ? __ldg(tab + col[i]) : -1;
-        r.off[i] = off[i];
-        col[i] += dcol;
-        off[i] += doff;
-        if (off[i] >= a.page) {
-          off[i] -= a.page;
-          col[i]++;
-        }
+      r.pg = left && pos < len && pos >= lowest ? __ldg(tab + col) : -1;
+      r.off = off;
+      col += dcol;
+      off += doff;
+      if (off >= a.page) {
+        off -= a.page;
+        col++;
       }
       pos += PT;
       if (left) left--;
@@ -602,22 +595,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     auto place = [&](const Pages& p) {
       Rows r;
       r.any = p.kvh >= 0;
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        r.at[i] = p.pg[i] < 0 ? -1 : (((long long)p.pg[i] * a.page + p.off[i]) * a.n_kv + p.kvh) * a.hd + l8 * 4;
+      r.at = p.pg < 0 ? -1 : (((long long)p.pg * a.page + p.off) * a.n_kv + p.kvh) * a.hd + l8 * 4;
       return r;
     };
-    auto load = [&](float4 (&v)[2][NV], const float* cache, const Rows& r) {
+    auto load = [&](float4 (&v)[1][NV], const float* cache, const Rows& r) {
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int u = 0; u < NV; u++) {
-          v[i][u] = make_float4(0, 0, 0, 0);
-          if (r.at[i] >= 0 && u * 32 + l8 * 4 < a.hd)
-            v[i][u] = __ldg(reinterpret_cast<const float4*>(cache + r.at[i] + u * 32));
-        }
+      for (int u = 0; u < NV; u++) {
+        v[0][u] = make_float4(0, 0, 0, 0);
+        if (r.at >= 0 && u * 32 + l8 * 4 < a.hd)
+          v[0][u] = __ldg(reinterpret_cast<const float4*>(cache + r.at + u * 32));
+      }
     };
-    float4 xk[2][NV], xv[2][NV];
+    float4 xk[1][NV], xv[1][NV];
     Pages pages = ask();
     Rows next = place(pages);
     pages = ask();
@@ -631,21 +620,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       const int s = n & 1, use = n >> 1;
       uint8_t* st = sm + s * L::STAGE;
       if (use && !(ok = wait(&qk_done[s], use - 1))) break;
-      int ek[2], ev[2];
-      px_rows<NV>(xk, st, L::PART, PT, jj, ek);
+      int ek[1], ev[1];
+      px_rows<NV, 1>(xk, st, L::PART, PT, jj, ek);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[s]);
       load(xk, a.kc, next);
       if (use && !(ok = wait(&pv_done[s], use - 1))) break;
-      px_rows<NV>(xv, st + 2 * L::PART, L::PART, PT, jj, ev);
+      px_rows<NV, 1>(xv, st + 2 * L::PART, L::PART, PT, jj, ev);
       if (l8 == 0) {  // (the softmax is done with the stage's last scales: P was used)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          kup[s][jj + 2 * i] = px_up(ek[i]);
-          vexp[s][jj + 2 * i] = (float)(ev[i] - 140);
-          vdown[s][jj + 2 * i] = px_down(ev[i]);
-        }
+        kup[s][jj] = px_up(ek[0]);
+        vexp[s][jj] = (float)(ev[0] - 140);
+        vdown[s][jj] = px_down(ev[0]);
       }
       fence_async_smem();
       __syncwarp();
