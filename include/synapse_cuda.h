@@ -545,6 +545,24 @@ syn_status_t syn_cuda_generate_speculative(syn_cuda_model_t *m, size_t seq, int3
                                            size_t n_steps, size_t k, size_t draft_layers,
                                            int32_t *out_tokens, size_t *drafted,
                                            size_t *accepted);
+/* Beam search (no counterpart in the reference): prefills the n_prompt tokens
+ * into the empty sequence `seq` and keeps the `beams` continuations with the
+ * largest sum of log-probabilities, in the sequences seq .. seq+beams-1 (all
+ * empty), for n_steps tokens, chained on the device: each step is one graph
+ * (the step's layers with syn_cuda_attention_decode_shared, or for INT8 models
+ * the decode attention in the reference's order; syn_cuda_beam_select) and one
+ * reordering of the contexts. A beam that generates eos (< 0: none) ends: it keeps
+ * its score and is filled up with eos; the search ends with n_steps or, tested
+ * every 16 steps, when all beams have ended. out_tokens: [beams][n_steps], best
+ * first; out_scores: [beams] or NULL. Sequence seq+i then holds the context of
+ * hypothesis i but for its last generated token, as after syn_cuda_generate.
+ * Equal values go to the lower beam, the larger logit, the lower token. Paged
+ * models at one rank only (SYN_ERR_UNSUPPORTED), beams <= 64. All pages are
+ * taken before the first step: the prompt's, and for each beam those that it
+ * writes to. On an error the sequences are empty again. */
+syn_status_t syn_cuda_generate_beam(syn_cuda_model_t *m, size_t seq, const int32_t *prompt,
+                                    size_t n_prompt, size_t beams, size_t n_steps,
+                                    int32_t eos, int32_t *out_tokens, float *out_scores);
 syn_status_t syn_cuda_model_seq_len(const syn_cuda_model_t *m, size_t seq, size_t *len);
 syn_status_t syn_cuda_model_reset(syn_cuda_model_t *m, size_t seq);
 syn_status_t syn_cuda_model_truncate(syn_cuda_model_t *m, size_t seq, size_t new_len);

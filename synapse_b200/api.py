@@ -940,6 +940,23 @@ class Model:
                 "generate_speculative")
         return [tok] + out.tolist(), nd.value, na.value
 
+    def generate_beam(self, prompt, steps, beams=4, eos=-1, seq=0):
+        """Beam search over the prompt (syn_cuda_generate_beam) in the empty
+        sequences [seq, seq + beams) of a paged model: (tokens int32
+        [beams, steps], best first and filled up with eos; sums of
+        log-probabilities f32 [beams])."""
+        import numpy as np
+        ids = np.ascontiguousarray(np.asarray(prompt, dtype=np.int32).reshape(-1))
+        if steps < 1 or beams < 1 or seq < 0:
+            raise SynapseError(2, "generate_beam")
+        out = np.empty((beams, steps), dtype=np.int32)
+        scores = np.empty(beams, dtype=np.float32)
+        _check(lib().syn_cuda_generate_beam(
+            self.handle, seq, ids.ctypes.data_as(ctypes.c_void_p), ids.size, beams, steps, eos,
+            out.ctypes.data_as(ctypes.c_void_p), scores.ctypes.data_as(ctypes.c_void_p)),
+            "generate_beam")
+        return out, scores
+
     def seq_len(self, seq=0):
         v = ctypes.c_size_t()
         _check(lib().syn_cuda_model_seq_len(self.handle, seq, ctypes.byref(v)), "model_seq_len")

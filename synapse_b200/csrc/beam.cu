@@ -195,7 +195,7 @@ void (*append_kernel(int lp))(const AppendArgs) {
 // ranked by counting. Which CTA is last changes no result.
 // Bound by HBM for many rows (4 bytes a logit), by latency for few.
 // ---------------------------------------------------------------------------
-constexpr int BS_THREADS = 256, BS_KMAX = 64, BS_BMAX = 64;
+constexpr int BS_THREADS = 256, BS_KMAX = (int)BEAMS_MAX, BS_BMAX = (int)BEAMS_MAX;
 
 __device__ __forceinline__ uint32_t ord32(float x) {  // order-preserving, > 0 for every float
   const uint32_t u = __float_as_uint(x + 0.0f);       // (-0 becomes 0)
@@ -648,7 +648,30 @@ int beam_tiles(size_t rows, size_t vocab, int sms) {
 }
 constexpr size_t BS_GROUPS = 65536;  // arrival counters, at the front of the scratch
 
+// A few numbers a step; in the step's graph, so that nothing of it changes with the position.
+__global__ void k_beam_note(int* len, const int* slots, int n, int advance, const int32_t* tok,
+                            const int32_t* par, int32_t* hist, int32_t* hist_parent, int ld) {
+  griddep_wait();
+  griddep_launch();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int s = slots[i], at = len[s] + advance;
+    if (at < ld) {
+      hist[(size_t)s * ld + at] = tok[i];
+      hist_parent[(size_t)s * ld + at] = par[i];
+      len[s] = at;
+    }
+  }
+}
+
 }  // namespace
+
+syn_status_t launch_beam_note(syn_cuda_kvcache_t* c, const int* slots, size_t n, int advance,
+                              const int32_t* tok, const int32_t* par, int32_t* hist,
+                              int32_t* hist_parent, int ld, cudaStream_t st) {
+  return launched(launch_pdl(k_beam_note, dim3(1), dim3(64), 0, st, c->d_len, slots, (int)n, advance,
+                             tok, par, hist, hist_parent, ld),
+                  "k_beam_note");
+}
 
 syn_status_t more_smem(const void* fn, size_t bytes) {
   static std::mutex mu;

@@ -302,6 +302,12 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 // pages reserved).
 syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& a, int* err,
                                 cudaStream_t st);
+// Tokens and parents of n beams kept at their sequences' position (d_len + advance, which
+// becomes the length; slots on the device): hist[slot * ld + position], parents likewise.
+syn_status_t launch_beam_note(syn_cuda_kvcache_t* c, const int* slots, size_t n, int advance,
+                              const int32_t* tok, const int32_t* par, int32_t* hist,
+                              int32_t* hist_parent, int ld, cudaStream_t st);
+constexpr size_t BEAMS_MAX = 64;  // beams of a group, continuations of a selection
 // Lets a kernel have `bytes` of dynamic shared memory on the current device (asked of the
 // runtime once per kernel and device; always with the same bytes for a kernel).
 syn_status_t more_smem(const void* fn, size_t bytes);

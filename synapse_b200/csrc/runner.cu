@@ -22,6 +22,7 @@
 #include <map>
 #include <new>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "internal.cuh"
@@ -270,6 +271,17 @@ struct syn_cuda_model_s {
   std::map<std::pair<size_t, int>, cudaGraphExec_t> graphs;
   std::map<std::pair<size_t, int>, int> eager_runs;
   std::map<size_t, cudaGraphExec_t> chain_graphs;  // chained decode step per batch
+  // beam search (allocated by the first syn_cuda_generate_beam): the sum of log-probabilities,
+  // the parent and the end flag of each beam, parents per position beside `hist`
+  syn_cuda_decode_plan_t* plan = nullptr;  // of the block formats; INT8 keeps its exact order
+  float* beam_score = nullptr;
+  int32_t* beam_parent = nullptr;
+  uint8_t* beam_fin = nullptr;
+  uint8_t* beam_fin_h = nullptr;  // pinned
+  int32_t* hist_parent = nullptr;
+  void* beam_scratch = nullptr;
+  // captured steps; what a step's launches are made from
+  std::map<std::tuple<size_t, bool, int32_t, void*, void*, void*, void*>, cudaGraphExec_t> beam_graphs;
 };
 
 namespace {
@@ -355,9 +367,28 @@ syn_status_t mm(syn_cuda_model_s* m, const syn_cuda_weight_t* w, const float* x,
 // logits and greedy tokens for every row into the span buffers, no cache
 // length advanced. nlayers < L runs only the first nlayers layers (the
 // reference's layer-skipping draft, pipeline.rs:281-330).
+// beam: a chained step of beams (sequences `slots`): attention by the plan where there is one, the best
+// continuations instead of each row's greedy token.
+struct BeamStep {
+  syn_cuda_decode_plan_t* plan;  // or nullptr
+  int32_t eos;                   // -1: none
+};
+
+// The `rows` best continuations of `beams` rows of logits: scores, parents and end flags into
+// the model's arrays, tokens into tok, both kept beside the sequences' next position.
+syn_status_t beam_best(syn_cuda_model_s* m, size_t beams, size_t rows, int32_t eos, int advance) {
+  syn_status_t s = launch_beam_select(
+      m->logits, m->V, 1, beams, m->V, m->beam_score, eos >= 0 ? m->beam_fin : nullptr, eos, rows,
+      m->beam_score, m->beam_parent, m->tok, eos >= 0 ? m->beam_fin : nullptr, m->beam_scratch,
+      m->ctx->sms, m->st);
+  if (s) return s;
+  return launch_beam_note(m->cache, m->slots_d, rows, advance, m->tok, m->beam_parent, m->hist,
+                          m->hist_parent, (int)(m->max_seq + 1), m->st);
+}
+
 syn_status_t forward(syn_cuda_model_s* m, size_t rows, bool prefill, size_t seq, bool want_logits,
                      bool chained = false, size_t nlayers = 0, bool span = false,
-                     const int* slots = nullptr) {
+                     const int* slots = nullptr, const BeamStep* beam = nullptr) {
   cudaStream_t st = m->st;
   syn_status_t s;
   const size_t h = m->h;
@@ -411,6 +442,7 @@ syn_status_t forward(syn_cuda_model_s* m, size_t rows, bool prefill, size_t seq,
     a.layer = li;
     a.out = m->att;
     s = span      ? launch_attn_span_args(a, seq, rows, m->ctx->err, st)
+        : beam && beam->plan ? launch_attn_shared(beam->plan, a, m->ctx->err, st)
         : prefill ? launch_attn_prefill_args(a, seq, rows, m->ctx->err, st)
                   : launch_attn_decode_args(a, rows, m->ctx->err, st);
     if (s) return s;
@@ -465,6 +497,7 @@ syn_status_t forward(syn_cuda_model_s* m, size_t rows, bool prefill, size_t seq,
                                    cudaMemcpyDeviceToHost, st));
     return SYN_OK;
   }
+  if (beam) return beam_best(m, rows, rows, beam->eos, 1);
   // vocab-parallel LM head. A greedy step without host logits gathers each
   // rank's argmax state over its slice (16 bytes per row), not the logits;
   // SYN_TP_ARGMAX_PAIRS=0 gathers the logits always.
@@ -1027,6 +1060,170 @@ syn_status_t syn_cuda_generate_speculative(syn_cuda_model_t* m, size_t seq, int3
   return SYN_OK;
 }
 
+namespace {
+
+// Buffers and plan of beam searches: once for a model.
+syn_status_t beam_buffers(syn_cuda_model_s* m) {
+  if (m->beam_scratch) return SYN_OK;
+  syn_status_t s;
+  const size_t most = std::min<size_t>(m->max_batch, BEAMS_MAX);
+  size_t bytes = 0;
+  for (size_t b = 1; b <= most; b++)
+    bytes = std::max({bytes, beam_scratch_bytes(b, m->V, b, m->ctx->sms),
+                      beam_scratch_bytes(1, m->V, b, m->ctx->sms)});
+  if (!m->plan && !m->int8) {
+    s = syn_cuda_decode_plan_create(m->cache, m->hq_l, &m->plan);
+    if (s && s != SYN_ERR_UNSUPPORTED) return s;  // (other heads: each row's whole context)
+  }
+  if (!m->beam_score && (s = dev_alloc_t(m, &m->beam_score, most))) return s;
+  if (!m->beam_parent && (s = dev_alloc_t(m, &m->beam_parent, most))) return s;
+  if (!m->beam_fin && (s = dev_alloc_t(m, &m->beam_fin, most))) return s;
+  if (!m->hist_parent && (s = dev_alloc_t(m, &m->hist_parent, m->max_batch * (m->max_seq + 1)))) return s;
+  if (!m->beam_fin_h) SYN_CUDA_TRY(cudaMallocHost(&m->beam_fin_h, BEAMS_MAX));
+  void* scratch = nullptr;
+  if ((s = dev_alloc(m, &scratch, bytes))) return s;
+  SYN_CUDA_TRY(cudaMemset(scratch, 0, bytes));
+  SYN_CUDA_TRY(cudaDeviceSynchronize());
+  m->beam_scratch = scratch;
+  return SYN_OK;
+}
+
+// One step of every beam: by its graph where there is one (or `capture` makes it).
+syn_status_t beam_step(syn_cuda_model_s* m, size_t beams, bool shared, const BeamStep& bs, bool capture) {
+  // (growing scratch buffers move: their addresses are part of the key)
+  const auto key = std::make_tuple(beams, shared, bs.eos, (void*)m->ctx->part, (void*)m->ctx->cnt,
+                                   (void*)m->ctx->abuf, (void*)m->cache->part);
+  auto it = m->beam_graphs.find(key);
+  if (it == m->beam_graphs.end() && !capture)
+    return forward(m, beams, false, 0, false, true, 0, false, m->slots_d, &bs);
+  if (it == m->beam_graphs.end()) {
+    if (m->beam_graphs.size() >= 16) {  // (each search ends with its stream drained)
+      for (auto& kv : m->beam_graphs) cudaGraphExecDestroy(kv.second);
+      m->beam_graphs.clear();
+    }
+    cudaGraph_t graph = nullptr;
+    SYN_CUDA_TRY(cudaStreamBeginCapture(m->st, cudaStreamCaptureModeThreadLocal));
+    syn_status_t s = forward(m, beams, false, 0, false, true, 0, false, m->slots_d, &bs);
+    cudaError_t e = cudaStreamEndCapture(m->st, &graph);
+    if (s == SYN_OK && e != cudaSuccess) s = cuda_status_r(e, "cudaStreamEndCapture");
+    if (s) {
+      if (graph) cudaGraphDestroy(graph);
+      return s;
+    }
+    cudaGraphExec_t exec = nullptr;
+    e = cudaGraphInstantiate(&exec, graph, 0);
+    cudaGraphDestroy(graph);
+    if (e != cudaSuccess) return cuda_status_r(e, "cudaGraphInstantiate");
+    it = m->beam_graphs.emplace(key, exec).first;
+  }
+  SYN_CUDA_TRY(cudaGraphLaunch(it->second, m->st));
+  return SYN_OK;
+}
+
+// Prompt, then n_steps tokens for each beam; *steps_run of them before every beam had ended.
+syn_status_t beam_search(syn_cuda_model_s* m, size_t seq, const int32_t* prompt, size_t n,
+                         size_t beams, size_t n_steps, int32_t eos, size_t* steps_run) {
+  syn_cuda_kvcache_t* c = m->cache;
+  cudaStream_t st = m->st;
+  syn_status_t s;
+  int32_t first;
+  if ((s = syn_cuda_prefill(m, seq, prompt, n, nullptr, &first))) return s;
+  int32_t seqs[BEAMS_MAX];
+  for (size_t b = 0; b < beams; b++) seqs[b] = m->slots_h[b] = (int32_t)(seq + b);
+  SYN_CUDA_TRY(cudaMemcpyAsync(m->slots_d, m->slots_h, beams * sizeof(int), cudaMemcpyHostToDevice, st));
+  SYN_CUDA_TRY(cudaMemsetAsync(m->beam_score, 0, beams * sizeof(float), st));
+  SYN_CUDA_TRY(cudaMemsetAsync(m->beam_fin, 0, beams, st));
+  for (size_t b = 1; b < beams; b++)
+    if ((s = syn_cuda_kvcache_fork(c, seq, seq + b, n, st))) return s;
+  for (size_t b = 0; b < beams; b++)  // every page that the steps will write
+    if ((s = kv_reserve(c, seq + b, n + n_steps - 1, st))) return s;
+  BeamStep bs{m->plan, eos};
+  size_t shared = 0;
+  if (m->plan) {
+    if ((s = syn_cuda_decode_plan_set(m->plan, 1, &beams, seqs, st))) return s;
+    if ((s = syn_cuda_decode_plan_prefix(m->plan, 0, &shared))) return s;
+  }
+  if ((s = beam_best(m, 1, beams, eos, 0))) return s;
+  for (size_t t = 1; t < n_steps; t++) {
+    // the first step sizes the scratch buffers; the second is captured
+    if ((s = beam_step(m, beams, shared > 0, bs, t > 1 && use_graphs()))) return s;
+    for (size_t b = 0; b < beams; b++) c->len[seq + b]++;
+    if (beams > 1) {
+      if ((s = launch_kv_reorder(c, beams, seqs, m->beam_parent, beams, &c->len[seq], st))) return s;
+      for (size_t b = 0; b < beams; b++) {
+        c->n_stale += !c->stale[seq + b];
+        c->stale[seq + b] = std::max<uint8_t>(c->stale[seq + b], 1);
+      }
+    }
+    *steps_run = t + 1;
+    if (eos >= 0 && t % 16 == 0 && t + 1 < n_steps) {
+      SYN_CUDA_TRY(cudaMemcpyAsync(m->beam_fin_h, m->beam_fin, beams, cudaMemcpyDeviceToHost, st));
+      SYN_CUDA_TRY(cudaStreamSynchronize(st));
+      if (std::all_of(m->beam_fin_h, m->beam_fin_h + beams, [](uint8_t f) { return f != 0; })) break;
+    }
+  }
+  return SYN_OK;
+}
+
+}  // namespace
+
+syn_status_t syn_cuda_generate_beam(syn_cuda_model_t* m, size_t seq, const int32_t* prompt,
+                                    size_t n_prompt, size_t beams, size_t n_steps, int32_t eos,
+                                    int32_t* out_tokens, float* out_scores) {
+  if (!m || !prompt || !out_tokens) return SYN_ERR_NULL_PTR;
+  if (!m->finalized || !n_prompt || !n_steps || !beams) return SYN_ERR_INVALID_ARG;
+  if (m->tp > 1 || !m->kv_page) return SYN_ERR_UNSUPPORTED;
+  if (beams > BEAMS_MAX || m->V > 1u << 25) return SYN_ERR_UNSUPPORTED;
+  if (seq >= m->max_batch || beams > m->max_batch - seq || beams > m->V) return SYN_ERR_INVALID_ARG;
+  if (eos >= 0 && (size_t)eos >= m->V) return SYN_ERR_INVALID_ARG;
+  if (n_prompt > m->max_seq || n_steps - 1 > m->max_seq - n_prompt) return SYN_ERR_INVALID_ARG;  // CacheFull
+  syn_cuda_kvcache_t* c = m->cache;
+  for (size_t b = 0; b < beams; b++)
+    if (c->len[seq + b]) return SYN_ERR_INVALID_ARG;  // a search starts its sequences
+  DeviceGuard g(m->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  syn_status_t s = beam_buffers(m);
+  if (s) return s;
+  size_t run = 1;
+  s = beam_search(m, seq, prompt, n_prompt, beams, n_steps, eos < 0 ? -1 : eos, &run);
+  std::vector<int32_t> tok(beams * run), par(beams * run);
+  if (s == SYN_OK) {
+    const size_t ld = (m->max_seq + 1) * sizeof(int32_t), at = seq * (m->max_seq + 1) + n_prompt;
+    SYN_CUDA_TRY(cudaMemcpyAsync(m->err_h, m->ctx->err, sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    SYN_CUDA_TRY(cudaMemcpy2DAsync(tok.data(), run * sizeof(int32_t), m->hist + at, ld,
+                                   run * sizeof(int32_t), beams, cudaMemcpyDeviceToHost, m->st));
+    SYN_CUDA_TRY(cudaMemcpy2DAsync(par.data(), run * sizeof(int32_t), m->hist_parent + at, ld,
+                                   run * sizeof(int32_t), beams, cudaMemcpyDeviceToHost, m->st));
+    if (out_scores)
+      SYN_CUDA_TRY(cudaMemcpyAsync(out_scores, m->beam_score, beams * sizeof(float),
+                                   cudaMemcpyDeviceToHost, m->st));
+    SYN_CUDA_TRY(cudaStreamSynchronize(m->st));
+    if ((s = *m->err_h)) {
+      int32_t zero = 0;
+      cudaMemcpy(m->ctx->err, &zero, sizeof(zero), cudaMemcpyHostToDevice);
+      *m->err_h = 0;
+    }
+  }
+  // (pages back: those of dropped beams, and those reserved beyond an early end)
+  for (size_t b = 0; b < beams; b++) {
+    if (s) {
+      c->len[seq + b] = 0;
+      launch_kv_set(c, seq + b, 0, 0, m->st);
+    }
+    const syn_status_t r = kv_release(c, seq + b, c->len[seq + b], m->st);
+    if (!s) s = r;
+  }
+  if (s) return s;
+  for (size_t b = 0; b < beams; b++) {  // a hypothesis from its end: token, then parent
+    size_t at = b;
+    for (size_t t = n_steps; t-- > 0;) {
+      out_tokens[b * n_steps + t] = t < run ? tok[at * run + t] : eos;
+      if (t < run) at = (size_t)par[at * run + t];
+    }
+  }
+  return SYN_OK;
+}
+
 syn_status_t syn_cuda_model_seq_len(const syn_cuda_model_t* m, size_t seq, size_t* len) {
   if (!m || !len) return SYN_ERR_NULL_PTR;
   if (!m->finalized) return SYN_ERR_INVALID_ARG;
@@ -1059,6 +1256,8 @@ syn_status_t syn_cuda_model_destroy(syn_cuda_model_t* m) {
   if (m->st) cudaStreamSynchronize(m->st);
   for (auto& kv : m->graphs) cudaGraphExecDestroy(kv.second);
   for (auto& kv : m->chain_graphs) cudaGraphExecDestroy(kv.second);
+  for (auto& kv : m->beam_graphs) cudaGraphExecDestroy(kv.second);
+  if (m->plan) syn_cuda_decode_plan_destroy(m->plan);
   for (auto& ly : m->layers) {
     if (ly.qkv) syn_cuda_weight_destroy(ly.qkv);
     if (ly.o) syn_cuda_weight_destroy(ly.o);
@@ -1072,6 +1271,7 @@ syn_status_t syn_cuda_model_destroy(syn_cuda_model_t* m) {
   if (m->tok_h) cudaFreeHost(m->tok_h);
   if (m->span_tok_h) cudaFreeHost(m->span_tok_h);
   if (m->slots_h) cudaFreeHost(m->slots_h);
+  if (m->beam_fin_h) cudaFreeHost(m->beam_fin_h);
   if (m->logits_h) cudaFreeHost(m->logits_h);
   if (m->err_h) cudaFreeHost(m->err_h);
   if (m->st) cudaStreamDestroy(m->st);
