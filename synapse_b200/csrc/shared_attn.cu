@@ -336,9 +336,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     }
     return __all_sync(0xffffffffu, done) != 0;
   };
-  griddep_launch();
   // The plan, the lengths, the page table and the shared pages are from before k_begin, which
-  // let this kernel begin when they were in place: only the queries have to be waited for.
+  // let this kernel begin when they were in place: only the queries have to be waited for (and
+  // k_span, which reads what k_begin wrote and does not wait itself, begins after that).
   const int* start = a.meta + a.mv.start() + blockIdx.x;
   const int i0 = start[0], i1 = start[1];
   int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
     const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     bool ok = true;
     griddep_wait();
+    griddep_launch();
     for (int it = i0; it < i1 && ok; it++) {
       const Item item = px_item(a, it);
       const bool busy = (warp & 3) * 32 < item.m;  // else no row of this warp is one
@@ -1065,17 +1066,16 @@ __global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
 
 // ---------------------------------------------------------------------------
 // The parts of a query row: k_span's of its own positions, and of its prefix
-// k_span's or k_prefix's. A warp per (row, head). (Maxima are in units of log2.)
+// k_span's or k_prefix's. A CTA per (row, head): warp w takes records w, w + 4, ...,
+// up to eight of them in flight before their weights are known, since what bounds
+// this is the latency of its two loads. (Maxima are in units of log2.)
 // ---------------------------------------------------------------------------
-constexpr int JN_WARPS = 4;
+constexpr int JN_WARPS = 4, JN_BLOCK = 32;  // records at a time
 
 __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
+  __shared__ __align__(16) float red[JN_WARPS][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
-  const int i = blockIdx.x * JN_WARPS + warp, b = i / a.n_heads, head = i - b * a.n_heads;
-  if (b >= a.rows) {
-    griddep_wait();
-    return;
-  }
+  const int b = blockIdx.x / a.n_heads, head = blockIdx.x - b * a.n_heads;
   const int kvh = head / a.G, g = head - kvh * a.G;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
   // Records first + c * step, c < n. (The plan and k_begin's jobs may be read before the
@@ -1101,31 +1101,33 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
   auto rec = [&](int c) {
     return c < own.n ? own.first + (size_t)c * own.step : pre.first + (size_t)(c - own.n) * pre.step;
   };
+  const bool act = lane * 4 < hd;
+  float4 x[JN_BLOCK / JN_WARPS];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int e = 0; e < JN_BLOCK / JN_WARPS; e++) {
+      const int c = c0 + warp + e * JN_WARPS;
+      if (act && c < n) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd) + lane);
+    }
+  };
   griddep_wait();
   const float2 none = make_float2(-INFINITY, 0.0f);
   const float2 mine = lane < n ? __ldcg(&a.pml[rec(lane)]) : none;
+  fetch(0);
   float M = mine.x;
   for (int c = 32 + lane; c < n; c += 32) M = fmaxf(M, __ldcg(&a.pml[rec(c)]).x);
   M = warp_max(M);
   float4 o = make_float4(0, 0, 0, 0);
   float sum = 0.0f;
-  const bool act = lane * 4 < hd;
-  for (int c0 = 0; c0 < n; c0 += 32) {
+  for (int c0 = 0; c0 < n; c0 += JN_BLOCK) {
     const float2 ml = c0 == 0 ? mine : c0 + lane < n ? __ldcg(&a.pml[rec(c0 + lane)]) : none;
+    if (c0) fetch(c0);
     const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
     sum = fmaf(f, ml.y, sum);
-    const int k = min(32, n - c0);
-    for (int c = 0; c < k; c += 8) {  // eight records' loads in flight
-      float4 x[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        x[e] = make_float4(0, 0, 0, 0);
-        // (a part that saw nothing may hold anything)
-        if (__shfl_sync(0xffffffffu, f, (c + e) & 31) != 0.0f && act && c + e < k) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c0 + c + e) * hd) + lane);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float fc = __shfl_sync(0xffffffffu, f, (c + e) & 31);
+    for (int e = 0; e < JN_BLOCK / JN_WARPS; e++) {
+      const float fc = __shfl_sync(0xffffffffu, f, warp + e * JN_WARPS);
+      if (fc != 0.0f && act) {  // (a part that saw nothing may hold anything)
         o.x = fmaf(x[e].x, fc, o.x);
         o.y = fmaf(x[e].y, fc, o.y);
         o.z = fmaf(x[e].z, fc, o.z);
@@ -1134,15 +1136,13 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
     }
   }
   griddep_launch();
+  *reinterpret_cast<float4*>(&red[warp][lane * 4]) = o;
   sum = warp_sum(sum);
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f * sum;  // (NaN stays)
-  if (act) {
-    float* orow = a.out + (long long)b * a.ldo + (long long)head * hd + lane * 4;
-    orow[0] = o.x * inv;
-    orow[1] = o.y * inv;
-    orow[2] = o.z * inv;
-    orow[3] = o.w * inv;
-  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < hd)
+    a.out[(long long)b * a.ldo + (long long)head * hd + d] = ((red[0][d] + red[1][d]) + (red[2][d] + red[3][d])) * inv;
 }
 
 syn_status_t launched(cudaError_t e, const char* where) {
@@ -1241,9 +1241,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->sms), dim3(SP_WARPS * 32), span_smem(c->hd), st, a),
                "k_span");
   if (s) return s;
-  const size_t joins = p->rows * p->n_heads;
-  return launched(launch_pdl(k_join, dim3((unsigned)((joins + JN_WARPS - 1) / JN_WARPS)), dim3(JN_WARPS * 32), 0,
-                             st, a),
+  return launched(launch_pdl(k_join, dim3((unsigned)(p->rows * p->n_heads)), dim3(JN_WARPS * 32), 0, st, a),
                   "k_join");
 }
 
