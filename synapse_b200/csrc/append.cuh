@@ -47,8 +47,15 @@ template <int VEC> struct ApVec;
 template <> struct ApVec<4> { using T = float4; };
 template <> struct ApVec<1> { using T = float; };
 
-template <int VEC, int LP, bool ONE, int HC>
-__device__ __forceinline__ void append_rows(const AppendArgs& a) {
+// What else becomes of a rotated q row: find(row, head) before the wait for the kernels before,
+// take(...) with its lanes' elements j, j + LP, ... of each half.
+struct NoTaker {
+  __device__ void find(int, int) {}
+  template <int VEC, int LP, typename T> __device__ void take(int, int, const T (&)[2], const T (&)[2]) {}
+};
+
+template <int VEC, int LP, bool ONE, int HC, typename Taker = NoTaker>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, Taker taker = Taker()) {
   static_assert(ONE || HC == 1, "several heads are held in registers");
   using T = typename ApVec<VEC>::T;
   const int heads = a.n_heads + 2 * a.n_kv, half = a.hd >> 1, nv = half / VEC;
@@ -67,6 +74,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a) {
                                      : a.v + (long long)(h - a.n_heads - a.n_kv) * a.hd) +
            (long long)row * a.ld;
   };
+  if (live && HC == 1 && h0 < a.n_heads) taker.find(row, h0);
   griddep_wait();
   griddep_launch();
   T x1[HC], x2[HC];
@@ -132,7 +140,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a) {
                       : (is_v ? a.vc + (size_t)(h - a.n_heads - a.n_kv) * a.hd
                               : a.kc + (size_t)(h - a.n_heads) * a.hd) +
                             (size_t)slot * a.n_kv * a.hd;
-    for (int j = lane; j < nv; j += LP) {
+    T r1[2] = {}, r2[2] = {};  // (half a head row of up to 128 elements is two steps of 32 lanes)
+    for (int j = lane, step = 0; j < nv; j += LP, step ^= 1) {
       T b1, b2, c, sn;
       if (ONE) {
         b1 = x1[i];
@@ -170,7 +179,10 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a) {
       }
       reinterpret_cast<T*>(dst)[j] = b1;
       reinterpret_cast<T*>(dst + half)[j] = b2;
+      r1[ONE ? 0 : step] = b1;
+      r2[ONE ? 0 : step] = b2;
     }
+    if (is_q) taker.template take<VEC, LP>(lane, nv, r1, r2);
   }
 }
 

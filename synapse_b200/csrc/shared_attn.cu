@@ -36,6 +36,8 @@ struct syn_cuda_decode_plan_s {
   std::vector<size_t> prefix, shrunk;  // per row: shared positions; the sequence's state at _set
   // device
   float* q = nullptr;        // rotated queries [batch][n_heads * hd]
+  uint8_t* qparts = nullptr; // k_prefix's: as fp16 parts, job by job (QParts)
+  float* qup = nullptr;      // their rows' scales
   int* meta = nullptr;       // MetaView, copied from meta_h
   int* meta_h = nullptr;     // pinned
   cudaEvent_t copied = nullptr;
@@ -65,11 +67,12 @@ struct Job {      // prefix work of one (group, tile of query rows, KV head)
   int len;        // shared positions
   int part0;      // first partial record; split i is at part0 + i * m
   int splits;
+  int q0;         // query rows of the jobs before
 };
 struct Item {     // a CTA's share of a job: key tiles t0 .. t1, partial records from part
   int row0, m0, m, kvh;
   int len, t0, t1, part;
-  int seq, lowest, pad0, pad1;  // lowest: no row of the job sees a position below (set on the device)
+  int seq, lowest, q0, pad;  // lowest: no row of the job sees a position below (set on the device)
 };
 
 // k_span's work: the positions of one row behind its prefix (n = 0), or the
@@ -102,13 +105,15 @@ struct Meta {
   __host__ __device__ int start() const { return 4 * rows; }     // [ctas + 1] items of each CTA
   __host__ __device__ int items() const { return (start() + ctas + 1 + 3) / 4 * 4; }
   __host__ __device__ int jobs() const { return items() + 12 * max_items; }
-  __host__ __device__ int unit_of() const { return jobs() + 7 * max_jobs; }  // k_span's prefix unit of the row, -1
+  __host__ __device__ int unit_of() const { return jobs() + 8 * max_jobs; }  // k_span's prefix unit of the row, -1
   __host__ __device__ int units() const { return unit_of() + rows; }          // prefixes first, then the rows
   __host__ __device__ int total() const { return units() + 5 * (rows + rows / 2); }
 };
 
 struct SharedArgs {
   const float* q;  // rotated
+  uint8_t* qparts;
+  float* qup;
   int n_heads, n_kv, hd, G;
   const float *kc, *vc;  // this layer
   const int* ptab;       // nullptr: contiguous
@@ -137,7 +142,7 @@ struct SharedArgs {
 //   16 warps load K and V rows (8 lanes a row) straight into registers, a tile
 //     ahead, and write them as fp16 hi + lo parts, x' = x 2^-e = hi + lo with
 //     lo = fp16(x' - hi) and e from the row's largest element: 22 bits,
-//     whatever the rows' magnitudes. An item's Q goes the same way first;
+//     whatever the rows' magnitudes. (k_begin has left Q in this form.)
 //   one thread issues tcgen05.mma: S = Qh Kh + Qh Kl + Ql Kh and, with the
 //     softmax's P split the same way, O += Ph Vh + Ph Vl + Pl Vh. Q and P are
 //     A operands in tensor memory. K and V lie alike, [key][hd] in swizzled
@@ -167,9 +172,8 @@ template <int HDP>
 struct PxSmem {
   static constexpr int PART = PT * HDP * 2;   // one fp16 part of K or V
   static constexpr int STAGE = 4 * PART;      // K hi, K lo, V hi, V lo
-  static constexpr int QPART = PM * HDP * 2;  // one part of Q
-  static constexpr int Q = 2 * STAGE;
-  static constexpr int BYTES = Q + 2 * QPART + 1024;
+  static constexpr int O = 2 * STAGE;         // O on its way out: [8 warps][32 rows][HDP / 2]
+  static constexpr int BYTES = O + PM * HDP * 4 + 1024;
 };
 
 // Item it, less the tiles that no row sees. Whole warps.
@@ -258,41 +262,30 @@ __device__ __forceinline__ void pair_sync(int id) {  // the two warps of the sam
   asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
 
-// NR rows, j, j + 2, of an operand of `rows` rows, 8 lanes a row (lane l has the
-// float4s l, l + 8, ...): the fp16 parts into `part` and psize bytes behind it; the
-// rows' exponents.
-template <int NV, int NR>
-__device__ __forceinline__ void px_rows(const float4 (&v)[NR][NV], uint8_t* part, int psize, int rows, int j,
-                                        int (&eb)[NR]) {
+// Row k of an operand of PT rows, 8 lanes a row (lane l has the float4s l, l + 8, ...): the
+// fp16 parts into `part` and psize bytes behind it; the row's exponent.
+template <int NV>
+__device__ __forceinline__ int px_row(const float4 (&v)[NV], uint8_t* part, int psize, int k) {
   const int l8 = threadIdx.x & 7;
-  float m[NR];
+  float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NR; i++) {
-    m[i] = 0.0f;
+  for (int u = 0; u < NV; u++)
+    m = fmaxf(fmaxf(fmaxf(m, fabsf(v[u].x)), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w)));
 #pragma unroll
-    for (int u = 0; u < NV; u++)
-      m[i] = fmaxf(fmaxf(fmaxf(m[i], fabsf(v[i][u].x)), fabsf(v[i][u].y)), fmaxf(fabsf(v[i][u].z), fabsf(v[i][u].w)));
+  for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const int eb = px_exp(m);
+  const f32x2 down = pk(px_down(eb), px_down(eb));
+  uint8_t* row = part + (k >> 3) * 1024 + (k & 7) * 128 + (l8 & 1) * 8;
+#pragma unroll
+  for (int u = 0; u < NV; u++) {
+    uint2 hi, lo;
+    split2(mul2(pk(v[u].x, v[u].y), down), hi.x, lo.x);
+    split2(mul2(pk(v[u].z, v[u].w), down), hi.y, lo.y);
+    uint8_t* p = row + (u >> 1) * PT * 128 + ((((u & 1) * 4 + (l8 >> 1)) ^ (k & 7)) << 4);
+    *reinterpret_cast<uint2*>(p) = hi;
+    *reinterpret_cast<uint2*>(p + psize) = lo;
   }
-#pragma unroll
-  for (int o = 4; o; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < NR; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
-#pragma unroll
-  for (int i = 0; i < NR; i++) {
-    const int k = j + 2 * i;
-    eb[i] = px_exp(m[i]);
-    const f32x2 down = pk(px_down(eb[i]), px_down(eb[i]));
-    uint8_t* row = part + (k >> 3) * 1024 + (k & 7) * 128 + (l8 & 1) * 8;
-#pragma unroll
-    for (int u = 0; u < NV; u++) {
-      uint2 hi, lo;
-      split2(mul2(pk(v[i][u].x, v[i][u].y), down), hi.x, lo.x);
-      split2(mul2(pk(v[i][u].z, v[i][u].w), down), hi.y, lo.y);
-      uint8_t* p = row + (u >> 1) * rows * 128 + ((((u & 1) * 4 + (l8 >> 1)) ^ (k & 7)) << 4);
-      *reinterpret_cast<uint2*>(p) = hi;
-      *reinterpret_cast<uint2*>(p + psize) = lo;
-    }
-  }
+  return eb;
 }
 
 template <int HDP>
@@ -305,7 +298,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t kfull[2], vfull[2], pfull[2], qk_done[2], pv_done[2], qfull;
-  __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT], qup[PM];
+  __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT];
   __shared__ float pmax[2][2][PM];  // [tile parity][half of the keys][row]
   __shared__ uint32_t tbase_sh;
   __shared__ int fail;
@@ -366,46 +359,20 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       }
       float cq = 0.0f;
       int low = 0;
-      // the item's queries, as fp16 parts (their place may still hold the last item's O)
-      if (ord) asm volatile("bar.sync 5, %0;" ::"n"(32 * PX_SOFT) : "memory");
-#pragma unroll 1
-      for (int g = 0; g < PM && g + warp * 8 < item.m; g += 64) {
-        const int l8 = lane & 7, j = g + warp * 8 + (((lane >> 3) & 1) << 2 | lane >> 4);
-        float4 v[2][NV];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const int m = item.m0 + j + 2 * i;
-          const float* src =
-              a.q + ((size_t)(item.row0 + m / a.G) * a.n_heads + item.kvh * a.G + m % a.G) * a.hd;
-#pragma unroll
-          for (int u = 0; u < NV; u++) {
-            v[i][u] = make_float4(0, 0, 0, 0);
-            if (j + 2 * i < item.m && u * 32 + l8 * 4 < a.hd)
-              v[i][u] = *reinterpret_cast<const float4*>(src + u * 32 + l8 * 4);
-          }
-        }
-        int eb[2];
-        px_rows<NV, 2>(v, sm + L::Q, L::QPART, PM, j, eb);
-        if (l8 == 0) {
-          qup[j] = px_up(eb[0]);
-          qup[j + 2] = px_up(eb[1]);
-        }
-      }
-      asm volatile("bar.sync 5, %0;" ::"n"(32 * PX_SOFT) : "memory");
-      if (busy) {
-        cq = qup[r] * a.scale * 1.4426950408889634f;
-        if (a.window && r < item.m)
+      if (busy) {  // half h brings Q's part h (the last item's products are done: its O was read)
+        const bool is = r < item.m;
+        if (is) cq = a.qup[item.q0 + r] * a.scale * 1.4426950408889634f;
+        if (a.window && is)
           low = max(0, a.len[a.meta[a.mv.seq() + item.row0 + (item.m0 + r) / a.G]] + 1 - a.window);
-        // (the last item's products are done: its O was read) half h brings Q's part h
         tc_fence_after();
-        const uint8_t* q = sm + L::Q + h * L::QPART + (r >> 3) * 1024 + (r & 7) * 128;
+        const uint4* q = reinterpret_cast<const uint4*>(a.qparts + (size_t)item.q0 * (HDP * 4)) + h * (HDP / 8) * item.m + r;
 #pragma unroll
-        for (int c = 0; c < HDP / 8; c += 4) {  // 16-byte chunks
-          uint4 u[4];
+        for (int c = 0; c < HDP / 8; c += 8) {  // 16-byte chunks
+          uint4 u[8];
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            u[e] = *reinterpret_cast<const uint4*>(q + ((c + e) >> 3) * (PM * 128) + ((((c + e) & 7) ^ (r & 7)) << 4));
+          for (int e = 0; e < 8; e++) u[e] = is && (c + e) * 8 < a.hd ? q[(c + e) * item.m] : make_uint4(0, 0, 0, 0);
           tc_st16(tl + C_Q + h * QC + c * 4, reinterpret_cast<const uint32_t*>(u));
+          tc_st16(tl + C_Q + h * QC + c * 4 + 16, reinterpret_cast<const uint32_t*>(u + 4));
         }
         tc_wait_st();
         tc_fence_before();
@@ -526,9 +493,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
                             : make_float2(M - P_TOP, la + pmax[n & 1][1][r]);
         pair_sync(pair);  // (the slot is the next item's)
-        // O: from rows to whole lines by way of the queries' place (its readers are long past)
+        // O: from rows to whole lines
         constexpr int CH = HDP / 8;  // 16-byte chunks of a row's half
-        uint8_t* stage = sm + L::Q + warp * (32 * CH * 16);
+        uint8_t* stage = sm + L::O + warp * (32 * CH * 16);
         for (int c = 0; c < HDP / 2; c += 32) {
           float o[32];
           tc_ld32(tl + C_O + h * (HDP / 2) + c, o);
@@ -599,15 +566,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       r.at = p.pg < 0 ? -1 : (((long long)p.pg * a.page + p.off) * a.n_kv + p.kvh) * a.hd + l8 * 4;
       return r;
     };
-    auto load = [&](float4 (&v)[1][NV], const float* cache, const Rows& r) {
+    auto load = [&](float4 (&v)[NV], const float* cache, const Rows& r) {
 #pragma unroll
       for (int u = 0; u < NV; u++) {
-        v[0][u] = make_float4(0, 0, 0, 0);
+        v[u] = make_float4(0, 0, 0, 0);
         if (r.at >= 0 && u * 32 + l8 * 4 < a.hd)
-          v[0][u] = __ldg(reinterpret_cast<const float4*>(cache + r.at + u * 32));
+          v[u] = __ldg(reinterpret_cast<const float4*>(cache + r.at + u * 32));
       }
     };
-    float4 xk[1][NV], xv[1][NV];
+    float4 xk[NV], xv[NV];
     Pages pages = ask();
     Rows next = place(pages);
     pages = ask();
@@ -621,18 +588,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       const int s = n & 1, use = n >> 1;
       uint8_t* st = sm + s * L::STAGE;
       if (use && !(ok = wait(&qk_done[s], use - 1))) break;
-      int ek[1], ev[1];
-      px_rows<NV, 1>(xk, st, L::PART, PT, jj, ek);
+      const int ek = px_row<NV>(xk, st, L::PART, jj);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[s]);
       load(xk, a.kc, next);
       if (use && !(ok = wait(&pv_done[s], use - 1))) break;
-      px_rows<NV, 1>(xv, st + 2 * L::PART, L::PART, PT, jj, ev);
+      const int ev = px_row<NV>(xv, st + 2 * L::PART, L::PART, jj);
       if (l8 == 0) {  // (the softmax is done with the stage's last scales: P was used)
-        kup[s][jj] = px_up(ek[0]);
-        vexp[s][jj] = (float)(ev[0] - 140);
-        vdown[s][jj] = px_down(ev[0]);
+        kup[s][jj] = px_up(ek);
+        vexp[s][jj] = (float)(ev - 140);
+        vdown[s][jj] = px_down(ev);
       }
       fence_async_smem();
       __syncwarp();
@@ -832,13 +798,77 @@ __device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int 
   }
 }
 
-// The append, and in the last `deal` blocks the shares.
-template <int VEC, int LP, bool ONE>
+// A rotated query row as k_prefix wants it, x' = x 2^-e = hi + lo: of a job's m rows the hi parts
+// and then the lo parts, each [HDP / 8][m] chunks of 16 bytes (a thread per row reads whole lines).
+struct QParts {
+  const SharedArgs& a;
+  uint8_t* at = nullptr;  // the row's first chunk; nullptr: no job
+  float* up = nullptr;
+  int m = 0;
+  __device__ QParts(const SharedArgs& a) : a(a) {}
+  __device__ __forceinline__ void find(int row, int head) {  // (the plan: from before this kernel)
+    const int job0 = a.meta[a.mv.job_of() + row];
+    if (job0 < 0) return;
+    const int kvh = head / a.G, i = a.meta[a.mv.local() + row] * a.G + head - kvh * a.G;
+    const Job job = reinterpret_cast<const Job*>(a.meta + a.mv.jobs())[job0 + i / PM * a.n_kv + kvh];
+    m = job.m;
+    up = a.qup + job.q0 + i - job.m0;
+    at = a.qparts + (size_t)job.q0 * (a.hd > 64 ? 512 : 256) + (i - job.m0) * 16;
+  }
+  template <int VEC, int LP, typename T>
+  __device__ __forceinline__ void take(int lane, int nv, const T (&r1)[2], const T (&r2)[2]) {
+    if (!at) return;  // (the same for the LP lanes of the row)
+    constexpr int STEPS = VEC == 4 ? 1 : 2;
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++)
+        mx = fmaxf(mx, fmaxf(fabsf(reinterpret_cast<const float*>(&r1[i])[e]), fabsf(reinterpret_cast<const float*>(&r2[i])[e])));
+    const uint32_t mask = (LP == 32 ? 0xffffffffu : (1u << (LP & 31)) - 1) << (threadIdx.x & 31 & ~(LP - 1));
+#pragma unroll
+    for (int o = LP / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o));
+    const int eb = px_exp(mx), lo = (a.hd > 64 ? 16 : 8) * m * 16;
+    if (lane == 0) *up = px_up(eb);
+    const float down = px_down(eb);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++)
+      if (lane + i * LP < nv)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float* f = reinterpret_cast<const float*>(h ? &r2[i] : &r1[i]);
+          const int d = h * (a.hd >> 1) + (lane + i * LP) * VEC;  // 8 elements a chunk
+          uint8_t* p = at + (d >> 3) * m * 16 + (d & 7) * 2;
+          if constexpr (VEC == 4) {
+            uint2 x, y;
+            split2(mul2(pk(f[0], f[1]), pk(down, down)), x.x, y.x);
+            split2(mul2(pk(f[2], f[3]), pk(down, down)), x.y, y.y);
+            *reinterpret_cast<uint2*>(p) = x;
+            *reinterpret_cast<uint2*>(p + lo) = y;
+          } else {
+            uint32_t x, y;
+            split2(mul2(pk(f[0], 0.0f), pk(down, down)), x, y);
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)x;
+            *reinterpret_cast<uint16_t*>(p + lo) = (uint16_t)y;
+          }
+        }
+    const int over = a.hd + lane;  // the rest of the last chunk
+    if ((a.hd & 7) && over < (a.hd | 7) + 1) {
+      uint8_t* p = at + (over >> 3) * m * 16 + (over & 7) * 2;
+      *reinterpret_cast<uint16_t*>(p) = 0;
+      *reinterpret_cast<uint16_t*>(p + lo) = 0;
+    }
+  }
+};
+
+// The append, and in the last `deal` blocks the shares. PARTS: with k_prefix behind it.
+template <int VEC, int LP, bool ONE, bool PARTS>
 __global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ AppendArgs p,
                                                       const __grid_constant__ SharedArgs a, int deal) {
   const int block = (int)blockIdx.x - ((int)gridDim.x - deal);
   if (block < 0) {
-    append_rows<VEC, LP, ONE, 1>(p);
+    if constexpr (PARTS) append_rows<VEC, LP, ONE, 1>(p, QParts(a));
+    else append_rows<VEC, LP, ONE, 1>(p);
   } else {
     griddep_wait();
     griddep_launch();
@@ -1151,6 +1181,14 @@ syn_status_t launched(cudaError_t e, const char* where) {
   return SYN_ERR_CUDA;
 }
 
+template <bool PARTS>
+void (*begin_kernel(const AppendShape& sh))(const AppendArgs, const SharedArgs, int) {
+  return !sh.vec       ? k_begin<1, 32, false, PARTS>
+         : sh.lp == 4 ? k_begin<4, 4, true, PARTS>
+         : sh.lp == 8 ? k_begin<4, 8, true, PARTS>
+                      : k_begin<4, 16, true, PARTS>;
+}
+
 // Most jobs and items of a batch of `batch` rows (groups of two or more share).
 size_t max_jobs(size_t batch, size_t n_kv, size_t G) {
   return n_kv * (batch * G / PM + batch / 2 + 1);
@@ -1182,6 +1220,8 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   const size_t rows_per_layer = c->page ? c->n_pages * c->page : c->batch * c->max_seq;
   SharedArgs a;
   a.q = p->q;
+  a.qparts = p->qparts;
+  a.qup = p->qup;
   a.n_heads = (int)p->n_heads;
   a.n_kv = (int)c->n_kv;
   a.hd = (int)c->hd;
@@ -1215,10 +1255,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
     ap.seq_of = p->meta + a.mv.seq();
     ap.rows = a.rows;
     const AppendShape sh = append_shape(ap);
-    void (*kern)(const AppendArgs, const SharedArgs, int) = !sh.vec       ? k_begin<1, 32, false>
-                                                            : sh.lp == 4  ? k_begin<4, 4, true>
-                                                            : sh.lp == 8  ? k_begin<4, 8, true>
-                                                                          : k_begin<4, 16, true>;
+    void (*kern)(const AppendArgs, const SharedArgs, int) = p->jobs ? begin_kernel<true>(sh) : begin_kernel<false>(sh);
     const size_t per = AP_THREADS / sh.lp, blocks = (p->rows * (p->n_heads + 2 * c->n_kv) + per - 1) / per;
     const int deal = (std::max(a.warps, a.span_jobs) + AP_THREADS - 1) / AP_THREADS;
     s = launched(launch_pdl(kern, dim3((unsigned)(blocks + deal)), dim3(AP_THREADS), 0, st, ap, a, deal), "k_begin");
@@ -1278,6 +1315,9 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
     return SYN_ERR_UNSUPPORTED;
   }
   cudaError_t e = cudaMalloc(&p->q, c->batch * n_heads * c->hd * sizeof(float));
+  const size_t qbytes = c->batch * n_heads * (c->hd > 64 ? 512 : 256);
+  if (e == cudaSuccess) e = cudaMalloc(&p->qparts, qbytes);
+  if (e == cudaSuccess) e = cudaMalloc(&p->qup, c->batch * n_heads * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->meta, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMallocHost(&p->meta_h, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
@@ -1302,6 +1342,8 @@ syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
   DeviceGuard g(p->device);
   cudaDeviceSynchronize();
   cudaFree(p->q);
+  cudaFree(p->qparts);
+  cudaFree(p->qup);
   cudaFree(p->meta);
   if (p->meta_h) cudaFreeHost(p->meta_h);
   cudaFree(p->po);
@@ -1350,6 +1392,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   Unit* units = reinterpret_cast<Unit*>(h + mv.units());
   int nj = 0, nu = 0, uj = 0;
   size_t tiles = 0, r0 = 0;
+  int q0 = 0;
   for (size_t i = 0; i < n_groups; i++) {
     const size_t n = group_rows[i];
     size_t shared = 0;  // leading positions in pages that all rows hold
@@ -1381,7 +1424,9 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     } else if (shared)
       for (int m0 = 0; m0 < (int)n * G; m0 += PM)
         for (int kvh = 0; kvh < (int)c->n_kv; kvh++) {
-          jobs[nj++] = Job{(int)r0, m0, std::min(PM, (int)n * G - m0), kvh, (int)shared, 0, 0};
+          const int m = std::min(PM, (int)n * G - m0);
+          jobs[nj++] = Job{(int)r0, m0, m, kvh, (int)shared, 0, 0, q0};
+          q0 += m;
           tiles += (shared + PT - 1) / PT;
         }
     r0 += n;
@@ -1393,7 +1438,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   size_t ni = 0, part = 0, done = 0, jt = 0;
   auto item_of = [&](const Job& job, size_t t0, size_t t1) {
     return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
-                seqs[job.row0], 0, 0, 0};
+                seqs[job.row0], 0, job.q0, 0};
   };
   int cta = 0;
   if (nj && nj <= mv.ctas) {
