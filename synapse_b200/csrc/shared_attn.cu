@@ -47,6 +47,7 @@ struct syn_cuda_decode_plan_s {
   size_t part_rows = 0;      // records of po / pml
   void* shares = nullptr;    // k_span's shares and jobs (Share, SpanJob), written by k_begin
   int units = 0, span_jobs = 0, jobs = 0;  // k_span's units and jobs; k_prefix's jobs
+  int prefix_ctas = 0, span_sms = 0;       // of their launches
 };
 
 namespace syn {
@@ -54,7 +55,8 @@ namespace {
 
 constexpr int PT = 64;         // keys of a prefix tile
 constexpr int PM = 128;        // query rows of a prefix job
-constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: warps of a CTA, keys of a tile
+constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: computing warps of a CTA, keys of a tile
+constexpr int SP_THREADS = 64 * SP_WARPS;
 constexpr int SP_V = 8;        // most query vectors of a k_span job
 constexpr int SP_FEW = 8;      // a group of at most so many query rows per KV head goes to k_span
 constexpr int ROWS_MAX = 512;  // rows of a plan
@@ -681,14 +683,16 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
 // ---------------------------------------------------------------------------
 // Few query vectors over a range of positions: each row's own positions, and
 // prefixes of few query rows. All jobs' tiles of 32 keys, one after another, are
-// dealt to all warps in equal, contiguous shares (the lengths are read on the
-// device), so uneven rows cost nothing. A warp works alone: bulk copies bring
-// the tile's K and V rows into its ring of three half tiles (16 bytes of padding
-// a row keep a lane per row free of bank conflicts); lane = key for the scores,
-// with q broadcast from shared memory, so no sum crosses lanes; lane = four
-// columns for the weighted sum, with the weights broadcast. A key costs about
-// 6 + 5 NQ instructions for NQ query vectors, against 43 cycles of an SM's share of
-// HBM for its 1 KB (head dim 128).
+// dealt to all computing warps in equal, contiguous shares (the lengths are read on
+// the device), so uneven rows cost nothing. Beside each computing warp a copying one
+// brings the K and V rows, a bulk copy a row, into the ring of three half tiles (16
+// bytes of padding a row keep a lane per row free of bank conflicts); lane = key for
+// the scores, with q broadcast from shared memory, so no sum crosses lanes; lane =
+// four columns for the weighted sum, with the weights broadcast. For four query
+// vectors a tile of 128 columns takes 1500 cycles for the scores, 270 for the weights and
+// 1300 for the sum, against 1400 of an SM's share of HBM for four warps' tiles. A warp
+// that copies for itself spends 2000 more on that: 32 rows behind 2048 shared
+// positions took 45 us instead of 38.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float redux_max(float x) {
   float y;
@@ -876,21 +880,46 @@ __global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ Ap
   }
 }
 
-// Tiles [k0, k1) of a job, by one warp; the record of each query vector. HD: the
-// head dim where it is 64 or 128, else 0.
-template <int LPR, int HD, int NQ>
-__device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job, int k0, int k1, size_t rec,
-                                         uint8_t* ring, float* qs, float2* ps, uint64_t* bars, uint32_t& used) {
-  constexpr int SUBS = 32 / LPR;
-  const int lane = threadIdx.x & 31, hd = HD ? HD : a.hd, stride = hd * 4 + 16, slot_bytes = SP_T * stride;
-  const int sub = lane / LPR, l4 = (lane % LPR) * 4;
-  // the ring: K and V of a tile in turn; `used` counts the fills of all jobs
-  const int nt = k1 - k0;
+// N floats, to or from shared memory
+template <int N>
+__device__ __forceinline__ void weights(float* to, const float* from) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int v = 0; v < N; v += 4) *reinterpret_cast<float4*>(to + v) = *reinterpret_cast<const float4*>(from + v);
+  } else {
+#pragma unroll
+    for (int v = 0; v < N; v++) to[v] = from[v];
+  }
+}
+
+// A warp's ring of half tiles (K and V of a tile in turn): `used` counts those that this side, the
+// copying or the computing warp, is past.
+struct SpanRing {
+  uint8_t* at;
+  int slot_bytes;
+  uint64_t *full, *empty;
+  uint32_t slot = 0, turn = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SP_SLOTS) {
+      slot = 0;
+      turn++;
+    }
+  }
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+    bool ok = mbar_try_wait(bar + slot, parity);
+    if (!ok) ok = mbar_wait_bounded(bar + slot, parity);
+    return __all_sync(0xffffffffu, ok) != 0;
+  }
+};
+
+// Tiles [k0, k1) of a job into the ring, lane = key.
+__device__ __forceinline__ bool span_fill(const SharedArgs& a, const SpanJob& job, int k0, int k1, int hd,
+                                          SpanRing& ring) {
+  const int lane = threadIdx.x & 31, stride = hd * 4 + 16;
   // the place of this lane's key in the tile that is asked for next
   int pos = job.r0 + k0 * SP_T + lane, col = a.ptab ? pos / a.page : 0, off = pos - col * a.page;
   const int dcol = a.ptab ? SP_T / a.page : 0, doff = SP_T - dcol * a.page;
-  long long at = -1;  // offset of its row in the cache, -1 = none
-  auto ask = [&]() {
+  auto ask = [&]() {  // offset of its row in the cache, -1 = none
     long long row = -1;
     if (pos < job.r1) {
       if (a.ptab) {
@@ -900,7 +929,6 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
         row = (long long)job.seq * a.max_seq + pos;
       }
     }
-    at = row < 0 ? -1 : (row * a.n_kv + job.kvh) * hd;
     pos += SP_T;
     col += dcol;
     off += doff;
@@ -908,25 +936,46 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
       off -= a.page;
       col++;
     }
+    return row < 0 ? -1 : (row * a.n_kv + job.kvh) * hd;
   };
-  uint32_t fslot = used % SP_SLOTS, rslot = fslot, rpar = (used / SP_SLOTS) & 1;
-  auto fill = [&](const float* cache) {  // the next half tile (K or V) into the next slot
-    uint64_t* bar = bars + fslot;
+  auto fill = [&](const float* cache, long long at) {
+    if (ring.turn && !ring.wait(ring.empty, (ring.turn - 1) & 1)) return false;
+    uint64_t* bar = ring.full + ring.slot;
     const uint32_t rows = __popc(__ballot_sync(0xffffffffu, at >= 0));
-    fence_async_smem();  // (the slot's last readers are past; order their accesses before the copy's)
     if (lane == 0) mbar_expect_tx(bar, rows * hd * 4);
     __syncwarp();
-    if (at >= 0) bulk_g2s(ring + fslot * slot_bytes + lane * stride, cache + at, hd * 4, bar);
-    fslot = fslot == SP_SLOTS - 1 ? 0 : fslot + 1;
+    if (at >= 0) bulk_g2s(ring.at + ring.slot * ring.slot_bytes + lane * stride, cache + at, hd * 4, bar);
+    ring.next();
+    return true;
   };
+  long long next = ask();
+  for (int k = k0; k < k1; k++) {
+    const long long at = next;
+    if (k + 1 < k1) next = ask();
+    if (!fill(a.kc, at) || !fill(a.vc, at)) return false;
+  }
+  return true;
+}
+
+// Tiles [k0, k1) of a job, by one warp; the record of each query vector. HD: the
+// head dim where it is 64 or 128, else 0.
+template <int LPR, int HD, int NQ>
+__device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job, int k0, int k1, size_t rec,
+                                         SpanRing& ring, float* qs, float* ps) {
+  constexpr int SUBS = 32 / LPR;
+  const int lane = threadIdx.x & 31, hd = HD ? HD : a.hd, stride = hd * 4 + 16;
+  const int sub = lane / LPR, l4 = (lane % LPR) * 4;
+  const int nt = k1 - k0;
   const uint8_t* tile = nullptr;
   auto ready = [&]() {  // the next half tile is in `tile`
-    bool ok = mbar_try_wait(bars + rslot, rpar);
-    if (!ok) ok = mbar_wait_bounded(bars + rslot, rpar);
-    tile = ring + rslot * slot_bytes;
-    rpar ^= rslot == SP_SLOTS - 1;
-    rslot = rslot == SP_SLOTS - 1 ? 0 : rslot + 1;
-    return __all_sync(0xffffffffu, ok) != 0;
+    tile = ring.at + ring.slot * ring.slot_bytes;
+    return ring.wait(ring.full, ring.turn & 1);
+  };
+  auto past = [&]() {
+    fence_async_smem();  // (this warp's reads before the copies that follow)
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ring.empty + ring.slot);
+    ring.next();
   };
   float m[NQ], l[NQ];
   f32x2 o[NQ][2];
@@ -936,14 +985,6 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
     l[v] = 0.0f;
     o[v][0] = o[v][1] = 0;
   }
-  ask();
-  fill(a.kc);
-  fill(a.vc);
-  if (nt > 1) {
-    ask();
-    fill(a.kc);
-  }
-  used += 2 * nt;
   // queries, times scale * log2(e)
   const float qscale = a.scale * 1.4426950408889634f;
   int low[NQ];
@@ -986,10 +1027,10 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
         acc2(acc[v][1], x.y, q.y);
       }
     }
-    __syncwarp();  // (all have read the slot)
-    if (k + 1 < nt) fill(a.vc);
-    // softmax weights, twice each for the packed sums
+    past();
+    // softmax weights
     float corr[NQ];
+    float w[NQ];
     bool grown = false;
 #pragma unroll
     for (int v = 0; v < NQ; v++) {
@@ -1002,7 +1043,7 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
       const float p = mx == -INFINITY ? 0.0f : ex2(x - mx);
       l[v] = fmaf(l[v], corr[v], p);
       m[v] = mx;
-      ps[lane * NQ + v] = make_float2(p, p);
+      w[v] = p;
     }
     if (grown) {
 #pragma unroll
@@ -1011,25 +1052,24 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
         o[v][1] = mul2(o[v][1], pk(corr[v], corr[v]));
       }
     }
+    weights<NQ>(ps + lane * NQ, w);
     __syncwarp();
     if (!ready()) return false;
     if (l4 < hd) {
 #pragma unroll 4
       for (int j = sub; j < nk; j += SUBS) {
         const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(tile + j * stride + l4 * 4);
-        const f32x2* p = reinterpret_cast<const f32x2*>(ps + j * NQ);
+        float p[NQ];
+        weights<NQ>(p, ps + j * NQ);
 #pragma unroll
         for (int v = 0; v < NQ; v++) {
-          acc2(o[v][0], p[v], x.x);
-          acc2(o[v][1], p[v], x.y);
+          const f32x2 pp = pk(p[v], p[v]);
+          acc2(o[v][0], pp, x.x);
+          acc2(o[v][1], pp, x.y);
         }
       }
     }
-    __syncwarp();
-    if (k + 2 < nt) {
-      ask();
-      fill(a.kc);
-    }
+    past();
   }
 #pragma unroll
   for (int v = 0; v < NQ; v++) {
@@ -1051,18 +1091,23 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
   return true;
 }
 
+// Warps 0 .. 3 compute, 4 .. 7 copy for them.
 template <int LPR, int HD>
-__global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
+__global__ void __launch_bounds__(SP_THREADS, 1) k_span(const SharedArgs a) {
   extern __shared__ __align__(16) uint8_t sraw[];
-  __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_SLOTS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slot_bytes = SP_T * (a.hd * 4 + 16), per_warp = SP_SLOTS * slot_bytes + SP_V * a.hd * 4 + SP_T * SP_V * 8;
-  uint8_t* ring = sraw + warp * per_warp;
-  float* qs = reinterpret_cast<float*>(ring + SP_SLOTS * slot_bytes);
-  float2* ps = reinterpret_cast<float2*>(qs + SP_V * a.hd);
-  if (lane < SP_SLOTS) mbar_init(&bars[warp][lane], 1);
-  mbar_fence_init();
-  __syncwarp();
+  __shared__ __align__(8) uint64_t full[SP_WARPS][SP_SLOTS], empty[SP_WARPS][SP_SLOTS];
+  const int warp = (threadIdx.x >> 5) % SP_WARPS, lane = threadIdx.x & 31, hd = HD ? HD : a.hd;
+  const bool copies = threadIdx.x >= SP_WARPS * 32;
+  const int slot_bytes = SP_T * (hd * 4 + 16), per_warp = SP_SLOTS * slot_bytes + SP_V * hd * 4 + SP_T * SP_V * 4;
+  SpanRing ring{sraw + warp * per_warp, slot_bytes, full[warp], empty[warp]};
+  float* qs = reinterpret_cast<float*>(ring.at + SP_SLOTS * slot_bytes);
+  float* ps = qs + SP_V * hd;
+  if (!copies && lane < SP_SLOTS) {
+    mbar_init(&full[warp][lane], 1);
+    mbar_init(&empty[warp][lane], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
   // Behind k_prefix this kernel needs nothing of it: k_begin is complete where k_prefix has
   // let it begin, and so it runs on every SM that k_prefix has left.
   if (!a.after_prefix) griddep_wait();
@@ -1070,7 +1115,6 @@ __global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
   const int gw = warp * gridDim.x + blockIdx.x;  // (neighbouring shares on different SMs)
   const int4 sh = __ldcg(reinterpret_cast<const int4*>(a.shares) + gw);
   int j = sh.x, k0 = sh.y, left = sh.z;
-  uint32_t used = 0;
   bool ok = true;
   while (left > 0 && ok) {
     union {
@@ -1082,10 +1126,11 @@ __global__ void __launch_bounds__(SP_WARPS * 32) k_span(const SharedArgs a) {
     const int k1 = min(job.nt, k0 + left);
     const size_t rec = a.span0 + (size_t)(gw + j) * SP_V;
     if (k1 > k0)
-      ok = job.nq > 4   ? span_job<LPR, HD, 8>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-           : job.nq > 2 ? span_job<LPR, HD, 4>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-           : job.nq > 1 ? span_job<LPR, HD, 2>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used)
-                        : span_job<LPR, HD, 1>(a, job, k0, k1, rec, ring, qs, ps, bars[warp], used);
+      ok = copies        ? span_fill(a, job, k0, k1, hd, ring)
+           : job.nq > 4 ? span_job<LPR, HD, 8>(a, job, k0, k1, rec, ring, qs, ps)
+           : job.nq > 2 ? span_job<LPR, HD, 4>(a, job, k0, k1, rec, ring, qs, ps)
+           : job.nq > 1 ? span_job<LPR, HD, 2>(a, job, k0, k1, rec, ring, qs, ps)
+                        : span_job<LPR, HD, 1>(a, job, k0, k1, rec, ring, qs, ps);
     left -= k1 - k0;
     k0 = 0;
     j++;
@@ -1202,7 +1247,7 @@ Meta meta_of(const syn_cuda_decode_plan_t* p) {
 
 // k_span: shared memory, and CTAs on an SM
 size_t span_smem(size_t hd) {
-  return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 8);
+  return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 4);
 }
 int span_ctas(size_t hd) { return span_smem(hd) > 112 * 1024 ? 1 : 2; }
 // Most k_span jobs of a batch
@@ -1240,8 +1285,8 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.pml = p->pml;
   a.rows = (int)p->rows;
   a.units = p->units;
-  a.warps = span_ctas(c->hd) * p->sms * SP_WARPS;
-  a.span0 = (int)(p->part_rows - (a.warps + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
+  a.warps = span_ctas(c->hd) * p->span_sms * SP_WARPS;
+  a.span0 = (int)(p->part_rows - (span_ctas(c->hd) * p->sms * SP_WARPS + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
   a.span_jobs = p->span_jobs;
   a.after_prefix = p->jobs > 0;
   a.shares = static_cast<Share*>(p->shares);
@@ -1266,7 +1311,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
     void (*kern)(const SharedArgs) = w ? k_prefix<128> : k_prefix<64>;
     const size_t smem = w ? PxSmem<128>::BYTES : PxSmem<64>::BYTES;
     if ((s = more_smem((const void*)kern, smem))) return s;
-    s = launched(launch_pdl(kern, dim3(p->sms), dim3(PX_THREADS), smem, st, a), "k_prefix");
+    s = launched(launch_pdl(kern, dim3(p->prefix_ctas), dim3(PX_THREADS), smem, st, a), "k_prefix");
     if (s) return s;
   }
   void (*span)(const SharedArgs) = c->hd == 128  ? k_span<32, 128>
@@ -1275,7 +1320,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
                                    : c->hd < 64  ? k_span<16, 0>
                                                  : k_span<32, 0>;
   if ((s = more_smem((const void*)span, span_smem(c->hd)))) return s;
-  s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->sms), dim3(SP_WARPS * 32), span_smem(c->hd), st, a),
+  s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->span_sms), dim3(SP_THREADS), span_smem(c->hd), st, a),
                "k_span");
   if (s) return s;
   return launched(launch_pdl(k_join, dim3((unsigned)(p->rows * p->n_heads)), dim3(JN_WARPS * 32), 0, st, a),
@@ -1431,6 +1476,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
         }
     r0 += n;
   }
+  p->prefix_ctas = p->span_sms = p->sms;
   // With no more jobs than CTAs, an item per CTA: the shortest items of which there are enough
   // CTAs for (a CTA that goes from one job to another drains its pipeline in between). Else
   // the tiles of all jobs, one after another, in equal shares.
@@ -1440,15 +1486,16 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
                 seqs[job.row0], 0, job.q0, 0};
   };
+  const int ctas = p->prefix_ctas;
   int cta = 0;
-  if (nj && nj <= mv.ctas) {
-    size_t most = (tiles + mv.ctas - 1) / mv.ctas;
+  if (nj && nj <= ctas) {
+    size_t most = (tiles + ctas - 1) / ctas;
     auto items_at = [&](size_t q) {
       size_t k = 0;
       for (int j = 0; j < nj; j++) k += (tiles_of(j) + q - 1) / q;
       return k;
     };
-    while (items_at(most) > (size_t)mv.ctas) most++;
+    while (items_at(most) > (size_t)ctas) most++;
     for (int j = 0; j < nj; j++) {
       Job& job = jobs[j];
       const size_t nt = tiles_of(j);
@@ -1461,9 +1508,9 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       }
     }
   }
-  for (int j = 0; cta < mv.ctas; cta++) {
+  for (int j = 0; cta < ctas; cta++) {
     h[mv.start() + cta] = (int)ni;
-    size_t share = nj > mv.ctas ? tiles * (cta + 1) / mv.ctas - done : 0;
+    size_t share = nj > ctas ? tiles * (cta + 1) / ctas - done : 0;
     done += share;
     while (share) {
       Job& job = jobs[j];
@@ -1479,7 +1526,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       }
     }
   }
-  h[mv.start() + mv.ctas] = (int)ni;
+  h[mv.start() + ctas] = (int)ni;
   for (size_t j = 0; j < rows; j++) {  // each row's own positions
     const int nch = (G + SP_V - 1) / SP_V;
     units[nu++] = Unit{(int)j, 0, h[mv.pre() + j], uj, nch};
