@@ -1434,11 +1434,8 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   p->seqs.assign(seqs, seqs + rows);
   p->prefix.assign(rows, 0);
   p->shrunk.assign(rows, 0);
-  Unit* units = reinterpret_cast<Unit*>(h + mv.units());
-  int nj = 0, nu = 0, uj = 0;
-  size_t tiles = 0, r0 = 0;
-  int q0 = 0;
-  for (size_t i = 0; i < n_groups; i++) {
+  size_t r0 = 0;
+  for (size_t i = 0; i < n_groups; r0 += group_rows[i++]) {
     const size_t n = group_rows[i];
     size_t shared = 0;  // leading positions in pages that all rows hold
     if (n > 1 && c->page) {
@@ -1452,50 +1449,108 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       }
       shared = col * c->page;
     }
-    const bool few = shared && n * G <= SP_FEW;
     for (size_t j = r0; j < r0 + n; j++) {
-      h[mv.seq() + j] = seqs[j];
-      h[mv.pre() + j] = (int)shared;
-      h[mv.job_of() + j] = shared && !few ? nj : -1;
-      h[mv.unit_of() + j] = few ? nu : -1;
-      h[mv.local() + j] = (int)(j - r0);
       p->prefix[j] = shared;
       if (c->page) p->shrunk[j] = c->shrunk[seqs[j]];
     }
-    if (few) {
-      const int nch = ((int)n * G + SP_V - 1) / SP_V;
-      units[nu++] = Unit{(int)r0, (int)n, (int)shared, uj, nch};
-      uj += (int)c->n_kv * nch;
-    } else if (shared)
-      for (int m0 = 0; m0 < (int)n * G; m0 += PM)
-        for (int kvh = 0; kvh < (int)c->n_kv; kvh++) {
-          const int m = std::min(PM, (int)n * G - m0);
-          jobs[nj++] = Job{(int)r0, m0, m, kvh, (int)shared, 0, 0, q0};
-          q0 += m;
-          tiles += (shared + PT - 1) / PT;
-        }
-    r0 += n;
   }
-  p->prefix_ctas = p->span_sms = p->sms;
-  // With no more jobs than CTAs, an item per CTA: the shortest items of which there are enough
-  // CTAs for (a CTA that goes from one job to another drains its pipeline in between). Else
-  // the tiles of all jobs, one after another, in equal shares.
+  Unit* units = reinterpret_cast<Unit*>(h + mv.units());
+  const int row_ch = (G + SP_V - 1) / SP_V;  // k_span jobs of a row and KV head
+  int nj = 0, nu = 0, uj = 0, widest = 0;
+  size_t tiles = 0, own = 0, longest = 0;  // k_prefix's; k_span's, of a row and in all, with 128 positions more
   auto tiles_of = [&](int j) { return ((size_t)jobs[j].len + PT - 1) / PT; };
-  size_t ni = 0, part = 0, done = 0, jt = 0;
-  auto item_of = [&](const Job& job, size_t t0, size_t t1) {
-    return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
-                seqs[job.row0], 0, job.q0, 0};
+  auto lay_out = [&](bool share) {
+    int q0 = 0;
+    nj = nu = uj = widest = 0;
+    tiles = own = longest = 0;
+    r0 = 0;
+    for (size_t i = 0; i < n_groups; r0 += group_rows[i++]) {
+      const size_t n = group_rows[i], shared = share ? p->prefix[r0] : 0;
+      const bool few = shared && n * G <= SP_FEW;
+      for (size_t j = r0; j < r0 + n; j++) {
+        h[mv.seq() + j] = seqs[j];
+        h[mv.pre() + j] = (int)shared;
+        h[mv.job_of() + j] = shared && !few ? nj : -1;
+        h[mv.unit_of() + j] = few ? nu : -1;
+        h[mv.local() + j] = (int)(j - r0);
+        const size_t t = (c->len[seqs[j]] - shared + 128) / SP_T + 1;
+        own += c->n_kv * row_ch * t;
+        longest = std::max(longest, t);
+      }
+      if (few) {
+        const int nch = ((int)n * G + SP_V - 1) / SP_V;
+        units[nu++] = Unit{(int)r0, (int)n, (int)shared, uj, nch};
+        uj += (int)c->n_kv * nch;
+        own += c->n_kv * nch * ((shared + SP_T - 1) / SP_T);
+      } else if (shared)
+        for (int m0 = 0; m0 < (int)n * G; m0 += PM)
+          for (int kvh = 0; kvh < (int)c->n_kv; kvh++) {
+            const int m = std::min(PM, (int)n * G - m0);
+            jobs[nj] = Job{(int)r0, m0, m, kvh, (int)shared, 0, 0, q0};
+            widest = std::max(widest, m);
+            q0 += m;
+            tiles += tiles_of(nj++);
+          }
+    }
+    for (size_t j = 0; j < rows; j++) {  // each row's own positions
+      units[nu++] = Unit{(int)j, 0, h[mv.pre() + j], uj, row_ch};
+      uj += (int)c->n_kv * row_ch;
+    }
   };
-  const int ctas = p->prefix_ctas;
-  int cta = 0;
-  if (nj && nj <= ctas) {
-    size_t most = (tiles + ctas - 1) / ctas;
+  auto most_of = [&](size_t n) {  // tiles of a CTA of k_prefix, with n of them
+    size_t most = (tiles + n - 1) / n;
     auto items_at = [&](size_t q) {
       size_t k = 0;
       for (int j = 0; j < nj; j++) k += (tiles_of(j) + q - 1) / q;
       return k;
     };
-    while (items_at(most) > (size_t)ctas) most++;
+    while ((size_t)nj <= n && items_at(most) > n) most++;
+    return most;
+  };
+  // What the kernels take (us, measured at head dim 128): k_prefix 7, and 1.6 + 0.008 m a tile of m
+  // query rows; k_span 4, 2.5 a tile of each warp, and k_join 1 for 32 records of a row. The rows are
+  // taken 128 positions on, as they grow before the plan is next set.
+  auto prefix_us = [&](int n) { return 7 + (1.6 + 0.008 * widest) * most_of(n); };
+  auto span_us = [&](int n) {
+    const size_t per = std::max<size_t>(1, (own + SP_WARPS * n - 1) / (SP_WARPS * n));
+    return 4 + 2.5 * per + longest / per / 32;
+  };
+  // SYN_PLAN_LAYOUT=1, 2 or 3 keeps to: every row for itself, k_span behind k_prefix, beside it.
+  const char* env = getenv("SYN_PLAN_LAYOUT");
+  const int only = env ? atoi(env) : 0;
+  lay_out(true);
+  p->prefix_ctas = p->span_sms = p->sms;
+  double best = span_us(p->sms) + (nj ? prefix_us(p->sms) : 0);
+  if (nj && only != 2) {
+    // k_span behind k_prefix, each on all SMs, or side by side, each on its own: 8 rows behind 2048
+    // positions take 19.1 us behind and 15.0 side by side, 64 rows behind 32768 169 and 181
+    double least = only == 3 ? 1e30 : 0.85 * best;
+    for (int n = 4; n < p->sms; n += 4) {
+      const double us = std::max(prefix_us(n), span_us(p->sms - n));
+      if (us < least) {
+        best = least = us;
+        p->prefix_ctas = n;
+        p->span_sms = p->sms - n;
+      }
+    }
+  }
+  // A short prefix is read by each row for itself: 56 rows behind 42 positions take 11.2 us so, and
+  // 20.3 with k_prefix.
+  lay_out(false);
+  if (only ? only == 1 : span_us(p->sms) < 0.85 * best) p->prefix_ctas = p->span_sms = p->sms;
+  else lay_out(true);
+  size_t ni = 0, part = 0, done = 0, jt = 0;
+  auto item_of = [&](const Job& job, size_t t0, size_t t1) {
+    return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
+                seqs[job.row0], 0, job.q0, 0};
+  };
+  // With no more jobs than CTAs, an item per CTA: the shortest items of which there are enough
+  // CTAs for (a CTA that goes from one job to another drains its pipeline in between). Else
+  // the tiles of all jobs, one after another, in equal shares.
+  const int ctas = p->prefix_ctas;
+  int cta = 0;
+  if (nj && nj <= ctas) {
+    const size_t most = most_of(ctas);
     for (int j = 0; j < nj; j++) {
       Job& job = jobs[j];
       const size_t nt = tiles_of(j);
@@ -1527,11 +1582,6 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     }
   }
   h[mv.start() + ctas] = (int)ni;
-  for (size_t j = 0; j < rows; j++) {  // each row's own positions
-    const int nch = (G + SP_V - 1) / SP_V;
-    units[nu++] = Unit{(int)j, 0, h[mv.pre() + j], uj, nch};
-    uj += (int)c->n_kv * nch;
-  }
   p->units = nu;
   p->span_jobs = uj;
   p->jobs = nj;

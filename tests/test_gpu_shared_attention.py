@@ -12,6 +12,12 @@ sb = pytest.importorskip("synapse_b200")
 U = 2.0 ** -24
 
 
+@pytest.fixture(autouse=True, params=["0", "1", "2", "3"], ids=["chosen", "rows", "behind", "beside"])
+def layout(request, monkeypatch):
+    """Each of the ways in which a plan lays out its work; by itself it takes the fastest."""
+    monkeypatch.setenv("SYN_PLAN_LAYOUT", request.param)
+
+
 def _rope(n, hd):
     f = 10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
     a = torch.arange(n, dtype=torch.float64)[:, None] * f
