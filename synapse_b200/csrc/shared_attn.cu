@@ -145,9 +145,13 @@ struct SharedArgs {
 //     ahead, and write them as fp16 hi + lo parts, x' = x 2^-e = hi + lo with
 //     lo = fp16(x' - hi) and e from the row's largest element: 22 bits,
 //     whatever the rows' magnitudes. (k_begin has left Q in this form.)
-//   one thread issues tcgen05.mma: S = Qh Kh + Qh Kl + Ql Kh and, with the
-//     softmax's P split the same way, O += Ph Vh + Ph Vl + Pl Vh. Q and P are
-//     A operands in tensor memory. K and V lie alike, [key][hd] in swizzled
+//   one thread issues tcgen05.mma: S = Qh Kl + Ql Kh + Qh Kh and, with the
+//     softmax's P split the same way, O += Ph Vh and O2 += Ph Vl + Pl Vh. Each
+//     product cuts its sum off below the accumulator's last bit, towards zero, and
+//     over thousands of keys that adds up: so the small products come first in S
+//     and have a sum of their own beside O (64 rows, 3500 keys an item: 1.3e-5 off
+//     with one sum, 5e-6 with two). Q and P are A operands in tensor memory, P in
+//     the place of its S. K and V lie alike, [key][hd] in swizzled
 //     128-byte rows: K-major for S, MN-major for O, so nothing is transposed;
 //   8 warps turn S into P, two threads per query row, 32 keys each.
 // Issuing blocks while the tensor pipe is busy (a product of 64 columns takes
@@ -295,8 +299,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   using L = PxSmem<HDP>;
   constexpr int QC = HDP / 2;   // tensor-memory columns of one part of Q
   constexpr int NV = HDP / 32;  // float4s of a row per lane
-  constexpr uint32_t C_Q = 0, C_S = 2 * QC, C_P = C_S + 2 * PT, C_O = C_P + 2 * PT, COLS = 512;
-  static_assert(C_O + HDP <= COLS, "tensor memory");
+  constexpr uint32_t C_Q = 0, C_S = 2 * QC, C_O = C_S + 2 * PT, C_O2 = C_O + HDP, COLS = 512;
+  static_assert(C_O2 + HDP <= COLS, "tensor memory");
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t kfull[2], vfull[2], pfull[2], qk_done[2], pv_done[2], qfull;
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = h * (HDP / 2); c < (h + 1) * (HDP / 2); c += 8) {
+            for (int c = h * HDP; c < (h + 1) * HDP; c += 8) {  // (of both sums)
               float o[8];
               tc_ld8(tl + C_O + c, o);
               tc_wait_ld();
@@ -451,8 +455,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             }
             tc_wait_st();
           }
-          if (use && !(ok = wait(&pv_done[s], use - 1))) break;  // P's last reader
-          tc_fence_after();
+          tc_fence_after();  // (both halves have read S; P takes its place)
           const float shift = M == -INFINITY ? 0.0f : P_TOP - M;
           const f32x2 shift2 = pk(shift, shift);
 #pragma unroll
@@ -471,8 +474,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
               l = fma2(e, vd.y, l);
               split2(e, hi[j / 2 + 1], lo[j / 2 + 1]);
             }
-            tc_st8(tl + C_P + s * PT + h * 16 + c / 2, hi);
-            tc_st8(tl + C_P + s * PT + 32 + h * 16 + c / 2, lo);
+            tc_st8(tl + C_S + s * PT + h * 16 + c / 2, hi);
+            tc_st8(tl + C_S + s * PT + 32 + h * 16 + c / 2, lo);
           }
           tc_wait_st();
           tc_fence_before();
@@ -502,6 +505,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           float o[32];
           tc_ld32(tl + C_O + h * (HDP / 2) + c, o);
           tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            float o2[8];
+            tc_ld8(tl + C_O2 + h * (HDP / 2) + c + j, o2);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[j + e] += o2[e];
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<float4*>(stage + (lane * CH + (((c + j) / 4) ^ (lane % CH))) * 16) =
@@ -622,17 +633,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       auto scores = [&](int k) {  // S of tile k
         const int s = k & 1, use = k >> 1;
         if (!(ok = wait(&kfull[s], use))) return;
+        if (use && !(ok = wait(&pv_done[s], use - 1))) return;  // P of the tile before last is there
         tc_fence_after();
         if (tc_elect()) {
           const uint32_t kb = k_lo + s * (L::STAGE >> 4), d = tb + C_S + s * PT, q = tb + C_Q;
+          auto at = [](int ks) { return (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32) >> 4; };
 #pragma unroll
           for (int ks = 0; ks < HDP / 16; ks++) {
-            const uint32_t o = (uint32_t)((ks >> 2) * PT * 128 + (ks & 3) * 32) >> 4;
-            if (ks == 0) tc_mma_ts<false>(d, q, kb, k_hi, id_s);
-            else tc_mma_ts<true>(d, q + ks * 8, kb + o, k_hi, id_s);
-            tc_mma_ts<true>(d, q + ks * 8, kb + (L::PART >> 4) + o, k_hi, id_s);
-            tc_mma_ts<true>(d, q + QC + ks * 8, kb + o, k_hi, id_s);
+            if (ks == 0) tc_mma_ts<false>(d, q, kb + (L::PART >> 4), k_hi, id_s);
+            else tc_mma_ts<true>(d, q + ks * 8, kb + (L::PART >> 4) + at(ks), k_hi, id_s);
+            tc_mma_ts<true>(d, q + QC + ks * 8, kb + at(ks), k_hi, id_s);
           }
+#pragma unroll
+          for (int ks = 0; ks < HDP / 16; ks++) tc_mma_ts<true>(d, q + ks * 8, kb + at(ks), k_hi, id_s);
           tc_commit(&qk_done[s]);
         }
         __syncwarp();
@@ -649,14 +662,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
           if (!ok || !(ok = wait(&pfull[s], use))) break;  // (after V: the softmax waits for its scales)
           tc_fence_after();
           if (tc_elect()) {
-            const uint32_t vb = v_lo + s * (L::STAGE >> 4), p = tb + C_P + s * PT, d = tb + C_O;
+            const uint32_t vb = v_lo + s * (L::STAGE >> 4), p = tb + C_S + s * PT, d = tb + C_O, d2 = tb + C_O2;
 #pragma unroll
             for (int ks = 0; ks < PT / 16; ks++) {
               const uint32_t o = ks * 2048 >> 4;
-              if (ks == 0 && t == 0) tc_mma_ts<false>(d, p, vb, v_hi, id_o);
-              else tc_mma_ts<true>(d, p + ks * 8, vb + o, v_hi, id_o);
-              tc_mma_ts<true>(d, p + ks * 8, vb + (L::PART >> 4) + o, v_hi, id_o);
-              tc_mma_ts<true>(d, p + 32 + ks * 8, vb + o, v_hi, id_o);
+              if (ks == 0 && t == 0) {
+                tc_mma_ts<false>(d, p, vb, v_hi, id_o);
+                tc_mma_ts<false>(d2, p, vb + (L::PART >> 4), v_hi, id_o);
+              } else {
+                tc_mma_ts<true>(d, p + ks * 8, vb + o, v_hi, id_o);
+                tc_mma_ts<true>(d2, p + ks * 8, vb + (L::PART >> 4) + o, v_hi, id_o);
+              }
+              tc_mma_ts<true>(d2, p + 32 + ks * 8, vb + o, v_hi, id_o);
             }
             tc_commit(&pv_done[s]);
           }
