@@ -362,7 +362,8 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
  * the schedule belong to the plan: its calls run in stream order, one at a
  * time; two streams or graphs that overlap need a plan each. _set is not for
  * captured streams; a captured attention call may be replayed after a later
- * _set of the same number of rows in groups that share (or not) as before.
+ * _set of the same number of rows in groups that share (or not) as before (which
+ * then keeps the captured call's choice of kernels, whatever the lengths).
  * head_dim <= 128; at most 512 rows in a plan. Destroy the plan before its cache. */
 typedef struct syn_cuda_decode_plan_s syn_cuda_decode_plan_t;
 syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t *cache, size_t n_heads,

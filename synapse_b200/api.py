@@ -666,6 +666,8 @@ class DecodePlan:
     def set(self, groups):
         """groups: lists of sequences; row r of an attention call is the r-th
         sequence of them all."""
+        if not self.cache.handle:
+            raise SynapseError(1, "decode_plan_set: the cache is closed")
         groups = [list(g) for g in groups]
         seqs, sizes = _int32s(s for g in groups for s in g), _sizes(len(g) for g in groups)
         _check(lib().syn_cuda_decode_plan_set(self.handle, len(sizes), sizes.buffer_info()[0],
@@ -698,6 +700,8 @@ def attention_decode_shared(plan, layer, qkv, q_norm, k_norm, eps, cos_t, sin_t,
     once (syn_cuda_attention_decode_shared); qkv rows [q | k | v]. Returns
     [rows, n_heads*hd]; the cache lengths are not advanced."""
     cache, n_heads = plan.cache, plan.n_heads
+    if not cache.handle:
+        raise SynapseError(1, "attention_decode_shared: the cache is closed")
     _check_qkv(cache, layer, qkv, n_heads, q_norm, k_norm, cos_t, sin_t)
     qd, kvd, ld = n_heads * cache.hd, cache.n_kv * cache.hd, qkv.shape[1]
     if qkv.shape[0] != plan.rows:

@@ -281,7 +281,7 @@ struct syn_cuda_model_s {
   int32_t* hist_parent = nullptr;
   void* beam_scratch = nullptr;
   // captured steps; what a step's launches are made from
-  std::map<std::tuple<size_t, bool, int32_t, void*, void*, void*, void*>, cudaGraphExec_t> beam_graphs;
+  std::map<std::tuple<size_t, int, int32_t, void*, void*, void*, void*>, cudaGraphExec_t> beam_graphs;
 };
 
 namespace {
@@ -358,17 +358,6 @@ syn_status_t mm(syn_cuda_model_s* m, const syn_cuda_weight_t* w, const float* x,
   return syn_cuda_qmatmul(m->ctx, w, x, rows, y, m->st);
 }
 
-// One forward over `rows` rows. Prefill: rows tokens of sequence `seq`.
-// Decode: rows sequences [0, rows), one token each.
-// chained: the step's input tokens are the previous step's outputs (m->tok),
-// and nothing is copied to the host.
-// span: rows are consecutive new positions of sequence `seq` (speculative
-// drafting and verification): attention through launch_attn_span_args,
-// logits and greedy tokens for every row into the span buffers, no cache
-// length advanced. nlayers < L runs only the first nlayers layers (the
-// reference's layer-skipping draft, pipeline.rs:281-330).
-// beam: a chained step of beams (sequences `slots`): attention by the plan where there is one, the best
-// continuations instead of each row's greedy token.
 struct BeamStep {
   syn_cuda_decode_plan_t* plan;  // or nullptr
   int32_t eos;                   // -1: none
@@ -386,6 +375,17 @@ syn_status_t beam_best(syn_cuda_model_s* m, size_t beams, size_t rows, int32_t e
                           m->hist_parent, (int)(m->max_seq + 1), m->st);
 }
 
+// One forward over `rows` rows. Prefill: rows tokens of sequence `seq`.
+// Decode: rows sequences [0, rows), one token each.
+// chained: the step's input tokens are the previous step's outputs (m->tok),
+// and nothing is copied to the host.
+// span: rows are consecutive new positions of sequence `seq` (speculative
+// drafting and verification): attention through launch_attn_span_args,
+// logits and greedy tokens for every row into the span buffers, no cache
+// length advanced. nlayers < L runs only the first nlayers layers (the
+// reference's layer-skipping draft, pipeline.rs:281-330).
+// beam: a chained step of beams (sequences `slots`): attention by the plan where there is one, the best
+// continuations instead of each row's greedy token.
 syn_status_t forward(syn_cuda_model_s* m, size_t rows, bool prefill, size_t seq, bool want_logits,
                      bool chained = false, size_t nlayers = 0, bool span = false,
                      const int* slots = nullptr, const BeamStep* beam = nullptr) {
@@ -1089,9 +1089,10 @@ syn_status_t beam_buffers(syn_cuda_model_s* m) {
 }
 
 // One step of every beam: by its graph where there is one (or `capture` makes it).
-syn_status_t beam_step(syn_cuda_model_s* m, size_t beams, bool shared, const BeamStep& bs, bool capture) {
+syn_status_t beam_step(syn_cuda_model_s* m, size_t beams, const BeamStep& bs, bool capture) {
   // (growing scratch buffers move: their addresses are part of the key)
-  const auto key = std::make_tuple(beams, shared, bs.eos, (void*)m->ctx->part, (void*)m->ctx->cnt,
+  const int layout = bs.plan ? decode_plan_layout(bs.plan) : 0;
+  const auto key = std::make_tuple(beams, layout, bs.eos, (void*)m->ctx->part, (void*)m->ctx->cnt,
                                    (void*)m->ctx->abuf, (void*)m->cache->part);
   auto it = m->beam_graphs.find(key);
   if (it == m->beam_graphs.end() && !capture)
@@ -1138,15 +1139,13 @@ syn_status_t beam_search(syn_cuda_model_s* m, size_t seq, const int32_t* prompt,
   for (size_t b = 0; b < beams; b++)  // every page that the steps will write
     if ((s = kv_reserve(c, seq + b, n + n_steps - 1, st))) return s;
   BeamStep bs{m->plan, eos};
-  size_t shared = 0;
-  if (m->plan) {
-    if ((s = syn_cuda_decode_plan_set(m->plan, 1, &beams, seqs, st))) return s;
-    if ((s = syn_cuda_decode_plan_prefix(m->plan, 0, &shared))) return s;
-  }
+  if (m->plan && (s = syn_cuda_decode_plan_set(m->plan, 1, &beams, seqs, st))) return s;
   if ((s = beam_best(m, 1, beams, eos, 0))) return s;
   for (size_t t = 1; t < n_steps; t++) {
+    // (by now all beams may come from one that wrote pages after the prompt, and the work has grown)
+    if (m->plan && t % 128 == 0 && (s = syn_cuda_decode_plan_set(m->plan, 1, &beams, seqs, st))) return s;
     // the first step sizes the scratch buffers; the second is captured
-    if ((s = beam_step(m, beams, shared > 0, bs, t > 1 && use_graphs()))) return s;
+    if ((s = beam_step(m, beams, bs, t > 1 && use_graphs()))) return s;
     for (size_t b = 0; b < beams; b++) c->len[seq + b]++;
     if (beams > 1) {
       if ((s = launch_kv_reorder(c, beams, seqs, m->beam_parent, beams, &c->len[seq], st))) return s;

@@ -18,6 +18,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <array>
+#include <map>
 #include <new>
 #include <vector>
 
@@ -48,6 +50,10 @@ struct syn_cuda_decode_plan_s {
   void* shares = nullptr;    // k_span's shares and jobs (Share, SpanJob), written by k_begin
   int units = 0, span_jobs = 0, jobs = 0;  // k_span's units and jobs; k_prefix's jobs
   int prefix_ctas = 0, span_sms = 0;       // of their launches
+  // The layout (CTAs of k_prefix; 0: none) that captured calls of a shape were made with: later
+  // sets of the shape keep to it, since a replay launches the same kernels and grids.
+  std::array<int, 4> shape{};  // rows, units, k_span's jobs and whether k_prefix has any, if all share
+  std::map<std::array<int, 4>, int> captured;
 };
 
 namespace syn {
@@ -58,7 +64,10 @@ constexpr int PM = 128;        // query rows of a prefix job
 constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: computing warps of a CTA, keys of a tile
 constexpr int SP_THREADS = 64 * SP_WARPS;
 constexpr int SP_V = 8;        // most query vectors of a k_span job
-constexpr int SP_FEW = 8;      // a group of at most so many query rows per KV head goes to k_span
+// A group of at most so many query rows per KV head goes to k_span, which reads its prefix once for 8
+// of them. 8 query rows behind 512, 2048, 8192 positions take 12.4, 17.1, 26.9 us there and
+// 13.4, 15.7, 27.4 in k_prefix; 16 (two readings) 13.2, 19.2, 35.2 and 14.3, 17.6, 28.5.
+constexpr int SP_FEW = 8;
 constexpr int ROWS_MAX = 512;  // rows of a plan
 constexpr int UNITS_MAX = ROWS_MAX + ROWS_MAX / 2;
 
@@ -164,6 +173,11 @@ struct SharedArgs {
 // O stays in tensor memory; it is rescaled only when the maximum grows by more
 // than 2^8 (P keeps 2^7 as its nominal top, so it stays below fp16's 2^16).
 // Waits are bounded (SYN_ERR_TIMEOUT).
+// 64 rows x 32 heads behind 32768 positions (8 KV heads of 128) take 163 us in all, 145
+// of them here: 2.5 us a tile, of which the products are 0.9; conversions and
+// softmax fill 56 % of the issue slots and wait for each other the rest. (8 converting
+// warps in place of 16: 176 us; a warp that issues among them: 303.) A CTA's first tile
+// takes 7 us, latencies of the page table, the rows, and 64 KB of O per item.
 // ---------------------------------------------------------------------------
 constexpr int PX_SOFT = 8, PX_CONV = 16;  // warps; then four of which one issues the products
 constexpr int PX_MMA_WARP = PX_SOFT + PX_CONV;
@@ -1274,6 +1288,10 @@ size_t span_jobs(size_t batch, size_t n_kv, size_t G) {
 
 }  // namespace
 
+int decode_plan_layout(const syn_cuda_decode_plan_t* p) {
+  return p->jobs ? p->prefix_ctas : p->units == (int)p->rows ? 0 : -1;
+}
+
 syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, int* err,
                                 cudaStream_t st) {
   syn_cuda_kvcache_t* c = p->cache;
@@ -1537,12 +1555,14 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   const int only = env ? atoi(env) : 0;
   lay_out(true);
   p->prefix_ctas = p->span_sms = p->sms;
+  p->shape = {(int)rows, nu, uj, nj > 0};
+  const auto kept = p->captured.find(p->shape);
   double best = span_us(p->sms) + (nj ? prefix_us(p->sms) : 0);
-  if (nj && only != 2) {
+  if (kept == p->captured.end() && nj && only != 2) {
     // k_span behind k_prefix, each on all SMs, or side by side, each on its own: 8 rows behind 2048
     // positions take 19.1 us behind and 15.0 side by side, 64 rows behind 32768 169 and 181
     double least = only == 3 ? 1e30 : 0.85 * best;
-    for (int n = 4; n < p->sms; n += 4) {
+    for (int n = 12; n < p->sms; n += 12) {
       const double us = std::max(prefix_us(n), span_us(p->sms - n));
       if (us < least) {
         best = least = us;
@@ -1554,8 +1574,14 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   // A short prefix is read by each row for itself: 56 rows behind 42 positions take 11.2 us so, and
   // 20.3 with k_prefix.
   lay_out(false);
-  if (only ? only == 1 : span_us(p->sms) < 0.85 * best) p->prefix_ctas = p->span_sms = p->sms;
-  else lay_out(true);
+  if (kept != p->captured.end() ? !kept->second : only ? only == 1 : span_us(p->sms) < 0.85 * best)
+    p->prefix_ctas = p->span_sms = p->sms;
+  else
+    lay_out(true);
+  if (kept != p->captured.end() && kept->second > 0 && kept->second < p->sms) {
+    p->prefix_ctas = kept->second;
+    p->span_sms = p->sms - kept->second;
+  }
   size_t ni = 0, part = 0, done = 0, jt = 0;
   auto item_of = [&](const Job& job, size_t t0, size_t t1) {
     return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
@@ -1640,6 +1666,9 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
   syn_status_t s;
   for (size_t i = 0; i < p->rows; i++)
     if ((s = kv_reserve(c, p->seqs[i], c->len[p->seqs[i]] + 1, st))) return s;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+  if (cs != cudaStreamCaptureStatusNone) p->captured[p->shape] = decode_plan_layout(p);
   AttnArgs a{const_cast<float*>(q), k, v, ld, p->n_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
              window, c, layer, out, ldo};
   return launch_attn_shared(p, a, nullptr, st);

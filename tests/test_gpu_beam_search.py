@@ -41,8 +41,8 @@ def _logp(x):
 class Plain:
     """Logits behind prompt + tokens, one hypothesis at a time; and the search."""
 
-    def __init__(self, ctx, cfg, w, fmt, prompt):
-        self.m = sb.Model(ctx, cfg, w, MAX_SEQ)
+    def __init__(self, ctx, cfg, w, fmt, prompt, max_seq=MAX_SEQ):
+        self.m = sb.Model(ctx, cfg, w, max_seq)
         self.n = len(prompt)
         _, self.first = self.m.forward_prefill(prompt)
         self.memo = {(): self.first}
@@ -94,6 +94,7 @@ def _check(plain, toks, scores, beams, steps, eos=-1):
     assert len({tuple(r) for r in toks.tolist()}) == beams
     for row, score in zip(toks.tolist(), scores):
         s, err = 0.0, 0.0
+        plain.logits(row[:-1])  # (and of all that lead there)
         for t, v in enumerate(row):
             x = plain.logits(row[:t])
             lp = _logp(x)
@@ -225,6 +226,21 @@ def test_graphs_and_eager_steps_agree(ctx, monkeypatch):
         assert np.array_equal(first[0], other[0])
         assert np.array_equal(first[1], other[1])
     m.close()
+
+
+def test_more_steps_than_a_plan_is_kept_for(ctx):
+    """300 steps: the plan is made again on the way, with what the beams share by then."""
+    cfg, w = _weights("Q4_0", "tiny-hd64")
+    plain = Plain(ctx, cfg, w, "Q4_0", PROMPTS[33], 340)
+    m = sb.Model(ctx, cfg, w, 340, max_batch=4, kv_page=16, kv_pages=2 + 4 * 20)
+    toks, scores = m.generate_beam(PROMPTS[33], 300, 4)
+    _check(plain, toks, scores, 4, 300)
+    _, lg = m.decode_slots([0, 1, 2, 3], toks[:, -1], want_logits=True)
+    for row, x in zip(toks.tolist(), lg):
+        want = plain.logits(row)
+        assert np.abs(x - want).max() <= 1e-3 * np.abs(want).max()
+    m.close()
+    plain.close()
 
 
 def test_pool_exhausted(ctx):

@@ -252,6 +252,30 @@ def test_captured_and_replayed_with_another_set(ctx):
     b.check(out=want)
 
 
+def test_captured_and_replayed_with_longer_prefixes(ctx):
+    """Of lengths for which a plan by itself would choose another layout, both ways."""
+    b = Batch(ctx, 8, 16, 128, 16, [32, 3000], [[1, 5, 0, 3] * 2, [2, 0, 40, 7] * 2], seed=8)
+    lens, qkv = list(b.lens), b.qkv
+    for first in (0, 1):
+        b.plan = sb.DecodePlan(b.cache, b.heads)
+        buf = torch.empty_like(qkv[:8])
+        b.plan.set([b.groups[first]])
+        sb.attention_decode_shared(b.plan, 0, buf, None, None, 1e-6, b.cos, b.sin)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sb.attention_decode_shared(b.plan, 0, buf, None, None, 1e-6, b.cos, b.sin)
+        got = torch.empty(16, 16 * 128, device="cuda")
+        for g in (1 - first, first):
+            b.plan.set([b.groups[g]])
+            buf.copy_(qkv[b.groups[g]])
+            sb.attention_decode_shared(b.plan, 0, buf, None, None, 1e-6, b.cos, b.sin)  # reserves
+            out.zero_()
+            graph.replay()
+            got[b.groups[g]] = out
+        torch.cuda.synchronize()
+        b.check(out=got, lens=lens)
+
+
 def test_two_plans_on_two_streams(ctx):
     b = Batch(ctx, 2, 8, 64, 16, [400, 401], [[3, 0, 5], [1, 1, 2]], seed=6)
     plans = [sb.DecodePlan(b.cache, 8) for _ in range(2)]
@@ -309,3 +333,8 @@ def test_refusals(ctx):
     assert e.value.status == 2
     b.plan.set([])
     assert sb.attention_decode_shared(b.plan, 0, b.qkv[:0], None, None, 1e-6, b.cos, b.sin).shape == (0, 256)
+    b.cache.close()
+    for act in (lambda: b.plan.set([[0]]), call):
+        with pytest.raises(sb.SynapseError) as e:
+            act()
+        assert e.value.status == 1
