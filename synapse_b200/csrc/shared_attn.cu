@@ -1542,10 +1542,10 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     while ((size_t)nj <= n && items_at(most) > n) most++;
     return most;
   };
-  // What the kernels take (us, measured at head dim 128): k_prefix 7, and 1.6 + 0.008 m a tile of m
-  // query rows; k_span 4, 2.5 a tile of each warp, and k_join 1 for 32 records of a row. The rows are
-  // taken 128 positions on, as they grow before the plan is next set.
-  auto prefix_us = [&](int n) { return 7 + (1.6 + 0.008 * widest) * most_of(n); };
+  // What the kernels take (us, measured at head dim 128): k_prefix 4 + 0.05 m for m query rows (at
+  // least 7) and 1.2 + 0.0165 m (at most 2.6) a tile; k_span 4, 2.5 a tile of each warp, and k_join 1 for 32 records
+  // of a row. The rows are taken 128 positions on, as they grow before the plan is next set.
+  auto prefix_us = [&](int n) { return std::max(7.0, 4 + 0.05 * widest) + std::min(2.6, 1.2 + 0.0165 * widest) * most_of(n); };
   auto span_us = [&](int n) {
     const size_t per = std::max<size_t>(1, (own + SP_WARPS * n - 1) / (SP_WARPS * n));
     return 4 + 2.5 * per + longest / per / 32;
@@ -1560,7 +1560,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   double best = span_us(p->sms) + (nj ? prefix_us(p->sms) : 0);
   if (kept == p->captured.end() && nj && only != 2) {
     // k_span behind k_prefix, each on all SMs, or side by side, each on its own: 8 rows behind 2048
-    // positions take 19.1 us behind and 15.0 side by side, 64 rows behind 32768 169 and 181
+    // positions take 19.1 us behind and 15.6 side by side, 64 rows behind 32768 are 7 % slower so
     double least = only == 3 ? 1e30 : 0.85 * best;
     for (int n = 12; n < p->sms; n += 12) {
       const double us = std::max(prefix_us(n), span_us(p->sms - n));
