@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <map>
 #include <mutex>
 #include <vector>
 
@@ -680,13 +681,14 @@ syn_status_t launch_beam_note(syn_cuda_kvcache_t* c, const int* slots, size_t n,
 
 syn_status_t more_smem(const void* fn, size_t bytes) {
   static std::mutex mu;
-  static std::vector<std::pair<const void*, int>> done;
+  static std::map<std::pair<const void*, int>, size_t> granted;
   int dev = 0;
   SYN_CUDA_TRY(cudaGetDevice(&dev));
   std::lock_guard<std::mutex> g(mu);
-  if (std::find(done.begin(), done.end(), std::make_pair(fn, dev)) != done.end()) return SYN_OK;
+  size_t& has = granted[{fn, dev}];
+  if (bytes <= has) return SYN_OK;
   SYN_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  done.push_back({fn, dev});
+  has = bytes;
   return SYN_OK;
 }
 

@@ -311,8 +311,8 @@ syn_status_t launch_beam_note(syn_cuda_kvcache_t* c, const int* slots, size_t n,
                               const int32_t* tok, const int32_t* par, int32_t* hist,
                               int32_t* hist_parent, int ld, cudaStream_t st);
 constexpr size_t BEAMS_MAX = 64;  // beams of a group, continuations of a selection
-// Lets a kernel have `bytes` of dynamic shared memory on the current device (asked of the
-// runtime once per kernel and device; always with the same bytes for a kernel).
+// Lets a kernel have `bytes` of dynamic shared memory on the current device (the runtime is asked
+// only where a kernel needs more than it has been given there).
 syn_status_t more_smem(const void* fn, size_t bytes);
 size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms);
 syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
