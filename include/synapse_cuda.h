@@ -358,7 +358,8 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
  * the batch's rows: n_groups groups of group_rows[g] sequences each (seqs, host
  * arrays, all distinct). _set finds for each group the leading pages that all
  * its sequences hold, and schedules their work; what a group does not share
- * (all of it on a contiguous cache) is computed row by row. The workspaces and
+ * (all of it on a contiguous cache) is computed row by row; so is what captured
+ * reorders may exchange with sequences that do not hold it. The workspaces and
  * the schedule belong to the plan: its calls run in stream order, one at a
  * time; two streams or graphs that overlap need a plan each. _set is not for
  * captured streams; a captured attention call may be replayed after a later
@@ -381,7 +382,8 @@ syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t *plan, siz
  * last `window`. Results within f32 reassociation of the reference order. The
  * lengths are not advanced. Cache positions that no row of a group sees (behind
  * its sequences, outside all windows) may hold anything. SYN_ERR_INVALID_ARG when a sequence was truncated,
- * reset or forked into since _set. */
+ * reset or forked into since _set, or when a reorder since then joined some of a group's sequences with
+ * one that did not hold the group's shared pages: _set describes the batch anew. */
 syn_status_t syn_cuda_attention_decode_shared(
     syn_cuda_decode_plan_t *plan, size_t layer, const float *q, const float *k, const float *v,
     size_t ld, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,

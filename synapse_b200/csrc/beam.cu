@@ -729,10 +729,15 @@ syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
   c->refs[old]--;
   c->refs[own] = 1;
   *e = own;
-  c->shrunk[seq]++;
+  kv_changed(c, seq);
   SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + seq * c->maxp + col, e, sizeof(int),
                                cudaMemcpyHostToDevice, st));
   return SYN_OK;
+}
+
+void kv_changed(syn_cuda_kvcache_t* c, size_t seq) {
+  c->shrunk[seq]++;
+  plans_changed(c, seq);
 }
 
 syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st) {
@@ -917,7 +922,7 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t* c, size_t src, size_t dst
     c->refs[to[full]] = 1;
     if ((s = kv_copy_page(c, from[full], to[full], tail, st))) return s;
   }
-  c->shrunk[dst]++;
+  kv_changed(c, dst);
   if (len)
     SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + dst * c->maxp, to, (full + (tail != 0)) * sizeof(int),
                                  cudaMemcpyHostToDevice, st));
@@ -946,6 +951,14 @@ syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int
   syn_status_t s;
   for (size_t i = 0; i < n; i++)
     if ((s = kv_own_page(c, seqs[i], st))) return s;
+  const bool captured = capturing(st);
+  for (size_t i = 0; i < n; i += beams) {
+    plans_reordered(c, seqs + i, beams);
+    std::vector<int32_t> mix(seqs + i, seqs + i + beams);
+    std::sort(mix.begin(), mix.end());
+    if (captured && std::find(c->mixes.begin(), c->mixes.end(), mix) == c->mixes.end())
+      c->mixes.push_back(std::move(mix));
+  }
   const size_t per = RO_MAX / beams * beams;
   for (size_t i0 = 0; i0 < n; i0 += per) {
     const size_t m = std::min(per, n - i0);
@@ -953,7 +966,7 @@ syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int
     for (size_t i = 0; i < m; i += beams) lens[i / beams] = c->len[seqs[i0 + i]];
     if ((s = launch_kv_reorder(c, m, seqs + i0, parents + i0, beams, lens, st))) return s;
   }
-  const uint8_t mark = capturing(st) ? 2 : 1;
+  const uint8_t mark = captured ? 2 : 1;
   for (size_t i = 0; i < n; i++) {
     c->n_stale += !c->stale[seqs[i]];
     c->stale[seqs[i]] = std::max(c->stale[seqs[i]], mark);

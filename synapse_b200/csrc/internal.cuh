@@ -2,6 +2,7 @@
 #pragma once
 
 #include <utility>
+#include <vector>
 
 #include "common.cuh"
 
@@ -54,6 +55,7 @@ struct syn_cuda_weight_s {
 // and truncate together). The device copy of the lengths is what kernels
 // read (so that a captured graph replays at the current position); the host
 // copy mirrors it for the CacheFull check.
+struct syn_cuda_decode_plan_s;
 struct syn_cuda_kvcache_s {
   int device;
   size_t max_seq, n_kv, hd, layers, batch;
@@ -82,6 +84,10 @@ struct syn_cuda_kvcache_s {
   uint8_t* stale;    // [batch]
   size_t n_stale;
   size_t* shrunk;    // [batch]
+  // The decode plans made on the cache, which are told what moves their sequences' pages, and the
+  // groups of the reorders that were captured, which a graph may run at any time.
+  std::vector<syn_cuda_decode_plan_s*> plans;
+  std::vector<std::vector<int32_t>> mixes;
 };
 
 namespace syn {
@@ -240,6 +246,8 @@ syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, 
 // Reads the table rows that were permuted on the device back to the host and
 // recounts the pages (synchronises the device; refused while `st` is captured).
 syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st);
+// Pages that seq shared may be its no longer: counted, and the plans told.
+void kv_changed(syn_cuda_kvcache_t* c, size_t seq);
 // Frees the pages of seq beyond position keep_len (drains `st` first).
 syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cudaStream_t st);
 // Decode step of sequences [0, batch): norm/RoPE/append of the new token,
@@ -301,6 +309,12 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 // What the launches of a plan's attention depend on beside its rows: k_prefix's CTAs, 0 when each
 // row reads all of its positions, -1 when groups share some without k_prefix.
 int decode_plan_layout(const syn_cuda_decode_plan_t* p);
+// A reorder of the group seqs[0 .. n): plans in which some but not all of them hold a group's shared
+// pages describe their rows no longer. _changed: the same for one sequence whose pages are its own now.
+void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n);
+void plans_changed(syn_cuda_kvcache_t* c, size_t seq);
+// The cache goes: its plans refuse every call but their end.
+void plans_orphaned(syn_cuda_kvcache_t* c);
 // Decode attention of a plan's rows (q, k, v, the layer and the output in a;
 // pages reserved).
 syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& a, int* err,

@@ -2152,7 +2152,7 @@ syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cuda
   SYN_CUDA_TRY(cudaStreamSynchronize(st));
   syn_status_t s = kv_sync(c, st);
   if (s) return s;
-  c->shrunk[seq]++;
+  kv_changed(c, seq);
   int* row = c->ptab_h + seq * c->maxp;
   const size_t keep = (keep_len + c->page - 1) / c->page;
   bool changed = false;
@@ -2318,6 +2318,7 @@ syn_status_t syn_cuda_kvcache_pages_free(const syn_cuda_kvcache_t* c, size_t* n)
 
 syn_status_t syn_cuda_kvcache_destroy(syn_cuda_kvcache_t* c) {
   if (!c) return SYN_ERR_NULL_PTR;
+  plans_orphaned(c);
   DeviceGuard g(c->device);
   cudaDeviceSynchronize();
   cudaFree(c->k);

@@ -27,6 +27,12 @@
 #include "internal.cuh"
 #include "tcgen05.cuh"
 
+// A group's rows share their leading positions: who holds those pages. A reorder among holders
+// leaves every row with them; one that brings in another sequence's context does not.
+struct PlanFamily {
+  std::vector<uint8_t> holds;  // [batch]: 1, and 2 for those that the group depends on (its rows, and
+};                             // whatever a captured reorder may exchange with them)
+
 // A batch of decode rows in groups. Built on the host by _set: which leading
 // pages each group shares, and the schedule of its prefix work.
 struct syn_cuda_decode_plan_s {
@@ -35,6 +41,8 @@ struct syn_cuda_decode_plan_s {
   size_t n_heads;
   size_t rows = 0, groups = 0;
   std::vector<int32_t> seqs;
+  std::vector<PlanFamily> families;    // of the groups that share
+  bool parted = false;                 // a reorder since _set has taken what a group shared from it
   std::vector<size_t> prefix, shrunk;  // per row: shared positions; the sequence's state at _set
   // device
   float* q = nullptr;        // rotated queries [batch][n_heads * hd]
@@ -1293,6 +1301,28 @@ size_t span_jobs(size_t batch, size_t n_kv, size_t G) {
 
 }  // namespace
 
+void plans_changed(syn_cuda_kvcache_t* c, size_t seq) {
+  for (auto* p : c->plans)
+    for (auto& f : p->families) {
+      p->parted |= f.holds[seq] == 2;
+      f.holds[seq] = 0;
+    }
+}
+
+void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n) {
+  for (auto* p : c->plans)
+    for (auto& f : p->families)
+      if (!std::all_of(seqs, seqs + n, [&](int32_t s) { return f.holds[s] != 0; }))
+        for (size_t i = 0; i < n; i++) {
+          p->parted |= f.holds[seqs[i]] == 2;
+          f.holds[seqs[i]] = 0;
+        }
+}
+
+void plans_orphaned(syn_cuda_kvcache_t* c) {
+  for (auto* p : c->plans) p->cache = nullptr;
+}
+
 int decode_plan_layout(const syn_cuda_decode_plan_t* p) {
   return p->jobs ? p->prefix_ctas : p->units == (int)p->rows ? 0 : -1;
 }
@@ -1418,6 +1448,7 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
     syn_cuda_decode_plan_destroy(p);
     return SYN_ERR_OUT_OF_MEMORY;
   }
+  c->plans.push_back(p);
   *out = p;
   return SYN_OK;
 }
@@ -1425,6 +1456,10 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
 syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
   if (!p) return SYN_ERR_NULL_PTR;
   DeviceGuard g(p->device);
+  if (p->cache) {
+    auto& plans = p->cache->plans;
+    plans.erase(std::remove(plans.begin(), plans.end(), p), plans.end());
+  }
   cudaDeviceSynchronize();
   cudaFree(p->q);
   cudaFree(p->qparts);
@@ -1444,6 +1479,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
                                       void* stream) {
   if (!p || (n_groups && (!group_rows || !seqs))) return SYN_ERR_NULL_PTR;
   syn_cuda_kvcache_t* c = p->cache;
+  if (!c) return SYN_ERR_INVALID_ARG;
   DeviceGuard g(p->device);
   if (!g.ok) return SYN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1474,6 +1510,24 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   p->seqs.assign(seqs, seqs + rows);
   p->prefix.assign(rows, 0);
   p->shrunk.assign(rows, 0);
+  p->families.clear();
+  p->parted = false;
+  // the sequences of a group, and those that a captured reorder may exchange with them at any time
+  auto related = [&](size_t r0, size_t n) {
+    std::vector<uint8_t> in(c->batch, 0);
+    for (size_t j = r0; j < r0 + n; j++) in[seqs[j]] = 2;
+    for (bool more = true; more;) {
+      more = false;
+      for (const auto& mix : c->mixes)
+        if (std::any_of(mix.begin(), mix.end(), [&](int32_t s) { return in[s]; }))
+          for (int32_t s : mix) {
+            more |= !in[s];
+            in[s] = 2;
+          }
+    }
+    return in;
+  };
+  auto pages = [&](size_t s) { return c->ptab_h + s * c->maxp; };
   size_t r0 = 0;
   for (size_t i = 0; i < n_groups; r0 += group_rows[i++]) {
     const size_t n = group_rows[i];
@@ -1481,13 +1535,15 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     if (n > 1 && c->page) {
       size_t most = c->len[seqs[r0]];
       for (size_t j = r0; j < r0 + n; j++) most = std::min(most, c->len[seqs[j]]);
-      size_t col = 0;
-      for (bool same = true; (col + 1) * c->page <= most; col++) {
-        const int pg = c->ptab_h[seqs[r0] * c->maxp + col];
-        for (size_t j = r0; j < r0 + n && same; j++) same = c->ptab_h[seqs[j] * c->maxp + col] == pg;
-        if (!same) break;
-      }
+      PlanFamily f{related(r0, n)};
+      const int* first = pages(seqs[r0]);
+      size_t col = most / c->page;
+      for (size_t s = 0; s < c->batch; s++)
+        if (f.holds[s]) col = std::mismatch(first, first + col, pages(s)).first - first;
       shared = col * c->page;
+      for (size_t s = 0; s < c->batch && shared; s++)
+        if (std::equal(first, first + col, pages(s))) f.holds[s] = std::max<uint8_t>(f.holds[s], 1);
+      if (shared) p->families.push_back(std::move(f));
     }
     for (size_t j = r0; j < r0 + n; j++) {
       p->prefix[j] = shared;
@@ -1655,9 +1711,10 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
                                               size_t ldo, void* stream) {
   if (!p || !q || !k || !v || !rope_cos || !rope_sin || !out) return SYN_ERR_NULL_PTR;
   syn_cuda_kvcache_t* c = p->cache;
-  if (layer >= c->layers) return SYN_ERR_INVALID_ARG;
+  if (!c || layer >= c->layers) return SYN_ERR_INVALID_ARG;
   if (!p->rows) return SYN_OK;
   if (ld < c->hd || ldo < p->n_heads * c->hd) return SYN_ERR_SHAPE_MISMATCH;
+  if (p->parted) return SYN_ERR_INVALID_ARG;
   for (size_t i = 0; i < p->rows; i++) {
     const int sq = p->seqs[i];
     if (c->len[sq] + 1 > c->max_seq) return SYN_ERR_INVALID_ARG;  // CacheFull

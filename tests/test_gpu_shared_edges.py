@@ -46,3 +46,86 @@ def test_head_dims_in_ascending_order():
     code = ASCENDING.format(root=os.path.dirname(tests), tests=tests)
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
     assert out.returncode == 0 and "ascending ok" in out.stdout, out.stdout + out.stderr
+
+
+def _refused(call, status=2):
+    with pytest.raises(sb.SynapseError) as e:
+        call()
+    assert e.value.status == status
+
+
+def test_reorder_across_the_plans_groups(ctx):
+    """Two groups of two, and a reorder of all four: the second group's context moves into the
+    first one. The plan has to be set again, and then describes the new contexts."""
+    b = Batch(ctx, 2, 4, 64, 16, [64, 64], [[3, 3], [3, 3]], seed=3)
+    b.check()
+    b.cache.reorder([0, 1, 2, 3], _ints(2, 1, 0, 3), 4)
+    _refused(lambda: _attend(b))
+    b.plan.set(b.groups)
+    b.check()
+    b.cache.reorder([0, 1], _ints(1, 0), 2)  # inside a group: the plan holds
+    b.check()
+
+
+def test_reorder_with_a_sequence_outside_the_plan(ctx):
+    """A beam that has ended is left out of the plan, and still takes part in the reorder."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 80], [[19, 19, 19, 19], [3]], seed=5)
+    b.plan.set([[0, 1, 2]])
+    # sequence 3 holds the same prompt: the shared pages stay what they are
+    b.cache.reorder([0, 1, 2, 3], _ints(3, 3, 0, 1), 4)
+    b.check(out=_attend(b, rows=[0, 1, 2]), lens=b.lens[:3])
+    # sequence 4 does not
+    b.cache.reorder([0, 1, 2, 4], _ints(3, 1, 2, 0), 4)
+    _refused(lambda: _attend(b, rows=[0, 1, 2]))
+    b.plan.set([[0, 1, 2]])
+    b.check(out=_attend(b, rows=[0, 1, 2]), lens=b.lens[:3])
+
+
+def test_reorder_through_a_sequence_outside_the_plan(ctx):
+    """Another prompt's context comes into a sequence behind the plan's back, and from there
+    into a row of the plan."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 64], [[3, 3, 3], [3]], seed=6)
+    b.plan.set([[0, 1]])
+    b.cache.reorder([2, 3], _ints(1, 0), 2)
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+    b.cache.reorder([0, 2], _ints(1, 0), 2)
+    _refused(lambda: _attend(b, rows=[0, 1]))
+    b.plan.set([[0, 1]])
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+
+
+def test_reorder_after_a_family_member_was_used_anew(ctx):
+    """A sequence that held the shared pages when the plan was set, and no longer does."""
+    b = Batch(ctx, 1, 4, 64, 16, [64], [[3, 3, 3]], seed=7, spare=12)
+    b.plan.set([[0, 1]])
+    b.cache.reset(2)
+    b.cache.advance(67, 2)
+    b.cache.reorder([0, 2], _ints(1, 0), 2)
+    _refused(lambda: _attend(b, rows=[0, 1]))
+    b.plan.set([[0, 1]])
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+
+
+def test_captured_reorder_across_the_plans_groups(ctx):
+    """A captured reorder may run at any time after a set: what its sequences do not all hold
+    is not taken as shared."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 64], [[3, 3], [3, 3]], seed=8)
+    par = _ints(0, 1, 2, 3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.cache.reorder([0, 1, 2, 3], par, 4)
+    _refused(lambda: _attend(b))
+    b.plan.set(b.groups)
+    for p in ([2, 1, 0, 3], [3, 3, 0, 1]):
+        par.copy_(_ints(*p))
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check()
+
+
+def test_a_plan_outlives_its_cache(ctx):
+    b = Batch(ctx, 1, 2, 64, 16, [40], [[3, 0]], seed=9)
+    b.cache.close()
+    _refused(lambda: b.plan.set([[0]]), 1)
+    b.plan.close()
