@@ -180,7 +180,9 @@ struct SharedArgs {
 // P_j = 2^{x_j - M} is the size of the whole contribution, and l = sum P_j 2^{-e_j}.
 // O stays in tensor memory; it is rescaled only when the maximum grows by more
 // than 2^8 (P keeps 2^7 as its nominal top, so it stays below fp16's 2^16).
-// Waits are bounded (SYN_ERR_TIMEOUT).
+// Waits are bounded (SYN_ERR_TIMEOUT). The two warps of the same query rows also wait for each other at
+// a barrier that is not, so a warp whose wait has run out does not leave by itself: it says so at
+// their next barrier, and both leave behind it.
 // 64 rows x 32 heads behind 32768 positions (8 KV heads of 128) take 155 us in all, 137
 // of them here: 2.4 us a tile, of which the products are 0.9; conversions and
 // softmax fill 58 % of the issue slots and wait for each other the rest. (8 converting
@@ -330,6 +332,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   __shared__ __align__(8) uint64_t kfull[2], vfull[2], pfull[2], qk_done[2], pv_done[2], qfull;
   __shared__ __align__(16) float kup[2][PT], vexp[2][PT], vdown[2][PT];
   __shared__ float pmax[2][2][PM];  // [tile parity][half of the keys][row]
+  __shared__ int gone[PX_SOFT];     // a softmax warp's wait has run out, told with an item's record
   __shared__ uint32_t tbase_sh;
   __shared__ int fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -416,8 +419,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       for (int t = item.t0; t < item.t1; t++, n++) {
         const int s = n & 1, use = n >> 1;
         // (the scales of the tile's rows come with V)
-        if (!(ok = wait(&vfull[s], use)) || !(ok = wait(&qk_done[s], use))) break;
-        if (busy) {
+        ok = wait(&vfull[s], use) && wait(&qk_done[s], use);
+        if (!busy && !ok) break;
+        if (busy) {  // (!ok: it goes on with what is there, as far as the barrier)
           tc_fence_after();
           f32x2 y[16];
           {
@@ -452,10 +456,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             unpk(y[j + 1], p, q);
             mx2 = fmaxf(fmaxf(mx2, p), q);
           }
-          mx = fmaxf(mx, mx2);
-          pmax[n & 1][h][r] = mx;
+          mx = fmaxf(mx, mx2);  // (no NaN: a NaN here is a warp that gives up)
+          pmax[n & 1][h][r] = ok ? mx : NAN;
           pair_sync(pair);
-          mx = fmaxf(mx, pmax[n & 1][h ^ 1][r]);
+          const float other = pmax[n & 1][h ^ 1][r];
+          if (!ok || __any_sync(0xffffffffu, other != other)) {
+            ok = false;
+            break;
+          }
+          mx = fmaxf(mx, other);
           // a new reference only when the old one is too far below (the same in both halves)
           const bool grow = mx > M + P_GROW;  // (also from -inf)
           const float ref = grow ? mx : M;
@@ -465,7 +474,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             const float f = !grow ? 1.0f : M == -INFINITY ? 0.0f : ex2(M - ref);
             M = ref;
             l = mul2(l, pk(f, f));
-            if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
+            wait(&pv_done[(n - 1) & 1], (n - 1) >> 1);  // (if it runs out, `fail` is set and the result void)
             tc_fence_after();
 #pragma unroll 1
             for (int c = h * HDP; c < (h + 1) * HDP; c += 8) {  // (of both sums)
@@ -509,14 +518,20 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       }
       if (!ok) break;
       // the item's record: O and l are both relative to 2^(M - P_TOP)
-      if (!(ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1))) break;
+      ok = wait(&pv_done[(n - 1) & 1], (n - 1) >> 1);
+      if (!busy && !ok) break;
       if (busy) {
         tc_fence_after();
         float la, lb;
         unpk(l, la, lb);
         la += lb;
         if (h == 1) pmax[n & 1][1][r] = la;
+        if (lane == 0) gone[warp] = !ok;
         pair_sync(pair);
+        if (!ok || gone[warp ^ 4]) {
+          ok = false;
+          break;
+        }
         const bool none = M == -INFINITY;
         if (h == 0 && r < item.m)
           a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
