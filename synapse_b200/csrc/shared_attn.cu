@@ -1195,6 +1195,11 @@ __global__ void __launch_bounds__(SP_THREADS, 1) k_span(const SharedArgs a) {
     j++;
   }
   if (!ok && lane == 0 && a.err) atomicExch(a.err, SYN_ERR_TIMEOUT);
+  if (!ok && copies)  // nothing may land in a CTA that has gone: each slot's last copies
+    for (int i = 0; i < SP_SLOTS; i++) {
+      const int turn = (int)ring.turn - (i >= (int)ring.slot);
+      if (turn >= 0) mbar_wait_bounded(ring.full + i, turn & 1);
+    }
   if (a.after_prefix) griddep_wait();  // (k_join waits for this kernel's end, and so for k_prefix's)
 }
 
