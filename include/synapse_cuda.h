@@ -376,6 +376,11 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t *plan, size_t n_gro
 /* Positions that row `row` shares with its group. */
 syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t *plan, size_t row,
                                          size_t *len);
+/* Reads and clears the plan's device-side error word, where its attention calls
+ * record what they find only while they run: SYN_ERR_TIMEOUT (a wait ran out),
+ * SYN_ERR_INVALID_ARG (a replayed graph has gone past max_seq or the pages that
+ * were reserved). The rows concerned hold no result then. Waits for the device. */
+syn_status_t syn_cuda_decode_plan_get_error(syn_cuda_decode_plan_t *plan, int32_t *status);
 /* syn_cuda_attention_decode_flash for the plan's rows (row r of q / k / v / out
  * is sequence r of the plan; q is left as it is): headwise norms, RoPE, K and V
  * appended at each sequence's length, attention over all its positions or the

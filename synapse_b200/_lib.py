@@ -95,6 +95,7 @@ SIGNATURES = {
     "syn_cuda_decode_plan_destroy": (c_st, [c_vp]),
     "syn_cuda_decode_plan_set": (c_st, [c_vp, c_size, c_vp, c_vp, c_vp]),
     "syn_cuda_decode_plan_prefix": (c_st, [c_vp, c_size, ctypes.POINTER(c_size)]),
+    "syn_cuda_decode_plan_get_error": (c_st, [c_vp, ctypes.POINTER(ctypes.c_int32)]),
     "syn_cuda_attention_decode_shared": (c_st, [c_vp, c_size, c_vp, c_vp, c_vp, c_size, c_vp, c_vp,
                                                 ctypes.c_float, c_vp, c_vp, c_size, c_vp, c_size,
                                                 c_vp]),

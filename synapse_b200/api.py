@@ -682,6 +682,13 @@ class DecodePlan:
                "decode_plan_prefix")
         return v.value
 
+    def get_error(self):
+        """Status that the attention calls have recorded on the device since the last call (0: none),
+        read and cleared; waits for the device (syn_cuda_decode_plan_get_error)."""
+        v = ctypes.c_int32()
+        _check(lib().syn_cuda_decode_plan_get_error(self.handle, ctypes.byref(v)), "decode_plan_get_error")
+        return v.value
+
     def close(self):
         if self.handle:
             lib().syn_cuda_decode_plan_destroy(self.handle)

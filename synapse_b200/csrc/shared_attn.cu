@@ -43,6 +43,7 @@ struct syn_cuda_decode_plan_s {
   std::vector<int32_t> seqs;
   std::vector<PlanFamily> families;    // of the groups that share
   bool parted = false;                 // a reorder since _set has taken what a group shared from it
+  int* err = nullptr;                  // device: where the public calls' kernels record what failed
   std::vector<size_t> prefix, shrunk;  // per row: shared positions; the sequence's state at _set
   // device
   float* q = nullptr;        // rotated queries [batch][n_heads * hd]
@@ -771,7 +772,8 @@ __device__ __forceinline__ int2 unit_range(const SharedArgs& a, const Unit& u) {
     return make_int2(lo, u.pre);
   }
   const int L = a.len[seq[u.row0]] + 1;
-  if (L > a.max_seq) {  // a replayed graph that has run past the cache
+  // a replayed graph that has run past the cache, or past the pages that were reserved
+  if (L > a.max_seq || (a.ptab && a.ptab[(size_t)seq[u.row0] * a.maxp + (L - 1) / a.page] < 0)) {
     if (a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
     return make_int2(0, 0);
   }
@@ -1460,6 +1462,8 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   if (e == cudaSuccess)
     e = cudaMalloc(&p->shares, p->sms * span_ctas(c->hd) * SP_WARPS * sizeof(Share) +
                                    span_jobs(c->batch, c->n_kv, G) * sizeof(SpanJob));
+  if (e == cudaSuccess) e = cudaMalloc(&p->err, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(p->err, 0, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(p->meta, 0, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&p->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -1489,6 +1493,7 @@ syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
   cudaFree(p->po);
   cudaFree(p->pml);
   cudaFree(p->shares);
+  cudaFree(p->err);
   if (p->copied) cudaEventDestroy(p->copied);
   delete p;
   return SYN_OK;
@@ -1723,6 +1728,18 @@ syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t* p, size_t
   return SYN_OK;
 }
 
+syn_status_t syn_cuda_decode_plan_get_error(syn_cuda_decode_plan_t* p, int32_t* status) {
+  if (!p || !status) return SYN_ERR_NULL_PTR;
+  DeviceGuard g(p->device);
+  if (!g.ok) return SYN_ERR_CUDA;
+  int v = 0;
+  SYN_CUDA_TRY(cudaDeviceSynchronize());
+  SYN_CUDA_TRY(cudaMemcpy(&v, p->err, sizeof(int), cudaMemcpyDeviceToHost));
+  SYN_CUDA_TRY(cudaMemset(p->err, 0, sizeof(int)));
+  *status = v;
+  return SYN_OK;
+}
+
 syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t layer,
                                               const float* q, const float* k, const float* v,
                                               size_t ld, const float* q_norm, const float* k_norm,
@@ -1753,7 +1770,7 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
   if (cs != cudaStreamCaptureStatusNone) p->captured[p->shape] = decode_plan_layout(p);
   AttnArgs a{const_cast<float*>(q), k, v, ld, p->n_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
              window, c, layer, out, ldo};
-  return launch_attn_shared(p, a, nullptr, st);
+  return launch_attn_shared(p, a, p->err, st);
 }
 
 }  // extern "C"

@@ -129,3 +129,40 @@ def test_a_plan_outlives_its_cache(ctx):
     b.cache.close()
     _refused(lambda: b.plan.set([[0]]), 1)
     b.plan.close()
+
+
+def test_errors_of_replays_are_reported(ctx):
+    """What a replay cannot do is kept in the plan's error word: a position behind max_seq, and
+    one for which no page was reserved."""
+    b = Batch(ctx, 1, 4, 64, 16, [40], [[7, 0]], seed=21)
+    c = b.cache  # max_seq 51
+    assert b.plan.get_error() == 0
+    b.check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _attend(b)
+    graph.replay()
+    torch.cuda.synchronize()
+    b.check(out=out)
+    assert b.plan.get_error() == 0
+    c.advance(1, 0)  # 48 positions: the next one needs a page
+    graph.replay()
+    assert b.plan.get_error() == 2
+    assert b.plan.get_error() == 0
+    b.lens[0] = 48
+    b.check()  # takes the page
+    graph.replay()
+    torch.cuda.synchronize()
+    b.check(out=out)
+    assert b.plan.get_error() == 0
+    c.advance(3, 0)
+    graph.replay()
+    assert b.plan.get_error() == 2
+
+
+def test_error_word_of_a_closed_plan(ctx):
+    b = Batch(ctx, 1, 2, 64, 16, [40], [[3, 0]], seed=22)
+    b.plan.close()
+    with pytest.raises(sb.SynapseError) as e:
+        b.plan.get_error()
+    assert e.value.status == 1
