@@ -362,9 +362,13 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
  * reorders may exchange with sequences that do not hold it. The workspaces and
  * the schedule belong to the plan: its calls run in stream order, one at a
  * time; two streams or graphs that overlap need a plan each. _set is not for
- * captured streams; a captured attention call may be replayed after a later
- * _set of the same number of rows in groups that share (or not) as before (which
- * then keeps the captured call's choice of kernels, whatever the lengths).
+ * captured streams; a captured attention call may be replayed after any later
+ * _set of the same number of rows, whatever its groups and lengths. (Where a call
+ * of so many rows was captured while no group of more than 8 query rows per KV head
+ * shared anything, or too little to gain by it, such groups are computed row by row in
+ * all later sets of as many rows: capture under the sharing that a graph is for.)
+ * Replayed after a _set of another number of rows it computes nothing: its output
+ * is NaN, and the plan's error word is SYN_ERR_INVALID_ARG.
  * head_dim <= 128; at most 512 rows in a plan. Destroy the plan before its cache. */
 typedef struct syn_cuda_decode_plan_s syn_cuda_decode_plan_t;
 syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t *cache, size_t n_heads,

@@ -306,8 +306,7 @@ syn_status_t launch_append_batch(const AttnArgs& a, float* q_out, size_t ldq, si
 syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
                                const int32_t* parents, size_t beams, const size_t* lens,
                                cudaStream_t st);
-// What the launches of a plan's attention depend on beside its rows: k_prefix's CTAs, 0 when each
-// row reads all of its positions, -1 when groups share some without k_prefix.
+// What the launches of a plan's attention depend on beside its rows: k_prefix's CTAs, 0 without it.
 int decode_plan_layout(const syn_cuda_decode_plan_t* p);
 // A reorder of the group seqs[0 .. n): plans in which some but not all of them hold a group's shared
 // pages describe their rows no longer. _changed: the same for one sequence whose pages are its own now.

@@ -18,7 +18,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <array>
 #include <map>
 #include <new>
 #include <vector>
@@ -59,10 +58,14 @@ struct syn_cuda_decode_plan_s {
   void* shares = nullptr;    // k_span's shares and jobs (Share, SpanJob), written by k_begin
   int units = 0, span_jobs = 0, jobs = 0;  // k_span's units and jobs; k_prefix's jobs
   int prefix_ctas = 0, span_sms = 0;       // of their launches
-  // The layout (CTAs of k_prefix; 0: none) that captured calls of a shape were made with: later
-  // sets of the shape keep to it, since a replay launches the same kernels and grids.
-  std::array<int, 4> shape{};  // rows, units, k_span's jobs and whether k_prefix has any, if all share
-  std::map<std::array<int, 4>, int> captured;
+  // How the captured calls of so many rows were laid out. A replay launches the same kernels and grids
+  // and reads the rest from the plan, so later sets of as many rows give k_prefix nothing to do where
+  // a graph has been made without it.
+  struct Captured {
+    bool without = false;  // k_prefix
+    int ctas = 0;          // of k_prefix, the last capture's
+  };
+  std::map<size_t, Captured> captured;
 };
 
 namespace syn {
@@ -115,14 +118,20 @@ struct SpanJob {
   int prefix, w0, nw, pad;
 };
 
-// Offsets (ints) of the arrays in the plan's metadata block.
+// What a plan's set has laid out, at the front of its metadata: rows, k_span's units (the last
+// `rows` are theirs) and jobs, and the CTAs that k_prefix's items are divided among. A replayed graph
+// goes by these, not by the set that it was captured under; only the number of rows has to be the same.
+struct Head {
+  int rows, units, span_jobs, ctas;
+};
+// Offsets (ints) of the arrays in the plan's metadata block, behind the Head.
 struct Meta {
   int rows, max_jobs, max_items, ctas;
-  __host__ __device__ int seq() const { return 0; }
-  __host__ __device__ int pre() const { return rows; }           // shared positions of each row
-  __host__ __device__ int job_of() const { return 2 * rows; }    // first job of the row's group, -1
-  __host__ __device__ int local() const { return 3 * rows; }     // row - first row of its group
-  __host__ __device__ int start() const { return 4 * rows; }     // [ctas + 1] items of each CTA
+  __host__ __device__ int seq() const { return 4; }
+  __host__ __device__ int pre() const { return seq() + rows; }       // shared positions of each row
+  __host__ __device__ int job_of() const { return seq() + 2 * rows; }  // first job of the row's group, -1
+  __host__ __device__ int local() const { return seq() + 3 * rows; }   // row - first row of its group
+  __host__ __device__ int start() const { return seq() + 4 * rows; }   // [ctas + 1] items of each CTA
   __host__ __device__ int items() const { return (start() + ctas + 1 + 3) / 4 * 4; }
   __host__ __device__ int jobs() const { return items() + 12 * max_items; }
   __host__ __device__ int unit_of() const { return jobs() + 8 * max_jobs; }  // k_span's prefix unit of the row, -1
@@ -144,9 +153,9 @@ struct SharedArgs {
   Meta mv;
   float* po;
   float2* pml;
-  int rows, units, span0;  // rows; k_span's units (the last `rows` are theirs) and its first record
-  int warps, span_jobs;    // of k_span
-  int after_prefix;        // k_prefix runs before it
+  int rows, span0;   // rows; k_span's first record
+  int warps;         // of k_span
+  int after_prefix;  // k_prefix runs before it
   struct Share* shares;
   struct SpanJob* sjobs;
   float* out;
@@ -206,6 +215,11 @@ struct PxSmem {
   static constexpr int O = 2 * STAGE;         // O on its way out: [8 warps][32 rows][HDP / 2]
   static constexpr int BYTES = O + PM * HDP * 4 + 1024;
 };
+
+__device__ __forceinline__ Head head_of(const SharedArgs& a) {
+  const int4 h = __ldg(reinterpret_cast<const int4*>(a.meta));
+  return Head{h.x, h.y, h.z, h.w};
+}
 
 // Item it, less the tiles that no row sees. Whole warps.
 __device__ __forceinline__ Item px_item(const SharedArgs& a, int it) {
@@ -366,8 +380,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   // The plan, the lengths, the page table and the shared pages are from before k_begin, which
   // let this kernel begin when they were in place: only the queries have to be waited for (and
   // k_span, which reads what k_begin wrote and does not wait itself, begins after that).
-  const int* start = a.meta + a.mv.start() + blockIdx.x;
-  const int i0 = start[0], i1 = start[1];
+  const Head head = head_of(a);
+  const int* start = a.meta + a.mv.start();
+  int c0 = blockIdx.x, c1 = c0 + 1;
+  if (head.ctas != (int)gridDim.x) {  // a set made for other grids: its CTAs' items, a few of them each
+    c0 = c0 * head.ctas / (int)gridDim.x;
+    c1 = c1 * head.ctas / (int)gridDim.x;
+  }
+  const int i0 = start[c0], i1 = head.rows == a.rows ? start[c1] : i0;
   int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
   int ord = 0;  // items with tiles so far
 
@@ -788,8 +808,9 @@ __device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int 
   __shared__ int starts[UNITS_MAX + 1], lows[UNITS_MAX], highs[UNITS_MAX], sums[AP_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
-  const int per = (a.units + AP_THREADS - 1) / AP_THREADS;
-  const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
+  const Head head = head_of(a);
+  const int nu = head.units, per = (nu + AP_THREADS - 1) / AP_THREADS;
+  const int u0 = min(nu, tid * per), u1 = min(nu, u0 + per);
   int sum = 0;
   for (int u = u0; u < u1; u++) {
     const Unit x = units[u];
@@ -815,12 +836,12 @@ __device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int 
     starts[u] = base;
     base += t;
   }
-  if (u1 == a.units) starts[a.units] = base;
+  if (u1 == nu) starts[nu] = base;
   __syncthreads();
-  const int total = starts[a.units], warps = min(a.warps, total);
+  const int total = starts[nu], warps = min(a.warps, total);
   // the last unit whose first tile (or job) is at or before x; an empty one starts where the next does
   auto find = [&](int x, auto&& at) {
-    int lo = 0, hi = a.units;
+    int lo = 0, hi = nu;
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (at(mid) <= x) lo = mid;
@@ -839,7 +860,7 @@ __device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int 
     }
     a.shares[w] = s;
   }
-  for (int j = block * AP_THREADS + tid; j < a.span_jobs; j += blocks * AP_THREADS) {
+  for (int j = block * AP_THREADS + tid; j < head.span_jobs; j += blocks * AP_THREADS) {
     const int u = find(j, [&](int i) { return units[i].job0; });
     const Unit x = units[u];
     const int jl = j - x.job0, kvh = jl / x.nch, v0 = (jl - kvh * x.nch) * SP_V;
@@ -931,7 +952,10 @@ template <int VEC, int LP, bool ONE, bool PARTS>
 __global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ AppendArgs p,
                                                       const __grid_constant__ SharedArgs a, int deal) {
   const int block = (int)blockIdx.x - ((int)gridDim.x - deal);
-  if (block < 0) {
+  if (head_of(a).rows != a.rows) {  // a replay after a set of another number of rows
+    griddep_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
+  } else if (block < 0) {
     if constexpr (PARTS) append_rows<VEC, LP, ONE, 1>(p, QParts(a));
     else append_rows<VEC, LP, ONE, 1>(p);
   } else {
@@ -1175,7 +1199,7 @@ __global__ void __launch_bounds__(SP_THREADS, 1) k_span(const SharedArgs a) {
   griddep_launch();
   const int gw = warp * gridDim.x + blockIdx.x;  // (neighbouring shares on different SMs)
   const int4 sh = __ldcg(reinterpret_cast<const int4*>(a.shares) + gw);
-  int j = sh.x, k0 = sh.y, left = sh.z;
+  int j = sh.x, k0 = sh.y, left = head_of(a).rows == a.rows ? sh.z : 0;
   bool ok = true;
   while (left > 0 && ok) {
     union {
@@ -1219,6 +1243,12 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
   const int b = blockIdx.x / a.n_heads, head = blockIdx.x - b * a.n_heads;
   const int kvh = head / a.G, g = head - kvh * a.G;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
+  const Head plan = head_of(a);
+  if (plan.rows != a.rows) {  // (as in k_begin: nothing was computed)
+    griddep_wait();
+    if (threadIdx.x < hd) a.out[(long long)b * a.ldo + (long long)head * hd + threadIdx.x] = NAN;
+    return;
+  }
   // Records first + c * step, c < n. (The plan and k_begin's jobs may be read before the
   // wait: k_span begins, and lets this kernel begin, after them.)
   struct Parts { size_t first; int n, step; };
@@ -1230,7 +1260,7 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
   };
   const int pu = a.meta[a.mv.unit_of() + b], job0 = a.meta[a.mv.job_of() + b];
   const int local = a.meta[a.mv.local() + b] * a.G + g;
-  const Parts own = span_parts(a.units - a.rows + b, g);
+  const Parts own = span_parts(plan.units - a.rows + b, g);
   Parts pre{0, 0, 0};
   if (pu >= 0) {
     pre = span_parts(pu, local);
@@ -1346,7 +1376,7 @@ void plans_orphaned(syn_cuda_kvcache_t* c) {
 }
 
 int decode_plan_layout(const syn_cuda_decode_plan_t* p) {
-  return p->jobs ? p->prefix_ctas : p->units == (int)p->rows ? 0 : -1;
+  return p->jobs ? p->prefix_ctas : 0;
 }
 
 syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, int* err,
@@ -1376,10 +1406,8 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.po = p->po;
   a.pml = p->pml;
   a.rows = (int)p->rows;
-  a.units = p->units;
   a.warps = span_ctas(c->hd) * p->span_sms * SP_WARPS;
   a.span0 = (int)(p->part_rows - (span_ctas(c->hd) * p->sms * SP_WARPS + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
-  a.span_jobs = p->span_jobs;
   a.after_prefix = p->jobs > 0;
   a.shares = static_cast<Share*>(p->shares);
   a.sjobs = reinterpret_cast<SpanJob*>(a.shares + a.warps);
@@ -1394,7 +1422,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
     const AppendShape sh = append_shape(ap);
     void (*kern)(const AppendArgs, const SharedArgs, int) = p->jobs ? begin_kernel<true>(sh) : begin_kernel<false>(sh);
     const size_t per = AP_THREADS / sh.lp, blocks = (p->rows * (p->n_heads + 2 * c->n_kv) + per - 1) / per;
-    const int deal = (std::max(a.warps, a.span_jobs) + AP_THREADS - 1) / AP_THREADS;
+    const int deal = (std::max(a.warps, p->span_jobs) + AP_THREADS - 1) / AP_THREADS;
     s = launched(launch_pdl(kern, dim3((unsigned)(blocks + deal)), dim3(AP_THREADS), 0, st, ap, a, deal), "k_begin");
     if (s) return s;
   }
@@ -1457,6 +1485,7 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   if (e == cudaSuccess) e = cudaMalloc(&p->qup, c->batch * n_heads * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->meta, p->meta_ints * sizeof(int));
   if (e == cudaSuccess) e = cudaMallocHost(&p->meta_h, p->meta_ints * sizeof(int));
+  if (e == cudaSuccess) std::fill(p->meta_h, p->meta_h + p->meta_ints, 0);  // (all of it is copied)
   if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->pml, p->part_rows * sizeof(float2));
   if (e == cudaSuccess)
@@ -1580,14 +1609,18 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   int nj = 0, nu = 0, uj = 0, widest = 0;
   size_t tiles = 0, own = 0, longest = 0;  // k_prefix's; k_span's, of a row and in all, with 128 positions more
   auto tiles_of = [&](int j) { return ((size_t)jobs[j].len + PT - 1) / PT; };
-  auto lay_out = [&](bool share) {
+  // few, many: whether groups of few query rows share their prefix (in k_span), and those of many
+  // (in k_prefix)
+  auto lay_out = [&](bool share_few, bool share_many) {
     int q0 = 0;
     nj = nu = uj = widest = 0;
     tiles = own = longest = 0;
     r0 = 0;
     for (size_t i = 0; i < n_groups; r0 += group_rows[i++]) {
-      const size_t n = group_rows[i], shared = share ? p->prefix[r0] : 0;
-      const bool few = shared && n * G <= SP_FEW;
+      const size_t n = group_rows[i];
+      const bool small = n * G <= SP_FEW;
+      const size_t shared = (small ? share_few : share_many) ? p->prefix[r0] : 0;
+      const bool few = shared && small;
       for (size_t j = r0; j < r0 + n; j++) {
         h[mv.seq() + j] = seqs[j];
         h[mv.pre() + j] = (int)shared;
@@ -1639,12 +1672,16 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   // SYN_PLAN_LAYOUT=1, 2 or 3 keeps to: every row for itself, k_span behind k_prefix, beside it.
   const char* env = getenv("SYN_PLAN_LAYOUT");
   const int only = env ? atoi(env) : 0;
-  lay_out(true);
+  const auto kept = p->captured.find(rows);
+  const bool many = kept == p->captured.end() || !kept->second.without;
+  const int ctas_kept = kept == p->captured.end() ? 0 : kept->second.ctas;
+  lay_out(true, many);
   p->prefix_ctas = p->span_sms = p->sms;
-  p->shape = {(int)rows, nu, uj, nj > 0};
-  const auto kept = p->captured.find(p->shape);
   double best = span_us(p->sms) + (nj ? prefix_us(p->sms) : 0);
-  if (kept == p->captured.end() && nj && only != 2) {
+  if (nj && ctas_kept) {
+    p->prefix_ctas = ctas_kept;
+    if (ctas_kept < p->sms) p->span_sms = p->sms - ctas_kept;
+  } else if (nj && only != 2) {
     // k_span behind k_prefix, each on all SMs, or side by side, each on its own: 8 rows behind 2048
     // positions take 19.1 us behind and 15.6 side by side, 64 rows behind 32768 are 7 % slower so
     double least = only == 3 ? 1e30 : 0.85 * best;
@@ -1659,15 +1696,12 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   }
   // A short prefix is read by each row for itself: 56 rows behind 42 positions take 11.2 us so, and
   // 20.3 with k_prefix.
-  lay_out(false);
-  if (kept != p->captured.end() ? !kept->second : only ? only == 1 : span_us(p->sms) < 0.85 * best)
+  const bool has_jobs = nj > 0;
+  lay_out(false, false);
+  if (has_jobs && ctas_kept ? false : only ? only == 1 : span_us(p->sms) < 0.85 * best)
     p->prefix_ctas = p->span_sms = p->sms;
   else
-    lay_out(true);
-  if (kept != p->captured.end() && kept->second > 0 && kept->second < p->sms) {
-    p->prefix_ctas = kept->second;
-    p->span_sms = p->sms - kept->second;
-  }
+    lay_out(true, many);
   size_t ni = 0, part = 0, done = 0, jt = 0;
   auto item_of = [&](const Job& job, size_t t0, size_t t1) {
     return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,
@@ -1711,6 +1745,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     }
   }
   h[mv.start() + ctas] = (int)ni;
+  *reinterpret_cast<Head*>(h) = Head{(int)rows, nu, uj, ctas};
   p->units = nu;
   p->span_jobs = uj;
   p->jobs = nj;
@@ -1767,7 +1802,11 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
     if ((s = kv_reserve(c, p->seqs[i], c->len[p->seqs[i]] + 1, st))) return s;
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
-  if (cs != cudaStreamCaptureStatusNone) p->captured[p->shape] = decode_plan_layout(p);
+  if (cs != cudaStreamCaptureStatusNone) {
+    auto& k = p->captured[p->rows];
+    if (p->jobs) k.ctas = p->prefix_ctas;
+    else k.without = true;
+  }
   AttnArgs a{const_cast<float*>(q), k, v, ld, p->n_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
              window, c, layer, out, ldo};
   return launch_attn_shared(p, a, p->err, st);

@@ -166,3 +166,76 @@ def test_error_word_of_a_closed_plan(ctx):
     with pytest.raises(sb.SynapseError) as e:
         b.plan.get_error()
     assert e.value.status == 1
+
+
+SETS = [[[0, 1, 2, 3], [4, 5, 6, 7]], [[0, 1], [2, 3, 4, 5, 6, 7]], [[0, 1, 2, 3, 4, 5, 6, 7]],
+        [[0], [1], [2], [3], [4], [5], [6], [7]], [[0, 1], [2, 3], [4, 5], [6, 7]],
+        [[0], [1, 2, 3, 4, 5, 6], [7]]]
+
+
+def _capture(b, groups):
+    b.plan = sb.DecodePlan(b.cache, b.heads)
+    b.plan.set(groups)
+    _attend(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _attend(b)
+    return graph, out
+
+
+@pytest.mark.parametrize("heads,prefix", [(1, 200), (4, 500), (4, 30), (16, 500)])
+@pytest.mark.parametrize("first", range(len(SETS)))
+def test_replay_after_any_set_of_as_many_rows(ctx, heads, prefix, first):
+    """Groups of other sizes, other numbers of groups, groups of few query rows and of many, and
+    rows for themselves, in the graph of one set: what the launches do is read from the plan."""
+    b = Batch(ctx, 1, heads, 64, 16, [prefix], [[5, 0, 40, 3, 17, 16, 1, 33]], seed=heads)
+    graph, out = _capture(b, SETS[first])
+    for later in SETS + [SETS[first]]:
+        b.plan.set(later)
+        b.qkv.copy_(_rand(b.qkv.shape, len(later) + first))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check(out=out)
+        b.check()  # an eager call of the same set
+    assert b.plan.get_error() == 0
+
+
+def test_two_graphs_of_one_plan(ctx):
+    """Captured under different sets: each replays under the other's, and under a third."""
+    b = Batch(ctx, 1, 4, 64, 16, [2000], [[5, 0, 40, 3, 17, 16, 1, 33]], seed=2)
+    b.plan.set(SETS[0])
+    _attend(b)
+    graphs = []
+    for groups in (SETS[2], SETS[0], SETS[1]):
+        b.plan.set(groups)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, _attend(b)))
+        graphs[-1] = (graph, graphs[-1][1])
+    for groups in SETS:
+        b.plan.set(groups)
+        for graph, out in graphs:
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            b.check(out=out)
+
+
+def test_replay_after_a_set_of_another_number_of_rows(ctx):
+    """No rows are computed, none appended; the output says so, and the plan's error word."""
+    b = Batch(ctx, 1, 8, 64, 16, [200], [[5, 0, 40, 3]], seed=4)
+    graph, out = _capture(b, [[0, 1, 2, 3]])
+    for groups in ([[0, 1, 2]], [[3]], []):
+        b.plan.set(groups)
+        before = [t.clone() for t in b.cache.pages()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out.isnan().all()
+        assert b.plan.get_error() == 2
+        assert all(torch.equal(x, y) for x, y in zip(before, b.cache.pages()))
+    b.plan.set([[0, 1, 2, 3]])
+    graph.replay()
+    torch.cuda.synchronize()
+    b.check(out=out)
+    assert b.plan.get_error() == 0
