@@ -58,15 +58,32 @@ struct ReorderArgs {
   int* ptab;
   int* done;  // finished blocks; zero between launches
   int maxp, page, row4;  // row4: float4s of one position
+  int max_seq;
   const int32_t* parents;
+  const int* len;  // the sequences' lengths on the device, where a replay finds the current ones
   int n, beams;
   int seq[RO_MAX];
-  int len[RO_MAX / 2];  // per group (beams >= 2)
 };
 
 __device__ __forceinline__ int ro_parent(const int32_t* par, int i, int beams) {
   const int p = par[i];
   return p >= 0 && p < beams ? p : i;  // out of range: the member keeps its own
+}
+
+// The parents of the group from member g0 on, and its length. A group whose lengths differ (a replay
+// finds them so; a call refuses them) stays as it is. Whole block.
+__device__ __forceinline__ int ro_group(const ReorderArgs& a, int g0, int* par) {
+  const int len = min(a.len[a.seq[g0]], a.max_seq);
+  int p = 0;
+  bool same = true;
+  if (threadIdx.x < a.beams) {
+    p = ro_parent(a.parents + g0, threadIdx.x, a.beams);
+    same = a.len[a.seq[g0 + threadIdx.x]] == len;
+  }
+  same = __syncthreads_and(same);
+  if (threadIdx.x < a.beams) par[threadIdx.x] = same ? p : threadIdx.x;
+  __syncthreads();
+  return len;
 }
 
 // Where member i's last page comes from: {member whose page it takes, 1 if
@@ -113,11 +130,9 @@ __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ Reorder
   griddep_launch();
   if (blockIdx.z < gridDim.z - 1) {
     const int i = blockIdx.y, g0 = i / a.beams * a.beams;
-    for (int j = tid; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
-    __syncthreads();
+    const int len = ro_group(a, g0, par), tail = len % a.page;
     if (tid == 0) t = ro_tail(par, i - g0, a.beams);
     __syncthreads();
-    const int len = a.len[i / a.beams], tail = len % a.page;
     if (t.y && tail) {
       const int col = len / a.page;
       const int src = a.ptab[(size_t)a.seq[g0 + par[i - g0]] * a.maxp + col];
@@ -135,8 +150,7 @@ __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ Reorder
       }
     }
   } else if (blockIdx.y < a.n / a.beams) {
-    const int g0 = blockIdx.y * a.beams, full = a.len[blockIdx.y] / a.page;
-    for (int j = tid; j < a.beams; j += 256) par[j] = ro_parent(a.parents + g0, j, a.beams);
+    const int g0 = blockIdx.y * a.beams, full = ro_group(a, g0, par) / a.page;
     for (int c0 = blockIdx.x * 8; c0 < full; c0 += gridDim.x * 8) {
       for (int u = tid; u < a.beams * 8; u += 256) {
         const int b = u >> 3, c = c0 + (u & 7);
@@ -154,12 +168,21 @@ __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ Reorder
   if (tid == 0) last = atomicAdd(a.done, 1) == (int)(gridDim.x * gridDim.y * gridDim.z) - 1;
   __syncthreads();
   if (!last) return;
-  if (tid < a.n) par[tid] = ro_parent(a.parents + tid / a.beams * a.beams, tid % a.beams, a.beams);
-  __syncthreads();
-  int entry = -1;
+  __shared__ int lens[RO_MAX];
   const int g0 = tid / a.beams * a.beams;
-  const size_t col = tid < a.n ? a.len[tid / a.beams] / a.page : 0;
-  const bool mine = tid < a.n && a.len[tid / a.beams] % a.page;
+  if (tid < a.n) {
+    par[tid] = ro_parent(a.parents + g0, tid - g0, a.beams);
+    lens[tid] = a.len[a.seq[tid]];
+  }
+  __syncthreads();
+  int entry = -1, len = 0;
+  if (tid < a.n) {
+    len = min(lens[g0], a.max_seq);
+    for (int j = g0; j < g0 + a.beams; j++)
+      if (lens[j] != len) len = 0;  // (as ro_group)
+  }
+  const size_t col = len / a.page;
+  const bool mine = len % a.page;
   if (mine) entry = a.ptab[(size_t)a.seq[g0 + ro_tail(par + g0, tid - g0, a.beams).x] * a.maxp + col];
   __syncthreads();
   if (mine) a.ptab[(size_t)a.seq[tid] * a.maxp + col] = entry;
@@ -707,21 +730,40 @@ syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, 
   return SYN_OK;
 }
 
+syn_status_t no_free_page() {
+  set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
+  return SYN_ERR_OUT_OF_MEMORY;
+}
+
 syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
   if (!c->page || c->stale[seq] == 1) return SYN_OK;  // (a reorder leaves private last pages)
   if (c->stale[seq] && !capturing(st)) {
     syn_status_t s = kv_sync(c, st);
     if (s) return s;
   }
+  return kv_copy_shared(c, seq, st);
+}
+
+syn_status_t kv_cut(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st) {
+  if (!c->page || c->stale[seq] != 2 || new_len % c->page == 0) return SYN_OK;
+  syn_status_t s = kv_sync(c, st);
+  if (s) return s;
+  const int* row = c->ptab_h + seq * c->maxp;
+  const size_t col = new_len / c->page;
+  if (row[col] < 0 || c->refs[row[col]] <= 1) return SYN_OK;
+  size_t free = c->n_free;
+  for (size_t i = col + 1; i < c->maxp; i++) free += row[i] >= 0 && c->refs[row[i]] == 1;
+  return free ? SYN_OK : no_free_page();
+}
+
+syn_status_t kv_copy_shared(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
+  if (!c->page) return SYN_OK;
   const size_t col = c->len[seq] / c->page;
   if (col >= c->maxp) return SYN_OK;
   int* e = c->ptab_h + seq * c->maxp + col;
   if (*e < 0 || c->refs[*e] <= 1) return SYN_OK;
   if (capturing(st)) return SYN_ERR_UNSUPPORTED;  // a replay would copy again
-  if (!c->n_free) {
-    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
-    return SYN_ERR_OUT_OF_MEMORY;
-  }
+  if (!c->n_free) return no_free_page();
   const int old = *e, own = c->free_pages[c->n_free - 1];
   syn_status_t s = kv_copy_page(c, old, own, c->len[seq] % c->page, st);
   if (s) return s;
@@ -772,17 +814,19 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
   a.done = c->d_ptab + c->batch * c->maxp;
   a.maxp = (int)c->maxp;
   a.page = (int)c->page;
+  a.max_seq = (int)c->max_seq;
   a.parents = parents;
+  a.len = c->d_len;
   a.n = (int)n;
   a.beams = (int)beams;
   size_t cols = 0, tail = 0;
   for (size_t i = 0; i < n; i++) a.seq[i] = seqs[i];
   for (size_t g = 0; g < n / beams; g++) {
-    a.len[g] = (int)lens[g];
     cols = std::max(cols, (lens[g] + c->page - 1) / c->page);
     tail = std::max(tail, lens[g] % c->page);
   }
-  if (!cols) return SYN_OK;
+  if (capturing(st)) tail = c->page - 1;  // (a replay's may be any)
+  else if (!cols) return SYN_OK;
   if (c->layers > 65534) return SYN_ERR_UNSUPPORTED;
   // about four 16-byte copies a thread, K and V: 28 layers x 20 beams x 28 rows of 4 KB (257 MB
   // read and written) take 39 us; one copy a thread takes 64
@@ -909,10 +953,7 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t* c, size_t src, size_t dst
   int *from = c->ptab_h + src * c->maxp, *to = c->ptab_h + dst * c->maxp;
   if (to[0] >= 0 && (s = kv_release(c, dst, 0, st))) return s;  // pages taken for a call, never committed
   const size_t full = len / c->page, tail = len % c->page;
-  if (tail && !c->n_free) {
-    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
-    return SYN_ERR_OUT_OF_MEMORY;
-  }
+  if (tail && !c->n_free) return no_free_page();
   for (size_t i = 0; i < full; i++) {
     to[i] = from[i];
     c->refs[to[i]]++;

@@ -241,6 +241,12 @@ syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaS
 // The page that the next position of seq goes into, if other sequences hold it
 // too, is replaced by a copy (SYN_ERR_UNSUPPORTED while `st` is captured).
 syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
+// The same where the host's table of seq is known to be current.
+syn_status_t kv_copy_shared(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
+// Whether seq can be cut back to new_len: one that a captured reorder may move gets its own copy of a
+// shared last page at once, for which there must be a page (the cut's own among them).
+syn_status_t kv_cut(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st);
+syn_status_t no_free_page();
 // Copies rows [0, rows) of page src to page dst, K and V of all layers.
 syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, cudaStream_t st);
 // Reads the table rows that were permuted on the device back to the host and
@@ -301,8 +307,8 @@ syn_status_t launch_kv_set(syn_cuda_kvcache_t* c, size_t seq, int value, int add
 // reserved) normalised, rotated and appended; q rows to q_out.
 syn_status_t launch_append_batch(const AttnArgs& a, float* q_out, size_t ldq, size_t n,
                                  const int32_t* seqs, const size_t* counts, cudaStream_t st);
-// Groups of `beams` sequences (seqs and lens on the host, parents on the
-// device) take over their parents' contexts; at most 256 sequences.
+// Groups of `beams` sequences (seqs and, for the size of the launch, lens on the
+// host, parents on the device) take over their parents' contexts; at most 256 sequences.
 syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
                                const int32_t* parents, size_t beams, const size_t* lens,
                                cudaStream_t st);

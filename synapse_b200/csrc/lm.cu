@@ -2129,10 +2129,7 @@ syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaS
   const size_t need = (new_len + c->page - 1) / c->page;
   size_t first = need, missing = 0;
   for (size_t i = 0; i < need; i++) missing += row[i] < 0;
-  if (missing > c->n_free) {
-    set_last_cuda_error(cudaErrorMemoryAllocation, "paged KV cache: no free page");
-    return SYN_ERR_OUT_OF_MEMORY;
-  }
+  if (missing > c->n_free) return no_free_page();
   for (size_t i = 0; i < need; i++) {
     if (row[i] >= 0) continue;
     row[i] = c->free_pages[--c->n_free];
@@ -2165,7 +2162,8 @@ syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cuda
   if (changed)
     SYN_CUDA_TRY(cudaMemcpy(c->d_ptab + seq * c->maxp, row, c->maxp * sizeof(int),
                             cudaMemcpyHostToDevice));
-  return SYN_OK;
+  // a graph may move the last page and write to it before any call for the sequence does
+  return c->stale[seq] == 2 && keep_len % c->page ? kv_copy_shared(c, seq, st) : SYN_OK;
 }
 
 __global__ void k_kv_advance_slots(int* len, const int* slots, int n) {
@@ -2407,7 +2405,9 @@ syn_status_t syn_cuda_kvcache_truncate(syn_cuda_kvcache_t* c, size_t seq, size_t
   if (seq >= c->batch) return SYN_ERR_INVALID_ARG;
   if (new_len >= c->len[seq]) return SYN_OK;  // kvcache.zig:109-113
   DeviceGuard g(c->device);
-  syn_status_t s = launch_kv_set(c, seq, (int)new_len, 0, (cudaStream_t)stream);
+  syn_status_t s = kv_cut(c, seq, new_len, (cudaStream_t)stream);
+  if (s) return s;
+  s = launch_kv_set(c, seq, (int)new_len, 0, (cudaStream_t)stream);
   if (s == SYN_OK) c->len[seq] = new_len;
   if (s == SYN_OK) s = kv_release(c, seq, new_len, (cudaStream_t)stream);
   return s;

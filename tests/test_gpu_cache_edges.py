@@ -1,0 +1,116 @@
+"""The paged cache under captured calls, few pages and long searches; the selection's largest
+sizes."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_beam_ops import _Mirror, _check_select, _rand, _rope  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+sb = pytest.importorskip("synapse_b200")
+
+
+def _ints(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("page,prompt", [(4, 0), (4, 7), (5, 5), (1, 2)])
+def test_captured_reorder_follows_the_lengths(ctx, page, prompt):
+    """One graph for every step: the reorder's positions are those of the replay."""
+    n = 4
+    cache = sb.KVCache(ctx, 40, 1, 8, 2, n, page, n * 40)
+    m, rng = _Mirror(cache), np.random.default_rng(page)
+    if prompt:
+        m.grow(0, prompt)
+        for s in range(1, n):
+            cache.fork(0, s)
+            m.ctxs[s] = list(m.ctxs[0])
+    par = _ints(0, 1, 2, 3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reorder(range(n), par, n)
+    for step in range(12):
+        for s in range(n):
+            m.grow(s, 1 + step % 2)
+        p = rng.integers(0, n, n)
+        par.copy_(torch.tensor(p, dtype=torch.int32))
+        graph.replay()
+        old = [list(c) for c in m.ctxs]
+        m.ctxs = [list(old[j]) for j in p]
+        m.check()
+    for s in range(n):
+        cache.reset(s)
+    assert cache.pages_free() == cache.n_pages
+
+
+def test_captured_reorder_of_unequal_lengths(ctx):
+    """A group whose lengths have parted by the replay stays as it is; the other one moves."""
+    cache = sb.KVCache(ctx, 40, 1, 8, 1, 4, 4, 60)
+    m = _Mirror(cache)
+    for s in range(4):
+        m.grow(s, 6)
+    par = _ints(1, 0, 1, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reorder(range(4), par, 2)
+    m.grow(1, 3)
+    graph.replay()
+    m.ctxs[2], m.ctxs[3] = m.ctxs[3], m.ctxs[2]
+    m.check()
+
+
+def test_cut_back_into_a_shared_page_before_a_replay(ctx):
+    """A sequence that a graph may permute and that is cut back into a page which others hold
+    gets its own copy at once: the replay writes there."""
+    cache = sb.KVCache(ctx, 40, 1, 8, 2, 5, 4, 30)
+    m = _Mirror(cache)
+    for s in range(2):
+        m.grow(s, 10)
+    cache.fork(0, 4)  # holds sequence 0's full pages
+    m.ctxs[4] = list(m.ctxs[0])
+    par = _ints(0, 1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reorder([0, 1], par, 2)
+    for s in range(2):
+        cache.truncate(6, s)
+        del m.ctxs[s][6:]
+    par.copy_(_ints(1, 1))
+    graph.replay()
+    m.ctxs[0] = list(m.ctxs[1])
+    m.check()  # (sequence 4 among them)
+    for s in (0, 1, 4):
+        m.grow(s, 5)
+    m.check()
+    for s in (0, 1, 4):
+        cache.reset(s)
+    assert cache.pages_free() == 30
+
+
+def test_cut_back_without_a_page_for_the_copy(ctx):
+    """Refused, and the sequence is as it was."""
+    cache = sb.KVCache(ctx, 40, 1, 8, 1, 4, 4, 8)
+    m = _Mirror(cache)
+    m.grow(0, 8)
+    cache.fork(0, 1)
+    m.ctxs[1] = list(m.ctxs[0])
+    par = _ints(0, 1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reorder([0, 1], par, 2)
+    m.grow(2, 24)  # every other page
+    assert cache.pages_free() == 0
+    with pytest.raises(sb.SynapseError) as e:
+        cache.truncate(6, 0)
+    assert e.value.status == 3
+    m.check()
+    cache.truncate(20, 2)
+    del m.ctxs[2][20:]
+    cache.truncate(6, 0)
+    del m.ctxs[0][6:]
+    m.check()
