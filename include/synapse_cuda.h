@@ -392,8 +392,9 @@ syn_status_t syn_cuda_decode_plan_get_error(syn_cuda_decode_plan_t *plan, int32_
  * is sequence r of the plan; q is left as it is): headwise norms, RoPE, K and V
  * appended at each sequence's length, attention over all its positions or the
  * last `window`. Results within f32 reassociation of the reference order. The
- * lengths are not advanced. Cache positions that no row of a group sees (behind
- * its sequences, outside all windows) may hold anything. SYN_ERR_INVALID_ARG when a sequence was truncated,
+ * lengths are not advanced. Cache positions that a row does not see (behind its
+ * sequence, outside its window) may hold anything; NaN and infinities that it sees
+ * go where the formula takes them (such rows are computed once more, slowly). SYN_ERR_INVALID_ARG when a sequence was truncated,
  * reset or forked into since _set, or when a reorder since then joined some of a group's sequences with
  * one that did not hold the group's shared pages: _set describes the batch anew. */
 syn_status_t syn_cuda_attention_decode_shared(

@@ -543,21 +543,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       if (!busy && !ok) break;
       if (busy) {
         tc_fence_after();
-        float la, lb;
-        unpk(l, la, lb);
-        la += lb;
-        if (h == 1) pmax[n & 1][1][r] = la;
-        if (lane == 0) gone[warp] = !ok;
-        pair_sync(pair);
-        if (!ok || gone[warp ^ 4]) {
-          ok = false;
-          break;
-        }
-        const bool none = M == -INFINITY;
-        if (h == 0 && r < item.m)
-          a.pml[rec] = none ? make_float2(-INFINITY, 0.0f)
-                            : make_float2(M - P_TOP, la + pmax[n & 1][1][r]);
-        pair_sync(pair);  // (the slot is the next item's)
+        bool fine = true;
         // O: from rows to whole lines
         constexpr int CH = HDP / 8;  // 16-byte chunks of a row's half
         uint8_t* stage = sm + L::O + warp * (32 * CH * 16);
@@ -571,14 +557,35 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             tc_ld8(tl + C_O2 + h * (HDP / 2) + c + j, o2);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[j + e] += o2[e];
+            for (int e = 0; e < 8; e++) {
+              o[j + e] += o2[e];
+              fine &= fabsf(o[j + e]) < INFINITY;
+            }
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<float4*>(stage + (lane * CH + (((c + j) / 4) ^ (lane % CH))) * 16) =
                 make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
-        __syncwarp();
+        float la, lb;
+        unpk(l, la, lb);
+        la = fine ? la + lb : NAN;
+        if (h == 1) pmax[n & 1][1][r] = la;
+        if (lane == 0) gone[warp] = !ok;
+        pair_sync(pair);
+        if (!ok || gone[warp ^ 4]) {
+          ok = false;
+          break;
+        }
+        // Nothing seen, or a sum that says so where nothing finite was (k_join takes that row again)
+        la += pmax[n & 1][1][r];
+        if (M == -INFINITY && r < item.m) {
+          int first = 0;
+          if (a.window) first = a.len[a.meta[a.mv.seq() + item.row0 + (item.m0 + r) / a.G]] + 1 - a.window;
+          if (first < min(item.t1 * PT, item.len)) la = NAN;
+        }
+        if (h == 0 && r < item.m) a.pml[rec] = make_float2(M - P_TOP, la);
+        pair_sync(pair);  // (the slot is the next item's)
         const int c = lane % CH, col = h * (HDP / 2) + c * 4, r0 = (warp & 3) * 32;
 #pragma unroll 4
         for (int q = lane / CH; q < 32; q += 32 / CH) {
@@ -1121,11 +1128,12 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
     for (int v = 0; v < NQ; v++) {
       float x, y;
       unpk(add2(acc[v][0], acc[v][1]), x, y);
-      x = lane < nk && key >= low[v] ? x + y : -INFINITY;
+      const bool seen = lane < nk && key >= low[v];
+      x = seen ? x + y : -INFINITY;
       const float mx = fmaxf(m[v], redux_max(x));
       corr[v] = m[v] == -INFINITY ? 0.0f : ex2(m[v] - mx);
       grown |= mx != m[v];
-      const float p = mx == -INFINITY ? 0.0f : ex2(x - mx);
+      const float p = mx == -INFINITY && !seen ? 0.0f : ex2(x - mx);  // (NaN where only NaN and -inf are seen)
       l[v] = fmaf(l[v], corr[v], p);
       m[v] = mx;
       w[v] = p;
@@ -1165,7 +1173,8 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
     for (int s = LPR; s < 32; s <<= 1)
 #pragma unroll
       for (int e = 0; e < 4; e++) x[e] += __shfl_xor_sync(0xffffffffu, x[e], s);
-    const float sum = warp_sum(l[v]);
+    // (x * 0: nothing, or NaN)
+    const float sum = warp_sum(fmaf(x[0], 0.0f, fmaf(x[1], 0.0f, fmaf(x[2], 0.0f, fmaf(x[3], 0.0f, l[v])))));
     if (v < job.nq) {
       if (lane == 0) a.pml[rec + v] = make_float2(m[v], sum);
       if (sub == 0 && l4 < hd)
@@ -1237,7 +1246,61 @@ __global__ void __launch_bounds__(SP_THREADS, 1) k_span(const SharedArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int JN_WARPS = 4, JN_BLOCK = 32;  // records at a time
 
-__global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
+// A query row from its definition, over the positions that it sees: exp(s - M) without a guard, so that NaN
+// and infinities go where the formula takes them. The other kernels cannot do that (a running maximum
+// drops NaN, a tile's other rows multiply what they do not see by 0, fp16 parts of an infinity are
+// NaN): they leave a sum that is NaN, or values that are not finite, and the row comes here. Slow
+// (each key's row by one warp, twice), and never taken by finite operands whose products stay finite.
+__device__ __noinline__ float join_plain(const SharedArgs& a, int b, int head, float (*red)[128]) {
+  __shared__ double sums[JN_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd, kvh = head / a.G;
+  const int seq = a.meta[a.mv.seq() + b], L = min(a.len[seq] + 1, a.max_seq);
+  const bool act = lane * 4 < hd;
+  const float4 zero = make_float4(0, 0, 0, 0);
+  float4 q = zero;
+  if (act) q = *(reinterpret_cast<const float4*>(a.q + ((size_t)b * a.n_heads + head) * hd) + lane);
+  auto each = [&](auto&& take) {  // (score, the lane's columns of V)
+    for (int pos = (a.window ? max(0, L - a.window) : 0) + warp; pos < L; pos += JN_WARPS) {
+      long long row = (long long)seq * a.max_seq + pos;
+      if (a.ptab) {
+        const int pg = a.ptab[(size_t)seq * a.maxp + pos / a.page];
+        if (pg < 0) continue;
+        row = (long long)pg * a.page + pos % a.page;
+      }
+      const size_t at = ((size_t)row * a.n_kv + kvh) * hd + lane * 4;
+      float4 k = zero, v = zero;
+      if (act) {
+        k = *reinterpret_cast<const float4*>(a.kc + at);
+        v = *reinterpret_cast<const float4*>(a.vc + at);
+      }
+      take(warp_sum(fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)))) * a.scale, v);
+    }
+  };
+  float M = -INFINITY;
+  each([&](float s, const float4&) { M = fmaxf(M, s); });
+  if (lane == 0) red[warp][0] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  double l = 0.0, o[4] = {0.0, 0.0, 0.0, 0.0};
+  each([&](float s, const float4& v) {
+    const double p = expf(s - M);
+    l += p;
+    o[0] += p * v.x;
+    o[1] += p * v.y;
+    o[2] += p * v.z;
+    o[3] += p * v.w;
+  });
+  if (lane == 0) sums[warp] = l;
+  __syncthreads();
+  l = sums[0] + sums[1] + sums[2] + sums[3];
+  *reinterpret_cast<float4*>(&red[warp][lane * 4]) =
+      make_float4((float)(o[0] / l), (float)(o[1] / l), (float)(o[2] / l), (float)(o[3] / l));
+  __syncthreads();
+  const int d = threadIdx.x;
+  return (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+}
+
+__global__ void __launch_bounds__(JN_WARPS * 32) k_join(const __grid_constant__ SharedArgs a) {
   __shared__ __align__(16) float red[JN_WARPS][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
   const int b = blockIdx.x / a.n_heads, head = blockIdx.x - b * a.n_heads;
@@ -1312,8 +1375,10 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const SharedArgs a) {
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f * sum;  // (NaN stays)
   __syncthreads();
   const int d = threadIdx.x;
-  if (d < hd)
-    a.out[(long long)b * a.ldo + (long long)head * hd + d] = ((red[0][d] + red[1][d]) + (red[2][d] + red[3][d])) * inv;
+  float y = 0.0f;
+  if (d < hd) y = ((red[0][d] + red[1][d]) + (red[2][d] + red[3][d])) * inv;
+  if (__syncthreads_or(!(fabsf(y) < INFINITY))) y = join_plain(a, b, head, red);
+  if (d < hd) a.out[(long long)b * a.ldo + (long long)head * hd + d] = y;
 }
 
 syn_status_t launched(cudaError_t e, const char* where) {

@@ -239,3 +239,142 @@ def test_replay_after_a_set_of_another_number_of_rows(ctx):
     torch.cuda.synchronize()
     b.check(out=out)
     assert b.plan.get_error() == 0
+
+
+def _plain(b, window=0):
+    """The definition in 64 bits, each row over the positions that it sees: [rows, kv, G, hd]
+    and the weights' bound on the f32 error of finite outputs."""
+    want, tol = [], []
+    heads, kv, hd = b.heads, b.kv, b.hd
+    x = b.qkv.view(len(b.lens), -1, hd)
+    for r, ln in enumerate(b.lens):
+        k, v = (t.double().clone() for t in b.kv_of(0, r, ln + 1))
+        k[ln] = _turn(x[r, heads:heads + kv], None, b.cos[ln], b.sin[ln], 1e-6)
+        v[ln] = x[r, heads + kv:].double()
+        q = _turn(x[r, :heads], None, b.cos[ln], b.sin[ln], 1e-6).view(kv, -1, hd)
+        lo = max(0, ln + 1 - window) if window else 0
+        k, v = k[lo:], v[lo:]
+        # (element by element: a library product may take 0 * inf another way)
+        s = (q[:, :, None] * k.transpose(0, 1)[:, None]).sum(-1) / hd ** 0.5
+        p = torch.exp(s - s.amax(-1, keepdim=True))  # NaN and infinities go their way
+        p = p / p.sum(-1, keepdim=True)
+        want.append((p[..., None] * v.transpose(0, 1)[:, None]).sum(-2))
+        fin = [t.nan_to_num(0.0, 0.0, 0.0) for t in (q, k, v, p)]
+        mag = torch.einsum("hgd,lhd->hgl", fin[0].abs(), fin[1].abs()).amax(-1) / hd ** 0.5
+        es = mag * (12 + hd / 8 + 8 + 6) * U
+        rel = 2 * es + (len(k) / 64 + 64 + 8 + 12) * U
+        tol.append(rel[..., None] * torch.einsum("hgl,lhd->hgd", fin[3], fin[2].abs()) + 1e-30)
+    return torch.stack(want), torch.stack(tol)
+
+
+def _check_as_plain(b, window=0):
+    """NaN and infinities where the definition has them (tolerances of finite outputs as in
+    Batch.check), twice."""
+    want, tol = _plain(b, window)
+    for _ in range(2):
+        got = _attend(b, window=window).view(want.shape).double()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.isinf(), want.isinf())
+        assert torch.equal(got[got.isinf()], want[want.isinf()])
+        fine = want.isfinite()
+        assert ((got - want).abs()[fine] <= tol[fine]).all()
+    if b.hd in (64, 128):  # the row-by-row kernel's NaN are in the same places
+        other = sb.attention_decode(b.cache, 0, b.qkv.clone(), b.heads, None, None, 1e-6, b.cos, b.sin,
+                                    window=window, batch=len(b.lens), flash=True).view(want.shape)
+        assert torch.equal(other.isnan(), want.isnan())
+
+
+SHAPES = [(1, 2, 64, 16, [96], [[40, 20]]),          # few query rows
+          (2, 16, 128, 16, [300], [[3, 70, 0, 33]]),  # a tensor-core prefix
+          (1, 12, 96, 5, [130, 60], [[4, 4], [70, 1]])]
+
+
+def _place(b, seq, pos):
+    t = b.cache.device_table()[seq].cpu()
+    return int(t[pos // b.page]) * b.page + pos % b.page
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_queries_give_their_own_rows_nan(ctx, shape, bad):
+    b = Batch(ctx, *shape, seed=11)
+    b.qkv.view(len(b.lens), -1, b.hd)[1, b.heads - 1] = bad  # one head of one row
+    _check_as_plain(b)
+    got = _attend(b).view(len(b.lens), b.kv, -1, b.hd)
+    assert got[1, -1, -1].isnan().all() and got.isnan().sum() == b.hd
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("first,n", [(0, 1), (0, 96), (17, 3), (33, 32)])
+def test_nan_keys(ctx, shape, first, n):
+    """In the first tile, as whole tiles, in between: NaN for every row that sees them, not zero."""
+    b = Batch(ctx, *shape, seed=12)
+    k, _ = b.cache.pages(0)
+    for pos in range(first, first + n):
+        k.view(-1, b.kv, b.hd)[_place(b, 0, pos), 0] = float("nan")
+    _check_as_plain(b)
+    assert _attend(b).view(len(b.lens), b.kv, -1)[0, 0].isnan().all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_nan_in_a_rows_own_positions(ctx, shape):
+    b = Batch(ctx, *shape, seed=13)
+    r = max(range(len(b.lens)), key=lambda i: b.lens[i])
+    k, v = (t.view(-1, b.kv, b.hd) for t in b.cache.pages(0))
+    k[_place(b, r, b.lens[r] - 1), -1, 3] = float("nan")
+    _check_as_plain(b)
+    k[_place(b, r, b.lens[r] - 1), -1, 3] = 0.0
+    v[_place(b, r, b.lens[r] - 1), -1, 3] = float("nan")
+    _check_as_plain(b)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_infinite_values_stay_in_their_columns(ctx, shape):
+    """An infinity in V reaches its own column; the other columns keep that row's finite
+    elements. With both signs in one column: NaN."""
+    b = Batch(ctx, *shape, seed=14)
+    v = b.cache.pages(0)[1].view(-1, b.kv, b.hd)
+    v[_place(b, 0, 20), 0, 5] = float("inf")
+    v[_place(b, 0, 21), 0, 6] = float("-inf")
+    v[_place(b, 0, 22), 0, 7] = float("inf")
+    v[_place(b, 0, 50), 0, 7] = float("-inf")
+    _check_as_plain(b)
+    row = _attend(b).view(len(b.lens), b.kv, -1, b.hd)[0, 0, 0]
+    assert row[5] == float("inf") and row[6] == -float("inf") and row[7].isnan()
+    assert row.isfinite().sum() == b.hd - 3
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_infinite_keys(ctx, shape):
+    """A score of +inf makes its row NaN (inf - inf), one of -inf weighs nothing."""
+    b = Batch(ctx, *shape, seed=15)
+    k, _ = b.cache.pages(0)
+    k.view(-1, b.kv, b.hd)[_place(b, 0, 2), 0, 1] = float("inf")
+    _check_as_plain(b)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("window", [20, 45, 64])
+def test_what_one_row_sees_and_another_does_not(ctx, shape, window):
+    """Rows of a group end at different positions, so their windows begin at different ones: bad
+    rows of the cache reach those that see them and no others."""
+    b = Batch(ctx, *shape, seed=16)
+    lens = sorted(b.lens[i] for i in b.groups[0])
+    k, v = (t.view(-1, b.kv, b.hd) for t in b.cache.pages(0))
+    pos = max(0, lens[0] + 1 - window)  # the first that the shortest row sees
+    if pos < b.plan.prefix(b.groups[0][0]):
+        v[_place(b, b.groups[0][0], pos), 0, 2] = float("inf")
+        _check_as_plain(b, window)
+        k[_place(b, b.groups[0][0], pos), 0, 2] = float("nan")
+    _check_as_plain(b, window)
+
+
+def test_scores_that_overflow(ctx):
+    """Finite rows whose products pass the largest float: infinite scores, as in f32."""
+    b = Batch(ctx, 1, 2, 64, 16, [96], [[40, 20]], seed=17)
+    b.qkv[:, :2 * 64] = 1e25
+    k, _ = b.cache.pages(0)
+    k.view(-1, 1, 64)[_place(b, 0, 0):_place(b, 0, 0) + 16] = -1e25
+    got = _attend(b)
+    one = sb.attention_decode(b.cache, 0, b.qkv.clone(), 2, None, None, 1e-6, b.cos, b.sin, batch=2, flash=True)
+    assert torch.equal(got.isnan(), one.isnan())
