@@ -37,7 +37,9 @@ struct AppendArgs {
   const int* ptab;
   int page, maxp, max_seq;
   const int* len;
-  const int* seq_of;  // device: one row of each sequence seq_of[row] (replaces the lists below)
+  const int* seq_of;  // device: one row of each sequence seq_of[row] (replaces the lists below) ...
+  const int* set_rows;  // ... if *set_rows is `rows`; else nothing
+  int* err;  // where a position without a page is reported; may be nullptr
   int rows;
   int n;
   int seq[AP_MAX];
@@ -92,7 +94,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, Taker taker = T
     sq = a.seq_of ? a.seq_of[row] : a.seq[s];
     pos = a.len[sq] + (a.seq_of ? 0 : row - a.row0[s]);
   }
-  const bool in = live && pos < a.max_seq;  // (a replayed graph may have run past the cache)
+  // (a replayed graph may have run past the cache, or its plan may have been set for other rows)
+  const bool in = live && pos < a.max_seq && (!a.seq_of || *a.set_rows == a.rows);
   const float* ct = a.cos_t + (size_t)pos * half;
   const float* st = a.sin_t + (size_t)pos * half;
   T c1, s1;
@@ -106,6 +109,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, Taker taker = T
     if (a.ptab) {
       const int pg = a.ptab[(size_t)sq * a.maxp + pos / a.page];
       slot = pg < 0 ? -1 : (long long)pg * a.page + pos % a.page;
+      if (pg < 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
     }
   }
 #pragma unroll
@@ -230,7 +234,8 @@ inline AppendArgs append_args(const AttnArgs& at, float* q_out, size_t ldq, size
   a.maxp = (int)c->maxp;
   a.max_seq = (int)c->max_seq;
   a.len = c->d_len;
-  a.seq_of = nullptr;
+  a.seq_of = a.set_rows = nullptr;
+  a.err = nullptr;
   a.n = 0;
   return a;
 }

@@ -297,6 +297,12 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
 
 __device__ __forceinline__ void prefetch_l2(const float* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <int N>
 __device__ __forceinline__ void more_regs() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -382,12 +388,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
   // k_span, which reads what k_begin wrote and does not wait itself, begins after that).
   const Head head = head_of(a);
   const int* start = a.meta + a.mv.start();
-  int c0 = blockIdx.x, c1 = c0 + 1;
+  int i0 = start[blockIdx.x], i1 = start[blockIdx.x + 1];
   if (head.ctas != (int)gridDim.x) {  // a set made for other grids: its CTAs' items, a few of them each
-    c0 = c0 * head.ctas / (int)gridDim.x;
-    c1 = c1 * head.ctas / (int)gridDim.x;
+    i0 = start[(int)blockIdx.x * head.ctas / (int)gridDim.x];
+    i1 = start[((int)blockIdx.x + 1) * head.ctas / (int)gridDim.x];
   }
-  const int i0 = start[c0], i1 = head.rows == a.rows ? start[c1] : i0;
+  if (head.rows != a.rows) i1 = i0;
   int n = 0;    // tiles so far; tile n uses stage n & 1 for the (n >> 1)-th time
   int ord = 0;  // items with tiles so far
 
@@ -477,18 +483,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             unpk(y[j + 1], p, q);
             mx2 = fmaxf(fmaxf(mx2, p), q);
           }
-          mx = fmaxf(mx, mx2);  // (no NaN: a NaN here is a warp that gives up)
-          pmax[n & 1][h][r] = ok ? mx : NAN;
+          mx = fmaxf(mx, mx2);
+          if (!ok) mx = NAN;  // (otherwise it never is: this warp gives up)
+          pmax[n & 1][h][r] = mx;
           pair_sync(pair);
-          const float other = pmax[n & 1][h ^ 1][r];
-          if (!ok || __any_sync(0xffffffffu, other != other)) {
+          mx = max_nan(mx, pmax[n & 1][h ^ 1][r]);
+          // a new reference only when the old one is too far below (the same in both halves)
+          const bool grow = !(mx <= M + P_GROW);  // (also from -inf)
+          const float ref = grow ? mx : M;
+          if (__any_sync(0xffffffffu, mx != mx)) {
             ok = false;
             break;
           }
-          mx = fmaxf(mx, other);
-          // a new reference only when the old one is too far below (the same in both halves)
-          const bool grow = mx > M + P_GROW;  // (also from -inf)
-          const float ref = grow ? mx : M;
           if (t == item.t0) {
             M = ref;
           } else if (__any_sync(0xffffffffu, grow)) {
@@ -543,7 +549,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
       if (!busy && !ok) break;
       if (busy) {
         tc_fence_after();
-        bool fine = true;
+        float la, lb;
+        unpk(l, la, lb);
+        la += lb;
+        if (h == 1) pmax[n & 1][1][r] = la;
+        if (lane == 0) gone[warp] = !ok;
+        pair_sync(pair);
+        if (!ok || gone[warp ^ 4]) {
+          ok = false;
+          break;
+        }
+        // (M = -inf: nothing seen, or nothing that weighs; the sum is NaN where a score was)
+        if (h == 0 && r < item.m) a.pml[rec] = make_float2(M - P_TOP, la + pmax[n & 1][1][r]);
+        pair_sync(pair);  // (the slot is the next item's)
         // O: from rows to whole lines
         constexpr int CH = HDP / 8;  // 16-byte chunks of a row's half
         uint8_t* stage = sm + L::O + warp * (32 * CH * 16);
@@ -557,35 +575,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1) k_prefix(const SharedArgs a) {
             tc_ld8(tl + C_O2 + h * (HDP / 2) + c + j, o2);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-              o[j + e] += o2[e];
-              fine &= fabsf(o[j + e]) < INFINITY;
-            }
+            for (int e = 0; e < 8; e++) o[j + e] += o2[e];
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<float4*>(stage + (lane * CH + (((c + j) / 4) ^ (lane % CH))) * 16) =
                 make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
-        float la, lb;
-        unpk(l, la, lb);
-        la = fine ? la + lb : NAN;
-        if (h == 1) pmax[n & 1][1][r] = la;
-        if (lane == 0) gone[warp] = !ok;
-        pair_sync(pair);
-        if (!ok || gone[warp ^ 4]) {
-          ok = false;
-          break;
-        }
-        // Nothing seen, or a sum that says so where nothing finite was (k_join takes that row again)
-        la += pmax[n & 1][1][r];
-        if (M == -INFINITY && r < item.m) {
-          int first = 0;
-          if (a.window) first = a.len[a.meta[a.mv.seq() + item.row0 + (item.m0 + r) / a.G]] + 1 - a.window;
-          if (first < min(item.t1 * PT, item.len)) la = NAN;
-        }
-        if (h == 0 && r < item.m) a.pml[rec] = make_float2(M - P_TOP, la);
-        pair_sync(pair);  // (the slot is the next item's)
         const int c = lane % CH, col = h * (HDP / 2) + c * 4, r0 = (warp & 3) * 32;
 #pragma unroll 4
         for (int q = lane / CH; q < 32; q += 32 / CH) {
@@ -799,8 +795,7 @@ __device__ __forceinline__ int2 unit_range(const SharedArgs& a, const Unit& u) {
     return make_int2(lo, u.pre);
   }
   const int L = a.len[seq[u.row0]] + 1;
-  // a replayed graph that has run past the cache, or past the pages that were reserved
-  if (L > a.max_seq || (a.ptab && a.ptab[(size_t)seq[u.row0] * a.maxp + (L - 1) / a.page] < 0)) {
+  if (L > a.max_seq) {  // a replayed graph that has run past the cache
     if (a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
     return make_int2(0, 0);
   }
@@ -815,12 +810,18 @@ __device__ __forceinline__ void deal_shares(const SharedArgs& a, int block, int 
   __shared__ int starts[UNITS_MAX + 1], lows[UNITS_MAX], highs[UNITS_MAX], sums[AP_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
+  // (loaded beside the number of units: there is room for as many as rows, and for half as many more)
+  const Unit mine = units[min(tid, a.mv.rows - 1)];
   const Head head = head_of(a);
+  if (head.rows != a.rows) {  // a replay after a set of another number of rows
+    if (block == 0 && tid == 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
+    return;
+  }
   const int nu = head.units, per = (nu + AP_THREADS - 1) / AP_THREADS;
   const int u0 = min(nu, tid * per), u1 = min(nu, u0 + per);
   int sum = 0;
   for (int u = u0; u < u1; u++) {
-    const Unit x = units[u];
+    const Unit x = u == tid && u < a.mv.rows ? mine : units[u];
     const int2 r = unit_range(a, x);
     const int t = (max(0, r.y - r.x) + SP_T - 1) / SP_T * a.n_kv * x.nch;
     starts[u] = t;
@@ -959,10 +960,7 @@ template <int VEC, int LP, bool ONE, bool PARTS>
 __global__ void __launch_bounds__(AP_THREADS) k_begin(const __grid_constant__ AppendArgs p,
                                                       const __grid_constant__ SharedArgs a, int deal) {
   const int block = (int)blockIdx.x - ((int)gridDim.x - deal);
-  if (head_of(a).rows != a.rows) {  // a replay after a set of another number of rows
-    griddep_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.err) atomicExch(a.err, SYN_ERR_INVALID_ARG);
-  } else if (block < 0) {
+  if (block < 0) {
     if constexpr (PARTS) append_rows<VEC, LP, ONE, 1>(p, QParts(a));
     else append_rows<VEC, LP, ONE, 1>(p);
   } else {
@@ -1173,8 +1171,7 @@ __device__ __forceinline__ bool span_job(const SharedArgs& a, const SpanJob& job
     for (int s = LPR; s < 32; s <<= 1)
 #pragma unroll
       for (int e = 0; e < 4; e++) x[e] += __shfl_xor_sync(0xffffffffu, x[e], s);
-    // (x * 0: nothing, or NaN)
-    const float sum = warp_sum(fmaf(x[0], 0.0f, fmaf(x[1], 0.0f, fmaf(x[2], 0.0f, fmaf(x[3], 0.0f, l[v])))));
+    const float sum = warp_sum(l[v]);
     if (v < job.nq) {
       if (lane == 0) a.pml[rec + v] = make_float2(m[v], sum);
       if (sub == 0 && l4 < hd)
@@ -1249,12 +1246,13 @@ constexpr int JN_WARPS = 4, JN_BLOCK = 32;  // records at a time
 // A query row from its definition, over the positions that it sees: exp(s - M) without a guard, so that NaN
 // and infinities go where the formula takes them. The other kernels cannot do that (a running maximum
 // drops NaN, a tile's other rows multiply what they do not see by 0, fp16 parts of an infinity are
-// NaN): they leave a sum that is NaN, or values that are not finite, and the row comes here. Slow
+// NaN): they leave a sum or a value that is not finite, and the row comes here. Slow
 // (each key's row by one warp, twice), and never taken by finite operands whose products stay finite.
 __device__ __noinline__ float join_plain(const SharedArgs& a, int b, int head, float (*red)[128]) {
   __shared__ double sums[JN_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd, kvh = head / a.G;
-  const int seq = a.meta[a.mv.seq() + b], L = min(a.len[seq] + 1, a.max_seq);
+  const int seq = a.meta[a.mv.seq() + b], L = a.len[seq] + 1;
+  if (L > a.max_seq) return 0.0f;  // (reported where the shares are dealt)
   const bool act = lane * 4 < hd;
   const float4 zero = make_float4(0, 0, 0, 0);
   float4 q = zero;
@@ -1307,7 +1305,7 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const __grid_constant__ 
   const int kvh = head / a.G, g = head - kvh * a.G;
   const Unit* units = reinterpret_cast<const Unit*>(a.meta + a.mv.units());
   const Head plan = head_of(a);
-  if (plan.rows != a.rows) {  // (as in k_begin: nothing was computed)
+  if (plan.rows != a.rows) {  // (as in deal_shares: nothing was computed)
     griddep_wait();
     if (threadIdx.x < hd) a.out[(long long)b * a.ldo + (long long)head * hd + threadIdx.x] = NAN;
     return;
@@ -1341,6 +1339,7 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < JN_BLOCK / JN_WARPS; e++) {
       const int c = c0 + warp + e * JN_WARPS;
+      x[e] = make_float4(0, 0, 0, 0);
       if (act && c < n) x[e] = __ldcg(reinterpret_cast<const float4*>(a.po + rec(c) * hd) + lane);
     }
   };
@@ -1361,12 +1360,10 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < JN_BLOCK / JN_WARPS; e++) {
       const float fc = __shfl_sync(0xffffffffu, f, warp + e * JN_WARPS);
-      if (fc != 0.0f && act) {  // (a part that saw nothing may hold anything)
-        o.x = fmaf(x[e].x, fc, o.x);
-        o.y = fmaf(x[e].y, fc, o.y);
-        o.z = fmaf(x[e].z, fc, o.z);
-        o.w = fmaf(x[e].w, fc, o.w);
-      }
+      o.x = fmaf(x[e].x, fc, o.x);  // (0 times what is not finite too: the row is taken again)
+      o.y = fmaf(x[e].y, fc, o.y);
+      o.z = fmaf(x[e].z, fc, o.z);
+      o.w = fmaf(x[e].w, fc, o.w);
     }
   }
   griddep_launch();
@@ -1377,7 +1374,7 @@ __global__ void __launch_bounds__(JN_WARPS * 32) k_join(const __grid_constant__ 
   const int d = threadIdx.x;
   float y = 0.0f;
   if (d < hd) y = ((red[0][d] + red[1][d]) + (red[2][d] + red[3][d])) * inv;
-  if (__syncthreads_or(!(fabsf(y) < INFINITY))) y = join_plain(a, b, head, red);
+  if (__syncthreads_or(!(fabsf(y) < INFINITY) || M == -INFINITY)) y = join_plain(a, b, head, red);
   if (d < hd) a.out[(long long)b * a.ldo + (long long)head * hd + d] = y;
 }
 
@@ -1483,6 +1480,8 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   {
     AppendArgs ap = append_args(at, p->q, qd, 0);
     ap.seq_of = p->meta + a.mv.seq();
+    ap.set_rows = p->meta;
+    ap.err = err;
     ap.rows = a.rows;
     const AppendShape sh = append_shape(ap);
     void (*kern)(const AppendArgs, const SharedArgs, int) = p->jobs ? begin_kernel<true>(sh) : begin_kernel<false>(sh);
