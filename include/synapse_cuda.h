@@ -278,7 +278,9 @@ syn_status_t syn_cuda_kvcache_create(syn_cuda_ctx_t *ctx, size_t max_seq,
  * a pool of n_pages pages of `page` positions; a sequence takes pages as it
  * grows (append, advance and the attention entry points) and returns them
  * on truncate / reset. No free page -> SYN_ERR_OUT_OF_MEMORY. page = 0 is
- * the contiguous cache. _view is unsupported on a paged cache. */
+ * the contiguous cache. _view is unsupported on a paged cache. A call on a
+ * captured stream takes its pages when it is captured; its replays find them in the table
+ * and leave the table alone. */
 syn_status_t syn_cuda_kvcache_create_paged(syn_cuda_ctx_t *ctx, size_t max_seq,
                                            size_t n_kv_heads, size_t head_dim,
                                            size_t num_layers, size_t batch, size_t page,

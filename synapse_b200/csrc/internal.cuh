@@ -238,6 +238,8 @@ struct AttnArgs {
 // table, copied to the device on `st`); SYN_ERR_OUT_OF_MEMORY when the pool
 // is exhausted. No-op for a contiguous cache.
 syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st);
+// The host's entries [first, first + n) of seq's table to the device, never as part of a graph.
+syn_status_t kv_put_table(syn_cuda_kvcache_t* c, size_t seq, size_t first, size_t n, cudaStream_t st);
 // The page that the next position of seq goes into, if other sequences hold it
 // too, is replaced by a copy (SYN_ERR_UNSUPPORTED while `st` is captured).
 syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);

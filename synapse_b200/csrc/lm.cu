@@ -2136,10 +2136,30 @@ syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaS
     c->refs[row[i]] = 1;
     first = std::min(first, i);
   }
-  if (first < need)
-    SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + seq * c->maxp + first, row + first,
-                                 (need - first) * sizeof(int), cudaMemcpyHostToDevice, st));
-  return SYN_OK;
+  return first < need ? kv_put_table(c, seq, first, need - first, st) : SYN_OK;
+}
+
+// On a captured stream the copy would become part of the graph, and every replay would put the
+// host's entries of that time back over what a reorder has made of them. There it is made at once,
+// beside the capture: nothing reads entries behind a sequence's length before then.
+syn_status_t kv_put_table(syn_cuda_kvcache_t* c, size_t seq, size_t first, size_t n, cudaStream_t st) {
+  const size_t at = seq * c->maxp + first, bytes = n * sizeof(int);
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+  if (cs == cudaStreamCaptureStatusNone) {
+    SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + at, c->ptab_h + at, bytes, cudaMemcpyHostToDevice, st));
+    return SYN_OK;
+  }
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  SYN_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+  cudaStream_t side = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(c->d_ptab + at, c->ptab_h + at, bytes, cudaMemcpyHostToDevice, side);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(side);
+  if (side) cudaStreamDestroy(side);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return e == cudaSuccess ? SYN_OK : cuda_status(e, "kv_put_table");
 }
 
 // Returns the pages of sequence seq beyond position keep_len to the free

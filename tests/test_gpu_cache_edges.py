@@ -114,3 +114,63 @@ def test_cut_back_without_a_page_for_the_copy(ctx):
     cache.truncate(6, 0)
     del m.ctxs[0][6:]
     m.check()
+
+
+def test_page_taken_while_capturing(ctx):
+    """A captured append that takes a page, without a call before it: its replays find the page,
+    and leave the table to the reorders in between."""
+    kv, hd, page, n = 1, 8, 4, 4
+    cache = sb.KVCache(ctx, 32, kv, hd, 1, n, page, 40)
+    m = _Mirror(cache)
+    m.grow(0, 8)  # full pages only
+    for s in range(1, n):
+        cache.fork(0, s)
+        m.ctxs[s] = list(m.ctxs[0])
+    cos, sin = _rope(32, hd)
+    qkv = torch.zeros(n, 3 * hd, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sb.qk_norm_rope_kv_append_batch(cache, 0, range(n), [1] * n, qkv, 1, None, None, 1e-6, cos, sin)
+
+    def step(value):
+        qkv[:, 2 * hd:] = -torch.arange(n, device="cuda")[:, None] - value
+        graph.replay()
+        for s in range(n):
+            cache.advance(1, s)
+            m.ctxs[s].append(s + value)
+
+    def check():  # V rows are stored as they come
+        table, v = cache.device_table().cpu(), cache.pages(0)[1].reshape(-1, hd).cpu()
+        for s, want in enumerate(m.ctxs):
+            pos = torch.arange(len(want))
+            got = v[table[s][pos // page].long() * page + pos % page]
+            assert torch.equal(got, -torch.tensor(want)[:, None].expand_as(got)), s
+    step(100.0)
+    check()
+    for value, p in ((200.0, [1, 0, 3, 2]), (300.0, [1, 2, 3, 0])):
+        cache.reorder(range(n), _ints(*p), n)
+        m.ctxs = [list(m.ctxs[j]) for j in p]
+        check()
+        step(value)
+        check()
+
+
+def test_page_taken_while_capturing_and_given_back(ctx):
+    """A sequence that was cut back since has no page for the replay, which then writes nothing."""
+    cache = sb.KVCache(ctx, 32, 1, 8, 1, 2, 4, 6)
+    cos, sin = _rope(32, 8)
+    qkv = torch.full((1, 24), 5.0, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sb.qk_norm_rope_kv_append_batch(cache, 0, [0], [1], qkv, 1, None, None, 1e-6, cos, sin)
+    cache.reset(0)
+    assert cache.pages_free() == 6
+    for p in cache.pages():
+        p.zero_()
+    cache.advance(20, 1)  # all of the first one's pages, and more
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(float(p.abs().sum()) == 0 for p in cache.pages())
+    assert int((cache.device_table()[0] >= 0).sum()) == 0
