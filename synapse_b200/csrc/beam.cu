@@ -763,7 +763,12 @@ syn_status_t kv_copy_shared(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) 
   int* e = c->ptab_h + seq * c->maxp + col;
   if (*e < 0 || c->refs[*e] <= 1) return SYN_OK;
   if (capturing(st)) return SYN_ERR_UNSUPPORTED;  // a replay would copy again
-  if (!c->n_free) return no_free_page();
+  if (!c->n_free) {  // (those of dropped beams are counted only when a table is read back)
+    syn_status_t s = kv_sync(c, st);
+    if (s) return s;
+    if (c->refs[*e] <= 1) return SYN_OK;
+    if (!c->n_free) return no_free_page();
+  }
   const int old = *e, own = c->free_pages[c->n_free - 1];
   syn_status_t s = kv_copy_page(c, old, own, c->len[seq] % c->page, st);
   if (s) return s;

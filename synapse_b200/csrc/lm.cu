@@ -2127,14 +2127,16 @@ syn_status_t kv_reserve(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaS
   }
   int* row = c->ptab_h + seq * c->maxp;
   const size_t need = (new_len + c->page - 1) / c->page;
-  size_t first = need, missing = 0;
-  for (size_t i = 0; i < need; i++) missing += row[i] < 0;
-  if (missing > c->n_free) return no_free_page();
-  for (size_t i = 0; i < need; i++) {
-    if (row[i] >= 0) continue;
+  size_t first = need;  // (a row is filled from the front)
+  while (first && row[first - 1] < 0) first--;
+  if (need - first > c->n_free) {  // those of dropped beams are counted only when a table is read back
+    syn_status_t s = kv_sync(c, st);
+    if (s && s != SYN_ERR_UNSUPPORTED) return s;
+    if (need - first > c->n_free) return no_free_page();
+  }
+  for (size_t i = first; i < need; i++) {
     row[i] = c->free_pages[--c->n_free];
     c->refs[row[i]] = 1;
-    first = std::min(first, i);
   }
   return first < need ? kv_put_table(c, seq, first, need - first, st) : SYN_OK;
 }

@@ -174,3 +174,55 @@ def test_page_taken_while_capturing_and_given_back(ctx):
     torch.cuda.synchronize()
     assert all(float(p.abs().sum()) == 0 for p in cache.pages())
     assert int((cache.device_table()[0] >= 0).sum()) == 0
+
+
+def test_search_runs_in_the_pages_that_its_beams_hold(ctx):
+    """Append, advance and reorder in turn, all beams from one: the pages of dropped beams are
+    found again before a call is refused."""
+    n, page, top = 4, 4, 64
+    # the longest context once, and of each beam the page it writes and one before
+    cache = sb.KVCache(ctx, top, 1, 8, 2, n, page, top // page + 2 * n)
+    m = _Mirror(cache)
+    m.grow(0, 16)
+    for s in range(1, n):
+        cache.fork(0, s)
+        m.ctxs[s] = list(m.ctxs[0])
+    for step in range(top - 16):
+        for s in range(n):
+            m.grow(s, 1)
+        cache.reorder(range(n), _ints(*[step % n] * n), n)
+        m.ctxs = [list(m.ctxs[step % n]) for _ in range(n)]
+    m.check()
+    for s in range(n):
+        cache.reset(s)
+    with pytest.raises(sb.SynapseError) as e:  # none left: refused, and nothing taken
+        for s in range(n):
+            cache.advance(top, s)
+    assert e.value.status == 3
+    for s in range(n):
+        cache.reset(s)
+    assert cache.pages_free() == cache.n_pages
+
+
+def test_batched_calls_find_dropped_pages(ctx):
+    """The same for the batched append and for a plan's attention."""
+    n, page, hd = 4, 4, 8
+    cos, sin = _rope(64, hd)
+    for kind in ("append", "attention"):
+        cache = sb.KVCache(ctx, 64, 1, hd, 1, n, page, 64 // page + 2 * n)
+        cache.advance(16, 0)
+        for s in range(1, n):
+            cache.fork(0, s)
+        plan = sb.DecodePlan(cache, 1)
+        plan.set([list(range(n))])
+        qkv = _rand((n, 3 * hd), 1)
+        for step in range(64 - 17):
+            if kind == "append":
+                sb.qk_norm_rope_kv_append_batch(cache, 0, range(n), [1] * n, qkv, 1, None, None, 1e-6, cos, sin)
+            else:
+                sb.attention_decode_shared(plan, 0, qkv, None, None, 1e-6, cos, sin)
+            for s in range(n):
+                cache.advance(1, s)
+            cache.reorder(range(n), _ints(*[step % n] * n), n)
+        torch.cuda.synchronize()
+        assert cache.length(0) == 63
