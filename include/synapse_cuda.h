@@ -339,8 +339,8 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t *cache, size_t src, size_t
  * at the next truncate, reset or fork of any sequence, which read the tables
  * back, and before a call is refused for want of a page (not while its stream is
  * captured). May be captured: a replay goes by the lengths of its own time, and leaves
- * a group whose lengths differ then as it is; a sequence reordered by a graph has its table read
- * back at every such call, and a truncate that leaves it in a page that others
+ * a group whose lengths differ then as it is; after a reorder by a graph the tables are read
+ * back at every truncate, reset and fork (appends, advances and attention do not wait), and a truncate that leaves it in a page that others
  * hold copies that page at once (SYN_ERR_OUT_OF_MEMORY without a free one, nothing
  * changed). Paged caches only. */
 syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t *cache, size_t n,

@@ -736,12 +736,8 @@ syn_status_t no_free_page() {
 }
 
 syn_status_t kv_own_page(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
-  if (!c->page || c->stale[seq] == 1) return SYN_OK;  // (a reorder leaves private last pages)
-  if (c->stale[seq] && !capturing(st)) {
-    syn_status_t s = kv_sync(c, st);
-    if (s) return s;
-  }
-  return kv_copy_shared(c, seq, st);
+  // (a reorder leaves private last pages, and kv_release sees to it that one by a graph finds them so)
+  return c->page && c->stale[seq] ? SYN_OK : kv_copy_shared(c, seq, st);
 }
 
 syn_status_t kv_cut(syn_cuda_kvcache_t* c, size_t seq, size_t new_len, cudaStream_t st) {

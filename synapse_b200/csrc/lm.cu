@@ -2188,6 +2188,22 @@ syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cuda
   return c->stale[seq] == 2 && keep_len % c->page ? kv_copy_shared(c, seq, st) : SYN_OK;
 }
 
+// Rows k and v (blockIdx.y) to positions pos .. pos + n of the sequence with page table ptab.
+__global__ void __launch_bounds__(256) k_kv_append_rows(float* kc, float* vc, const int* ptab, size_t page,
+                                                        size_t pos, const float* k, const float* v, size_t n,
+                                                        size_t row) {
+  griddep_wait();
+  griddep_launch();
+  float* cache = blockIdx.y ? vc : kc;
+  const float* from = blockIdx.y ? v : k;
+  for (size_t t = blockIdx.x; t < n; t += gridDim.x) {
+    const int pg = ptab[(pos + t) / page];
+    if (pg < 0) continue;  // (given back since the call was captured)
+    float* to = cache + ((size_t)pg * page + (pos + t) % page) * row;
+    for (size_t i = threadIdx.x; i < row; i += 256) to[i] = from[t * row + i];
+  }
+}
+
 __global__ void k_kv_advance_slots(int* len, const int* slots, int n) {
   griddep_wait();
   griddep_launch();
@@ -2374,6 +2390,15 @@ syn_status_t syn_cuda_kvcache_view(const syn_cuda_kvcache_t* c, size_t layer, si
   return SYN_OK;
 }
 
+static syn_status_t append_by_table(syn_cuda_kvcache_t* c, size_t layer, size_t seq, const float* k,
+                                    const float* v, size_t n, cudaStream_t st) {
+  const size_t row = c->n_kv * c->hd, base = layer * c->n_pages * c->page * row;
+  return cuda_status(launch_pdl(k_kv_append_rows, dim3((unsigned)std::min<size_t>(n, 1024), 2), dim3(256), 0, st,
+                                c->k + base, c->v + base, (const int*)c->d_ptab + seq * c->maxp, c->page,
+                                c->len[seq], k, v, n, row),
+                     "k_kv_append_rows");
+}
+
 syn_status_t syn_cuda_kvcache_append(syn_cuda_kvcache_t* c, size_t layer, size_t seq,
                                      const float* k, const float* v, size_t n_tokens,
                                      void* stream) {
@@ -2385,9 +2410,12 @@ syn_status_t syn_cuda_kvcache_append(syn_cuda_kvcache_t* c, size_t layer, size_t
   const size_t row = c->n_kv * c->hd;
   cudaStream_t st = (cudaStream_t)stream;
   if (c->page) {  // page by page
-    syn_status_t s = c->stale[seq] ? kv_sync(c, st) : SYN_OK;
-    if (s == SYN_OK) s = kv_reserve(c, seq, c->len[seq] + n_tokens, st);
+    syn_status_t s = kv_reserve(c, seq, c->len[seq] + n_tokens, st);
     if (s) return s;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    SYN_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+    // (where a reorder has moved the pages, or may have by the time of a replay, the device knows them)
+    if (c->stale[seq] || cs != cudaStreamCaptureStatusNone) return append_by_table(c, layer, seq, k, v, n_tokens, st);
     const size_t base = layer * c->n_pages * c->page;
     for (size_t t = 0; t < n_tokens;) {
       const size_t pos = c->len[seq] + t, in = pos % c->page;

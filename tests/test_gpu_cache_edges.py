@@ -226,3 +226,86 @@ def test_batched_calls_find_dropped_pages(ctx):
             cache.reorder(range(n), _ints(*[step % n] * n), n)
         torch.cuda.synchronize()
         assert cache.length(0) == 63
+
+
+def _grow(m, seq, n):
+    """_Mirror.grow, with values that are made on the device (nothing waits for it)."""
+    for _ in range(n):
+        m.tick += 1
+        for layer in range(m.c.layers):
+            x = torch.full((1, m.c.n_kv * m.c.hd), m.tick + 0.25 * layer, device="cuda")
+            m.c.append(layer, x, -x, seq)
+        m.c.advance(1, seq)
+        m.ctxs[seq].append(float(m.tick))
+
+
+def test_growing_calls_after_a_captured_reorder_do_not_wait(ctx):
+    """Sequences that a graph may permute at any time: appends, advances and attention find
+    their pages on the device, with no wait for it."""
+    n, hd, page = 4, 64, 4
+    cache = sb.KVCache(ctx, 64, 1, hd, 2, n, page, 60)
+    m = _Mirror(cache)
+    m.grow(0, 9)
+    for s in range(1, n):
+        cache.fork(0, s)
+        m.ctxs[s] = list(m.ctxs[0])
+    par = _ints(0, 1, 2, 3)
+    cos, sin = _rope(64, hd)
+    plan = sb.DecodePlan(cache, 1)
+    qkv = torch.zeros(n, 3 * hd, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reorder(range(n), par, n)
+    plan.set([list(range(n))])
+    # (every kernel once: a first launch loads it)
+    sb.qk_norm_rope_kv_append_batch(cache, 0, range(n), [1] * n, qkv, 1, None, None, 1e-6, cos, sin)
+    sb.attention_decode_shared(plan, 0, qkv, None, None, 1e-6, cos, sin)
+    for s in range(n):
+        _grow(m, s, 1)
+    for p in ([1, 1, 3, 0], [2, 0, 1, 1]):
+        par.copy_(torch.tensor(p, dtype=torch.int32))
+        torch.cuda.synchronize()
+        busy = torch.cuda.Event()
+        torch.cuda._sleep(900_000_000)  # about half a second
+        busy.record()
+        graph.replay()
+        m.ctxs = [list(m.ctxs[j]) for j in p]
+        sb.qk_norm_rope_kv_append_batch(cache, 0, range(n), [1] * n, qkv, 1, None, None, 1e-6, cos, sin)
+        sb.attention_decode_shared(plan, 1, qkv, None, None, 1e-6, cos, sin)
+        for s in range(n):
+            _grow(m, s, 3)  # (append and advance; over a page's end)
+        assert not busy.query()
+        m.check()
+    for s in range(n):
+        cache.reset(s)
+    assert cache.pages_free() == 60
+
+
+def test_captured_append_follows_a_reorder(ctx):
+    """The rows of a replay go to the pages that its sequences have by then."""
+    cache = sb.KVCache(ctx, 32, 1, 8, 2, 2, 4, 12)
+    m = _Mirror(cache)
+    for s in range(2):
+        m.grow(s, 9)
+    rows = torch.zeros(2, 3, 8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for s in range(2):
+            for layer in range(2):
+                cache.append(layer, rows[s], rows[s], s)
+    cache.reorder([0, 1], _ints(1, 0), 2)
+    m.ctxs.reverse()
+    for s in range(2):
+        rows[s] = 100.0 * (s + 1) + torch.arange(3, device="cuda")[:, None]
+    graph.replay()
+    torch.cuda.synchronize()
+    m.check()
+    table = cache.device_table().cpu()
+    for s in range(2):
+        pos = torch.arange(9, 12)
+        slot = table[s][pos // 4].long() * 4 + pos % 4
+        for t in cache.pages():
+            for layer in range(2):
+                assert torch.equal(t[layer].reshape(-1, 8)[slot], rows[s])
