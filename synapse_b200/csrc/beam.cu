@@ -667,13 +667,23 @@ __global__ void __launch_bounds__(BS_THREADS, 4) k_beam_select(const BeamArgs a)
   beam_pick(a, g, raw, keys, keys2);
 }
 
+// Elements that beam_pick needs room for, with segments of t tiles: k lists of k, or the heads that
+// reach the threads' k-th best.
+size_t beam_cap(size_t beams, size_t vocab, size_t k, int t) {
+  const size_t seg = (size_t)BS_TILE * t, lists = beams * ((vocab + seg - 1) / seg);
+  return std::max({k * k, k * ((lists + BS_THREADS - 1) / BS_THREADS), (size_t)BS_CAP / 2});
+}
+constexpr size_t BS_SMEM = 200 * 1024;
+
 // Tiles of a segment: as few as give at most two CTAs on every SM,
-// at most 8 (uneven waves then cost less than longer segments save).
-int beam_tiles(size_t rows, size_t vocab, int sms) {
+// at most 8 (uneven waves then cost less than longer segments save) unless a group's
+// lists would not fit (64 beams and continuations of 13 million tokens or more).
+int beam_tiles(size_t rows, size_t beams, size_t vocab, size_t k, int sms) {
   const size_t tiles = (vocab + BS_TILE - 1) / BS_TILE;
-  for (int t = 1; t < 8; t++)
-    if (rows * ((tiles + t - 1) / t) <= 2 * (size_t)sms) return t;
-  return 8;
+  int t = 1;
+  while (t < 8 && rows * ((tiles + t - 1) / t) > 2 * (size_t)sms) t++;
+  while (beam_cap(beams, vocab, k, t) * 2 * sizeof(uint64_t) > BS_SMEM) t++;
+  return t;
 }
 constexpr size_t BS_GROUPS = 65536;  // arrival counters, at the front of the scratch
 
@@ -870,8 +880,8 @@ syn_status_t launch_append_batch(const AttnArgs& at, float* q_out, size_t ldq, s
   return SYN_OK;
 }
 
-size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms) {
-  const size_t seg = (size_t)BS_TILE * beam_tiles(rows, vocab, sms), nseg = (vocab + seg - 1) / seg;
+size_t beam_scratch_bytes(size_t rows, size_t beams, size_t vocab, size_t k, int sms) {
+  const size_t seg = (size_t)BS_TILE * beam_tiles(rows, beams, vocab, k, sms), nseg = (vocab + seg - 1) / seg;
   return BS_GROUPS * sizeof(int) + rows * nseg * (k * sizeof(uint64_t) + sizeof(float2));
 }
 
@@ -886,7 +896,7 @@ syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t
   a.beams = (int)beams;
   a.vocab = (int)vocab;
   a.k = (int)k;
-  a.tiles = beam_tiles(rows, vocab, sms);
+  a.tiles = beam_tiles(rows, beams, vocab, k, sms);
   a.nseg = (int)((vocab + (size_t)BS_TILE * a.tiles - 1) / ((size_t)BS_TILE * a.tiles));
   a.vec = ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   a.scores = scores;
@@ -899,15 +909,11 @@ syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t
   a.out_p = out_p;
   a.out_t = out_t;
   a.out_f = out_f;
-  const size_t lists = beams * a.nseg;
-  // k lists of k, or the heads that reach the threads' k-th best
-  const size_t cap = std::max({k * k, k * ((lists + BS_THREADS - 1) / BS_THREADS), (size_t)BS_CAP / 2});
-  const size_t smem = cap * 2 * sizeof(uint64_t);
+  const size_t cap = beam_cap(beams, vocab, k, a.tiles), smem = cap * 2 * sizeof(uint64_t);
   a.cap = (int)cap;
-  if (smem > 200 * 1024) return SYN_ERR_UNSUPPORTED;
   void (*kern)(const BeamArgs) = a.tiles > 2 ? k_beam_select<16> : k_beam_select<8>;
   if (smem > 40 * 1024) {
-    syn_status_t s = more_smem((const void*)kern, 200 * 1024);
+    syn_status_t s = more_smem((const void*)kern, BS_SMEM);
     if (s) return s;
   }
   return launched(launch_pdl(kern, dim3((unsigned)a.nseg, (unsigned)rows), dim3(BS_THREADS), smem, st, a),
@@ -1067,7 +1073,7 @@ syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t* ctx, const float* logits, size
   if (!g.ok) return SYN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
   syn_status_t s = grow_scratch(&ctx->beam, &ctx->beam_bytes,
-                                beam_scratch_bytes(groups * beams, vocab, k, ctx->sms), st);
+                                beam_scratch_bytes(groups * beams, beams, vocab, k, ctx->sms), st);
   if (s) return s;
   return launch_beam_select(logits, ld, groups, beams, vocab, scores, finished, eos, k, out_scores,
                             out_parents, out_tokens, out_finished, ctx->beam, ctx->sms, st);

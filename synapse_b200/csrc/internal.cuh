@@ -335,7 +335,7 @@ constexpr size_t BEAMS_MAX = 64;  // beams of a group, continuations of a select
 // Lets a kernel have `bytes` of dynamic shared memory on the current device (the runtime is asked
 // only where a kernel needs more than it has been given there).
 syn_status_t more_smem(const void* fn, size_t bytes);
-size_t beam_scratch_bytes(size_t rows, size_t vocab, size_t k, int sms);
+size_t beam_scratch_bytes(size_t rows, size_t beams, size_t vocab, size_t k, int sms);
 syn_status_t launch_beam_select(const float* x, size_t ld, size_t groups, size_t beams,
                                 size_t vocab, const float* scores, const uint8_t* fin, int eos,
                                 size_t k, float* out_s, int32_t* out_p, int32_t* out_t,

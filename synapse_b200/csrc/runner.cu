@@ -1069,8 +1069,8 @@ syn_status_t beam_buffers(syn_cuda_model_s* m) {
   const size_t most = std::min<size_t>(m->max_batch, BEAMS_MAX);
   size_t bytes = 0;
   for (size_t b = 1; b <= most; b++)
-    bytes = std::max({bytes, beam_scratch_bytes(b, m->V, b, m->ctx->sms),
-                      beam_scratch_bytes(1, m->V, b, m->ctx->sms)});
+    bytes = std::max({bytes, beam_scratch_bytes(b, b, m->V, b, m->ctx->sms),
+                      beam_scratch_bytes(1, 1, m->V, b, m->ctx->sms)});
   if (!m->plan && !m->int8) {
     s = syn_cuda_decode_plan_create(m->cache, m->hq_l, &m->plan);
     if (s && s != SYN_ERR_UNSUPPORTED) return s;  // (other heads: each row's whole context)

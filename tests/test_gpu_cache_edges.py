@@ -309,3 +309,36 @@ def test_captured_append_follows_a_reorder(ctx):
         for t in cache.pages():
             for layer in range(2):
                 assert torch.equal(t[layer].reshape(-1, 8)[slot], rows[s])
+
+
+@pytest.mark.parametrize("vocab", [(1 << 24) + 3, 1 << 25])
+def test_select_of_the_largest_vocabularies(ctx, vocab):
+    """64 beams and 64 continuations: the header's limits, all at once."""
+    beams = k = 64
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(beams, vocab, generator=g, device="cuda")
+    x[torch.arange(beams), torch.randint(0, vocab, (beams,), generator=g, device="cuda")] = 9.0
+    scores = -torch.rand(beams, generator=g, device="cuda")
+    s, p, t, f = (o[0] for o in sb.beam_select(ctx, x, scores, beams, k=k))
+    # each beam's k best logits in 64 bits; within a beam logits decide, and equal ones go to the
+    # lower token
+    val, tok, beam = [], [], []
+    for b in range(beams):
+        top, at = torch.topk(x[b], k + 8)
+        lse = torch.logsumexp(x[b].double(), 0)
+        val.append(scores[b].double() + (top.double() - lse))
+        tok.append(at)
+        beam.append(torch.full_like(at, b))
+    val, tok, beam = torch.cat(val), torch.cat(tok), torch.cat(beam)
+    best = val.sort(descending=True).values[:k]
+    # as for smaller vocabularies: a thread's chain has an addition for every two tiles of its
+    # segment, of which there are 800 at most, so ceil(16384 / 800 / 2) = 11 of the 16 counted there
+    tol = 2 * 86 * 2.0 ** -24
+    mine = scores[p.long()].double() + (x[p.long(), t.long()].double()
+                                        - torch.stack([torch.logsumexp(x[b].double(), 0) for b in p.tolist()]))
+    assert ((mine - best).abs() <= tol).all()
+    assert ((s.double() - best).abs() <= tol + 2.0 ** -24 * best.abs()).all()
+    assert len({(a, b) for a, b in zip(p.tolist(), t.tolist())}) == k
+    for b in set(p.tolist()):
+        took = x[b, t[p == b].long()]
+        assert torch.equal(took, torch.topk(x[b], len(took)).values)
