@@ -526,6 +526,13 @@ def _index(v):
     return int(v)
 
 
+def _int32(v):
+    """An int32 argument of the C ABI (ctypes would take another number modulo 2^32)."""
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise SynapseError(2, f"{v} is no int32")
+    return int(v)
+
+
 def _int32s(values):
     """An int32 array of the C ABI; values that are no such numbers are refused."""
     try:
@@ -755,7 +762,7 @@ def beam_select(ctx, logits, scores, beams, k=None, finished=None, eos=-1):
     if rows:
         _check(lib().syn_cuda_beam_select(
             ctx.handle, logits.data_ptr(), ld if rows > 1 else vocab, g, beams, vocab,
-            scores.data_ptr(), _addr(finished), int(eos), k, s.data_ptr(), p.data_ptr(),
+            scores.data_ptr(), _addr(finished), _int32(eos), k, s.data_ptr(), p.data_ptr(),
             t.data_ptr(), f.data_ptr(), _raw_stream(ctx.device)), "beam_select")
     return s, p, t, f
 
@@ -960,6 +967,7 @@ class Model:
         ids = np.ascontiguousarray(np.asarray(prompt, dtype=np.int32).reshape(-1))
         if steps < 1 or beams < 1 or seq < 0:
             raise SynapseError(2, "generate_beam")
+        eos = _int32(eos)
         out = np.empty((beams, steps), dtype=np.int32)
         scores = np.empty(beams, dtype=np.float32)
         _check(lib().syn_cuda_generate_beam(

@@ -342,3 +342,12 @@ def test_select_of_the_largest_vocabularies(ctx, vocab):
     for b in set(p.tolist()):
         took = x[b, t[p == b].long()]
         assert torch.equal(took, torch.topk(x[b], len(took)).values)
+
+
+def test_select_end_tokens_that_are_no_int32(ctx):
+    x, s, fin = _rand((2, 50), 1), _rand((2,), 2), torch.zeros(2, dtype=torch.uint8, device="cuda")
+    for eos in (2 ** 32 + 9, 2 ** 31, -2 ** 31 - 1):
+        with pytest.raises(sb.SynapseError) as e:
+            sb.beam_select(ctx, x, s, 2, finished=fin, eos=eos)
+        assert e.value.status == 2
+    sb.beam_select(ctx, x, s, 2, finished=fin, eos=9)
