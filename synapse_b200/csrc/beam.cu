@@ -32,9 +32,9 @@ bool capturing(cudaStream_t st) {
 // One page's first rows to another page: grid (chunks, layers, K / V)
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) k_kv_copy_page(float4* k, float4* v, size_t layer4,
-                                                      size_t src4, size_t dst4, int n4) {
+                                                      size_t src4, size_t dst4, size_t n4) {
   float4* p = (blockIdx.z ? v : k) + blockIdx.y * layer4;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n4; i += gridDim.x * 256)
+  for (size_t i = blockIdx.x * 256 + threadIdx.x; i < n4; i += gridDim.x * 256)
     p[dst4 + i] = p[src4 + i];
 }
 
@@ -70,20 +70,16 @@ __device__ __forceinline__ int ro_parent(const int32_t* par, int i, int beams) {
   return p >= 0 && p < beams ? p : i;  // out of range: the member keeps its own
 }
 
-// The parents of the group from member g0 on, and its length. A group whose lengths differ (a replay
-// finds them so; a call refuses them) stays as it is. Whole block.
+// The parents of the group from member g0 on, and its length; 0, so that nothing moves, where the
+// lengths differ (a replay finds them so; a call refuses them). Whole block.
 __device__ __forceinline__ int ro_group(const ReorderArgs& a, int g0, int* par) {
   const int len = min(a.len[a.seq[g0]], a.max_seq);
-  int p = 0;
   bool same = true;
   if (threadIdx.x < a.beams) {
-    p = ro_parent(a.parents + g0, threadIdx.x, a.beams);
+    par[threadIdx.x] = ro_parent(a.parents + g0, threadIdx.x, a.beams);
     same = a.len[a.seq[g0 + threadIdx.x]] == len;
   }
-  same = __syncthreads_and(same);
-  if (threadIdx.x < a.beams) par[threadIdx.x] = same ? p : threadIdx.x;
-  __syncthreads();
-  return len;
+  return __syncthreads_and(same) ? len : 0;
 }
 
 // Where member i's last page comes from: {member whose page it takes, 1 if
@@ -138,11 +134,11 @@ __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ Reorder
       const int src = a.ptab[(size_t)a.seq[g0 + par[i - g0]] * a.maxp + col];
       const int dst = a.ptab[(size_t)a.seq[g0 + t.x] * a.maxp + col];
       if (src >= 0 && dst >= 0) {
-        const int n4 = tail * a.row4;
+        const size_t n4 = (size_t)tail * a.row4;
         const size_t s4 = (size_t)src * a.page * a.row4, d4 = (size_t)dst * a.page * a.row4;
         float4* k = a.k + blockIdx.z * a.layer4;
         float4* v = a.v + blockIdx.z * a.layer4;
-        for (int j = blockIdx.x * 256 + tid; j < n4; j += gridDim.x * 256) {
+        for (size_t j = blockIdx.x * 256 + tid; j < n4; j += gridDim.x * 256) {
           const float4 x = k[s4 + j], y = v[s4 + j];
           k[d4 + j] = x;
           v[d4 + j] = y;
@@ -727,12 +723,12 @@ syn_status_t more_smem(const void* fn, size_t bytes) {
 
 syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, cudaStream_t st) {
   const size_t row4 = c->n_kv * c->hd / 4, page4 = c->page * row4;
-  const int n4 = (int)(rows * row4);
+  const size_t n4 = rows * row4;
   if (!n4) return SYN_OK;
   for (size_t l0 = 0; l0 < c->layers; l0 += 32768) {
     const unsigned nl = (unsigned)std::min<size_t>(c->layers - l0, 32768);
     const size_t layer4 = c->n_pages * page4;
-    k_kv_copy_page<<<dim3((unsigned)std::min(8, (n4 + 255) / 256), nl, 2), 256, 0, st>>>(
+    k_kv_copy_page<<<dim3((unsigned)std::min<size_t>(8, (n4 + 255) / 256), nl, 2), 256, 0, st>>>(
         reinterpret_cast<float4*>(c->k) + l0 * layer4, reinterpret_cast<float4*>(c->v) + l0 * layer4,
         layer4, src * page4, dst * page4, n4);
   }
