@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "append.cuh"
@@ -976,7 +977,7 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t* c, size_t src, size_t dst
 }
 
 syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* seqs,
-                                      const int32_t* parents, size_t beams, void* stream) {
+                                      const int32_t* parents, size_t beams, void* stream) try {
   if (!c || !seqs || !parents) return SYN_ERR_NULL_PTR;
   if (!c->page) return SYN_ERR_UNSUPPORTED;
   if (!n) return SYN_OK;
@@ -1016,13 +1017,15 @@ syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int
     c->stale[seqs[i]] = std::max(c->stale[seqs[i]], mark);
   }
   return SYN_OK;
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
     syn_cuda_kvcache_t* c, size_t layer, size_t n_seqs, const int32_t* seqs, const size_t* n_tokens,
     const float* q, const float* k, const float* v, size_t ld, size_t n_heads, const float* q_norm,
     const float* k_norm, float eps, const float* rope_cos, const float* rope_sin, float* q_out,
-    size_t ldq, void* stream) {
+    size_t ldq, void* stream) try {
   if (!c || !seqs || !n_tokens || !q || !k || !v || !rope_cos || !rope_sin || !q_out)
     return SYN_ERR_NULL_PTR;
   if (layer >= c->layers) return SYN_ERR_INVALID_ARG;
@@ -1048,6 +1051,8 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
   AttnArgs a{const_cast<float*>(q), k, v, ld, n_heads, q_norm, k_norm, eps, rope_cos, rope_sin, 0, c,
              layer, nullptr, 0};
   return launch_append_batch(a, q_out, ldq, n_seqs, seqs, n_tokens, st);
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t* ctx, const float* logits, size_t ld,

@@ -1168,7 +1168,7 @@ syn_status_t beam_search(syn_cuda_model_s* m, size_t seq, const int32_t* prompt,
 
 syn_status_t syn_cuda_generate_beam(syn_cuda_model_t* m, size_t seq, const int32_t* prompt,
                                     size_t n_prompt, size_t beams, size_t n_steps, int32_t eos,
-                                    int32_t* out_tokens, float* out_scores) {
+                                    int32_t* out_tokens, float* out_scores) try {
   if (!m || !prompt || !out_tokens) return SYN_ERR_NULL_PTR;
   if (!m->finalized || !n_prompt || !n_steps || !beams) return SYN_ERR_INVALID_ARG;
   if (m->tp > 1 || !m->kv_page) return SYN_ERR_UNSUPPORTED;
@@ -1221,6 +1221,8 @@ syn_status_t syn_cuda_generate_beam(syn_cuda_model_t* m, size_t seq, const int32
     }
   }
   return SYN_OK;
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 syn_status_t syn_cuda_model_seq_len(const syn_cuda_model_t* m, size_t seq, size_t* len) {

@@ -1565,7 +1565,12 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
     syn_cuda_decode_plan_destroy(p);
     return SYN_ERR_OUT_OF_MEMORY;
   }
-  c->plans.push_back(p);
+  try {
+    c->plans.push_back(p);
+  } catch (const std::bad_alloc&) {
+    syn_cuda_decode_plan_destroy(p);
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
   *out = p;
   return SYN_OK;
 }
@@ -1594,7 +1599,7 @@ syn_status_t syn_cuda_decode_plan_destroy(syn_cuda_decode_plan_t* p) {
 
 syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups,
                                       const size_t* group_rows, const int32_t* seqs,
-                                      void* stream) {
+                                      void* stream) try {
   if (!p || (n_groups && (!group_rows || !seqs))) return SYN_ERR_NULL_PTR;
   syn_cuda_kvcache_t* c = p->cache;
   if (!c) return SYN_ERR_INVALID_ARG;
@@ -1625,11 +1630,11 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   int* h = p->meta_h;
   Job* jobs = reinterpret_cast<Job*>(h + mv.jobs());
   Item* items = reinterpret_cast<Item*>(h + mv.items());
+  p->parted = true;  // (until all of it is in place)
   p->seqs.assign(seqs, seqs + rows);
   p->prefix.assign(rows, 0);
   p->shrunk.assign(rows, 0);
   p->families.clear();
-  p->parted = false;
   // the sequences of a group, and those that a captured reorder may exchange with them at any time
   auto related = [&](size_t r0, size_t n) {
     std::vector<uint8_t> in(c->batch, 0);
@@ -1817,12 +1822,15 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
   p->groups = n_groups;
   SYN_CUDA_TRY(cudaMemcpyAsync(p->meta, h, p->meta_ints * sizeof(int), cudaMemcpyHostToDevice, st));
   SYN_CUDA_TRY(cudaEventRecord(p->copied, st));
+  p->parted = false;
   return SYN_OK;
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 syn_status_t syn_cuda_decode_plan_prefix(const syn_cuda_decode_plan_t* p, size_t row, size_t* len) {
   if (!p || !len) return SYN_ERR_NULL_PTR;
-  if (row >= p->rows) return SYN_ERR_INVALID_ARG;
+  if (row >= p->rows || p->parted) return SYN_ERR_INVALID_ARG;
   *len = p->prefix[row];
   return SYN_OK;
 }
@@ -1844,13 +1852,13 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
                                               size_t ld, const float* q_norm, const float* k_norm,
                                               float eps, const float* rope_cos,
                                               const float* rope_sin, size_t window, float* out,
-                                              size_t ldo, void* stream) {
+                                              size_t ldo, void* stream) try {
   if (!p || !q || !k || !v || !rope_cos || !rope_sin || !out) return SYN_ERR_NULL_PTR;
   syn_cuda_kvcache_t* c = p->cache;
   if (!c || layer >= c->layers) return SYN_ERR_INVALID_ARG;
+  if (p->parted) return SYN_ERR_INVALID_ARG;
   if (!p->rows) return SYN_OK;
   if (ld < c->hd || ldo < p->n_heads * c->hd) return SYN_ERR_SHAPE_MISMATCH;
-  if (p->parted) return SYN_ERR_INVALID_ARG;
   for (size_t i = 0; i < p->rows; i++) {
     const int sq = p->seqs[i];
     if (c->len[sq] + 1 > c->max_seq) return SYN_ERR_INVALID_ARG;  // CacheFull
@@ -1874,6 +1882,8 @@ syn_status_t syn_cuda_attention_decode_shared(syn_cuda_decode_plan_t* p, size_t 
   AttnArgs a{const_cast<float*>(q), k, v, ld, p->n_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
              window, c, layer, out, ldo};
   return launch_attn_shared(p, a, p->err, st);
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 }  // extern "C"

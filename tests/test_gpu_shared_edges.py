@@ -378,3 +378,15 @@ def test_scores_that_overflow(ctx):
     got = _attend(b)
     one = sb.attention_decode(b.cache, 0, b.qkv.clone(), 2, None, None, 1e-6, b.cos, b.sin, batch=2, flash=True)
     assert torch.equal(got.isnan(), one.isnan())
+
+
+def test_a_parted_plan_says_so_everywhere(ctx):
+    """Not only the attention call, of rows or of none, but what it would say of its rows too."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 64], [[3, 3], [3, 3]], seed=31)
+    assert b.plan.prefix(1) == 64
+    b.cache.reorder([0, 1, 2, 3], _ints(2, 1, 0, 3), 4)
+    _refused(lambda: b.plan.prefix(1))
+    _refused(lambda: _attend(b))
+    b.plan.set(b.groups)
+    assert b.plan.prefix(1) == 0
+    b.check()
