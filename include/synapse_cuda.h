@@ -375,7 +375,9 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
  * all later sets of as many rows: capture under the sharing that a graph is for.)
  * Replayed after a _set of another number of rows it computes nothing: its output
  * is NaN, and the plan's error word is SYN_ERR_INVALID_ARG.
- * head_dim <= 128; at most 512 rows in a plan. Destroy the plan before its cache. */
+ * head_dim <= 128; at most 512 rows in a plan, and 2^30 tiles of 32 positions that are
+ * computed row by row (rows x KV heads x ceil(heads a KV head / 8) x positions / 32): else
+ * SYN_ERR_UNSUPPORTED, and the plan has to be set again. Destroy the plan before its cache. */
 typedef struct syn_cuda_decode_plan_s syn_cuda_decode_plan_t;
 syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t *cache, size_t n_heads,
                                          syn_cuda_decode_plan_t **out);

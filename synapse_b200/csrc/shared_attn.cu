@@ -1771,6 +1771,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     p->prefix_ctas = p->span_sms = p->sms;
   else
     lay_out(true, many);
+  if (own > 1u << 30) return SYN_ERR_UNSUPPORTED;  // (the device counts k_span's tiles in 32 bits)
   size_t ni = 0, part = 0, done = 0, jt = 0;
   auto item_of = [&](const Job& job, size_t t0, size_t t1) {
     return Item{job.row0, job.m0, job.m,     job.kvh, job.len, (int)t0, (int)t1, (int)part,

@@ -390,3 +390,22 @@ def test_a_parted_plan_says_so_everywhere(ctx):
     b.plan.set(b.groups)
     assert b.plan.prefix(1) == 0
     b.check()
+
+
+def test_more_tiles_than_32_bits_count(ctx, monkeypatch):
+    """512 rows behind 2^26 shared positions, each by itself: refused, and the plan with it."""
+    monkeypatch.setenv("SYN_PLAN_LAYOUT", "1")
+    n, page = 512, 1 << 16
+    cache = sb.KVCache(ctx, (1 << 26) + page, 1, 4, 1, n, page, 1024 + n)
+    cache.advance(1 << 26, 0)
+    for s in range(1, n):
+        cache.fork(0, s)
+    plan = sb.DecodePlan(cache, 1)
+    plan.set([[0]])
+    _refused(lambda: plan.set([list(range(n))]), 12)
+    cos = torch.ones(cache.max_seq, 2, device="cuda")
+    _refused(lambda: sb.attention_decode_shared(plan, 0, torch.zeros(1, 12, device="cuda"), None, None, 1e-6, cos, cos))
+    _refused(lambda: plan.prefix(0))
+    plan.set([list(range(256))])
+    assert plan.prefix(255) == 1 << 26
+    cache.close()
