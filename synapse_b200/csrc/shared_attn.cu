@@ -1403,11 +1403,12 @@ Meta meta_of(const syn_cuda_decode_plan_t* p) {
   return Meta{(int)c->batch, (int)jobs, (int)(jobs + p->sms), p->sms};
 }
 
-// k_span: shared memory, and CTAs on an SM
+// k_span's shared memory. (One CTA on an SM, whatever it leaves free: 256 threads of up to 254 registers.
+// Twice the grid for heads of up to 60, where the memory would allow it, ran in two waves: 32 rows behind
+// 2048 positions, 600 of their own, took 37.3 us at head dim 32 and take 33.6; 34.6 and 30.4 at 48.)
 size_t span_smem(size_t hd) {
   return SP_WARPS * (SP_SLOTS * SP_T * (hd * 4 + 16) + SP_V * hd * 4 + SP_T * SP_V * 4);
 }
-int span_ctas(size_t hd) { return span_smem(hd) > 112 * 1024 ? 1 : 2; }
 // Most k_span jobs of a batch
 size_t span_jobs(size_t batch, size_t n_kv, size_t G) {
   return n_kv * (batch * ((G + SP_V - 1) / SP_V) + batch / 2 * (SP_FEW / SP_V));
@@ -1468,8 +1469,8 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
   a.po = p->po;
   a.pml = p->pml;
   a.rows = (int)p->rows;
-  a.warps = span_ctas(c->hd) * p->span_sms * SP_WARPS;
-  a.span0 = (int)(p->part_rows - (span_ctas(c->hd) * p->sms * SP_WARPS + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
+  a.warps = p->span_sms * SP_WARPS;
+  a.span0 = (int)(p->part_rows - (p->sms * SP_WARPS + span_jobs(c->batch, c->n_kv, a.G)) * SP_V);
   a.after_prefix = p->jobs > 0;
   a.shares = static_cast<Share*>(p->shares);
   a.sjobs = reinterpret_cast<SpanJob*>(a.shares + a.warps);
@@ -1504,7 +1505,7 @@ syn_status_t launch_attn_shared(syn_cuda_decode_plan_t* p, const AttnArgs& at, i
                                    : c->hd < 64  ? k_span<16, 0>
                                                  : k_span<32, 0>;
   if ((s = more_smem((const void*)span, span_smem(c->hd)))) return s;
-  s = launched(launch_pdl(span, dim3(span_ctas(c->hd) * p->span_sms), dim3(SP_THREADS), span_smem(c->hd), st, a),
+  s = launched(launch_pdl(span, dim3(p->span_sms), dim3(SP_THREADS), span_smem(c->hd), st, a),
                "k_span");
   if (s) return s;
   return launched(launch_pdl(k_join, dim3((unsigned)(p->rows * p->n_heads)), dim3(JN_WARPS * 32), 0, st, a),
@@ -1537,7 +1538,7 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   const size_t G = n_heads / c->n_kv;
   // per CTA than the batch's query rows; k_span records: 8 of each (warp, job) that meet
   const size_t prefix = c->batch * n_heads + (size_t)p->sms * std::min<size_t>(PM, c->batch * G);
-  const size_t span = (p->sms * span_ctas(c->hd) * SP_WARPS + span_jobs(c->batch, c->n_kv, G)) * SP_V;
+  const size_t span = (p->sms * SP_WARPS + span_jobs(c->batch, c->n_kv, G)) * SP_V;
   p->part_rows = prefix + span;
   if (p->part_rows > 0x7FFFFFFF) {
     delete p;
@@ -1553,7 +1554,7 @@ syn_status_t syn_cuda_decode_plan_create(syn_cuda_kvcache_t* c, size_t n_heads,
   if (e == cudaSuccess) e = cudaMalloc(&p->po, p->part_rows * c->hd * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&p->pml, p->part_rows * sizeof(float2));
   if (e == cudaSuccess)
-    e = cudaMalloc(&p->shares, p->sms * span_ctas(c->hd) * SP_WARPS * sizeof(Share) +
+    e = cudaMalloc(&p->shares, p->sms * SP_WARPS * sizeof(Share) +
                                    span_jobs(c->batch, c->n_kv, G) * sizeof(SpanJob));
   if (e == cudaSuccess) e = cudaMalloc(&p->err, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(p->err, 0, sizeof(int));
