@@ -338,11 +338,12 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t *cache, size_t src, size_t
  * Nothing synchronises. Pages that no member holds any more are counted free
  * at the next truncate, reset or fork of any sequence, which read the tables
  * back, and before a call is refused for want of a page (not while its stream is
- * captured). May be captured: a replay goes by the lengths of its own time, and leaves
- * a group whose lengths differ then as it is; after a reorder by a graph the tables are read
- * back at every truncate, reset and fork (appends, advances and attention do not wait), and a truncate that leaves it in a page that others
- * hold copies that page at once (SYN_ERR_OUT_OF_MEMORY without a free one, nothing
- * changed). Paged caches only. */
+ * captured). May be captured: a replay goes by the lengths of its own time, and
+ * leaves a group whose lengths differ then as it is. Once a reorder was captured, the
+ * tables are read back at every truncate, reset and fork (appends, advances and
+ * attention do not wait), and a truncate that leaves one of its sequences in a page
+ * that others hold copies that page at once (SYN_ERR_OUT_OF_MEMORY without a free
+ * one, nothing changed). Paged caches only. */
 syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t *cache, size_t n,
                                       const int32_t *seqs, const int32_t *parents,
                                       size_t beams, void *stream);
@@ -396,7 +397,10 @@ syn_status_t syn_cuda_decode_plan_get_error(syn_cuda_decode_plan_t *plan, int32_
 /* syn_cuda_attention_decode_flash for the plan's rows (row r of q / k / v / out
  * is sequence r of the plan; q is left as it is): headwise norms, RoPE, K and V
  * appended at each sequence's length, attention over all its positions or the
- * last `window`. Results within f32 reassociation of the reference order. The
+ * last `window`. Results within f32 reassociation of the reference order, but for what a
+ * group of more than 8 query rows per KV head shares: there q, K, V and the weights
+ * enter the products with 22 bits, and the sums are cut off towards zero (64 rows behind
+ * 32768 positions: 4.9e-6 relative, f32 in one order 3.5e-6). The
  * lengths are not advanced. Cache positions that a row does not see (behind its
  * sequence, outside its window) may hold anything; NaN and infinities that it sees
  * go where the formula takes them (such rows are computed once more, slowly). SYN_ERR_INVALID_ARG when a sequence was truncated,
@@ -408,8 +412,10 @@ syn_status_t syn_cuda_attention_decode_shared(
     const float *rope_sin, size_t window, float *out, size_t ldo, void *stream);
 /* The k best continuations of each group of beams. Row g*beams + b of logits
  * (stride ld) is beam b of group g; a candidate (b, t) has the value
- * scores[g*beams+b] + logits[t] - logsumexp(logits), compared in 64 bits; equal
- * values go to the lower beam, then to the larger logit, then to the lower
+ * scores[g*beams+b] + logits[t] - logsumexp(logits), compared in 64 bits. The
+ * sum of exponentials is an f32 sum of f32 terms (within 5.2e-6 relative): inside a beam the
+ * order is the logits' own, candidates of different beams that are closer than twice
+ * that may change places. Equal values go to the lower beam, then to the larger logit, then to the lower
  * token. NaN counts as -inf, +inf as the largest float. A beam with finished[row] != 0 (may be NULL) has the one candidate
  * (eos, its score); its others are -inf. Outputs [groups][k], best first:
  * value, beam within the group, token, and (optional) whether the

@@ -17,12 +17,15 @@ namespace syn {
 // is one step of its lanes, kept in registers between the sum and the rotation,
 // and HC heads of a row are under way at once, with the position found and its
 // angles read once for all of them. Single tokens of 32 sequences (48 head rows of
-// 128) take 2.4 us, the launch's own time; 7 ragged prompts (189 MB read and
-// written) 41.6 us, 70 % of what a copy of them takes.
+// 128) take 2.5 us, the launch's own time; 7 ragged prompts (189 MB read and
+// written) 42.7 us, 69 % of what a copy of them takes.
 // ---------------------------------------------------------------------------
 constexpr int AP_MAX = 256;  // sequences per launch (by value)
 constexpr int AP_THREADS = 256;
-constexpr size_t AP_FILL = 600;  // blocks from which a launch fills the device
+// Blocks from which a launch fills the device: from there on HC is 2. 32 head rows of 128 a token, one
+// and two heads a lane group: 8 tokens 2.8 and 3.4 us, 89 tokens 3.2 and 3.6, 281 tokens 4.4 and 4.0, 920
+// tokens 10.0 and 8.3, 5736 tokens 53.4 and 43.1.
+constexpr size_t AP_FILL = 600;
 
 struct AppendArgs {
   const float *q, *k, *v;

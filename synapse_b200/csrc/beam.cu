@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) k_kv_copy_page(float4* k, float4* v, size
 // the page of a member that has no child, matched in ascending order. No page
 // is both read and written, so the copies need no second buffer. The last block
 // to finish writes the tail entries, so one launch does it all (two took 48 us where
-// this takes 38.6: 4 x 8 beams, 28 layers, 257 MB of copies, the copy rate; 5.9 us for
+// this takes 39.3: 4 x 8 beams, 28 layers, 257 MB of copies, the copy rate; 6.1 us for
 // 4 beams of 16 layers, latency).
 // ---------------------------------------------------------------------------
 constexpr int RO_MAX = 256;  // sequences per call (by value in the launch)
@@ -117,7 +117,8 @@ __device__ __forceinline__ int2 ro_tail(const int* par, int i, int beams) {
 
 // grid (chunks, n, layers + 1): the copies of each layer; then, column chunks by group, the
 // table entries of full pages. Those of the last pages, which the copies go by, are
-// written by the block that finishes last.
+// written by the block that finishes last. (The lengths from the device, for the replays, cost 4 x 8
+// beams 0.7 us of 39.3.)
 __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ ReorderArgs a) {
   __shared__ int par[RO_MAX], old[RO_MAX][9];
   __shared__ int2 t;
@@ -218,8 +219,8 @@ void (*append_kernel(int lp))(const AppendArgs) {
 // lets too many through), one on the elements that are left, and what reaches it
 // ranked by counting. Which CTA is last changes no result.
 // Bound by HBM for many rows (4 bytes a logit): 160 rows of 128256 take 34.6 us, a third of
-// the copy rate, in 2.7 waves of segments. By latency for few: 8.5 us for 4 rows
-// of 32000, 12 for 8 of 151936, a chain of pass, bound, list and join.
+// the copy rate, in 2.2 waves of segments (1280 CTAs, four on an SM). By latency for few: 8.4 us for
+// 4 rows of 32000, 12.3 for 8 of 151936, a chain of pass, bound, list and join.
 // ---------------------------------------------------------------------------
 constexpr int BS_THREADS = 256, BS_KMAX = (int)BEAMS_MAX, BS_BMAX = (int)BEAMS_MAX;
 
@@ -672,7 +673,7 @@ size_t beam_cap(size_t beams, size_t vocab, size_t k, int t) {
 }
 constexpr size_t BS_SMEM = 200 * 1024;
 
-// Tiles of a segment: as few as give at most two CTAs on every SM,
+// Tiles of a segment: as few as give at most two CTAs on every SM (which has room for four),
 // at most 8 (uneven waves then cost less than longer segments save) unless a group's
 // lists would not fit (64 beams and continuations of 13 million tokens or more).
 int beam_tiles(size_t rows, size_t beams, size_t vocab, size_t k, int sms) {

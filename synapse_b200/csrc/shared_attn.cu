@@ -77,8 +77,9 @@ constexpr int SP_WARPS = 4, SP_T = 32, SP_SLOTS = 3;  // k_span: computing warps
 constexpr int SP_THREADS = 64 * SP_WARPS;
 constexpr int SP_V = 8;        // most query vectors of a k_span job
 // A group of at most so many query rows per KV head goes to k_span, which reads its prefix once for 8
-// of them. 8 query rows behind 512, 2048, 8192 positions take 12.4, 17.1, 26.9 us there and
-// 13.4, 15.7, 27.4 in k_prefix; 16 (two readings) 13.2, 19.2, 35.2 and 14.3, 17.6, 28.5.
+// of them. 8 query rows of 128 behind 512, 2048, 8192 positions take 12.7, 17.2, 26.8 us there and
+// 14.1, 17.3, 28.1 in k_prefix; 16 (two readings) 13.4, 19.7, 36.2 and 14.8, 18.4, 29.0. (8 rows of 64
+// behind 512: 12.9 and 12.2.)
 constexpr int SP_FEW = 8;
 constexpr int ROWS_MAX = 512;  // rows of a plan
 constexpr int UNITS_MAX = ROWS_MAX + ROWS_MAX / 2;
@@ -193,10 +194,10 @@ struct SharedArgs {
 // Waits are bounded (SYN_ERR_TIMEOUT). The two warps of the same query rows also wait for each other at
 // a barrier that is not, so a warp whose wait has run out does not leave by itself: it says so at
 // their next barrier, and both leave behind it.
-// 64 rows x 32 heads behind 32768 positions (8 KV heads of 128) take 155 us in all, 137
+// 64 rows x 32 heads behind 32768 positions (8 KV heads of 128) take 153 us in all, 140
 // of them here: 2.4 us a tile, of which the products are 0.9; conversions and
-// softmax fill 58 % of the issue slots and wait for each other the rest. (8 converting
-// warps in place of 16: 176 us; a warp that issues among them: 303.) A CTA's first tile
+// softmax fill 69 % of the issue slots and wait for each other the rest. (When it was built: 8
+// converting warps in place of 16, 176 us; a warp that issues among them, 303.) A CTA's first tile
 // takes 7 us, latencies of the page table, the rows, and 64 KB of O per item.
 // ---------------------------------------------------------------------------
 constexpr int PX_SOFT = 8, PX_CONV = 16;  // warps; then four of which one issues the products
@@ -1731,7 +1732,7 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     while ((size_t)nj <= n && items_at(most) > n) most++;
     return most;
   };
-  // What the kernels take (us, measured at head dim 128): k_prefix 4 + 0.05 m for m query rows (at
+  // What the kernels take (us, measured at head dim 128 and used for all): k_prefix 4 + 0.05 m for m query rows (at
   // least 7) and 1.2 + 0.0165 m (at most 2.6) a tile; k_span 4, 2.5 a tile of each warp, and k_join 1 for 32 records
   // of a row. The rows are taken 128 positions on, as they grow before the plan is next set.
   auto prefix_us = [&](int n) { return std::max(7.0, 4 + 0.05 * widest) + std::min(2.6, 1.2 + 0.0165 * widest) * most_of(n); };

@@ -278,6 +278,7 @@ def _check_as_plain(b, window=0):
         assert torch.equal(got[got.isinf()], want[want.isinf()])
         fine = want.isfinite()
         assert ((got - want).abs()[fine] <= tol[fine]).all()
+    assert b.plan.get_error() == 0
     if b.hd in (64, 128):  # the row-by-row kernel's NaN are in the same places
         other = sb.attention_decode(b.cache, 0, b.qkv.clone(), b.heads, None, None, 1e-6, b.cos, b.sin,
                                     window=window, batch=len(b.lens), flash=True).view(want.shape)
