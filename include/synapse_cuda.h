@@ -374,8 +374,10 @@ syn_status_t syn_cuda_qk_norm_rope_kv_append_batch(
  * of so many rows was captured while no group of more than 8 query rows per KV head
  * shared anything, or too little to gain by it, such groups are computed row by row in
  * all later sets of as many rows: capture under the sharing that a graph is for.)
- * Replayed after a _set of another number of rows it computes nothing: its output
- * is NaN, and the plan's error word is SYN_ERR_INVALID_ARG.
+ * Replayed after a _set of another number of rows, or after a reorder, truncate or
+ * reset that took from a group what it shared, it computes nothing: its output is NaN,
+ * and the plan's error word is SYN_ERR_INVALID_ARG. (A captured reorder takes it away
+ * when it is captured: set the plan again before either graph runs.)
  * head_dim <= 128; at most 512 rows in a plan, and 2^30 tiles of 32 positions that are
  * computed row by row (rows x KV heads x ceil(heads a KV head / 8) x positions / 32): else
  * SYN_ERR_UNSUPPORTED, and the plan has to be set again. Destroy the plan before its cache. */

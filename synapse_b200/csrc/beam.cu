@@ -780,15 +780,15 @@ syn_status_t kv_copy_shared(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) 
   c->refs[old]--;
   c->refs[own] = 1;
   *e = own;
-  kv_changed(c, seq);
+  kv_changed(c, seq, st);
   SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + seq * c->maxp + col, e, sizeof(int),
                                cudaMemcpyHostToDevice, st));
   return SYN_OK;
 }
 
-void kv_changed(syn_cuda_kvcache_t* c, size_t seq) {
+void kv_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
   c->shrunk[seq]++;
-  plans_changed(c, seq);
+  plans_changed(c, seq, st);
 }
 
 syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st) {
@@ -968,7 +968,7 @@ syn_status_t syn_cuda_kvcache_fork(syn_cuda_kvcache_t* c, size_t src, size_t dst
     c->refs[to[full]] = 1;
     if ((s = kv_copy_page(c, from[full], to[full], tail, st))) return s;
   }
-  kv_changed(c, dst);
+  kv_changed(c, dst, st);
   if (len)
     SYN_CUDA_TRY(cudaMemcpyAsync(c->d_ptab + dst * c->maxp, to, (full + (tail != 0)) * sizeof(int),
                                  cudaMemcpyHostToDevice, st));
@@ -999,7 +999,7 @@ syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int
     if ((s = kv_own_page(c, seqs[i], st))) return s;
   const bool captured = capturing(st);
   for (size_t i = 0; i < n; i += beams) {
-    plans_reordered(c, seqs + i, beams);
+    plans_reordered(c, seqs + i, beams, st);
     std::vector<int32_t> mix(seqs + i, seqs + i + beams);
     std::sort(mix.begin(), mix.end());
     if (captured && std::find(c->mixes.begin(), c->mixes.end(), mix) == c->mixes.end())

@@ -255,7 +255,7 @@ syn_status_t kv_copy_page(syn_cuda_kvcache_t* c, int src, int dst, size_t rows, 
 // recounts the pages (synchronises the device; refused while `st` is captured).
 syn_status_t kv_sync(syn_cuda_kvcache_t* c, cudaStream_t st);
 // Pages that seq shared may be its no longer: counted, and the plans told.
-void kv_changed(syn_cuda_kvcache_t* c, size_t seq);
+void kv_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
 // Frees the pages of seq beyond position keep_len (drains `st` first).
 syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cudaStream_t st);
 // Decode step of sequences [0, batch): norm/RoPE/append of the new token,
@@ -317,9 +317,10 @@ syn_status_t launch_kv_reorder(syn_cuda_kvcache_t* c, size_t n, const int32_t* s
 // What the launches of a plan's attention depend on beside its rows: k_prefix's CTAs, 0 without it.
 int decode_plan_layout(const syn_cuda_decode_plan_t* p);
 // A reorder of the group seqs[0 .. n): plans in which some but not all of them hold a group's shared
-// pages describe their rows no longer. _changed: the same for one sequence whose pages are its own now.
-void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n);
-void plans_changed(syn_cuda_kvcache_t* c, size_t seq);
+// pages describe their rows no longer. _changed: the same for one sequence that is shorter than what it
+// shared. Calls of such a plan are refused, and replays that follow on `st` compute nothing.
+void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n, cudaStream_t st);
+void plans_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
 // The cache goes: its plans refuse every call but their end.
 void plans_orphaned(syn_cuda_kvcache_t* c);
 // Decode attention of a plan's rows (q, k, v, the layer and the output in a;

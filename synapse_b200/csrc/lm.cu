@@ -2171,7 +2171,7 @@ syn_status_t kv_release(syn_cuda_kvcache_t* c, size_t seq, size_t keep_len, cuda
   SYN_CUDA_TRY(cudaStreamSynchronize(st));
   syn_status_t s = kv_sync(c, st);
   if (s) return s;
-  kv_changed(c, seq);
+  kv_changed(c, seq, st);
   int* row = c->ptab_h + seq * c->maxp;
   const size_t keep = (keep_len + c->page - 1) / c->page;
   bool changed = false;

@@ -29,6 +29,7 @@
 // A group's rows share their leading positions: who holds those pages. A reorder among holders
 // leaves every row with them; one that brings in another sequence's context does not.
 struct PlanFamily {
+  size_t len;                  // shared positions
   std::vector<uint8_t> holds;  // [batch]: 1, and 2 for those that the group depends on (its rows, and
 };                             // whatever a captured reorder may exchange with them)
 
@@ -1417,22 +1418,34 @@ size_t span_jobs(size_t batch, size_t n_kv, size_t G) {
 
 }  // namespace
 
-void plans_changed(syn_cuda_kvcache_t* c, size_t seq) {
-  for (auto* p : c->plans)
-    for (auto& f : p->families) {
-      p->parted |= f.holds[seq] == 2;
-      f.holds[seq] = 0;
-    }
+namespace {
+
+// A sequence holds a family's pages no longer.
+void family_loses(syn_cuda_decode_plan_t* p, PlanFamily& f, size_t seq, cudaStream_t st) {
+  if (f.holds[seq] == 2 && !p->parted) {
+    p->parted = true;
+    // No number of rows is this one, so what was captured computes nothing until the next set. (A
+    // captured reorder moves nothing yet, and must not do this whenever it is replayed.)
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    cudaStreamIsCapturing(st, &cs);
+    if (cs == cudaStreamCaptureStatusNone) cudaMemsetAsync(p->meta, 0xff, sizeof(int), st);
+  }
+  f.holds[seq] = 0;
 }
 
-void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n) {
+}  // namespace
+
+void plans_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
+  for (auto* p : c->plans)
+    for (auto& f : p->families)
+      if (c->len[seq] < f.len) family_loses(p, f, seq, st);
+}
+
+void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n, cudaStream_t st) {
   for (auto* p : c->plans)
     for (auto& f : p->families)
       if (!std::all_of(seqs, seqs + n, [&](int32_t s) { return f.holds[s] != 0; }))
-        for (size_t i = 0; i < n; i++) {
-          p->parted |= f.holds[seqs[i]] == 2;
-          f.holds[seqs[i]] = 0;
-        }
+        for (size_t i = 0; i < n; i++) family_loses(p, f, seqs[i], st);
 }
 
 void plans_orphaned(syn_cuda_kvcache_t* c) {
@@ -1660,12 +1673,12 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
     if (n > 1 && c->page) {
       size_t most = c->len[seqs[r0]];
       for (size_t j = r0; j < r0 + n; j++) most = std::min(most, c->len[seqs[j]]);
-      PlanFamily f{related(r0, n)};
+      PlanFamily f{0, related(r0, n)};
       const int* first = pages(seqs[r0]);
       size_t col = most / c->page;
       for (size_t s = 0; s < c->batch; s++)
         if (f.holds[s]) col = std::mismatch(first, first + col, pages(s)).first - first;
-      shared = col * c->page;
+      f.len = shared = col * c->page;
       for (size_t s = 0; s < c->batch && shared; s++)
         if (std::equal(first, first + col, pages(s))) f.holds[s] = std::max<uint8_t>(f.holds[s], 1);
       if (shared) p->families.push_back(std::move(f));

@@ -410,3 +410,44 @@ def test_more_tiles_than_32_bits_count(ctx, monkeypatch):
     plan.set([list(range(256))])
     assert plan.prefix(255) == 1 << 26
     cache.close()
+
+
+def test_replay_after_a_group_was_parted(ctx):
+    """A replay asks nobody: the plan itself says that its rows are not what they were."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 64], [[3, 3], [3, 3]], seed=41, spare=8)
+    graph, out = _capture(b, b.groups)
+
+    def void():
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out.isnan().all() and b.plan.get_error() == 2
+
+    def right():
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check(out=out)
+        assert b.plan.get_error() == 0
+    right()
+    b.cache.reorder([0, 1, 2, 3], _ints(2, 1, 0, 3), 4)
+    void()
+    b.plan.set(b.groups)  # shares nothing now
+    right()
+    b = Batch(ctx, 1, 4, 64, 16, [64], [[3, 3, 5]], seed=42, spare=8)
+    graph, out = _capture(b, b.groups)
+    b.cache.reorder([0, 1], _ints(1, 0), 2)  # inside the group
+    right()
+    b.cache.truncate(66, 2)  # of its own positions
+    b.lens[2] = 66
+    right()
+    b.cache.truncate(50, 2)  # of the shared ones
+    void()
+    b.lens[2] = 50
+    b.plan.set(b.groups)
+    b.check()
+    right()
+    b.cache.reset(0)
+    void()
+    b.lens[0] = 0
+    b.plan.set(b.groups)
+    b.check()
+    right()
