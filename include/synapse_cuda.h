@@ -425,7 +425,8 @@ syn_status_t syn_cuda_attention_decode_shared(
  * such token, finished must be NULL). The outputs may be the inputs where
  * k == beams. beams, k <= 64, k <= beams*vocab, vocab <= 2^25, at most 65535
  * rows. Scratch belongs to the
- * context, as for syn_cuda_qmatmul. */
+ * context and grows as for syn_cuda_qmatmul; what a captured call uses stays until the
+ * context is destroyed. */
 syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t *ctx, const float *logits, size_t ld,
                                   size_t groups, size_t beams, size_t vocab,
                                   const float *scores, const uint8_t *finished,

@@ -1060,7 +1060,7 @@ syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t* ctx, const float* logits, size
                                   size_t groups, size_t beams, size_t vocab, const float* scores,
                                   const uint8_t* finished, int32_t eos, size_t k, float* out_scores,
                                   int32_t* out_parents, int32_t* out_tokens, uint8_t* out_finished,
-                                  void* stream) {
+                                  void* stream) try {
   if (!ctx || !logits || !scores || !out_scores || !out_parents || !out_tokens)
     return SYN_ERR_NULL_PTR;
   if (!groups) return SYN_OK;
@@ -1074,11 +1074,21 @@ syn_status_t syn_cuda_beam_select(syn_cuda_ctx_t* ctx, const float* logits, size
   DeviceGuard g(ctx->device);
   if (!g.ok) return SYN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
-  syn_status_t s = grow_scratch(&ctx->beam, &ctx->beam_bytes,
-                                beam_scratch_bytes(groups * beams, beams, vocab, k, ctx->sms), st);
+  const size_t bytes = beam_scratch_bytes(groups * beams, beams, vocab, k, ctx->sms);
+  const bool captured = capturing(st);
+  if (bytes > ctx->beam_bytes && ctx->beam_captured && !captured) {
+    ctx->beam_kept.push_back(ctx->beam);
+    ctx->beam = nullptr;
+    ctx->beam_bytes = 0;
+    ctx->beam_captured = false;
+  }
+  syn_status_t s = grow_scratch(&ctx->beam, &ctx->beam_bytes, bytes, st);
   if (s) return s;
+  ctx->beam_captured |= captured;
   return launch_beam_select(logits, ld, groups, beams, vocab, scores, finished, eos, k, out_scores,
                             out_parents, out_tokens, out_finished, ctx->beam, ctx->sms, st);
+} catch (const std::bad_alloc&) {
+  return SYN_ERR_OUT_OF_MEMORY;
 }
 
 }  // extern "C"

@@ -248,6 +248,7 @@ syn_status_t syn_cuda_context_destroy(syn_cuda_ctx_t* ctx) {
     cudaFree(ctx->cnt);
     cudaFree(ctx->abuf);
     cudaFree(ctx->beam);
+    for (void* kept : ctx->beam_kept) cudaFree(kept);
     cudaFree(ctx->err);
     tp_release(ctx);
   }

@@ -20,6 +20,8 @@ struct syn_cuda_ctx_s {
   size_t abuf_bytes;
   void* beam;        // beam selection: the segments' candidates and sums
   size_t beam_bytes;
+  bool beam_captured;            // a graph holds `beam`, so it is not freed when it has to grow ...
+  std::vector<void*> beam_kept;  // ... but kept here
   int* err;          // device-side error word (e.g. SYN_ERR_TIMEOUT)
   void* nccl;        // tensor-parallel communicator (ncclComm_t) or nullptr
   int tp_rank, tp_world;

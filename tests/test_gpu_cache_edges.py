@@ -351,3 +351,29 @@ def test_select_end_tokens_that_are_no_int32(ctx):
             sb.beam_select(ctx, x, s, 2, finished=fin, eos=eos)
         assert e.value.status == 2
     sb.beam_select(ctx, x, s, 2, finished=fin, eos=9)
+
+
+def test_captured_select_outlives_a_larger_one():
+    """The context's scratch grows between a capture and its replay: the graph's own stays."""
+    ctx = sb.Context(0)
+    x, s = _rand((4, 3000), 1, 3.0), _rand((4,), 2)
+    want = [t.clone() for t in sb.beam_select(ctx, x, s, 4)]
+    graphs = []
+    for rows in (4, 4, 64, 512):
+        big, bs = _rand((rows, 20000), rows, 3.0), _rand((rows,), 3)
+        sb.beam_select(ctx, big, bs, 4)  # (grows from the third on)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sb.beam_select(ctx, x, s, 4)
+        graphs.append((graph, out))
+    fill = [torch.full((1 << 22,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]
+    for graph, out in graphs + graphs:
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+    assert all(int((t != 7).sum()) == 0 for t in fill)
+    del graphs, graph
+    ctx.close()
