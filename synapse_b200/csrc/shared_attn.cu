@@ -1250,8 +1250,8 @@ constexpr int JN_WARPS = 4, JN_BLOCK = 32;  // records at a time
 // and infinities go where the formula takes them. The other kernels cannot do that (a running maximum
 // drops NaN, a tile's other rows multiply what they do not see by 0, fp16 parts of an infinity are
 // NaN): they leave a sum or a value that is not finite, and the row comes here. A query or a score that
-// is NaN decides it; otherwise it is slow (each key's row by one warp, twice): 64
-// rows x 4 heads that see an infinite V element among 32768 positions take 11.4 ms, NaN queries no longer than others.
+// is NaN decides it, in no more time than a finite row; otherwise it is slow (each key's row by one warp,
+// twice): 64 rows x 4 heads that see an infinite V element among 32768 positions take 11.4 ms.
 // Never taken by finite operands whose products stay finite.
 __device__ __noinline__ float join_plain(const SharedArgs& a, int b, int head, float (*red)[128]) {
   __shared__ double sums[JN_WARPS];
