@@ -1005,6 +1005,7 @@ syn_status_t syn_cuda_kvcache_reorder(syn_cuda_kvcache_t* c, size_t n, const int
     if (captured && std::find(c->mixes.begin(), c->mixes.end(), mix) == c->mixes.end())
       c->mixes.push_back(std::move(mix));
   }
+  if (captured) plans_mixed(c, st);
   const size_t per = RO_MAX / beams * beams;
   for (size_t i0 = 0; i0 < n; i0 += per) {
     const size_t m = std::min(per, n - i0);

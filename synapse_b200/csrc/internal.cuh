@@ -323,6 +323,9 @@ int decode_plan_layout(const syn_cuda_decode_plan_t* p);
 // shared. Calls of such a plan are refused, and replays that follow on `st` compute nothing.
 void plans_reordered(syn_cuda_kvcache_t* c, const int32_t* seqs, size_t n, cudaStream_t st);
 void plans_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st);
+// A reorder was captured (its groups are in c->mixes): from now on plans depend on all that it may
+// exchange with their rows.
+void plans_mixed(syn_cuda_kvcache_t* c, cudaStream_t st);
 // The cache goes: its plans refuse every call but their end.
 void plans_orphaned(syn_cuda_kvcache_t* c);
 // Decode attention of a plan's rows (q, k, v, the layer and the output in a;

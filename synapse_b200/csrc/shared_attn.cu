@@ -1455,7 +1455,30 @@ void family_loses(syn_cuda_decode_plan_t* p, PlanFamily& f, size_t seq, cudaStre
   f.holds[seq] = 0;
 }
 
+// Whoever a captured reorder may exchange with a sequence that the group depends on is depended on too; and
+// a holder that one may exchange with a sequence that is none is no holder for long.
+void family_close(syn_cuda_decode_plan_t* p, PlanFamily& f, cudaStream_t st) {
+  for (bool more = true; more;) {
+    more = false;
+    for (const auto& mix : p->cache->mixes) {
+      const bool all = std::all_of(mix.begin(), mix.end(), [&](int32_t s) { return f.holds[s] != 0; });
+      const bool core = std::any_of(mix.begin(), mix.end(), [&](int32_t s) { return f.holds[s] == 2; });
+      for (int32_t s : mix) {
+        const uint8_t was = f.holds[s];
+        if (!all) family_loses(p, f, s, st);
+        else if (core) f.holds[s] = 2;
+        more |= f.holds[s] != was;
+      }
+    }
+  }
+}
+
 }  // namespace
+
+void plans_mixed(syn_cuda_kvcache_t* c, cudaStream_t st) {
+  for (auto* p : c->plans)
+    for (auto& f : p->families) family_close(p, f, st);
+}
 
 void plans_changed(syn_cuda_kvcache_t* c, size_t seq, cudaStream_t st) {
   for (auto* p : c->plans)
@@ -1703,7 +1726,10 @@ syn_status_t syn_cuda_decode_plan_set(syn_cuda_decode_plan_t* p, size_t n_groups
       f.len = shared = col * c->page;
       for (size_t s = 0; s < c->batch && shared; s++)
         if (std::equal(first, first + col, pages(s))) f.holds[s] = std::max<uint8_t>(f.holds[s], 1);
-      if (shared) p->families.push_back(std::move(f));
+      if (shared) {
+        family_close(p, f, st);
+        p->families.push_back(std::move(f));
+      }
     }
     for (size_t j = r0; j < r0 + n; j++) {
       p->prefix[j] = shared;

@@ -451,3 +451,46 @@ def test_replay_after_a_group_was_parted(ctx):
     b.plan.set(b.groups)
     b.check()
     right()
+
+
+def _captured_reorder(b, seqs):
+    par = torch.arange(len(seqs), dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.cache.reorder(seqs, par, len(seqs))
+    return graph, par
+
+
+def test_what_a_captured_reorder_depends_on_is_used_anew(ctx):
+    """A reorder of holders is captured after the set; one of them, outside the plan, then gets another
+    context, which a replay would bring to the plan's rows."""
+    b = Batch(ctx, 1, 4, 64, 16, [64], [[3, 3, 3, 3]], seed=51, spare=12)
+    b.plan.set([[0, 1]])
+    # 3 reaches the rows through 2 only, and was captured first
+    graphs = [_captured_reorder(b, s) for s in ([2, 3], [0, 2])]
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+    b.cache.reset(3)
+    b.cache.advance(67, 3)
+    _refused(lambda: _attend(b, rows=[0, 1]))
+    b.plan.set([[0, 1]])
+    for graph, par in graphs:
+        par.copy_(_ints(1, 0))
+        graph.replay()
+    torch.cuda.synchronize()
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+
+
+def test_a_holder_that_a_captured_reorder_may_replace(ctx):
+    """Captured before the set: a sequence that holds the shared pages may have another context by the time
+    an ordinary reorder brings it into the group."""
+    b = Batch(ctx, 1, 4, 64, 16, [64, 64], [[3, 3, 3], [3]], seed=52)
+    graph, par = _captured_reorder(b, [2, 3])
+    b.plan.set([[0, 1]])
+    par.copy_(_ints(1, 0))
+    graph.replay()
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
+    b.cache.reorder([0, 2], _ints(1, 0), 2)
+    _refused(lambda: _attend(b, rows=[0, 1]))
+    b.plan.set([[0, 1]])
+    b.check(out=_attend(b, rows=[0, 1]), lens=b.lens[:2])
